@@ -257,6 +257,196 @@ QWN_CUDA_ABI_API int qwn_hip_ext_kv_attention_device_noalloc(QwnCudaContextHandl
                                                              uint32_t query_heads, uint32_t position,
                                                              float scale, void *stream);
 
+/* ---- operators of a batched serving step --------------------------------
+ * What lies between the projections when many sequences are decoded at once:
+ * the residual's addition with RMSNorm and the projections' int8 input, the
+ * paged 4-bit KV cache, and the logits' penalties and masks.  Each takes a
+ * request struct of device pointers that a caller builds once and passes
+ * every step; strides are in elements (0: rows back to back), and no pointer
+ * needs more alignment than its element.  A request's outputs may not overlap its inputs except
+ * where it says so.  Sizes that only the device knows (a batch's row starts,
+ * cached lengths, page numbers, token ids) are read there, so a captured
+ * step replays with new ones; each is checked there, and what points outside
+ * the buffers that the host described is left out.  No counterpart in the
+ * reference. */
+#define QWN_HIP_DTYPE_F32 0u
+#define QWN_HIP_DTYPE_F16 1u
+#define QWN_HIP_DTYPE_BF16 2u
+
+/* h = x + residual (rounded to dtype; residual NULL: h = x)
+ * y = h * norm / sqrt(mean(h^2) + eps), rounded once to fp32 from 64 bits
+ * scales[t] = amax / 127 (1 where amax is 0), q8 = rint(y / scale): the
+ * per-token quantization of qwn_hip_ext_quantize_device on y, bit for bit.
+ * A token whose y are not all finite has the scale NaN and zeros in q8. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t tokens;
+    uint32_t cols;
+    uint32_t dtype;                /* of x, residual, residual_out and y */
+    uint32_t x_stride;
+    uint32_t residual_stride;
+    uint32_t residual_out_stride;
+    uint32_t y_stride;
+    uint32_t q8_stride;            /* q8 is zero from cols to here */
+    float eps;
+    uint32_t reserved;
+    const void *x;                 /* [tokens][x_stride] */
+    const void *residual;          /* NULL, or [tokens][residual_stride] */
+    void *residual_out;            /* NULL, or h [tokens][residual_out_stride]; may be x or residual
+                                      with that one's stride */
+    const float *norm;             /* [cols] */
+    void *y;                       /* NULL, or [tokens][y_stride] */
+    int8_t *q8;                    /* NULL, or [tokens][q8_stride] (then scales too) */
+    float *scales;                 /* [tokens] */
+} QwnHipNormRequest;
+QWN_CUDA_ABI_API int qwn_hip_ext_norm_quantize_device(QwnCudaContextHandle *context,
+                                                      const QwnHipNormRequest *request, void *stream);
+
+/* A paged KV cache held in 4 bits: `pages` pages of page_tokens tokens (a
+ * power of two from 16 to 1024), handed to sequences by the caller through a
+ * page table.  A token's K or V of one head (head_dim up to 256) is held per
+ * group of 64 channels as an f16 minimum, an f16 step = (max - min) / 15 and
+ * codes rint((x - minimum) / step) in 0 .. 15; it stands for minimum + step *
+ * code.  Values that are not finite are held as zero, finite ones clamped to
+ * the range of f16.  rope_dims (even, 0: none) channels of every key, as
+ * pairs (i, i + rope_dims / 2), are rotated by position * rope_theta^(-2 i /
+ * rope_dims) on the way in, in 64 bits.  Charged to the context's budget; one
+ * cache per layer. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t pages;
+    uint32_t page_tokens;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t rope_dims;
+    float rope_theta;
+} QwnHipPagedKvOptions;
+typedef struct {
+    QwnCudaAbiHeader header;
+    void *opaque;
+} QwnHipPagedKvHandle;
+QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_create(QwnCudaContextHandle *context, const QwnHipPagedKvOptions *options,
+                                                 QwnHipPagedKvHandle *out);
+/* Waits for the device: no call of any stream may still use the cache. */
+QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_destroy(QwnCudaContextHandle *context, QwnHipPagedKvHandle *cache);
+
+/* A ragged batch.  Sequence s brings the rows starts[s] .. starts[s + 1] - 1
+ * of the step's tensors (none, one, or many), its tokens past[s], past[s] + 1,
+ * ...; slot t of it lies in page page_table[s][t / page_tokens].  Rows behind
+ * starts[sequences] belong to no sequence: they are not read, and outputs keep
+ * what they held there.  A sequence whose past is negative or whose rows do
+ * not lie in 0 .. tokens is left out; slots whose page is not one of the
+ * cache's (or lies past table_stride) are not stored, and not attended to. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t sequences;
+    uint32_t tokens;               /* rows of the step's tensors */
+    uint32_t table_stride;         /* pages of a row of the table */
+    uint32_t reserved;
+    const int32_t *starts;         /* device [sequences + 1], ascending */
+    const int32_t *past;           /* device [sequences]: tokens before this step's */
+    const int32_t *page_table;     /* device [sequences][table_stride] */
+} QwnHipPagedBatch;
+
+/* Stores the batch's keys (rotated) and values at their slots, and, if query
+ * is given, writes the rotated queries.  A position is the token's slot, or
+ * positions[row].  Sequences may share pages (a common prefix), but a slot may
+ * be named once in a call. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    const QwnHipPagedBatch *batch;
+    uint32_t dtype;                /* of key, value, query and query_out */
+    uint32_t query_heads;
+    uint32_t key_stride;
+    uint32_t value_stride;
+    uint32_t query_stride;
+    uint32_t query_out_stride;
+    const void *key;               /* [tokens][key_stride]: [kv_heads][head_dim] */
+    const void *value;             /* [tokens][value_stride] */
+    const void *query;             /* NULL, or [tokens][query_stride]: [query_heads][head_dim] */
+    void *query_out;               /* [tokens][query_out_stride]; may be query with its stride */
+    const int32_t *positions;      /* NULL, or [tokens] */
+} QwnHipPagedAppendRequest;
+QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_append_device(QwnCudaContextHandle *context, QwnHipPagedKvHandle *cache,
+                                                        const QwnHipPagedAppendRequest *request, void *stream);
+
+/* The values that the batch's tokens (its rows, as the append stored them)
+ * stand for, fp32 [tokens][stride] of keys and values (either may be NULL). */
+QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_read_device(QwnCudaContextHandle *context, QwnHipPagedKvHandle *cache,
+                                                      const QwnHipPagedBatch *batch, float *keys, float *values,
+                                                      uint32_t stride, void *stream);
+
+/* Causal attention of the batch's rows over the cache, the batch's own tokens
+ * appended before: token past[s] + i of sequence s attends to its slots 0 ..
+ * past[s] + i, query head h to KV head h / (query_heads / kv_heads).  A row
+ * that attends to nothing is zeros; a row whose query is not finite is NaN.
+ * fp32 queries are computed to fp32 (22 bits of query and probability in the
+ * matrix products), f16 and bf16 ones with f16 probabilities.  The workspace
+ * (qwn_hip_ext_paged_kv_attention_workspace_bytes, the same for every batch
+ * of a cache; 0 for a request that is refused; 16-byte aligned) holds nothing
+ * between calls, and may not be shared by calls that run at the same time. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    const QwnHipPagedBatch *batch;
+    uint32_t dtype;                /* of query and output */
+    uint32_t query_heads;          /* a multiple of the cache's kv_heads */
+    uint32_t query_stride;
+    uint32_t output_stride;
+    const void *query;             /* [tokens][query_stride]: [query_heads][head_dim] */
+    void *output;                  /* [tokens][output_stride] */
+    void *workspace;
+    float scale;
+    uint32_t reserved;
+} QwnHipPagedAttentionRequest;
+QWN_CUDA_ABI_API uint64_t qwn_hip_ext_paged_kv_attention_workspace_bytes(QwnCudaContextHandle *context,
+                                                                         QwnHipPagedKvHandle *cache,
+                                                                         const QwnHipPagedAttentionRequest *request);
+QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_attention_device(QwnCudaContextHandle *context, QwnHipPagedKvHandle *cache,
+                                                           const QwnHipPagedAttentionRequest *request, void *stream);
+
+/* The logits of a batch before the greedy choice (or a caller's sampler):
+ * tokens of the row's history: l > 0 ? l / repetition : l * repetition, and
+ * for those it holds `count` > 0 times behind its first prompt_counts[row]
+ * entries l -= frequency * count + presence; l += the sum of the token's
+ * biases (a token may come several times); l = -inf where the token's bit of
+ * the row's mask is 0.  In 64 bits, rounded to fp32 and then to dtype.  ids: the first
+ * index of the largest value, -1 for a row that nothing is left of (every
+ * value -inf or NaN).  Tokens outside 0 .. vocab - 1 in a list are padding.
+ * A row's part of a list is list[starts[row]] .. list[starts[row + 1] - 1],
+ * none if that does not lie in the list's capacity.  Row r reads mask row
+ * mask_index[r] (none if that is not one), or r where mask_index is NULL. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t rows;                 /* up to 65535 */
+    uint32_t vocab;
+    uint32_t dtype;                /* of logits and out */
+    uint32_t in_stride;
+    uint32_t out_stride;
+    uint32_t history_capacity;     /* entries of history */
+    uint32_t bias_capacity;        /* entries of bias_tokens and bias_values */
+    uint32_t mask_rows;
+    uint32_t mask_stride;          /* words of a mask row */
+    uint32_t reserved;
+    const void *logits;            /* [rows][in_stride] */
+    void *out;                     /* [rows][out_stride]; may be logits with its stride */
+    const int32_t *history;        /* NULL, or token ids, every row's prompt and what it generated */
+    const int32_t *history_starts; /* [rows + 1] */
+    const int32_t *prompt_counts;  /* NULL (none), or [rows] */
+    const float *repetition;       /* NULL (1), or [rows] */
+    const float *presence;         /* NULL (0), or [rows] */
+    const float *frequency;        /* NULL (0), or [rows] */
+    const int32_t *bias_tokens;    /* NULL, or token ids */
+    const float *bias_values;
+    const int32_t *bias_starts;    /* [rows + 1] */
+    const uint32_t *mask;          /* NULL, or [mask_rows][mask_stride]: bit t % 32 of word t / 32 */
+    const int32_t *mask_index;     /* NULL, or [rows] */
+    int32_t *ids;                  /* NULL, or [rows] */
+    void *workspace;               /* for ids: qwn_hip_ext_logits_workspace_bytes(), 8-byte aligned */
+} QwnHipLogitsRequest;
+QWN_CUDA_ABI_API uint64_t qwn_hip_ext_logits_workspace_bytes(uint32_t rows, uint32_t vocab);
+QWN_CUDA_ABI_API int qwn_hip_ext_logits_process_device(QwnCudaContextHandle *context,
+                                                       const QwnHipLogitsRequest *request, void *stream);
+
 /* Debug: the integer sums of the GEMV for one token, computed by the same
  * device code as the GEMV (host pointers, synchronous).  HyperVSQ-2:
  * out[row][block*8 + octant] = sum (code-1)*a; Q4_0: out[row][block] =

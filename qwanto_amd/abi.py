@@ -60,6 +60,10 @@ EXT_EXPORTS = (
     "qwn_hip_ext_gemm_mfma_group_device", "qwn_hip_ext_upload_batch", "qwn_hip_ext_plan_residency",
     "qwn_hip_ext_debug_mfma_int_sums", "qwn_hip_ext_debug_kv_read",
     "qwn_hip_ext_kv_attention_device_noalloc",
+    "qwn_hip_ext_norm_quantize_device", "qwn_hip_ext_paged_kv_create", "qwn_hip_ext_paged_kv_destroy",
+    "qwn_hip_ext_paged_kv_append_device", "qwn_hip_ext_paged_kv_read_device",
+    "qwn_hip_ext_paged_kv_attention_workspace_bytes", "qwn_hip_ext_paged_kv_attention_device",
+    "qwn_hip_ext_logits_workspace_bytes", "qwn_hip_ext_logits_process_device",
 )
 DECODER_EXPORTS = (
     "qwn_hip_decoder_create", "qwn_hip_decoder_destroy", "qwn_hip_decoder_reset",
@@ -70,6 +74,13 @@ DECODER_EXPORTS = (
 
 GEMV_INPUT = {"image": 0, "f32": 1, "rmsnorm": 2, "swiglu": 3}
 GEMV_OUTPUT = {"store": 0, "add": 1, "argmax": 2, "swiglu": 3}
+ACTIVATION = {"f32": 0, "f16": 1, "bf16": 2}
+
+# The null stream itself (hipStreamLegacy) as a `stream` argument, for callers
+# whose other work is on it (torch's default stream): None is the context's own
+# stream, ordered with the null stream but not the same one, and every change
+# between the two costs the GPU a wait.
+NULL_STREAM = 1
 
 
 class Header(ctypes.Structure):
@@ -202,6 +213,52 @@ class DecoderStats(_Versioned):
                 ("graph", ctypes.c_uint32), ("prefill_block_tokens", ctypes.c_uint32)]
 
 
+def _fields(kind, *names):
+    return [(n, kind) for n in names]
+
+
+class NormRequest(_Versioned):
+    _fields_ = [("header", Header)] + \
+        _fields(ctypes.c_uint32, "tokens", "cols", "dtype", "x_stride", "residual_stride", "residual_out_stride",
+                "y_stride", "q8_stride") + \
+        [("eps", ctypes.c_float), ("reserved", ctypes.c_uint32)] + \
+        _fields(ctypes.c_void_p, "x", "residual", "residual_out", "norm", "y", "q8", "scales")
+
+
+class PagedKvOptions(_Versioned):
+    _fields_ = [("header", Header)] + \
+        _fields(ctypes.c_uint32, "pages", "page_tokens", "kv_heads", "head_dim", "rope_dims") + \
+        [("rope_theta", ctypes.c_float)]
+
+
+class PagedBatch(_Versioned):
+    _fields_ = [("header", Header)] + _fields(ctypes.c_uint32, "sequences", "tokens", "table_stride", "reserved") + \
+        _fields(ctypes.c_void_p, "starts", "past", "page_table")
+
+
+class PagedAppendRequest(_Versioned):
+    _fields_ = [("header", Header), ("batch", ctypes.POINTER(PagedBatch))] + \
+        _fields(ctypes.c_uint32, "dtype", "query_heads", "key_stride", "value_stride", "query_stride",
+                "query_out_stride") + \
+        _fields(ctypes.c_void_p, "key", "value", "query", "query_out", "positions")
+
+
+class PagedAttentionRequest(_Versioned):
+    _fields_ = [("header", Header), ("batch", ctypes.POINTER(PagedBatch))] + \
+        _fields(ctypes.c_uint32, "dtype", "query_heads", "query_stride", "output_stride") + \
+        _fields(ctypes.c_void_p, "query", "output", "workspace") + \
+        [("scale", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
+class LogitsRequest(_Versioned):
+    _fields_ = [("header", Header)] + \
+        _fields(ctypes.c_uint32, "rows", "vocab", "dtype", "in_stride", "out_stride", "history_capacity",
+                "bias_capacity", "mask_rows", "mask_stride", "reserved") + \
+        _fields(ctypes.c_void_p, "logits", "out", "history", "history_starts", "prompt_counts", "repetition",
+                "presence", "frequency", "bias_tokens", "bias_values", "bias_starts", "mask", "mask_index", "ids",
+                "workspace")
+
+
 class Placement(ctypes.Structure):
     """QwnHipPlacement (the reference's QwnPlacement layout)."""
     _fields_ = [("name_hash", ctypes.c_uint64), ("byte_offset", ctypes.c_uint64),
@@ -326,6 +383,17 @@ class Library:
         lib.qwn_hip_ext_gemm_mfma_device.argtypes = [P(Handle), P(Handle), V, V, V, U32, U32, V]
         lib.qwn_hip_ext_gemm_mfma_group_device.argtypes = [P(Handle), P(Handle), U32, V, V, V, U32, U32, U32, V]
         lib.qwn_hip_ext_upload_batch.argtypes = [P(Handle), P(TensorUpload), U32, P(Handle)]
+        lib.qwn_hip_ext_norm_quantize_device.argtypes = [P(Handle), P(NormRequest), V]
+        lib.qwn_hip_ext_paged_kv_create.argtypes = [P(Handle), P(PagedKvOptions), P(Handle)]
+        lib.qwn_hip_ext_paged_kv_destroy.argtypes = [P(Handle), P(Handle)]
+        lib.qwn_hip_ext_paged_kv_append_device.argtypes = [P(Handle), P(Handle), P(PagedAppendRequest), V]
+        lib.qwn_hip_ext_paged_kv_read_device.argtypes = [P(Handle), P(Handle), P(PagedBatch), V, V, U32, V]
+        lib.qwn_hip_ext_paged_kv_attention_workspace_bytes.argtypes = [P(Handle), P(Handle), P(PagedAttentionRequest)]
+        lib.qwn_hip_ext_paged_kv_attention_workspace_bytes.restype = ctypes.c_uint64
+        lib.qwn_hip_ext_paged_kv_attention_device.argtypes = [P(Handle), P(Handle), P(PagedAttentionRequest), V]
+        lib.qwn_hip_ext_logits_workspace_bytes.argtypes = [U32, U32]
+        lib.qwn_hip_ext_logits_workspace_bytes.restype = ctypes.c_uint64
+        lib.qwn_hip_ext_logits_process_device.argtypes = [P(Handle), P(LogitsRequest), V]
         lib.qwn_hip_ext_plan_residency.argtypes = [V, V, V, V, U32, ctypes.c_uint64, ctypes.c_uint64, V, V]
         lib.qwn_hip_decoder_create.argtypes = [P(Handle), P(DecoderDesc), P(Handle)]
         lib.qwn_hip_decoder_destroy.argtypes = [P(Handle), P(Handle)]
@@ -608,6 +676,99 @@ class Context:
         self.lib.check("kv_attention_device", self.lib.lib.qwn_hip_ext_kv_attention_device(
             self._h, ctypes.byref(h), q_ptr, out_ptr, query_heads, position, scale, work_ptr,
             stream))
+
+    # -- a batched serving step -------------------------------------------------
+    # Requests hold device pointers, are built once and passed every step; the
+    # caller keeps the tensors behind them alive.  A stride of 0: rows back to back.
+    def norm_request(self, tokens: int, cols: int, dtype: str, x_ptr: int, norm_ptr: int, eps: float,
+                     residual_ptr: int | None = None, residual_out_ptr: int | None = None, y_ptr: int | None = None,
+                     q8_ptr: int | None = None, scales_ptr: int | None = None, x_stride: int = 0,
+                     residual_stride: int = 0, residual_out_stride: int = 0, y_stride: int = 0,
+                     q8_stride: int = 0) -> NormRequest:
+        return NormRequest(tokens=tokens, cols=cols, dtype=ACTIVATION[dtype], x_stride=x_stride,
+                           residual_stride=residual_stride, residual_out_stride=residual_out_stride,
+                           y_stride=y_stride, q8_stride=q8_stride, eps=eps, x=x_ptr, residual=residual_ptr,
+                           residual_out=residual_out_ptr, norm=norm_ptr, y=y_ptr, q8=q8_ptr, scales=scales_ptr)
+
+    def norm_quantize_device(self, req: NormRequest, stream: int | None = None) -> None:
+        self.lib.check("norm_quantize_device",
+                       self.lib.lib.qwn_hip_ext_norm_quantize_device(self._h, ctypes.byref(req), stream))
+
+    def paged_kv_create(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, rope_dims: int = 0,
+                        rope_theta: float = 0.0) -> Handle:
+        opts = PagedKvOptions(pages=pages, page_tokens=page_tokens, kv_heads=kv_heads, head_dim=head_dim,
+                              rope_dims=rope_dims, rope_theta=rope_theta)
+        h = Handle()
+        self.lib.check("paged_kv_create", self.lib.lib.qwn_hip_ext_paged_kv_create(
+            self._h, ctypes.byref(opts), ctypes.byref(h)))
+        return h
+
+    def paged_kv_destroy(self, h: Handle) -> None:
+        self.lib.check("paged_kv_destroy", self.lib.lib.qwn_hip_ext_paged_kv_destroy(self._h, ctypes.byref(h)))
+
+    def paged_batch(self, sequences: int, tokens: int, starts_ptr: int, past_ptr: int, table_ptr: int,
+                    table_stride: int) -> PagedBatch:
+        """One step's ragged batch: starts [sequences + 1], past [sequences] and
+        the page table [sequences][table_stride], int32 on the device."""
+        return PagedBatch(sequences=sequences, tokens=tokens, table_stride=table_stride, starts=starts_ptr,
+                          past=past_ptr, page_table=table_ptr)
+
+    def paged_append_request(self, batch: PagedBatch, dtype: str, k_ptr: int, v_ptr: int,
+                             q_ptr: int | None = None, q_out_ptr: int | None = None, query_heads: int = 0,
+                             positions_ptr: int | None = None, key_stride: int = 0, value_stride: int = 0,
+                             query_stride: int = 0, query_out_stride: int = 0) -> PagedAppendRequest:
+        return PagedAppendRequest(batch=ctypes.pointer(batch), dtype=ACTIVATION[dtype], query_heads=query_heads,
+                                  key_stride=key_stride, value_stride=value_stride, query_stride=query_stride,
+                                  query_out_stride=query_out_stride, key=k_ptr, value=v_ptr, query=q_ptr,
+                                  query_out=q_out_ptr, positions=positions_ptr)
+
+    def paged_kv_append_device(self, h: Handle, req: PagedAppendRequest, stream: int | None = None) -> None:
+        self.lib.check("paged_kv_append_device", self.lib.lib.qwn_hip_ext_paged_kv_append_device(
+            self._h, ctypes.byref(h), ctypes.byref(req), stream))
+
+    def paged_kv_read_device(self, h: Handle, batch: PagedBatch, k_ptr: int | None, v_ptr: int | None,
+                             stride: int = 0, stream: int | None = None) -> None:
+        self.lib.check("paged_kv_read_device", self.lib.lib.qwn_hip_ext_paged_kv_read_device(
+            self._h, ctypes.byref(h), ctypes.byref(batch), k_ptr, v_ptr, stride, stream))
+
+    def paged_attention_request(self, batch: PagedBatch, dtype: str, query_heads: int, q_ptr: int, out_ptr: int,
+                                scale: float, workspace_ptr: int | None = None, query_stride: int = 0,
+                                output_stride: int = 0) -> PagedAttentionRequest:
+        return PagedAttentionRequest(batch=ctypes.pointer(batch), dtype=ACTIVATION[dtype], query_heads=query_heads,
+                                     query_stride=query_stride, output_stride=output_stride, query=q_ptr,
+                                     output=out_ptr, workspace=workspace_ptr, scale=scale)
+
+    def paged_attention_workspace_bytes(self, h: Handle, req: PagedAttentionRequest) -> int:
+        return int(self.lib.lib.qwn_hip_ext_paged_kv_attention_workspace_bytes(self._h, ctypes.byref(h),
+                                                                                ctypes.byref(req)))
+
+    def paged_kv_attention_device(self, h: Handle, req: PagedAttentionRequest, stream: int | None = None) -> None:
+        self.lib.check("paged_kv_attention_device", self.lib.lib.qwn_hip_ext_paged_kv_attention_device(
+            self._h, ctypes.byref(h), ctypes.byref(req), stream))
+
+    def logits_workspace_bytes(self, rows: int, vocab: int) -> int:
+        return int(self.lib.lib.qwn_hip_ext_logits_workspace_bytes(rows, vocab))
+
+    def logits_request(self, rows: int, vocab: int, dtype: str, logits_ptr: int, out_ptr: int, in_stride: int = 0,
+                       out_stride: int = 0, history_ptr: int | None = None, history_starts_ptr: int | None = None,
+                       history_capacity: int = 0, prompt_counts_ptr: int | None = None,
+                       repetition_ptr: int | None = None, presence_ptr: int | None = None,
+                       frequency_ptr: int | None = None, bias_tokens_ptr: int | None = None,
+                       bias_values_ptr: int | None = None, bias_starts_ptr: int | None = None,
+                       bias_capacity: int = 0, mask_ptr: int | None = None, mask_rows: int = 0, mask_stride: int = 0,
+                       mask_index_ptr: int | None = None, ids_ptr: int | None = None,
+                       workspace_ptr: int | None = None) -> LogitsRequest:
+        return LogitsRequest(rows=rows, vocab=vocab, dtype=ACTIVATION[dtype], in_stride=in_stride, out_stride=out_stride,
+                             history_capacity=history_capacity, bias_capacity=bias_capacity, mask_rows=mask_rows,
+                             mask_stride=mask_stride, logits=logits_ptr, out=out_ptr, history=history_ptr,
+                             history_starts=history_starts_ptr, prompt_counts=prompt_counts_ptr,
+                             repetition=repetition_ptr, presence=presence_ptr, frequency=frequency_ptr,
+                             bias_tokens=bias_tokens_ptr, bias_values=bias_values_ptr, bias_starts=bias_starts_ptr,
+                             mask=mask_ptr, mask_index=mask_index_ptr, ids=ids_ptr, workspace=workspace_ptr)
+
+    def logits_process_device(self, req: LogitsRequest, stream: int | None = None) -> None:
+        self.lib.check("logits_process_device",
+                       self.lib.lib.qwn_hip_ext_logits_process_device(self._h, ctypes.byref(req), stream))
 
     # -- misc -----------------------------------------------------------------
     def telemetry(self) -> Telemetry:

@@ -5,6 +5,7 @@
 
 #include "qwn_cuda_abi.h"
 #include "qwn_internal.h"
+#include "qwn_paged.h"
 
 #include <algorithm>
 #include <mutex>
@@ -62,6 +63,11 @@ struct ResidentKv {
     void *allocation = nullptr;
 };
 
+struct ResidentPaged {
+    PagedKv c;
+    void *allocation = nullptr;
+};
+
 struct Decoder;  // qwn_decoder.hip
 
 // Weight upload pipeline: whole-row chunks of a host buffer are copied into
@@ -103,6 +109,7 @@ struct Context {
     DeviceBuffer dev_in, dev_out, dev_scales, dev_work, dev_img;
     std::vector<ResidentTensor *> tensors;
     std::vector<ResidentKv *> caches;
+    std::vector<ResidentPaged *> paged;
     std::vector<Decoder *> decoders;
     UploadPipe upload;
     DownloadPipe download;
@@ -117,6 +124,34 @@ template <typename T>
 bool header_ok(const T &s) {
     return s.header.abi_version == QWN_CUDA_ABI_VERSION && s.header.struct_size >= sizeof(T);
 }
+
+// A row stride of a request: 0 stands for rows back to back.
+inline uint32_t stride_or(uint32_t stride, uint64_t row) {
+    return stride ? stride : static_cast<uint32_t>(std::min<uint64_t>(row, UINT32_MAX));
+}
+
+// Makes `device` current for one call and the caller's device current again
+// after it.
+class DeviceScope {
+public:
+    explicit DeviceScope(int device) {
+        if ((error_ = hipGetDevice(&before_)) != hipSuccess || before_ == device) {
+            before_ = -1;
+            return;
+        }
+        error_ = hipSetDevice(device);
+    }
+    ~DeviceScope() {
+        if (before_ >= 0) (void)hipSetDevice(before_);
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+    hipError_t error() const { return error_; }
+
+private:
+    int before_ = -1;
+    hipError_t error_ = hipSuccess;
+};
 
 Context *context_of(const QwnCudaContextHandle *h);
 // Handles this context issued (lock held by the caller); null otherwise.
@@ -134,6 +169,9 @@ hipError_t download_rows(Context *ctx, float *dst, size_t dst_stride, const floa
 
 // Allocates what download_rows needs (it does so itself when first called).
 hipError_t ready_download(Context *ctx);
+
+// Releases a paged cache's device memory (context lock held).
+void destroy_paged(ResidentPaged *rp);
 
 // Releases a decoder's device memory and graph (context lock held).
 void destroy_decoder(Decoder *d);

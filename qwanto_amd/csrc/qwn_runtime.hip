@@ -626,8 +626,10 @@ QWN_CUDA_ABI_API int qwn_cuda_abi_context_destroy(QwnCudaContextHandle *handle) 
         ctx->decoders.clear();
         for (ResidentTensor *t : ctx->tensors) free_tensor(t);
         for (ResidentKv *c : ctx->caches) free_cache(c);
+        for (ResidentPaged *c : ctx->paged) destroy_paged(c);
         ctx->tensors.clear();
         ctx->caches.clear();
+        ctx->paged.clear();
         ctx->host_in.release();
         ctx->host_out.release();
         ctx->download.data.release();

@@ -1,0 +1,125 @@
+"""Helpers of the serving operators' tests: batches on the GPU, and the
+operators' definitions in 64 bits on the host."""
+import torch
+
+DEV = "cuda:0"
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+# half a step of a type's rounding, relative to the value
+HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+GROUP = 64
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(g, *shape):
+    return torch.randn(*shape, generator=g, dtype=torch.float32)
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def stream():
+    from qwanto_amd import abi
+    return torch.cuda.current_stream().cuda_stream or abi.NULL_STREAM
+
+
+def quantize8(y):
+    """The framework's per-token int8 quantization of fp32 y: (codes, scales)."""
+    amax = y.abs().amax(dim=1, keepdim=True)
+    scale = torch.where(amax > 0, amax / torch.full_like(amax, 127.0), torch.ones_like(amax))
+    inv = torch.ones_like(scale) / scale
+    return (y * inv).clamp(-127.0, 127.0).round().to(torch.int8), scale[:, 0]
+
+
+def levels(x):
+    """The cache's 4-bit form of fp32 x [..., head_dim]: (values float64, step, minimum of
+    every channel, the quotient each code is rounded from)."""
+    x = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).clamp(-65504.0, 65504.0)
+    values, steps, mins, quotients = [], [], [], []
+    for c in range(0, x.shape[-1], GROUP):
+        g = x[..., c:c + GROUP]
+        lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+        m = lo.half().double()
+        s = ((hi - lo) / torch.full_like(lo, 15.0)).half().double()
+        t = torch.where(s > 0, (g.double() - m) / torch.where(s > 0, s, torch.ones_like(s)), torch.zeros_like(g.double()))
+        values.append(m + s * t.round().clamp(0, 15))
+        steps.append(s.expand_as(t))
+        mins.append(m.expand_as(t))
+        quotients.append(t)
+    cat = lambda v: torch.cat(v, dim=-1)  # noqa: E731
+    return cat(values), cat(steps), cat(mins), cat(quotients)
+
+
+def rotate(x, positions, rope, theta):
+    """[rows][heads][head_dim] rotated in 64 bits: pairs (i, i + rope / 2)."""
+    y = x.double().clone()
+    half = rope // 2
+    if half:
+        freq = theta ** (-2.0 * torch.arange(half, dtype=torch.float64) / rope)
+        ang = (positions.double()[:, None] * freq)[:, None]
+        a, b = x[..., :half].double(), x[..., half:rope].double()
+        y[..., :half] = a * ang.cos() - b * ang.sin()
+        y[..., half:rope] = a * ang.sin() + b * ang.cos()
+    return y
+
+
+class Cache:
+    """A paged cache of the library with its table, filled and read through the
+    public calls."""
+
+    def __init__(self, ctx, lengths, kv_heads, head_dim, page=16, rope=0, theta=1.0e6, extra=2, seed=0, width=None):
+        """`lengths`: slots each sequence may use."""
+        self.ctx, self.kv_heads, self.head_dim, self.page, self.rope, self.theta = ctx, kv_heads, head_dim, page, rope, theta
+        need = [-(-n // page) for n in lengths]
+        self.pages = sum(need) + extra
+        order = torch.randperm(self.pages, generator=gen(seed + 99)).to(torch.int32)
+        self.width = width or max(max(need), 1)
+        table = torch.full((len(lengths), self.width), -1, dtype=torch.int32)
+        at = 0
+        for s, n in enumerate(need):
+            table[s, :n] = order[at:at + n]
+            at += n
+        self.table_host = table
+        self.table = table.to(DEV)
+        self.h = ctx.paged_kv_create(self.pages, page, kv_heads, head_dim, rope_dims=rope, rope_theta=theta if rope else 0.0)
+        self.keep = []
+
+    def batch(self, past, new, pad=0, table=None):
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        s = torch.tensor(starts, dtype=torch.int32, device=DEV)
+        p = torch.tensor(past, dtype=torch.int32, device=DEV)
+        t = self.table if table is None else table
+        b = self.ctx.paged_batch(len(past), max(1, starts[-1] + pad), ptr(s), ptr(p), ptr(t), t.shape[1])
+        self.keep.append((s, p, t, b))
+        return b
+
+    def append(self, batch, k, v, dtype, q=None, q_out=None, heads=0, positions=None, **strides):
+        r = self.ctx.paged_append_request(batch, dtype, ptr(k), ptr(v), q_ptr=ptr(q), q_out_ptr=ptr(q_out),
+                                          query_heads=heads, positions_ptr=ptr(positions), **strides)
+        self.ctx.paged_kv_append_device(self.h, r, stream=stream())
+
+    def read(self, batch, fill=float("nan")):
+        out = torch.full((2, batch.tokens, self.kv_heads * self.head_dim), fill, device=DEV)
+        self.ctx.paged_kv_read_device(self.h, batch, ptr(out[0]), ptr(out[1]), stream=stream())
+        return out.cpu()
+
+    def request(self, batch, q, out, dtype, heads, scale, **strides):
+        r = self.ctx.paged_attention_request(batch, dtype, heads, ptr(q), ptr(out), scale, **strides)
+        n = self.ctx.paged_attention_workspace_bytes(self.h, r)
+        assert n > 0, "request refused"
+        work = torch.full((n,), 0xff, dtype=torch.uint8, device=DEV)   # NaN everywhere
+        r.workspace = ptr(work)
+        self.keep.append((work, r))
+        return r
+
+    def attend(self, batch, q, out, dtype, heads, scale, **strides):
+        self.ctx.paged_kv_attention_device(self.h, self.request(batch, q, out, dtype, heads, scale, **strides), stream=stream())
+
+    def close(self):
+        torch.cuda.synchronize()
+        self.ctx.paged_kv_destroy(self.h)

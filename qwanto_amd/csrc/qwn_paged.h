@@ -11,12 +11,14 @@
 //           (i >> 1) | (i & 1) << 2
 //   values  [load][lane 64][JW words]   lane 16 g + n: tokens 4 g .. 4 g + 3 of
 //           the channels 32 w + n (low byte pairs) and 32 w + 16 + n
-//   key scales, value scales            [token][group] f16 step, f16 minimum
+//   key scales, value scales            [token][group] f16 minimum, f16 step (the upper half)
 //
 // with JW = 4 words (2 at 64 channels) of the head's channels / 32, so that a
 // wave's load of 16 bytes a lane is one contiguous kilobyte and each word is
 // one lane's share of a v_mfma_f32_16x16x32_f16 operand: nibbles b and b + 4
-// are the two halves of one register.  Heads of 32 to 256 channels are stored
+// are the two halves of one register.  As they lie there, nibble 0 or 1 of a
+// half is an f16 of 2^-24 or 2^-20 times its code, a number below the normal
+// ones that the matrix cores take as it is.  Heads of 32 to 256 channels are stored
 // as 64, 128 or 256; the channels past head_dim are zeros.
 #pragma once
 
@@ -94,14 +96,17 @@ struct PagedBatch {
 struct PagedSequence {
     uint32_t row = 0, rows = 0, past = 0;
 };
-QWN_HD PagedSequence paged_sequence(const PagedBatch &b, uint32_t s) {
-    const int32_t r0 = b.starts[s], r1 = b.starts[s + 1], past = b.past[s];
+QWN_HD PagedSequence paged_rows(const PagedBatch &b, int32_t r0, int32_t r1, int32_t past) {
     PagedSequence q;
     if (r0 < 0 || r1 <= r0 || static_cast<uint32_t>(r1) > b.tokens || past < 0) return q;
     q.row = static_cast<uint32_t>(r0);
     q.rows = static_cast<uint32_t>(r1 - r0);
     q.past = static_cast<uint32_t>(past);
     return q;
+}
+
+QWN_HD PagedSequence paged_sequence(const PagedBatch &b, uint32_t s) {
+    return paged_rows(b, b.starts[s], b.starts[s + 1], b.past[s]);
 }
 
 // Page of a slot of sequence s; false where the table names none of the pool.
@@ -124,16 +129,18 @@ inline uint32_t paged_units_most(uint32_t sequences, uint32_t tokens) {
     return static_cast<uint32_t>(runs < tokens ? runs : tokens);
 }
 
-// Attention splits a list of `total` equal pieces of work among `workers`:
-// worker w takes pieces paged_share(w) .. paged_share(w + 1) - 1, and
-// paged_worker is the one that takes a piece.
+// Attention splits a list of `total` units of work among `workers`: worker w
+// takes units paged_share(w) .. paged_share(w + 1) - 1, and paged_worker is the
+// one that takes a unit.
 QWN_HD uint64_t paged_share(uint64_t total, uint32_t workers, uint32_t w) { return total * w / workers; }
-QWN_HD uint32_t paged_worker(uint64_t total, uint32_t workers, uint64_t piece) {
-    return static_cast<uint32_t>(((piece + 1) * workers - 1) / total);
+QWN_HD uint32_t paged_worker(uint64_t total, uint32_t workers, uint64_t unit) {
+    return static_cast<uint32_t>(((unit + 1) * workers - 1) / total);
 }
-// Of a block of work, pieces `first` and on, that no worker has whole, worker
-// w's partial sums: each worker keeps two, of the block that its first piece
-// belongs to and of the one that its last does.
+// A block of work is `start` units for its beginning, that no worker does
+// anything for, and one for each of its pieces, the first of them unit `first`.
+// Of a block whose pieces no worker has all of, worker w's partial sums: each
+// worker keeps two, of a block that it begins in the middle of (or at its first
+// piece) and of one that it does not come to the end of.
 QWN_HD uint32_t paged_partial(uint64_t total, uint32_t workers, uint64_t first, uint32_t w) {
     return 2 * w + (paged_share(total, workers, w) < first ? 1u : 0u);
 }

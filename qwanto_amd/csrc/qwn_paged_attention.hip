@@ -17,9 +17,21 @@
 // registers.
 //
 // fp32 queries and probabilities are split into two f16 halves (22 bits, two
-// products); f16 and bf16 ones take one.  Queries are first divided by a power
-// of two per row, probabilities by one per wave that covers the values' steps,
-// so that neither halves nor rounded values leave the range of f16.
+// products); f16 and bf16 ones take one.  With one product the codes go in
+// where they lie in a word, as f16 of 2^-24 and 2^-20 times their value
+// (qwn_paged.h): 5 instructions for 8 codes, where making them integers takes
+// 11.  The elements that meet the larger ones are divided by 16 beforehand, the
+// sums multiplied by 2^24 at the end.  (The matrix cores sum such operands to
+// 2e-7 of their magnitudes, integers to 5e-8: fp32 takes integers, less 8 to
+// halve what cancels.)  A probability that f16 rounds would count its error
+// times the code, although codes are 7.5 +- 5 and the values they make around
+// zero; the sum of the rounded weights, one more product with a row of ones,
+// takes 8 times that error out again.
+//
+// Queries are scaled by a power of two
+// per row to below 2^15, probabilities times steps by one per row and wave to
+// below 2^11 where their largest was met (2^15 a little past it): f16 then has
+// 25 binades and more below the largest, for the second halves as well.
 #include "qwn_context.h"
 #include "qwn_device.h"
 #include "qwn_hip_ext.h"
@@ -36,6 +48,7 @@ using namespace qwn;
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
@@ -45,8 +58,16 @@ constexpr int kThreads = kWaves * kWaveSize;
 constexpr uint32_t kRows = 16;                    // query rows of a block: the matrix cores' columns
 constexpr uint32_t kStep = 32;                    // tokens of a wave's step
 constexpr uint32_t kPiece = kStep * kWaves;       // tokens of a workgroup's step: the unit work is split in
-constexpr uint32_t kMostSlots = 0x7fffff80u;     // of a sequence: slot numbers stay in 32 bits
-constexpr uint32_t kWorkers = 512;                // workgroups: two of four waves on each CU
+constexpr uint32_t kWorkers = 768;                // workgroups at most: three of four waves on each CU
+constexpr uint32_t kStart = 3;                    // pieces that a block's beginning and end cost as much as
+// Contexts are not split up to so many slots, where there are few blocks or
+// many: 64 sequences of 1024 tokens, 8 KV heads, 20 us whole and 28 split and
+// merged; one of 512, 11 and 11.
+constexpr uint32_t kWholeSlots = 512, kWholeSlotsMany = 1024, kMany = 256;
+
+constexpr int kQueryBits = 15;                   // |query| < 2^15 in f16
+constexpr int kWeightBits = 11;                  // probability times step < 2^11 of the largest met,
+constexpr float kSlack = 4.0f;                   // and 2^4 more before the reference moves
 
 struct AttnArgs {
     PagedKv c;
@@ -56,86 +77,112 @@ struct AttnArgs {
     float *part_o;       // [worker][2][kRows][width]
     float2 *part_ml;     // [worker][2][kRows]: reference exponent, sum
     uint32_t query_stride, output_stride, query_heads, group;
+    uint32_t slots;      // of a sequence's row of the table
+    uint32_t workers;    // workgroups of the launch
+    bool whole;
     float scale;
 };
 
-// Work is a list of pieces of kPiece tokens: for each sequence, each block of
-// kRows query rows (a row is a token and one of the query heads of a KV head),
-// each KV head, the pieces of its context in order.  Worker w of W takes the
-// w-th share of the list, whatever the lengths of the sequences.
+// Work is a list: for each sequence, each block of kRows query rows (a row is a
+// token and one of the query heads of a KV head), each KV head, kStart units
+// for the block itself and one for each piece of kPiece tokens of its context.
+// Worker w of W takes the w-th share of the list, whatever the lengths of the
+// sequences.  (61 contexts of 1 to 8191 tokens, 32 heads, 8 KV heads: 30 us,
+// 44 with pieces alone, many short blocks meeting in some workers.)  Where no
+// context can be long (`whole`), a worker takes a block, and nothing is merged.
 struct Shape {
-    uint32_t blocks, pieces;  // of a sequence: row blocks, pieces of one block and head
+    uint32_t blocks, pieces, units;  // of a sequence: row blocks; pieces and units of one block and head
 };
-__device__ __forceinline__ Shape shape_of(const AttnArgs &a, uint32_t s) {
-    const PagedSequence q = paged_sequence(a.b, s);
+__device__ __forceinline__ Shape shape_of(const AttnArgs &a, const PagedSequence &q) {
     Shape r;
-    r.blocks = static_cast<uint32_t>((static_cast<uint64_t>(q.rows) * a.group + kRows - 1) / kRows);
+    r.blocks = (q.rows * a.group + kRows - 1) / kRows;
     // slots past the table are attended to by none
-    const uint64_t slots = min(min(static_cast<uint64_t>(q.past) + q.rows,
-                                   static_cast<uint64_t>(a.b.table_stride) << a.c.page_shift),
-                               static_cast<uint64_t>(kMostSlots));
-    r.pieces = q.rows ? static_cast<uint32_t>((slots + kPiece - 1) / kPiece) : 0u;
+    r.pieces = (min(q.past + q.rows, a.slots) + kPiece - 1) / kPiece;
+    r.units = a.whole ? 1u : kStart + r.pieces;
     return r;
 }
+__device__ __forceinline__ PagedSequence lane_sequence(const AttnArgs &a, uint32_t s) {
+    return s < a.b.sequences ? paged_sequence(a.b, s) : PagedSequence{};
+}
+__device__ __forceinline__ uint32_t units_of(const AttnArgs &a, const PagedSequence &q) {
+    const Shape h = shape_of(a, q);
+    return h.blocks * a.c.kv_heads * h.units;
+}
+// A sequence that every lane asks for.
+__device__ __forceinline__ PagedSequence sequence_of(const AttnArgs &a, uint32_t s) {
+    return paged_rows(a.b, scalar_load(a.b.starts + s), scalar_load(a.b.starts + s + 1), scalar_load(a.b.past + s));
+}
 
-// 64-bit prefix over the batch, 64 sequences a step: the sequence that holds
-// piece `index`, the pieces before it, and the whole list's length.
-struct Place {
-    uint32_t seq;
-    uint64_t before;
+// The list's length, and the first 64 sequences in the lanes: what most batches
+// are found by without a second look.
+struct List {
+    PagedSequence q;           // of lane l: sequence l,
+    uint32_t n, end;           // its units, and those of the sequences up to it
+    uint32_t total;
 };
-__device__ __forceinline__ uint64_t scan64(uint64_t v) {
+__device__ __forceinline__ List list_of(const AttnArgs &a) {
+    List l;
     const uint32_t lane = threadIdx.x % kWaveSize;
-#pragma unroll
-    for (int off = 1; off < kWaveSize; off <<= 1) {
-        const uint64_t o = __shfl_up(v, off);
-        if (lane >= static_cast<uint32_t>(off)) v += o;
-    }
-    return v;
+    l.q = lane_sequence(a, lane);
+    l.n = units_of(a, l.q);
+    l.end = wave_scan(l.n);
+    l.total = lane_of(l.end, kWaveSize - 1);
+    for (uint32_t s0 = kWaveSize; s0 < a.b.sequences; s0 += kWaveSize)
+        l.total += lane_of(wave_scan(units_of(a, lane_sequence(a, s0 + lane))), kWaveSize - 1);
+    return l;
 }
-__device__ __forceinline__ uint64_t pieces_of(const AttnArgs &a, uint32_t s) {
-    const Shape h = shape_of(a, s);
-    return static_cast<uint64_t>(h.blocks) * a.c.kv_heads * h.pieces;
-}
-__device__ __forceinline__ uint64_t total_pieces(const AttnArgs &a) {
-    uint64_t n = 0;
-    for (uint32_t s0 = 0; s0 < a.b.sequences; s0 += kWaveSize) {
-        const uint32_t s = s0 + threadIdx.x % kWaveSize;
-        if (s < a.b.sequences) n += pieces_of(a, s);
-    }
-    for (int off = kWaveSize / 2; off > 0; off >>= 1) n += __shfl_xor(n, off);
-    return n;
-}
-__device__ __forceinline__ Place find_piece(const AttnArgs &a, uint64_t index) {
-    uint64_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.b.sequences; s0 += kWaveSize) {
-        const uint32_t s = s0 + threadIdx.x % kWaveSize;
-        const uint64_t n = s < a.b.sequences ? pieces_of(a, s) : 0ull;
-        const uint64_t end = before + scan64(n);
-        const uint64_t past = __ballot(end > index);
-        if (past) {
-            const int first = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            return {s0 + first, __shfl(end, first) - __shfl(n, first)};
+// The sequence that holds unit `index` of the list, and the units before it.
+__device__ __forceinline__ PagedSequence find_place(const AttnArgs &a, const List &l, uint32_t index, uint32_t &seq,
+                                                    uint32_t &before) {
+    PagedSequence q = l.q;
+    uint32_t n = l.n, end = l.end;
+    before = 0;
+    for (uint32_t s0 = 0;; ) {
+        const uint64_t past = __ballot(before + end > index);
+        const int first = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : kWaveSize - 1;
+        if (past || s0 + kWaveSize >= a.b.sequences) {  // the second only past the list's end
+            seq = s0 + first;
+            before += lane_of(end, first) - lane_of(n, first);
+            return PagedSequence{lane_of(q.row, first), lane_of(q.rows, first), lane_of(q.past, first)};
         }
-        before = __shfl(end, kWaveSize - 1);
+        before += lane_of(end, kWaveSize - 1);
+        s0 += kWaveSize;
+        q = lane_sequence(a, s0 + threadIdx.x % kWaveSize);
+        n = units_of(a, q);
+        end = wave_scan(n);
     }
-    return {a.b.sequences, before};
 }
 
-__device__ __forceinline__ uint64_t share(uint64_t total, uint32_t w) { return paged_share(total, kWorkers, w); }
+// Workgroups that get work: all, or one for each unit.
+__device__ __forceinline__ uint32_t workers_of(const AttnArgs &a, uint32_t total) { return min(total, a.workers); }
 
-// Half b (0: nibbles 0 .. 3, 1: 4 .. 7) pairs of a code word as f16: nibbles
-// p and p + 4 in the two halves of a register.  1024 + code is the f16 with
-// the code in its last bits.
+// A code word's 8 codes as f16, for one product with halves (WHOLE false):
+// nibbles p and p + 4 as they lie, times 2^-24 (p even) or 2^-20; for two
+// products (WHOLE): the codes less 8.  1024 + code is the f16 with the code in
+// its last bits.
+template <bool WHOLE>
 __device__ __forceinline__ v2h codes2(uint32_t word, int p) {
-    const uint32_t bits = ((word >> (4 * p)) & 0x000f000fu) | 0x64006400u;
-    const v2h base = {static_cast<_Float16>(1024.0f), static_cast<_Float16>(1024.0f)};
-    return __builtin_bit_cast(v2h, bits) - base;
+    if constexpr (WHOLE) {
+        const v2h base = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
+        return __builtin_bit_cast(v2h, ((word >> (4 * p)) & 0x000f000fu) | 0x64006400u) - base;
+    }
+    return __builtin_bit_cast(v2h, (p >= 2 ? word >> 8 : word) & (p % 2 ? 0x00f000f0u : 0x000f000fu));
 }
+template <bool WHOLE>
 __device__ __forceinline__ v8h codes8(uint32_t word) {
-    const v2h a = codes2(word, 0), b = codes2(word, 1), c = codes2(word, 2), d = codes2(word, 3);
+    const v2h a = codes2<WHOLE>(word, 0), b = codes2<WHOLE>(word, 1), c = codes2<WHOLE>(word, 2), d = codes2<WHOLE>(word, 3);
     return (v8h){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// What element i of an operand that meets codes8 is multiplied by, and what
+// makes up for it together with the codes' own factor.
+template <bool WHOLE>
+__device__ constexpr float balance(int i) { return !WHOLE && (i >> 1) % 2 ? 0.0625f : 1.0f; }
+
+__device__ __forceinline__ v2h to_halves(float a, float b) {
+    return __builtin_convertvector((v2f){a, b}, v2h);
+}
+__device__ __forceinline__ float step_of(uint32_t w) { return half_to_float(w >> 16); }
+__device__ __forceinline__ float least_of(uint32_t w) { return half_to_float(w & 0xffffu); }
 
 // x as NP halves that add up to it.
 template <int NP>
@@ -146,10 +193,13 @@ template <int NP>
 __device__ __forceinline__ Halves<NP> halves(const float x[8]) {
     Halves<NP> h;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const _Float16 hi = static_cast<_Float16>(x[i]);
-        h.p[0][i] = hi;
-        if constexpr (NP == 2) h.p[1][i] = static_cast<_Float16>(x[i] - static_cast<float>(hi));
+    for (int i = 0; i < 8; i += 2) {
+        const v2h hi = to_halves(x[i], x[i + 1]);
+        h.p[0][i] = hi[0], h.p[0][i + 1] = hi[1];
+        if constexpr (NP == 2) {
+            const v2h lo = to_halves(x[i] - static_cast<float>(hi[0]), x[i + 1] - static_cast<float>(hi[1]));
+            h.p[1][i] = lo[0], h.p[1][i + 1] = lo[1];
+        }
     }
     return h;
 }
@@ -163,10 +213,9 @@ __device__ __forceinline__ float across_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// What a lane reads of a step's two tiles.
-template <int W>
-struct Tiles {
-    uint32_t k[2][W / 32], v[2][W / 32], ks[2][4 * (W / 64)], vs[2][4 * (W / 64)];
+// A step's tiles by their pages; ok: the table names them.
+struct Pages {
+    uint32_t page[2];
     bool ok[2];
 };
 template <int N>
@@ -182,31 +231,62 @@ __device__ __forceinline__ void load_words(uint32_t *dst, const uint8_t *src) {
         dst[0] = x[0], dst[1] = x[1];
     }
 }
-template <int W>
-__device__ __forceinline__ void load_tiles(const AttnArgs &a, uint32_t s, uint32_t head, uint32_t token, uint32_t lane,
-                                           Tiles<W> &t) {
+// s and token are the same in every lane.
+__device__ __forceinline__ Pages find_pages(const AttnArgs &a, uint32_t s, uint32_t token) {
+    Pages p;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t at = (token + kPagedTile * i) >> a.c.page_shift;
+        const bool in = at < a.b.table_stride;
+        const int32_t page = scalar_load(a.b.table + static_cast<size_t>(s) * a.b.table_stride + (in ? at : 0u));
+        p.ok[i] = in && page >= 0 && static_cast<uint32_t>(page) < a.c.pages;
+        p.page[i] = p.ok[i] ? static_cast<uint32_t>(page) : 0u;
+    }
+    return p;
+}
+// The keys' half of a step's tiles, or the values'.
+template <int W, bool KEYS>
+__device__ __forceinline__ void load_tiles(const AttnArgs &a, const Pages &p, uint32_t head, uint32_t token, uint32_t lane,
+                                           uint32_t (&codes)[2][W / 32], uint32_t (&scales)[2][W / 16]) {
     constexpr int JW = W >= 128 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const uint32_t slot = token + kPagedTile * i;
-        uint32_t page = 0;
-        t.ok[i] = paged_page(a.c, a.b, s, slot, page);
-        const uint8_t *block =
-            a.c.pool + paged_block_at(a.c, t.ok[i] ? page : 0u, (slot & (a.c.page_tokens - 1)) / kPagedTile, head);
+        const uint32_t tile = ((token + kPagedTile * i) & (a.c.page_tokens - 1)) / kPagedTile;
+        const uint8_t *block = a.c.pool + paged_block_at(a.c, p.page[i], tile, head);
 #pragma unroll
-        for (int j = 0; j < W / 32; j += JW) {
-            load_words<JW>(t.k[i] + j, block + 4 * paged_word(W, lane, j));
-            load_words<JW>(t.v[i] + j, block + paged_values_at(W) + 4 * paged_word(W, lane, j));
-        }
-        constexpr int G = W / 64;
-        load_words<4 * G>(t.ks[i], block + paged_key_scales_at(W) + lane / 16 * (16 * G));
-        load_words<4 * G>(t.vs[i], block + paged_value_scales_at(W) + lane / 16 * (16 * G));
+        for (int j = 0; j < W / 32; j += JW)
+            load_words<JW>(codes[i] + j, block + (KEYS ? 0u : paged_values_at(W)) + 4 * paged_word(W, lane, j));
+        load_words<W / 16>(scales[i], block + (KEYS ? paged_key_scales_at(W) : paged_value_scales_at(W)) + lane / 16 * (W / 4));
     }
 }
 
+// The 8 channels of a query row from c0, zeros past the head's.
+template <typename T>
+__device__ __forceinline__ void load_query(const T *row, uint32_t c0, uint32_t n, float x[8]) {
+    constexpr int VEC = 16 / sizeof(T);
+    if (c0 + 8 <= n) {
+#pragma unroll
+        for (int h = 0; h < 8; h += VEC) {
+            const Vec<T, VEC> v = load_vec<T, VEC>(row + c0 + h);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[h + i] = to_float(v.v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = c0 + i < n ? to_float(row[c0 + i]) : 0.0f;
+    }
+}
+
+// A worker goes through its pieces block by block; in a block its four waves
+// take every fourth step of 32 tokens, each with its own maxima and sums, and
+// meet in LDS at the end.  A step's keys are read again as soon as the scores
+// are there, its values once they are used: the other half of the step's work
+// hides each, in one set of registers.  Bound by HBM in the long run, by the
+// searches and loads that a block starts with where contexts are short.
 template <typename T, int W>
-__global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_kernel(AttnArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
+    constexpr bool WHOLE = NP == 2;
     constexpr int J = W / 32, G = W / 64, C = W / 16;
     constexpr int kPad = W + 4;
     __shared__ float merge_o[kWaves][kRows][kPad];
@@ -214,88 +294,96 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnArgs a) {
     const uint32_t lane = threadIdx.x % kWaveSize;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const uint32_t n = lane % 16, g = lane / 16;
-    const uint64_t total = total_pieces(a);
-    const uint64_t begin = share(total, blockIdx.x), end = share(total, blockIdx.x + 1);
-    if (begin >= end) return;
-    Place at = find_piece(a, begin);
-    for (uint64_t u = begin; u < end;) {
-        // the block and head of piece u, and this worker's pieces of it
-        Shape h = shape_of(a, at.seq);
-        uint64_t in_seq = static_cast<uint64_t>(h.blocks) * a.c.kv_heads * h.pieces;
-        while (u - at.before >= in_seq) {
-            at.before += in_seq;
-            ++at.seq;
-            h = shape_of(a, at.seq);
-            in_seq = static_cast<uint64_t>(h.blocks) * a.c.kv_heads * h.pieces;
+    const List list = list_of(a);
+    const uint32_t workers = workers_of(a, list.total);
+    if (blockIdx.x >= workers) return;
+    const uint32_t begin = static_cast<uint32_t>(paged_share(list.total, workers, blockIdx.x));
+    const uint32_t end = static_cast<uint32_t>(paged_share(list.total, workers, blockIdx.x + 1));
+    uint32_t s, before;
+    PagedSequence q = find_place(a, list, begin, s, before);
+    for (uint32_t u = begin; u < end;) {
+        // the block and head of unit u, and this worker's pieces of it
+        Shape h = shape_of(a, q);
+        while (u - before >= h.blocks * a.c.kv_heads * h.units) {
+            before += h.blocks * a.c.kv_heads * h.units;
+            q = sequence_of(a, ++s);
+            h = shape_of(a, q);
         }
-        const uint32_t s = at.seq;
-        const PagedSequence q = paged_sequence(a.b, s);
-        const uint64_t in = u - at.before;
-        const uint32_t item = static_cast<uint32_t>(in / h.pieces), piece0 = static_cast<uint32_t>(in % h.pieces);
+        const uint32_t item = (u - before) / h.units, at = (u - before) % h.units;
+        const uint32_t first = u - at + (a.whole ? 0u : kStart);  // the unit of its first piece
+        if (u < first) u = min(first, end);
+        if (u == end) break;
         const uint32_t block = item / a.c.kv_heads, head = item % a.c.kv_heads;
-        const uint32_t count = static_cast<uint32_t>(min(static_cast<uint64_t>(h.pieces - piece0), end - u));
-        const bool whole = piece0 == 0 && count == h.pieces;
+        const uint32_t piece0 = u - first;
+        const uint32_t count = a.whole ? h.pieces : min(h.pieces - piece0, end - u);
+        const uint32_t rows = min(kRows, q.rows * a.group - block * kRows);
+        const uint32_t most = min(q.past + (block * kRows + rows - 1) / a.group + 1, a.slots);  // slots any row sees
+        const uint32_t least_seen = q.past + block * kRows / a.group + 1;                        // slots every row sees
+        const uint32_t t_end = min(most, (piece0 + count) * kPiece);
+        uint32_t t0 = piece0 * kPiece + wave * kStep;
+        uint32_t k[2][J], v[2][J], ks[2][4 * G], vs[2][4 * G];
+        Pages pk = find_pages(a, s, t0), pv = pk;
+        load_tiles<W, true>(a, pk, head, t0, lane, k, ks);
+        load_tiles<W, false>(a, pv, head, t0, lane, v, vs);
+        // where nothing follows a step's loads are issued again: how many are in
+        // flight does not depend on a branch, and no wait is for more than it needs
+        uint32_t next = t0 + kPiece < t_end ? t0 + kPiece : t0;
+        Pages pn = find_pages(a, s, next);
 
         // this lane's query row (column n): token and head, its visible slots
-        const uint64_t r = static_cast<uint64_t>(block) * kRows + n;
-        const bool real = r < static_cast<uint64_t>(q.rows) * a.group;
-        const uint32_t tok = real ? static_cast<uint32_t>(r / a.group) : 0u;
-        const uint32_t qh = head * a.group + static_cast<uint32_t>(r % a.group);
+        const bool real = n < rows;
+        const uint32_t r = block * kRows + (real ? n : 0u), tok = r / a.group;
         const uint32_t visible = real ? q.past + tok + 1 : 0u;
-        const uint64_t last_row = min(static_cast<uint64_t>(block) * kRows + kRows, static_cast<uint64_t>(q.rows) * a.group) - 1;
-        const uint32_t most = q.past + static_cast<uint32_t>(last_row / a.group) + 1;  // slots any row of the block sees
         const T *qp = static_cast<const T *>(a.query) + static_cast<size_t>(q.row + tok) * a.query_stride +
-                      static_cast<size_t>(qh) * a.c.head_dim;
-
+                      static_cast<size_t>(head * a.group + r % a.group) * a.c.head_dim;
         Halves<NP> qf[J];
         float qsum[G], row_mul;
         {
             float x[J][8], top = 0.0f;
 #pragma unroll
+            for (int j = 0; j < J; ++j) load_query(qp, 32 * j + 8 * g, a.c.head_dim, x[j]);
+#pragma unroll
             for (int j = 0; j < J; ++j)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t ch = 32 * j + 8 * g + i;
-                    x[j][i] = real && ch < a.c.head_dim ? to_float(qp[ch]) : 0.0f;
+                    if (!real) x[j][i] = 0.0f;
                     top = fmaxf(top, fabsf(x[j][i]));
                 }
             top = across_max(top);
             int e = 0;  // top < 2^e
             if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
-            e = max(e, -126);
-            const float down = ldexpf(1.0f, -e);
-            row_mul = a.scale * 1.44269504088896340736f * ldexpf(1.0f, e);
+            e = max(e, -100);
+            const float up = ldexpf(1.0f, kQueryBits - e);
+            row_mul = a.scale * 1.44269504088896340736f * ldexpf(1.0f, e - kQueryBits + (WHOLE ? 0 : 24));
 #pragma unroll
             for (int gg = 0; gg < G; ++gg) qsum[gg] = 0.0f;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    x[j][i] *= down;
+                    x[j][i] *= up;
+                    qsum[j / 2] += x[j][i];
+                    x[j][i] *= balance<WHOLE>(i);
                 }
                 qf[j] = halves<NP>(x[j]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) qsum[j / 2] += x[j][i];
             }
 #pragma unroll
-            for (int gg = 0; gg < G; ++gg) qsum[gg] = across_sum(qsum[gg]);
+            for (int gg = 0; gg < G; ++gg) {
+                qsum[gg] = across_sum(qsum[gg]) * (WHOLE ? 1.0f : 0x1p-24f);
+                if (top == INFINITY) qsum[gg] = __builtin_nanf("");  // not finite: NaN, whatever the codes are
+            }
         }
 
-        v4f acc[C];
+        v4f acc[C], weights[G];
         float low[G], sum = 0.0f, m = -INFINITY, ref = 0.0f;
-        int vexp = -24;  // below every step that is not zero
+        uint32_t steps = 0;  // no step of a value met so far is larger: f16 bits above, 0xffff below
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int gg = 0; gg < G; ++gg) low[gg] = 0.0f;
+        for (int gg = 0; gg < G; ++gg) low[gg] = 0.0f, weights[gg] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 
-        const uint32_t t_end = min(most, (piece0 + count) * kPiece);
-        for (uint32_t t0 = piece0 * kPiece + wave * kStep; t0 < t_end; t0 += kPiece) {
-            Tiles<W> t;
-            load_tiles<W>(a, s, head, t0, lane, t);
-            // scores of the lane's 8 tokens
-            float sc[8], step_top = 0.0f;
-            bool see[8];
+        for (; t0 < t_end; t0 += kPiece) {
+            float sc[8];
 #pragma unroll
             for (int i2 = 0; i2 < 2; ++i2) {
                 v4f d[G];
@@ -303,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnArgs a) {
                 for (int gg = 0; gg < G; ++gg) d[gg] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    const v8h kc = codes8(t.k[i2][j]);
+                    const v8h kc = codes8<WHOLE>(k[i2][j]);
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
                         d[j / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qf[j].p[p], d[j / 2], 0, 0, 0);
@@ -313,41 +401,57 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnArgs a) {
                     float x = 0.0f;
 #pragma unroll
                     for (int gg = 0; gg < G; ++gg) {
-                        const uint32_t w = t.ks[i2][i * G + gg];
-                        x = fmaf(half_to_float(w & 0xffffu), d[gg][i], x);
-                        x = fmaf(half_to_float(w >> 16), qsum[gg], x);
+                        const uint32_t w = ks[i2][i * G + gg];
+                        x = fmaf(step_of(w), d[gg][i], x);
+                        x = fmaf(WHOLE ? fmaf(8.0f, step_of(w), least_of(w)) : least_of(w), qsum[gg], x);
                     }
-                    const uint32_t slot = t0 + kPagedTile * i2 + 4 * g + i;
-                    see[4 * i2 + i] = t.ok[i2] && slot < visible;
-                    sc[4 * i2 + i] = see[4 * i2 + i] ? x * row_mul : -INFINITY;
-                    // tokens that no row sees may hold anything
-                    const bool live = t.ok[i2] && slot < most;
-#pragma unroll
-                    for (int gg = 0; gg < G; ++gg) {
-                        if (!live) t.vs[i2][i * G + gg] = 0;
-                        step_top = fmaxf(step_top, half_to_float(t.vs[i2][i * G + gg] & 0xffffu));
-                    }
+                    sc[4 * i2 + i] = x * row_mul;
                 }
             }
-            float mx = m;
+            const Pages pg = pv;
+            const uint32_t now = next;
+            pk = pn;
+            load_tiles<W, true>(a, pk, head, now, lane, k, ks);
+            next = t0 + 2 * kPiece < t_end ? t0 + 2 * kPiece : now;
+            pn = find_pages(a, s, next);
+            uint32_t top = 0;
+            if (t0 + kStep > least_seen || !pg.ok[0] || !pg.ok[1]) {  // not all tokens for all rows
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sc[i]);
-            mx = across_max(mx);
-            step_top = across_max(step_top);
-            const int e = static_cast<int>(__builtin_bit_cast(uint32_t, step_top) >> 23) - 126;  // steps < 2^e
-            const int ve = max(vexp, e);
-            const float next = mx == -INFINITY ? 0.0f : mx + static_cast<float>(ve);
-            if (__any(mx > m || ve > vexp)) {
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t slot = t0 + kPagedTile * (i / 4) + 4 * g + i % 4;
+                    if (!pg.ok[i / 4] || slot >= visible) sc[i] = -INFINITY;
+                    // tokens that no row sees may hold any (finite) numbers
+#pragma unroll
+                    for (int gg = 0; gg < G; ++gg)
+                        if (pg.ok[i / 4] && slot < most) top = max(top, vs[i / 4][(i % 4) * G + gg]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8 * G; ++i) top = max(top, vs[i / (4 * G)][i % (4 * G)]);
+            }
+            float mx = sc[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i]);
+            // a new reference only where a score is well past the last one's or a
+            // step larger: rare once a few steps are done
+            if (__any(mx > m + kSlack || top > steps)) {
+                mx = across_max(fmaxf(mx, m));
+                top = max(top, steps);
+                top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+                top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+                steps = top | 0xffffu;
+                // steps < 2^e; 2^-24 is the smallest that is not zero
+                const int e = max(-24, static_cast<int>(__builtin_bit_cast(uint32_t, step_of(top)) >> 23) - 126);
+                const float moved = mx == -INFINITY ? 0.0f : mx + static_cast<float>(e - kWeightBits);
                 // nothing seen yet: sums of zeros, whatever the reference was
-                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - next);
+                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - moved);
 #pragma unroll
                 for (int c = 0; c < C; ++c) acc[c] *= alpha;
 #pragma unroll
-                for (int gg = 0; gg < G; ++gg) low[gg] *= alpha;
+                for (int gg = 0; gg < G; ++gg) low[gg] *= alpha, weights[gg] *= alpha;
                 sum *= alpha;
                 m = mx;
-                vexp = ve;
-                ref = next;
+                ref = moved;
             }
             float p[8];
 #pragma unroll
@@ -361,22 +465,29 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnArgs a) {
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t w = t.vs[i / 4][(i % 4) * G + gg];
-                    x[i] = p[i] * half_to_float(w & 0xffffu);
-                    low[gg] = fmaf(p[i], half_to_float(w >> 16), low[gg]);
+                    const uint32_t w = vs[i / 4][(i % 4) * G + gg];
+                    low[gg] = fmaf(p[i], fmaf(8.0f, step_of(w), least_of(w)), low[gg]);
+                    x[i] = fmaf(p[i] * balance<WHOLE>(i), step_of(w), 0.0f);
                 }
                 pf[gg] = halves<NP>(x);
+                if constexpr (!WHOLE) {
+                    const _Float16 one = static_cast<_Float16>(1.0f), more = static_cast<_Float16>(16.0f);
+                    weights[gg] = __builtin_amdgcn_mfma_f32_16x16x32_f16((v8h){one, one, more, more, one, one, more, more},
+                                                                        pf[gg].p[0], weights[gg], 0, 0, 0);
+                }
             }
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int w = c / 2, b = (c % 2) * 2;
-                const v2h x0 = codes2(t.v[0][w], b), x1 = codes2(t.v[0][w], b + 1);
-                const v2h x2 = codes2(t.v[1][w], b), x3 = codes2(t.v[1][w], b + 1);
+                const v2h x0 = codes2<WHOLE>(v[0][w], b), x1 = codes2<WHOLE>(v[0][w], b + 1);
+                const v2h x2 = codes2<WHOLE>(v[1][w], b), x3 = codes2<WHOLE>(v[1][w], b + 1);
                 const v8h vc = {x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 #pragma unroll
-                for (int k = 0; k < NP; ++k)
-                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pf[c / 4].p[k], acc[c], 0, 0, 0);
+                for (int kk = 0; kk < NP; ++kk)
+                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pf[c / 4].p[kk], acc[c], 0, 0, 0);
             }
+            pv = pk;
+            load_tiles<W, false>(a, pv, head, now, lane, v, vs);
         }
 
         // the four waves' results of the block: lane (g, n) has channels
@@ -385,15 +496,18 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnArgs a) {
 #pragma unroll
         for (int gg = 0; gg < G; ++gg) low[gg] = across_sum(low[gg]);
         __syncthreads();  // the previous block's results are read
+        if (real) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const v4f o = acc[c] + low[c / 4];
-            *reinterpret_cast<v4f *>(&merge_o[wave][n][16 * c + 4 * g]) = o;
+            for (int c = 0; c < C; ++c) {
+                const v4f o = WHOLE ? acc[c] + low[c / 4] : acc[c] * 0x1p24f - 8.0f * weights[c / 4] + low[c / 4];
+                *reinterpret_cast<v4f *>(&merge_o[wave][n][16 * c + 4 * g]) = o;
+            }
+            if (g == 0) merge_ml[wave][n] = make_float2(m == -INFINITY ? -INFINITY : ref, sum);
         }
-        if (g == 0) merge_ml[wave][n] = make_float2(m == -INFINITY ? -INFINITY : ref, sum);
         __syncthreads();
-        const uint32_t part = paged_partial(total, kWorkers, u - piece0, blockIdx.x);
-        for (uint32_t i = threadIdx.x; i < kRows * W; i += kThreads) {
+        const bool whole = count == h.pieces;
+        const uint32_t part = paged_partial(list.total, workers, first, blockIdx.x);
+        for (uint32_t i = threadIdx.x; i < rows * W; i += kThreads) {
             const uint32_t row = i / W, ch = i % W;
             float top = -INFINITY;
 #pragma unroll
@@ -406,67 +520,103 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnArgs a) {
                 o = fmaf(merge_o[w][row][ch], f, o);
                 l = fmaf(merge_ml[w][row].y, f, l);
             }
-            const uint64_t rr = static_cast<uint64_t>(block) * kRows + row;
-            if (rr >= static_cast<uint64_t>(q.rows) * a.group) continue;
             if (whole) {
-                if (ch < a.c.head_dim) {
-                    T *dst = static_cast<T *>(a.output) + (static_cast<size_t>(q.row) + rr / a.group) * a.output_stride +
-                             static_cast<size_t>(head * a.group + rr % a.group) * a.c.head_dim;
-                    dst[ch] = from_float<T>(l == 0.0f ? 0.0f : o / l);
-                }
+                const uint32_t rr = block * kRows + row;
+                T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + rr / a.group) * a.output_stride +
+                         static_cast<size_t>(head * a.group + rr % a.group) * a.c.head_dim;
+                if (ch < a.c.head_dim) dst[ch] = from_float<T>(l == 0.0f ? 0.0f : o / l);
             } else {
                 const size_t at_part = static_cast<size_t>(part) * kRows + row;
                 a.part_o[at_part * W + ch] = o;
                 if (ch == 0) a.part_ml[at_part] = make_float2(top, l);
             }
         }
-        u += count;
+        u += a.whole ? 1u : count;
     }
 }
 
 // Blocks that several workers shared: their partial sums joined.  grid (row
-// blocks of the batch at most, KV heads).
+// blocks of the batch at most, KV heads, kMergeParts): part z takes rows z, z +
+// kMergeParts, ... of a block.  W / 4 threads hold 4 channels each of a row;
+// where a part has fewer rows than the workgroup has such groups, several
+// groups share a row's partials and meet in LDS.
+constexpr uint32_t kMergeParts = 4;
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
+    constexpr uint32_t kLanes = W / 4, kGroups = kThreads / kLanes;
+    __shared__ v4f part_o[kGroups][kLanes];
+    __shared__ float2 part_ml[kGroups];
+    const List list = list_of(a);
     uint32_t s, block;
-    if (!find_in(a.b, blockIdx.x, [&](uint32_t i) { return shape_of(a, i).blocks; }, s, block)) return;
+    if (!find_in(a.b, blockIdx.x, [&](uint32_t i) {
+            return shape_of(a, i < kWaveSize ? list.q : paged_sequence(a.b, i)).blocks;
+        }, s, block))
+        return;
     const uint32_t head = blockIdx.y;
-    const uint64_t total = total_pieces(a);
-    uint64_t before = 0;
-    for (uint32_t s0 = 0; s0 < s; s0 += kWaveSize) {
-        const uint32_t i = s0 + threadIdx.x % kWaveSize;
-        uint64_t v = i < s ? pieces_of(a, i) : 0ull;
-        for (int off = kWaveSize / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
-        before += v;
+    const uint32_t total = list.total, workers = workers_of(a, total);
+    uint32_t before = 0;
+    PagedSequence q;
+    if (s < kWaveSize) {
+        before = lane_of(list.end, s) - lane_of(list.n, s);
+        q = PagedSequence{lane_of(list.q.row, s), lane_of(list.q.rows, s), lane_of(list.q.past, s)};
+    } else {
+        for (uint32_t s0 = 0; s0 < s; s0 += kWaveSize) {
+            const uint32_t i = s0 + threadIdx.x % kWaveSize;
+            before += lane_of(wave_scan(i < s ? units_of(a, paged_sequence(a.b, i)) : 0u), kWaveSize - 1);
+        }
+        q = sequence_of(a, s);
     }
-    const Shape h = shape_of(a, s);
-    const PagedSequence q = paged_sequence(a.b, s);
-    const uint64_t first = before + (static_cast<uint64_t>(block) * a.c.kv_heads + head) * h.pieces;
-    const uint32_t w0 = paged_worker(total, kWorkers, first), w1 = paged_worker(total, kWorkers, first + h.pieces - 1);
+    const Shape h = shape_of(a, q);
+    const uint32_t first = before + (block * a.c.kv_heads + head) * h.units + kStart;
+    const uint32_t w0 = paged_worker(total, workers, first), w1 = paged_worker(total, workers, first + h.pieces - 1);
     if (w0 == w1) return;  // one worker had it all, and wrote it
-    const uint64_t rows = min(static_cast<uint64_t>(kRows), static_cast<uint64_t>(q.rows) * a.group - static_cast<uint64_t>(block) * kRows);
-    for (uint32_t i = threadIdx.x; i < rows * W; i += kThreads) {
-        const uint32_t row = i / W, ch = i % W;
-        float top = -INFINITY;
-        for (uint32_t w = w0; w <= w1; ++w)
-            if (share(total, w) < share(total, w + 1))
-                top = fmaxf(top, a.part_ml[static_cast<size_t>(paged_partial(total, kWorkers, first, w)) * kRows + row].x);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float o = 0.0f, l = 0.0f;
-        for (uint32_t w = w0; w <= w1; ++w) {
-            if (share(total, w) >= share(total, w + 1)) continue;
-            const size_t at = static_cast<size_t>(paged_partial(total, kWorkers, first, w)) * kRows + row;
-            const float2 ml = a.part_ml[at];
-            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-            o = fmaf(a.part_o[at * W + ch], f, o);
-            l = fmaf(ml.y, f, l);
+    const uint32_t p0 = paged_partial(total, workers, first, w0), n = w1 - w0 + 1;
+    const uint32_t all = min(kRows, q.rows * a.group - block * kRows);
+    if (blockIdx.z >= all) return;
+    const uint32_t rows = (all - blockIdx.z + kMergeParts - 1) / kMergeParts;
+    uint32_t share = 1;  // groups of a row
+    while (2 * share * rows <= kGroups) share *= 2;
+    const uint32_t group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, mine = group % share;
+    for (uint32_t r0 = 0; r0 < rows; r0 += kGroups / share) {
+        const uint32_t r = r0 + group / share, row = blockIdx.z + r * kMergeParts;
+        v4f o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        float top = -INFINITY, l = 0.0f;
+        if (r < rows) {
+#pragma unroll 4
+            for (uint32_t i = mine; i < n; i += share) {
+                // the first worker's partial may be its second, the others' are their first
+                const size_t at = static_cast<size_t>(i ? 2 * (w0 + i) : p0) * kRows + row;
+                const float2 ml = a.part_ml[at];
+                const v4f x = *reinterpret_cast<const v4f *>(a.part_o + at * W + 4 * lane);
+                const float next = fmaxf(top, ml.x), base = next == -INFINITY ? 0.0f : next;
+                const float f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(ml.x - base);
+                o = o * f0 + x * f1;
+                l = l * f0 + ml.y * f1;
+                top = next;
+            }
         }
-        if (ch < a.c.head_dim) {
-            const uint64_t rr = static_cast<uint64_t>(block) * kRows + row;
-            T *dst = static_cast<T *>(a.output) + (static_cast<size_t>(q.row) + rr / a.group) * a.output_stride +
-                     static_cast<size_t>(head * a.group + rr % a.group) * a.c.head_dim;
-            dst[ch] = from_float<T>(l == 0.0f ? 0.0f : o / l);
+        if (share > 1) {  // then this loop is run once
+            part_o[group][lane] = o;
+            if (lane == 0) part_ml[group] = make_float2(top, l);
+            __syncthreads();
+            if (mine != 0) continue;
+            for (uint32_t i = 1; i < share; ++i) top = fmaxf(top, part_ml[group + i].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+            o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+            l = 0.0f;
+            for (uint32_t i = 0; i < share; ++i) {
+                const float f = __builtin_amdgcn_exp2f(part_ml[group + i].x - base);
+                o += part_o[group + i][lane] * f;
+                l += part_ml[group + i].y * f;
+            }
         }
+        if (r >= rows) continue;
+        const uint32_t rr = block * kRows + row;
+        T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + rr / a.group) * a.output_stride +
+                 static_cast<size_t>(head * a.group + rr % a.group) * a.c.head_dim;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * lane + i < a.c.head_dim) dst[4 * lane + i] = from_float<T>(l == 0.0f ? 0.0f : o[i] / l);
     }
 }
 
@@ -475,22 +625,20 @@ size_t partial_bytes(uint32_t width) {
 }
 
 template <typename T, int W>
-hipError_t launch_width(const AttnArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_attention_kernel<T, W>), dim3(kWorkers), dim3(kThreads), 0, stream, a);
+hipError_t launch_width(AttnArgs a, uint32_t blocks, hipStream_t stream) {
+    a.whole = a.slots <= (blocks * a.c.kv_heads >= kMany ? kWholeSlotsMany : kWholeSlots);
+    a.workers = a.whole ? blocks * a.c.kv_heads : W == 256 ? kWorkers / 3 : kWorkers;  // of 256 channels: one on each CU
+    hipLaunchKernelGGL((paged_attention_kernel<T, W>), dim3(a.workers), dim3(kThreads), 0, stream, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    // a sequence's rows fill blocks but for its last one
-    const uint64_t rows = static_cast<uint64_t>(a.b.tokens) * a.group;
-    const uint64_t blocks = std::min<uint64_t>(rows, rows / kRows + std::min(a.b.sequences, a.b.tokens));
-    if (blocks > 0x7fffffffu) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((paged_merge_kernel<T, W>), dim3(static_cast<uint32_t>(blocks), a.c.kv_heads), dim3(kThreads), 0, stream, a);
+    if (e != hipSuccess || a.whole) return e;
+    hipLaunchKernelGGL((paged_merge_kernel<T, W>), dim3(blocks, a.c.kv_heads, kMergeParts), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 template <typename T>
-hipError_t launch_paged_attention(const AttnArgs &a, hipStream_t stream) {
-    return a.c.width == 64    ? launch_width<T, 64>(a, stream)
-           : a.c.width == 128 ? launch_width<T, 128>(a, stream)
-                              : launch_width<T, 256>(a, stream);
+hipError_t launch_paged_attention(const AttnArgs &a, uint32_t blocks, hipStream_t stream) {
+    return a.c.width == 64    ? launch_width<T, 64>(a, blocks, stream)
+           : a.c.width == 128 ? launch_width<T, 128>(a, blocks, stream)
+                              : launch_width<T, 256>(a, blocks, stream);
 }
 
 // The request as the kernels take it (lock held): what a workspace is sized
@@ -541,6 +689,17 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_attention_device(QwnCudaContextHandle 
         set_error("paged attention workspace must be 16-byte aligned");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
+    // row blocks and pieces of the batch at most: counted in 32 bits
+    const uint64_t rows = static_cast<uint64_t>(a.b.tokens) * a.group;
+    const uint64_t blocks = std::min<uint64_t>(rows, rows / kRows + std::min(a.b.sequences, a.b.tokens));
+    const uint64_t slots = std::min<uint64_t>(static_cast<uint64_t>(a.b.table_stride) << a.c.page_shift, 0x7fffff80u);
+    if (rows > 0x7fffffffu || blocks * a.c.kv_heads > 0x7fffffffu ||
+        blocks * a.c.kv_heads > 0x7fffffffull / (kStart + (slots + kPiece - 1) / kPiece)) {
+        set_error("paged attention: %u tokens of %u heads over %llu slots are too many for one call", a.b.tokens,
+                  r->query_heads, static_cast<unsigned long long>(slots));
+        return QWN_CUDA_STATUS_UNSUPPORTED;
+    }
+    a.slots = static_cast<uint32_t>(slots);
     DeviceScope device(ctx->device);
     if (device.error() != hipSuccess) return hip_fail("paged attention device", device.error());
     a.query = r->query;
@@ -549,9 +708,9 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_attention_device(QwnCudaContextHandle 
     a.part_ml = static_cast<float2 *>(r->workspace);
     a.part_o = reinterpret_cast<float *>(a.part_ml + static_cast<size_t>(kWorkers) * 2 * kRows);
     hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
-    const hipError_t e = r->dtype == QWN_HIP_DTYPE_F32   ? launch_paged_attention<float>(a, s)
-                         : r->dtype == QWN_HIP_DTYPE_F16 ? launch_paged_attention<f16>(a, s)
-                                                         : launch_paged_attention<bf16>(a, s);
+    const hipError_t e = r->dtype == QWN_HIP_DTYPE_F32   ? launch_paged_attention<float>(a, static_cast<uint32_t>(blocks), s)
+                         : r->dtype == QWN_HIP_DTYPE_F16 ? launch_paged_attention<f16>(a, static_cast<uint32_t>(blocks), s)
+                                                         : launch_paged_attention<bf16>(a, static_cast<uint32_t>(blocks), s);
     if (e != hipSuccess) return hip_fail("paged attention launch", e);
     ctx->telemetry.kv_cache_kernel_count++;
     return QWN_CUDA_STATUS_OK;

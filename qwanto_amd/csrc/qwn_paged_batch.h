@@ -15,14 +15,28 @@ ResidentPaged *paged_of(Context *ctx, const QwnHipPagedKvHandle &h);
 // A caller's batch as kernels take it; false where it is not one.
 bool batch_of(const QwnHipPagedBatch *b, PagedBatch &out);
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {  // inclusive
-    const uint32_t lane = threadIdx.x % kWaveSize;
-#pragma unroll
-    for (int off = 1; off < kWaveSize; off <<= 1) {
-        const uint32_t o = __shfl_up(v, off);
-        if (lane >= static_cast<uint32_t>(off)) v += o;
-    }
-    return v;
+// A read of what no kernel of the call writes, at an address that every lane
+// shares: through the scalar cache, apart from the vector loads in flight.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T *p) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) T *>(reinterpret_cast<uintptr_t>(p));
+}
+
+// Inclusive sum over the wave's lanes (row shifts, then the rows' totals).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+    return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = scan_step<0x111, 0xf>(v);   // row_shr:1
+    v = scan_step<0x112, 0xf>(v);
+    v = scan_step<0x114, 0xf>(v);
+    v = scan_step<0x118, 0xf>(v);
+    v = scan_step<0x142, 0xa>(v);   // row_bcast:15 into rows 1, 3
+    return scan_step<0x143, 0xc>(v);  // row_bcast:31 into rows 2, 3
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
 
 // The sequence whose units (weight(s) of them) hold number `index`, counted
@@ -39,12 +53,10 @@ __device__ __forceinline__ bool find_in(const PagedBatch &b, uint32_t index, W w
         if (past) {
             const int first = __ffsll(static_cast<unsigned long long>(past)) - 1;
             seq = s0 + first;
-            at = index - (__shfl(end, first) - __shfl(n, first));
-            seq = __builtin_amdgcn_readfirstlane(seq);
-            at = __builtin_amdgcn_readfirstlane(at);
+            at = index - (lane_of(end, first) - lane_of(n, first));
             return true;
         }
-        index -= __shfl(end, kWaveSize - 1);
+        index -= lane_of(end, kWaveSize - 1);
     }
     return false;
 }

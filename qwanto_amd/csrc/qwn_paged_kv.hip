@@ -109,8 +109,8 @@ __device__ __forceinline__ uint32_t quantize8(const float *x, uint32_t c0, uint3
 }
 
 __device__ __forceinline__ uint32_t scale_word(f16 step, f16 least) {
-    return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, step)) |
-           static_cast<uint32_t>(__builtin_bit_cast(uint16_t, least)) << 16;
+    return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, least)) |
+           static_cast<uint32_t>(__builtin_bit_cast(uint16_t, step)) << 16;
 }
 
 // Nibbles 0 .. 7 into the order of a key word (qwn_paged.h): even nibbles to
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_read_kernel(ReadArgs a) 
             if (k < from || k >= to || ch >= D) return;
             const uint32_t sc = scales[(first + k) * groups + ch / kPagedGroup];
             out[static_cast<size_t>(q.row + slot0 + k - q.past) * a.stride + head * D + ch] =
-                fmaf(half_to_float(sc & 0xffffu), static_cast<float>(code), half_to_float(sc >> 16));
+                fmaf(half_to_float(sc >> 16), static_cast<float>(code), half_to_float(sc & 0xffffu));
         };
         if (is_key) {
             const uint32_t k = w / (words / 4), c0 = w % (words / 4) * 8;

@@ -122,19 +122,22 @@ static int units() {
 // reads those of each block's workers: the same ones, each written once.
 static int split() {
     std::srand(2);
-    for (int round = 0; round < 4000; ++round) {
-        const uint32_t workers = 1 + std::rand() % 40;
+    for (int round = 0; round < 6000; ++round) {
+        const uint32_t start = std::rand() % 4;
         std::vector<uint64_t> first, pieces;
         uint64_t total = 0;
         for (int i = 1 + std::rand() % 12; i > 0; --i) {
-            first.push_back(total);
+            first.push_back(total + start);   // the first piece's unit
             pieces.push_back(1 + std::rand() % (std::rand() % 2 ? 3 : 90));
-            total += pieces.back();
+            total += start + pieces.back();
         }
+        uint32_t workers = 1 + std::rand() % 40;
+        if (workers > total) workers = static_cast<uint32_t>(total);
         std::map<uint32_t, std::pair<size_t, uint32_t>> written;  // partial -> (block, worker)
         std::vector<int> whole(first.size(), 0);
         for (uint32_t w = 0; w < workers; ++w) {
             const uint64_t b = paged_share(total, workers, w), e = paged_share(total, workers, w + 1);
+            CHECK(b < e);
             for (uint64_t u = b; u < e; ++u) CHECK(paged_worker(total, workers, u) == w);
             for (size_t i = 0; i < first.size(); ++i) {
                 const uint64_t from = first[i] > b ? first[i] : b;
@@ -157,8 +160,9 @@ static int split() {
             }
             CHECK(whole[i] == 0);
             for (uint32_t w = w0; w <= w1; ++w) {
-                if (paged_share(total, workers, w) >= paged_share(total, workers, w + 1)) continue;
-                const auto it = written.find(paged_partial(total, workers, first[i], w));
+                const uint32_t part = paged_partial(total, workers, first[i], w);
+                CHECK(w == w0 || part == 2 * w);   // what the merge takes for granted
+                const auto it = written.find(part);
                 CHECK(it != written.end() && it->second.first == i && it->second.second == w);
                 written.erase(it);
             }

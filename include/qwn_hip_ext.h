@@ -422,7 +422,7 @@ typedef struct {
     uint32_t dtype;                /* of logits and out */
     uint32_t in_stride;
     uint32_t out_stride;
-    uint32_t history_capacity;     /* entries of history */
+    uint32_t history_capacity;     /* entries of history, under 2^29 */
     uint32_t bias_capacity;        /* entries of bias_tokens and bias_values */
     uint32_t mask_rows;
     uint32_t mask_stride;          /* words of a mask row */

@@ -118,6 +118,41 @@ __device__ __forceinline__ float wave_max_all(float v) {
 }
 
 
+// The same of a 64-bit sum and of an unsigned maximum, to every lane.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_add_f64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROW_MASK, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROW_MASK, 0xf, true);
+    return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v = dpp_add_f64<0x111, 0xf>(v);
+    v = dpp_add_f64<0x112, 0xf>(v);
+    v = dpp_add_f64<0x114, 0xf>(v);
+    v = dpp_add_f64<0x118, 0xf>(v);
+    v = dpp_add_f64<0x142, 0xa>(v);
+    v = dpp_add_f64<0x143, 0xc>(v);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), 63);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), 63);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {  // 0 where no lane is moved from
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xf, true)));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = dpp_max_u32<0x111, 0xf>(v);
+    v = dpp_max_u32<0x112, 0xf>(v);
+    v = dpp_max_u32<0x114, 0xf>(v);
+    v = dpp_max_u32<0x118, 0xf>(v);
+    v = dpp_max_u32<0x142, 0xa>(v);
+    v = dpp_max_u32<0x143, 0xc>(v);
+    return __builtin_amdgcn_readlane(static_cast<int>(v), 63);
+}
+
+
 // ---- activation images --------------------------------------------------------
 
 // The value of lane ^ 1 / lane ^ 2 within each quad, by DPP quad

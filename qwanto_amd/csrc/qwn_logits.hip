@@ -12,8 +12,11 @@ namespace {
 using namespace qwn;
 
 constexpr int kThreads = 256;
-constexpr uint32_t kSlice = 4096;          // tokens of the vocabulary a workgroup takes
-constexpr uint32_t kSeen = 0x80000000u;    // in the history; the bits below count the generated ones
+constexpr uint32_t kSlice = 2048;          // tokens of the vocabulary a workgroup takes
+// of a token: in the history, with a bias, with several; the bits below count
+// the generated ones
+constexpr uint32_t kSeen = 1u << 31, kBias = 1u << 30, kBiases = 1u << 29;
+constexpr uint32_t kMostHistory = kBiases - 1;
 constexpr uint32_t kNone = 0xffffffffu;
 
 struct LogitsArgs {
@@ -49,96 +52,142 @@ __device__ __forceinline__ void range_of(const int32_t *starts, uint32_t r, uint
     to = ok ? static_cast<uint32_t>(b) : 0u;
 }
 
-// grid (slices of the vocabulary, rows).  A workgroup counts the row's
-// history and finds its biases among its own tokens in LDS (integer adds and
-// minima: their order does not matter), then passes over its slice of the
-// logits once.  The row's lists are read by every slice, from L2.  Touched
+// Entries [from, to) of a list, four to a load, f(index, entry) for each: every
+// thread's loads are issued together, four at a time.
+template <typename F>
+__device__ __forceinline__ void scan_list(const int32_t *list, uint32_t from, uint32_t to, F f) {
+    for (uint32_t i0 = from; i0 < to; i0 += 16 * kThreads) {
+        Vec<int32_t, 4> t[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t i = i0 + 4 * (threadIdx.x + kThreads * k);
+            if (i + 4 <= to) {
+                t[k] = load_vec<int32_t, 4>(list + i);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) t[k].v[e] = i + e < to ? list[i + e] : -1;
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) f(i0 + 4 * (threadIdx.x + kThreads * k) + e, static_cast<uint32_t>(t[k].v[e]));
+    }
+}
+
+// grid (slices of the vocabulary, rows).  A workgroup's slice of the logits is
+// loaded into registers; while it comes, the row's history is counted and its
+// biases are found among the slice's tokens in LDS (integer adds and ors: their
+// order does not matter).  Every slice reads the row's lists, from L2.  Touched
 // logits are computed in 64 bits and rounded once.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
     constexpr int VEC = 16 / sizeof(T);
+    constexpr int N = kSlice / (kThreads * VEC);  // vectors of a thread
     __shared__ __attribute__((aligned(16))) uint32_t counts[kSlice];
-    __shared__ __attribute__((aligned(16))) uint32_t owner[kSlice];  // the first of the token's biases in the list
-    __shared__ uint32_t again[kSlice / 32];                            // tokens with more than one
+    __shared__ float biases[kSlice];              // where kBias is set and kBiases is not
     __shared__ uint64_t red[kThreads / kWaveSize];
     const uint32_t r = blockIdx.y, v0 = blockIdx.x * kSlice, v1 = min(a.vocab, v0 + kSlice), tid = threadIdx.x;
+    const T *in = static_cast<const T *>(a.logits) + static_cast<size_t>(r) * a.in_stride;
+    T *out = static_cast<T *>(a.out) + static_cast<size_t>(r) * a.out_stride;
     uint32_t h0 = 0, h1 = 0, b0 = 0, b1 = 0;
     if (a.history) range_of(a.history_starts, r, a.history_capacity, h0, h1);
     if (a.bias_tokens) range_of(a.bias_starts, r, a.bias_capacity, b0, b1);
-    const bool lists = h1 > h0 || b1 > b0;
-    if (lists) {
-        for (uint32_t i = tid; i < kSlice / 4; i += kThreads) {
-            reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
-            reinterpret_cast<uint4 *>(owner)[i] = make_uint4(kNone, kNone, kNone, kNone);
-        }
-        for (uint32_t i = tid; i < kSlice / 32; i += kThreads) again[i] = 0;
-        __syncthreads();
-        const int32_t prompt = a.prompt_counts ? a.prompt_counts[r] : 0;
-        for (uint32_t i = h0 + tid; i < h1; i += kThreads) {
-            const uint32_t t = static_cast<uint32_t>(a.history[i]);
-            if (t < v0 || t >= v1) continue;
-            atomicOr(&counts[t - v0], kSeen);
-            if (static_cast<int32_t>(i - h0) >= prompt) atomicAdd(&counts[t - v0], 1u);
-        }
-        for (uint32_t i = b0 + tid; i < b1; i += kThreads) {
-            const uint32_t t = static_cast<uint32_t>(a.bias_tokens[i]);
-            if (t < v0 || t >= v1) continue;
-            if (atomicMin(&owner[t - v0], i) != kNone) atomicOr(&again[(t - v0) / 32], 1u << ((t - v0) % 32));
-        }
-        __syncthreads();
-    }
+    const int32_t m = a.mask_index ? a.mask_index[r] : static_cast<int32_t>(r);
+    const uint32_t *mask = a.mask && m >= 0 && static_cast<uint32_t>(m) < a.mask_rows ? a.mask + static_cast<size_t>(m) * a.mask_stride : nullptr;
+    const uint32_t prompt = a.prompt_counts ? static_cast<uint32_t>(max(0, a.prompt_counts[r])) : 0u;
     const double rep = a.repetition ? a.repetition[r] : 1.0f, pres = a.presence ? a.presence[r] : 0.0f,
                  freq = a.frequency ? a.frequency[r] : 0.0f;
-    const uint32_t *mask = nullptr;
-    if (a.mask) {
-        const int32_t m = a.mask_index ? a.mask_index[r] : static_cast<int32_t>(r);
-        if (m >= 0 && static_cast<uint32_t>(m) < a.mask_rows) mask = a.mask + static_cast<size_t>(m) * a.mask_stride;
+    Vec<T, VEC> x[N];
+    uint32_t allowed[N];  // the words that hold a vector's tokens: VEC divides 32
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const uint32_t v = v0 + (tid + kThreads * k) * VEC;
+        if (v + VEC <= v1) x[k] = load_vec<T, VEC>(in + v);
+        allowed[k] = mask && v < v1 ? mask[v / 32] : 0xffffffffu;
     }
-    const T *in = static_cast<const T *>(a.logits) + static_cast<size_t>(r) * a.in_stride;
-    T *out = static_cast<T *>(a.out) + static_cast<size_t>(r) * a.out_stride;
-    // the value of token v0 + k: x, after the row's lists
-    auto touched = [&](float x, uint32_t k) {
-        const uint32_t n = counts[k], o = owner[k];
-        if (n == 0 && o == kNone) return from_float<T>(x);
-        double y = x;
-        if (n & kSeen) y = y > 0.0 ? y / rep : y * rep;
-        const uint32_t made = n & ~kSeen;
-        if (made) y = y - static_cast<double>(made) * freq - pres;
-        if (o != kNone) {
-            double bias = a.bias_values[o];
-            if ((again[k / 32] >> (k % 32)) & 1u)  // all of them, in the list's order
-                for (uint32_t i = o + 1; i < b1; ++i)
-                    if (static_cast<uint32_t>(a.bias_tokens[i]) == v0 + k) bias += a.bias_values[i];
-            y += bias;
+    const bool lists = h1 > h0 || b1 > b0;
+    if (lists) {
+        for (uint32_t i = tid; i < kSlice / 4; i += kThreads) reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
+        lds_barrier();
+        scan_list(a.history, h0, h1, [&](uint32_t i, uint32_t t) {
+            if (t < v0 || t >= v1) return;
+            atomicOr(&counts[t - v0], kSeen);
+            if (i - h0 >= prompt) atomicAdd(&counts[t - v0], 1u);
+        });
+        scan_list(a.bias_tokens, b0, b1, [&](uint32_t, uint32_t t) {
+            if (t < v0 || t >= v1) return;
+            if (atomicOr(&counts[t - v0], kBias) & kBias) atomicOr(&counts[t - v0], kBiases);
+        });
+        lds_barrier();
+        if (b1 > b0) {
+            for (uint32_t i = b0 + tid; i < b1; i += kThreads) {
+                const uint32_t t = static_cast<uint32_t>(a.bias_tokens[i]);
+                if (t >= v0 && t < v1 && !(counts[t - v0] & kBiases)) biases[t - v0] = a.bias_values[i];
+            }
+            lds_barrier();
         }
-        if constexpr (sizeof(T) == 4) return static_cast<float>(y);
+    }
+    const double inv_rep = 1.0 / rep;
+    // the value of token v0 + k, with the row's lists' `n`: x after them
+    auto touched = [&](float x, uint32_t k, uint32_t n) {
+        double y = x;
+        if (n & kSeen) y *= y > 0.0 ? inv_rep : rep;
+        const uint32_t made = n & kMostHistory;
+        if (made) y = y - static_cast<double>(made) * freq - pres;
+        if (n & kBiases) {  // all of them, in the list's order
+            double bias = 0.0;
+            for (uint32_t i = b0; i < b1; ++i)
+                if (static_cast<uint32_t>(a.bias_tokens[i]) == v0 + k) bias += a.bias_values[i];
+            y += bias;
+        } else if (n & kBias) {
+            y += biases[k];
+        }
         return from_float<T>(static_cast<float>(y));
     };
-    uint64_t best = 0;
-    auto one = [&](T raw, uint32_t v) {
-        T y = lists ? touched(to_float(raw), v - v0) : raw;
-        if (mask && !((mask[v / 32] >> (v % 32)) & 1u)) y = from_float<T>(-INFINITY);
-        if (a.keys) best = max(best, greedy_key(to_float(y), v));
+    float best = -INFINITY;  // of the thread's tokens, in ascending order: NaN and -inf never win
+    uint32_t best_at = kNone;
+    auto finish = [&](T y, uint32_t v, uint32_t word) {
+        if (!((word >> (v % 32)) & 1u)) y = from_float<T>(-INFINITY);
+        const float f = to_float(y);
+        if (f > best) best = f, best_at = v;
         return y;
     };
-    for (uint32_t v = v0 + tid * VEC; v < v1; v += kThreads * VEC) {
-        if (v + VEC <= v1) {
-            const Vec<T, VEC> x = load_vec<T, VEC>(in + v);
-            Vec<T, VEC> y;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) y.v[i] = one(x.v[i], v + i);
-            store_vec<T, VEC>(out + v, y);
+    for (int k = 0; k < N; ++k) {
+        const uint32_t v = v0 + (tid + kThreads * k) * VEC;
+        if (v + VEC <= v1) {
+            if (lists) {
+#pragma unroll
+                for (int i0 = 0; i0 < VEC; i0 += 4) {
+                    const uint4 n = *reinterpret_cast<const uint4 *>(counts + (v - v0 + i0));
+                    if (n.x | n.y | n.z | n.w) {
+                        const uint32_t n4[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (n4[i]) x[k].v[i0 + i] = touched(to_float(x[k].v[i0 + i]), v - v0 + i0 + i, n4[i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[k].v[i] = finish(x[k].v[i], v + i, allowed[k]);
+            store_vec<T, VEC>(out + v, x[k]);
         } else {
-            for (uint32_t i = v; i < v1; ++i) out[i] = one(in[i], i);
+            for (uint32_t i = v; i < v1; ++i) {
+                T y = in[i];
+                if (lists && counts[i - v0]) y = touched(to_float(y), i - v0, counts[i - v0]);
+                out[i] = finish(y, i, allowed[k]);
+            }
         }
     }
     if (!a.keys) return;
-    best = wave_max_key(best);
-    if (tid % kWaveSize == 0) red[tid / kWaveSize] = best;
-    __syncthreads();
+    const uint64_t key = wave_max_key(greedy_key(best, best_at));
+    if (tid % kWaveSize == 0) red[tid / kWaveSize] = key;
+    lds_barrier();
     if (tid == 0) {
-        for (int w = 1; w < kThreads / kWaveSize; ++w) best = max(best, red[w]);
-        a.keys[static_cast<size_t>(r) * a.parts + blockIdx.x] = best;
+        uint64_t top = red[0];
+        for (int w = 1; w < kThreads / kWaveSize; ++w) top = max(top, red[w]);
+        a.keys[static_cast<size_t>(r) * a.parts + blockIdx.x] = top;
     }
 }
 
@@ -185,7 +234,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_logits_process_device(QwnCudaContextHandle *han
         set_error("logits request: a row stride is shorter than its row, or differs in place");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
-    if ((r->history && (!r->history_starts || r->history_capacity > 0x7fffffffu)) ||
+    if ((r->history && (!r->history_starts || r->history_capacity > kMostHistory)) ||
         (r->bias_tokens && (!r->bias_values || !r->bias_starts || r->bias_capacity > 0x7fffffffu)) ||
         (r->mask && (a.mask_stride < (r->vocab + 31) / 32 || r->mask_rows == 0 || (!r->mask_index && r->mask_rows < r->rows))) ||
         (r->ids && (!r->workspace || (reinterpret_cast<uintptr_t>(r->workspace) & 7u)))) {

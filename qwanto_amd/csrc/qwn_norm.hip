@@ -21,7 +21,7 @@ struct NormArgs {
 
 // Sum over the workgroup, in every thread; red holds a value per wave.
 __device__ __forceinline__ double block_sum(double v, double *red) {
-    for (int off = kWaveSize / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
+    v = wave_sum_f64(v);
     const uint32_t waves = blockDim.x / kWaveSize;
     if (waves == 1) return v;
     if (threadIdx.x % kWaveSize == 0) red[threadIdx.x / kWaveSize] = v;
@@ -31,7 +31,7 @@ __device__ __forceinline__ double block_sum(double v, double *red) {
     return s;
 }
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *red) {
-    for (int off = kWaveSize / 2; off > 0; off >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off)));
+    v = wave_max_u32(v);
     const uint32_t waves = blockDim.x / kWaveSize;
     if (waves == 1) return v;
     if (threadIdx.x % kWaveSize == 0) red[threadIdx.x / kWaveSize] = v;
@@ -211,13 +211,11 @@ hipError_t launch_norm(const NormArgs &a, uint32_t tokens, hipStream_t stream) {
     constexpr uint32_t VEC = 16 / sizeof(T);
     const uint32_t vectors = std::max(1u, a.cols / VEC);
     auto threads = [&](uint32_t vpt) { return ((vectors + vpt - 1) / vpt + kWaveSize - 1) / kWaveSize * kWaveSize; };
-    const uint32_t least = (vectors + 1023) / 1024;  // vectors a thread must hold
-    const uint32_t want = least;
-    if (want <= 1) {
-        hipLaunchKernelGGL((norm_quantize_kernel<T, 1>), dim3(tokens), dim3(threads(1)), 0, stream, a);
-    } else if (want <= 2) {
+    if (vectors <= 2 * 1024) {
+        // two vectors a thread: 4099 tokens of 2560 fp32 27 us (5.0 TB/s), one a
+        // thread 31 (fewer rows at a time), four 28; one token the same
         hipLaunchKernelGGL((norm_quantize_kernel<T, 2>), dim3(tokens), dim3(threads(2)), 0, stream, a);
-    } else if (want <= 4) {
+    } else if (vectors <= 4 * 1024) {
         hipLaunchKernelGGL((norm_quantize_kernel<T, 4>), dim3(tokens), dim3(threads(4)), 0, stream, a);
     } else {
         hipLaunchKernelGGL((norm_quantize_long_kernel<T>), dim3(tokens), dim3(1024), 0, stream, a);

@@ -108,10 +108,6 @@ __device__ __forceinline__ uint32_t units_of(const AttnArgs &a, const PagedSeque
     const Shape h = shape_of(a, q);
     return h.blocks * a.c.kv_heads * h.units;
 }
-// A sequence that every lane asks for.
-__device__ __forceinline__ PagedSequence sequence_of(const AttnArgs &a, uint32_t s) {
-    return paged_rows(a.b, scalar_load(a.b.starts + s), scalar_load(a.b.starts + s + 1), scalar_load(a.b.past + s));
-}
 
 // The list's length, and the first 64 sequences in the lanes: what most batches
 // are found by without a second look.
@@ -306,7 +302,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
         Shape h = shape_of(a, q);
         while (u - before >= h.blocks * a.c.kv_heads * h.units) {
             before += h.blocks * a.c.kv_heads * h.units;
-            q = sequence_of(a, ++s);
+            q = sequence_of(a.b, ++s);
             h = shape_of(a, q);
         }
         const uint32_t item = (u - before) / h.units, at = (u - before) % h.units;
@@ -547,24 +543,18 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
     __shared__ v4f part_o[kGroups][kLanes];
     __shared__ float2 part_ml[kGroups];
     const List list = list_of(a);
-    uint32_t s, block;
-    if (!find_in(a.b, blockIdx.x, [&](uint32_t i) {
-            return shape_of(a, i < kWaveSize ? list.q : paged_sequence(a.b, i)).blocks;
-        }, s, block))
-        return;
+    uint32_t s, block, before = 0;
+    PagedSequence q;
+    if (!find_in(a.b, blockIdx.x, [&](const PagedSequence &x) { return shape_of(a, x).blocks; }, s, block, q)) return;
     const uint32_t head = blockIdx.y;
     const uint32_t total = list.total, workers = workers_of(a, total);
-    uint32_t before = 0;
-    PagedSequence q;
     if (s < kWaveSize) {
         before = lane_of(list.end, s) - lane_of(list.n, s);
-        q = PagedSequence{lane_of(list.q.row, s), lane_of(list.q.rows, s), lane_of(list.q.past, s)};
     } else {
         for (uint32_t s0 = 0; s0 < s; s0 += kWaveSize) {
             const uint32_t i = s0 + threadIdx.x % kWaveSize;
             before += lane_of(wave_scan(i < s ? units_of(a, paged_sequence(a.b, i)) : 0u), kWaveSize - 1);
         }
-        q = sequence_of(a, s);
     }
     const Shape h = shape_of(a, q);
     const uint32_t first = before + (block * a.c.kv_heads + head) * h.units + kStart;

@@ -22,6 +22,11 @@ __device__ __forceinline__ T scalar_load(const T *p) {
     return *reinterpret_cast<const __attribute__((address_space(4))) T *>(reinterpret_cast<uintptr_t>(p));
 }
 
+// A sequence that every lane asks for.
+__device__ __forceinline__ PagedSequence sequence_of(const PagedBatch &b, uint32_t s) {
+    return paged_rows(b, scalar_load(b.starts + s), scalar_load(b.starts + s + 1), scalar_load(b.past + s));
+}
+
 // Inclusive sum over the wave's lanes (row shifts, then the rows' totals).
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t scan_step(uint32_t v) {
@@ -39,21 +44,23 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
     return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
 
-// The sequence whose units (weight(s) of them) hold number `index`, counted
+// The sequence whose units (weight(q) of them) hold number `index`, counted
 // over the sequences in order, and its number within the sequence; false past
 // the last.  Every wave searches for itself, 64 sequences a step.
 template <typename W>
-__device__ __forceinline__ bool find_in(const PagedBatch &b, uint32_t index, W weight, uint32_t &seq, uint32_t &at) {
+__device__ __forceinline__ bool find_in(const PagedBatch &b, uint32_t index, W weight, uint32_t &seq, uint32_t &at,
+                                        PagedSequence &q) {
     const uint32_t lane = threadIdx.x % kWaveSize;
     for (uint32_t s0 = 0; s0 < b.sequences; s0 += kWaveSize) {
         const uint32_t s = s0 + lane;
-        const uint32_t n = s < b.sequences ? weight(s) : 0u;
-        const uint32_t end = wave_scan(n);
+        const PagedSequence mine = s < b.sequences ? paged_sequence(b, s) : PagedSequence{};
+        const uint32_t n = weight(mine), end = wave_scan(n);
         const uint64_t past = __ballot(end > index);
         if (past) {
             const int first = __ffsll(static_cast<unsigned long long>(past)) - 1;
             seq = s0 + first;
             at = index - (lane_of(end, first) - lane_of(n, first));
+            q = PagedSequence{lane_of(mine.row, first), lane_of(mine.rows, first), lane_of(mine.past, first)};
             return true;
         }
         index -= lane_of(end, kWaveSize - 1);
@@ -61,8 +68,8 @@ __device__ __forceinline__ bool find_in(const PagedBatch &b, uint32_t index, W w
     return false;
 }
 
-__device__ __forceinline__ bool find_unit(const PagedBatch &b, uint32_t index, uint32_t &seq, uint32_t &at) {
-    return find_in(b, index, [&](uint32_t s) { return paged_units(paged_sequence(b, s)); }, seq, at);
+__device__ __forceinline__ bool find_unit(const PagedBatch &b, uint32_t index, uint32_t &seq, uint32_t &at, PagedSequence &q) {
+    return find_in(b, index, [](const PagedSequence &x) { return paged_units(x); }, seq, at, q);
 }
 
 }  // namespace qwn

@@ -28,57 +28,79 @@ struct AppendArgs {
     uint32_t key_stride, value_stride, query_stride, query_out_stride, query_heads;
 };
 
-// Elements [c0, c0 + 8) of a row of n, zeros past its end.
+// 8 elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T *row, uint32_t c0, uint32_t n, float v[8]) {
+struct Eight {
+    static constexpr int VEC = 16 / sizeof(T);
+    Vec<T, VEC> v[8 / VEC];
+
+    __device__ __forceinline__ T &raw(int i) { return v[i / VEC].v[i % VEC]; }
+    __device__ __forceinline__ float at(int i) const { return to_float(v[i / VEC].v[i % VEC]); }
+    // Elements [c0, c0 + 8) of a row of n, zeros past its end.
+    __device__ __forceinline__ void load(const T *row, uint32_t c0, uint32_t n) {
+        if (c0 + 8 <= n) {
+#pragma unroll
+            for (int h = 0; h < 8 / VEC; ++h) v[h] = load_vec<T, VEC>(row + c0 + h * VEC);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw(i) = c0 + i < n ? row[c0 + i] : from_float<T>(0.0f);
+        }
+    }
+    // Of the channels [c0, c0 + 8) of a head, the ones that they are paired
+    // with: pairs (i, i + half) of the first `rope` channels.
+    __device__ __forceinline__ void load_partners(const T *row, uint32_t c0, uint32_t n, uint32_t rope) {
+        const uint32_t half = rope / 2;
+        if (half % 8 == 0) {
+            load(row, c0 >= rope ? c0 : c0 < half ? c0 + half : c0 - half, n);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t c = c0 + i;
+                raw(i) = c < rope ? row[c < half ? c + half : c - half] : from_float<T>(0.0f);
+            }
+        }
+    }
+};
+template <typename T>
+__device__ __forceinline__ void store8(T *row, uint32_t c0, uint32_t n, const float v[8]) {
     if (c0 + 8 <= n) {
         constexpr int VEC = 16 / sizeof(T);
 #pragma unroll
         for (int h = 0; h < 8; h += VEC) {
-            const Vec<T, VEC> x = load_vec<T, VEC>(row + c0 + h);
+            Vec<T, VEC> x;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[h + i] = to_float(x.v[i]);
+            for (int i = 0; i < VEC; ++i) x.v[i] = from_float<T>(v[h + i]);
+            store_vec<T, VEC>(row + c0 + h, x);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c0 + i < n ? to_float(row[c0 + i]) : 0.0f;
+        for (int i = 0; i < 8; ++i)
+            if (c0 + i < n) row[c0 + i] = from_float<T>(v[i]);
     }
 }
 
-// The rotated channels [c0, c0 + 8) of a head: of the pairs (i, i + half) of
-// the first `rope` channels, cos and sin [half] of the row's position.
+// v, of channels [c0, c0 + 8), rotated with their partners o; cs: cos and sin
+// [half] of the position.
 template <typename T>
-__device__ __forceinline__ void load8_rotated(const T *row, uint32_t c0, uint32_t n, uint32_t rope, const double2 *cs,
-                                              float v[8]) {
-    load8(row, c0, n, v);
-    if (c0 >= rope) return;
+__device__ __forceinline__ void rotate8(float v[8], const Eight<T> &o, uint32_t c0, uint32_t rope, const double2 *cs) {
     const uint32_t half = rope / 2;
-    float o[8];
-    if (half % 8 == 0) {
-        load8(row, c0 < half ? c0 + half : c0 - half, n, o);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t c = c0 + i;
-            o[i] = c < rope ? to_float(row[c < half ? c + half : c - half]) : 0.0f;
-        }
-    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t c = c0 + i;
         if (c < rope) {
             const double2 t = cs[c < half ? c : c - half];
             const double s = c < half ? -t.y : t.y;
-            v[i] = static_cast<float>(static_cast<double>(v[i]) * t.x + static_cast<double>(o[i]) * s);
+            v[i] = static_cast<float>(static_cast<double>(v[i]) * t.x + static_cast<double>(o.at(i)) * s);
         }
     }
 }
 
 // The 4-bit codes (nibble i: channel c0 + i) of a lane's 8 channels of a
 // head, and the group's step and minimum in every lane of the 8 that hold it.
-// Channels past n count for nothing.  The quotient that a code is rounded
-// from is a 64-bit division: next to a border between two codes, and f16 and
-// bf16 inputs lie on borders, fewer bits would choose another one.
+// Channels past n count for nothing.  A code is the 64-bit quotient rounded,
+// halves to even: f16 and bf16 inputs lie on borders between two codes.  The
+// fp32 quotient is off by less than 2^-18 (three roundings of a number up to
+// 16), so only next to a border does the 64-bit one decide.
 __device__ __forceinline__ uint32_t quantize8(const float *x, uint32_t c0, uint32_t n, f16 &step, f16 &least) {
     constexpr float kMax = 65504.0f;  // the largest f16
     float v[8], lo = kMax, hi = -kMax;
@@ -97,13 +119,16 @@ __device__ __forceinline__ uint32_t quantize8(const float *x, uint32_t c0, uint3
     if (lo > hi) lo = hi = 0.0f;  // a group past the head's channels
     least = static_cast<f16>(lo);
     step = static_cast<f16>((hi - lo) / 15.0f);
-    const double d = static_cast<double>(step), m = static_cast<double>(least);
+    const float d = static_cast<float>(step), m = static_cast<float>(least), inv = d > 0.0f ? 1.0f / d : 0.0f;
     uint32_t codes = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const double t = d > 0.0 ? rint((static_cast<double>(v[i]) - m) / d) : 0.0;
-        const uint32_t code = t > 0.0 ? static_cast<uint32_t>(fmin(t, 15.0)) : 0u;
-        codes |= (c0 + i < n ? code : 0u) << (4 * i);
+        const float t = (v[i] - m) * inv;
+        float code = rintf(t);
+        if (fabsf(t - code) > 0.4999f && fabsf(t) < 17.0f)
+            code = static_cast<float>(rint((static_cast<double>(v[i]) - static_cast<double>(m)) / static_cast<double>(d)));
+        const uint32_t c = static_cast<uint32_t>(fminf(15.0f, fmaxf(0.0f, code)));
+        codes |= (c0 + i < n ? c : 0u) << (4 * i);
     }
     return codes;
 }
@@ -116,69 +141,74 @@ __device__ __forceinline__ uint32_t scale_word(f16 step, f16 least) {
 // Nibbles 0 .. 7 into the order of a key word (qwn_paged.h): even nibbles to
 // 0 .. 3, odd ones to 4 .. 7.
 __device__ __forceinline__ uint32_t key_order(uint32_t n) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= ((n >> (4 * i)) & 15u) << paged_key_bit(i);
-    return w;
+    auto gather = [](uint32_t x) {  // the low nibbles of the 4 bytes
+        x &= 0x0f0f0f0fu;
+        x = (x | x >> 4) & 0x00ff00ffu;
+        return (x | x >> 8) & 0xffffu;
+    };
+    return gather(n) | gather(n >> 4) << 16;
 }
 
-// One workgroup (or gridDim.y of them, which share its tasks) per aligned
-// group of 4 slots that new tokens reach: the tokens whose values share a
-// word.  The angles of its rows are computed once, in 64 bits: at position
-// 100000 an fp32 angle would be off by hundredths.  A task is 8 channels of
-// one head: of the values and keys of the group's tokens, or of one row's
-// queries.  Keys fill whole words.  A word of values is stored where the call
-// brings all 4 of its tokens; else its bits are changed by an exclusive or, so
-// that tokens of one word that come from two sequences of a call (a shared
-// page) do not lose each other.
+// The rows of the batch that bring tokens to unit `unit` of sequence s.
+struct Unit {
+    uint32_t slot, from, count, row;  // its first slot; of its 4 slots the first that is new; how many; the first's row
+};
+__device__ __forceinline__ Unit unit_of(const PagedSequence &q, uint32_t unit) {
+    Unit u;
+    u.slot = (q.past / kPagedUnit + unit) * kPagedUnit;
+    u.from = u.slot < q.past ? q.past - u.slot : 0u;
+    u.count = min(kPagedUnit, q.past + q.rows - u.slot) - u.from;
+    u.row = q.row + u.slot + u.from - q.past;
+    return u;
+}
+
+// A unit's values and keys: a task is 8 channels of one head of either, of all
+// its tokens, whose loads are issued together.  Keys fill whole words.  A word
+// of values is stored where the call brings all 4 of its tokens; else its bits
+// are changed by an exclusive or, so that tokens of one word that come from two
+// sequences of a call (a shared page) do not lose each other.
 template <typename T>
-__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
-    __shared__ double2 cs[kPagedUnit][128];
-    uint32_t s, unit;
-    if (!find_unit(a.b, blockIdx.x, s, unit)) return;
-    const PagedSequence q = paged_sequence(a.b, s);
-    const PagedKv &c = a.c;
-    const uint32_t slot0 = (q.past / kPagedUnit + unit) * kPagedUnit;
-    const uint32_t from = slot0 < q.past ? q.past - slot0 : 0u;                       // of the 4 slots
-    const uint32_t to = min(kPagedUnit, q.past + q.rows - slot0);
-    const uint32_t row0 = q.row + slot0 + from - q.past, count = to - from;           // rows of the batch
-    const uint32_t half = c.rope_dims / 2;
-    for (uint32_t i = threadIdx.x; i < count * half; i += kAppendThreads) {
-        const uint32_t k = i / half, f = i % half;
-        const double p = a.positions ? static_cast<double>(a.positions[row0 + k]) : static_cast<double>(slot0 + from + k);
-        double2 t;
-        sincos(p * c.freqs[f], &t.y, &t.x);
-        cs[k][f] = t;
-    }
-    __syncthreads();
-    uint32_t page = 0;
-    const bool stored = paged_page(c, a.b, s, slot0, page);
-    const uint32_t tile = (slot0 & (c.page_tokens - 1)) / kPagedTile, first = slot0 % kPagedTile;
-    const uint32_t lanes = c.width / 8, groups = c.width / kPagedGroup, D = c.head_dim;
-    const uint32_t kv_tasks = stored ? c.kv_heads * lanes : 0u, q_lanes = (D + 7) / 8;
-    const uint32_t tasks = a.query ? a.query_heads * q_lanes * count : 0u;
-    const uint32_t threads = kAppendThreads * gridDim.y, me = blockIdx.y * kAppendThreads + threadIdx.x;
-    const uint32_t kv_rounds = (2 * kv_tasks + kWaveSize - 1) / kWaveSize * kWaveSize;
-    // whole waves: lanes 8 .. 32 apart exchange below
-    for (uint32_t i = me; i < kv_rounds; i += threads) {
-        const bool real = i < 2 * kv_tasks, is_key = i >= kv_tasks;
+struct KvTask {
+    uint32_t head, lane;
+    bool real, is_key;
+    Eight<T> x[kPagedUnit], o[kPagedUnit];
+
+    __device__ __forceinline__ void load(const AppendArgs &a, const Unit &u, uint32_t i) {
+        const PagedKv &c = a.c;
+        const uint32_t lanes = c.width / 8, kv_tasks = c.kv_heads * lanes;
+        real = i < 2 * kv_tasks;
+        is_key = i >= kv_tasks;
         const uint32_t j = real ? i - (is_key ? kv_tasks : 0u) : 0u;
-        const uint32_t head = j / lanes, lane = j % lanes, c0 = lane * 8;
-        uint8_t *block = c.pool + paged_block_at(c, page, tile, head);
-        uint32_t codes[kPagedUnit] = {};
+        head = j / lanes;
+        lane = j % lanes;
 #pragma unroll
         for (uint32_t k = 0; k < kPagedUnit; ++k) {
-            if (k >= count) break;
-            float x[8];
+            if (k >= u.count) break;
+            const size_t row = u.row + k;
+            const T *src = (is_key ? static_cast<const T *>(a.key) + row * a.key_stride
+                                   : static_cast<const T *>(a.value) + row * a.value_stride) + head * c.head_dim;
+            x[k].load(src, lane * 8, c.head_dim);
+            if (is_key && c.rope_dims) o[k].load_partners(src, lane * 8, c.head_dim, c.rope_dims);
+        }
+    }
+
+    // Whole waves: lanes 1 to 4 apart exchange.
+    __device__ __forceinline__ void store(const AppendArgs &a, const Unit &u, uint32_t page, const double2 (*cs)[128]) {
+        const PagedKv &c = a.c;
+        const uint32_t tile = (u.slot & (c.page_tokens - 1)) / kPagedTile, first = u.slot % kPagedTile;
+        const uint32_t groups = c.width / kPagedGroup, c0 = lane * 8;
+        uint8_t *block = c.pool + paged_block_at(c, page, tile, head);
+        uint32_t codes[kPagedUnit] = {}, other[kPagedUnit];
+#pragma unroll
+        for (uint32_t k = 0; k < kPagedUnit; ++k) {
+            if (k >= u.count) break;
+            const uint32_t token = first + u.from + k;
             f16 step, least;
-            const uint32_t row = row0 + k, token = first + from + k;
-            if (is_key) {
-                load8_rotated(static_cast<const T *>(a.key) + static_cast<size_t>(row) * a.key_stride + head * D, c0, D,
-                              c.rope_dims, cs[k], x);
-            } else {
-                load8(static_cast<const T *>(a.value) + static_cast<size_t>(row) * a.value_stride + head * D, c0, D, x);
-            }
-            codes[k] = quantize8(x, c0, D, step, least);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = x[k].at(i);
+            if (is_key) rotate8(v, o[k], c0, c.rope_dims, cs[k]);
+            codes[k] = quantize8(v, c0, c.head_dim, step, least);
             if (!real) continue;
             if (lane % 8 == 0)
                 reinterpret_cast<uint32_t *>(block + (is_key ? paged_key_scales_at(c.width) : paged_value_scales_at(c.width)))
@@ -187,59 +217,127 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
         }
         // values: channels c0 .. c0 + 7 are columns n = c0 % 16 .. of the 16
         // wide half c0 / 16; the other half of their words is two lanes on
-        uint32_t other[kPagedUnit];
 #pragma unroll
         for (uint32_t k = 0; k < kPagedUnit; ++k) other[k] = __shfl_xor(codes[k], 2);
-        if (!real || is_key) continue;
-        const bool odd = (lane / 2) % 2;   // this lane's channels are the words' upper halves
+        if (!real || is_key) return;
+        const bool odd = (lane / 2) % 2;  // this lane's channels are the words' upper halves
         uint32_t *words = reinterpret_cast<uint32_t *>(block + paged_values_at(c.width));
-        const uint32_t c_even = c0 & ~16u;
 #pragma unroll
         for (uint32_t m = 0; m < 4; ++m) {
             const uint32_t i4 = odd ? 4 + m : m;  // of the lane pair's 8 columns the even lane writes 4, the odd lane 4
             uint32_t bits = 0, mask = 0;
 #pragma unroll
             for (uint32_t k = 0; k < kPagedUnit; ++k) {
-                if (k >= count) break;
+                if (k >= u.count) break;
                 const uint32_t mine = (codes[k] >> (4 * i4)) & 15u, theirs = (other[k] >> (4 * i4)) & 15u;
-                const uint32_t lo = paged_value_bit(from + k, 0), hi = paged_value_bit(from + k, 16);
+                const uint32_t lo = paged_value_bit(u.from + k, 0), hi = paged_value_bit(u.from + k, 16);
                 bits |= (odd ? theirs : mine) << lo | (odd ? mine : theirs) << hi;
                 mask |= 15u << lo | 15u << hi;
             }
-            uint32_t *w = words + paged_value_word(c.width, first, c_even + i4);
-            if (count == kPagedUnit) {
+            uint32_t *w = words + paged_value_word(c.width, first, (c0 & ~16u) + i4);
+            if (u.count == kPagedUnit) {
                 *w = bits;
             } else {
                 atomicXor(w, (*w ^ bits) & mask);
             }
         }
     }
-    for (uint32_t i = me; i < tasks; i += threads) {
-        const uint32_t k = i / (a.query_heads * q_lanes), j = i % (a.query_heads * q_lanes);
-        const uint32_t head = j / q_lanes, c0 = j % q_lanes * 8, row = row0 + k;
-        const T *src = static_cast<const T *>(a.query) + static_cast<size_t>(row) * a.query_stride + head * D;
-        T *dst = static_cast<T *>(a.query_out) + static_cast<size_t>(row) * a.query_out_stride + head * D;
-        // both channels of a pair in one thread: the query may be rotated in place
-        float x[8];
-        if (c0 >= c.rope_dims) {
-            load8(src, c0, D, x);
+};
+
+// A unit's queries: a task is 8 pairs of one head (both channels of a pair in
+// one thread: the query may be rotated in place), or 8 of the channels behind
+// the rotated ones, of all the unit's rows.
+template <typename T>
+struct QueryTask {
+    uint32_t head, c0, end;
+    bool real, pair;
+    Eight<T> x[kPagedUnit], y[kPagedUnit];
+
+    __device__ __forceinline__ void load(const AppendArgs &a, const Unit &u, uint32_t i) {
+        const uint32_t D = a.c.head_dim, rope = a.c.rope_dims, half = rope / 2;
+        const uint32_t pairs = (half + 7) / 8, lanes = pairs + (D - rope + 7) / 8;
+        real = i < a.query_heads * lanes;
+        if (!real) return;
+        head = i / lanes;
+        const uint32_t lane = i % lanes;
+        pair = lane < pairs;
+        c0 = pair ? lane * 8 : rope + (lane - pairs) * 8;
+        end = pair ? half : D;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c0 + e < D) dst[c0 + e] = from_float<T>(x[e]);
-            continue;
+        for (uint32_t k = 0; k < kPagedUnit; ++k) {
+            if (k >= u.count) break;
+            const T *src = static_cast<const T *>(a.query) + static_cast<size_t>(u.row + k) * a.query_stride + head * D;
+            x[k].load(src, c0, end);
+            if (pair) y[k].load(src + half, c0, half);
         }
+    }
+
+    __device__ __forceinline__ void store(const AppendArgs &a, const Unit &u, const double2 (*cs)[128]) {
+        if (!real) return;
+        const uint32_t half = a.c.rope_dims / 2;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t ch = c0 + e;
-            if (ch >= half) {
-                if (ch >= c.rope_dims && ch < D) dst[ch] = src[ch];
-                continue;
+        for (uint32_t k = 0; k < kPagedUnit; ++k) {
+            if (k >= u.count) break;
+            T *dst = static_cast<T *>(a.query_out) + static_cast<size_t>(u.row + k) * a.query_out_stride + head * a.c.head_dim;
+            float p[8], r[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = x[k].at(e);
+            if (pair) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const double2 t = cs[k][min(c0 + e, half - 1)];
+                    const double v = static_cast<double>(p[e]), w = static_cast<double>(y[k].at(e));
+                    p[e] = static_cast<float>(v * t.x - w * t.y);
+                    r[e] = static_cast<float>(v * t.y + w * t.x);
+                }
+                store8(dst + half, c0, half, r);
             }
-            const double2 t = cs[k][ch];
-            const double u = static_cast<double>(to_float(src[ch])), v = static_cast<double>(to_float(src[ch + half]));
-            dst[ch] = from_float<T>(static_cast<float>(u * t.x - v * t.y));
-            dst[ch + half] = from_float<T>(static_cast<float>(u * t.y + v * t.x));
+            store8(dst, c0, end, p);
         }
+    }
+};
+
+// grid (units of 4 slots at most, parts): the first kv_parts workgroups of a
+// unit take its values and keys, the others its queries, a task a thread.  The
+// angles of the unit's rows are computed once in each, in 64 bits (at position
+// 100000 an fp32 angle would be off by hundredths), while the tasks' loads are
+// in flight.
+template <typename T>
+__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a, uint32_t kv_parts) {
+    __shared__ double2 cs[kPagedUnit][128];
+    uint32_t s, unit;
+    PagedSequence q;
+    const uint32_t half = a.c.rope_dims / 2;
+    // ahead of the tasks' loads, which come back in order
+    const double freq = a.c.freqs[half ? threadIdx.x % half : 0u];
+    if (!find_unit(a.b, blockIdx.x, s, unit, q)) return;
+    const Unit u = unit_of(q, unit);
+    const uint32_t k0 = half ? threadIdx.x / half : kPagedUnit;
+    const int32_t own = a.positions && k0 < u.count ? a.positions[u.row + k0] : 0;
+    auto angles = [&] {
+        for (uint32_t i = threadIdx.x; i < u.count * half; i += kAppendThreads) {
+            const uint32_t k = i / half, f = i % half;
+            const bool first = i == threadIdx.x;
+            const double p = a.positions ? static_cast<double>(first ? own : a.positions[u.row + k])
+                                         : static_cast<double>(u.slot + u.from + k);
+            double2 t;
+            sincos(p * (first ? freq : a.c.freqs[f]), &t.y, &t.x);
+            cs[k][f] = t;
+        }
+        lds_barrier();
+    };
+    if (blockIdx.y < kv_parts) {
+        uint32_t page = 0;
+        if (!paged_page(a.c, a.b, s, u.slot, page)) return;
+        KvTask<T> task;
+        task.load(a, u, blockIdx.y * kAppendThreads + threadIdx.x);
+        angles();
+        task.store(a, u, page, cs);
+    } else {
+        QueryTask<T> task;
+        task.load(a, u, (blockIdx.y - kv_parts) * kAppendThreads + threadIdx.x);
+        angles();
+        task.store(a, u, cs);
     }
 }
 
@@ -250,47 +348,58 @@ struct ReadArgs {
     uint32_t stride;
 };
 
-// The fp32 values of the batch's tokens: a workgroup per aligned group of 4
-// slots, a thread a word of codes.
+// The fp32 values of the batch's tokens: a workgroup per unit of 4 slots; a
+// thread takes a word of keys (8 channels of a token) or four words of values
+// (4 channels twice, of 4 tokens).
 __global__ __launch_bounds__(kAppendThreads) void paged_read_kernel(ReadArgs a) {
     uint32_t s, unit;
-    if (!find_unit(a.b, blockIdx.x, s, unit)) return;
-    const PagedSequence q = paged_sequence(a.b, s);
+    PagedSequence q;
+    if (!find_unit(a.b, blockIdx.x, s, unit, q)) return;
     const PagedKv &c = a.c;
-    const uint32_t slot0 = (q.past / kPagedUnit + unit) * kPagedUnit;
-    const uint32_t from = slot0 < q.past ? q.past - slot0 : 0u;
-    const uint32_t to = min(kPagedUnit, q.past + q.rows - slot0);
+    const Unit u = unit_of(q, unit);
     uint32_t page = 0;
-    if (!paged_page(c, a.b, s, slot0, page)) return;
-    const uint32_t tile = (slot0 & (c.page_tokens - 1)) / kPagedTile, first = slot0 % kPagedTile;
-    const uint32_t D = c.head_dim, groups = c.width / kPagedGroup, words = c.width / 2;  // of the group's values and of its keys
-    for (uint32_t i = threadIdx.x; i < 2 * c.kv_heads * words; i += kAppendThreads) {
-        const bool is_key = i >= c.kv_heads * words;
-        const uint32_t j = i % (c.kv_heads * words), head = j / words, w = j % words;
+    if (!paged_page(c, a.b, s, u.slot, page)) return;
+    const uint32_t tile = (u.slot & (c.page_tokens - 1)) / kPagedTile, first = u.slot % kPagedTile;
+    const uint32_t D = c.head_dim, groups = c.width / kPagedGroup;
+    const uint32_t key_tasks = c.width / 2, value_tasks = c.width / 8, tasks = key_tasks + value_tasks;  // of a head
+    auto value = [](uint32_t scale, uint32_t code) {
+        return fmaf(half_to_float(scale >> 16), static_cast<float>(code), half_to_float(scale & 0xffffu));
+    };
+    for (uint32_t i = threadIdx.x; i < c.kv_heads * tasks; i += kAppendThreads) {
+        const uint32_t head = i / tasks, j = i % tasks;
         const uint8_t *block = c.pool + paged_block_at(c, page, tile, head);
-        const uint32_t *codes = reinterpret_cast<const uint32_t *>(block + (is_key ? 0u : paged_values_at(c.width)));
-        const uint32_t *scales = reinterpret_cast<const uint32_t *>(
-            block + (is_key ? paged_key_scales_at(c.width) : paged_value_scales_at(c.width)));
-        float *out = is_key ? a.keys : a.values;
-        if (!out) continue;
-        auto put = [&](uint32_t k, uint32_t ch, uint32_t code) {
-            if (k < from || k >= to || ch >= D) return;
-            const uint32_t sc = scales[(first + k) * groups + ch / kPagedGroup];
-            out[static_cast<size_t>(q.row + slot0 + k - q.past) * a.stride + head * D + ch] =
-                fmaf(half_to_float(sc >> 16), static_cast<float>(code), half_to_float(sc & 0xffffu));
-        };
-        if (is_key) {
-            const uint32_t k = w / (words / 4), c0 = w % (words / 4) * 8;
-            const uint32_t x = codes[paged_key_word(c.width, first + k, c0)];
+        float v[8];
+        if (j < key_tasks) {
+            const uint32_t k = j / (key_tasks / 4), c0 = j % (key_tasks / 4) * 8;
+            if (!a.keys || k < u.from || k >= u.from + u.count) continue;
+            const uint32_t x = reinterpret_cast<const uint32_t *>(block)[paged_key_word(c.width, first + k, c0)];
+            const uint32_t sc = reinterpret_cast<const uint32_t *>(block + paged_key_scales_at(c.width))[(first + k) * groups + c0 / kPagedGroup];
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) put(k, c0 + e, (x >> paged_key_bit(e)) & 15u);
-        } else {
-            const uint32_t ch = w / 16 * 32 + w % 16;
-            const uint32_t x = codes[paged_value_word(c.width, first, ch)];
+            for (uint32_t e = 0; e < 8; ++e) v[e] = value(sc, (x >> paged_key_bit(e)) & 15u);
+            store8(a.keys + static_cast<size_t>(u.row + k - u.from) * a.stride + head * D, c0, D, v);
+        } else if (a.values) {
+            const uint32_t m = j - key_tasks, ch = m / 4 * 32 + m % 4 * 4;  // channels ch .. + 3 and ch + 16 .. + 19
+            const uint32_t *codes = reinterpret_cast<const uint32_t *>(block + paged_values_at(c.width));
+            uint32_t x[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) x[e] = codes[paged_value_word(c.width, first, ch + e)];
 #pragma unroll
             for (uint32_t k = 0; k < kPagedUnit; ++k) {
-                put(k, ch, (x >> paged_value_bit(k, 0)) & 15u);
-                put(k, ch + 16, (x >> paged_value_bit(k, 16)) & 15u);
+                if (k < u.from || k >= u.from + u.count) continue;
+                const uint32_t sc = reinterpret_cast<const uint32_t *>(block + paged_value_scales_at(c.width))[(first + k) * groups + ch / kPagedGroup];
+                float *row = a.values + static_cast<size_t>(u.row + k - u.from) * a.stride + head * D;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    Vec<float, 4> y;
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) y.v[e] = value(sc, (x[e] >> paged_value_bit(k, 16 * h)) & 15u);
+                    const uint32_t at = ch + 16 * h;
+                    if (at + 4 <= D) {
+                        store_vec<float, 4>(row + at, y);
+                    } else {
+                        for (uint32_t e = 0; e < 4 && at + e < D; ++e) row[at + e] = y.v[e];
+                    }
+                }
             }
         }
     }
@@ -465,14 +574,17 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_append_device(QwnCudaContextHandle *ha
     a.positions = r->positions;
     a.query_heads = r->query ? r->query_heads : 0u;
     hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
-    const uint32_t units = paged_units_most(a.b.sequences, a.b.tokens);
-    const dim3 grid(units, 1);
+    // a thread a task of the values and keys; of the queries a task of one token
+    const uint32_t kv_parts = (2 * a.c.kv_heads * (a.c.width / 8) + kAppendThreads - 1) / kAppendThreads;
+    const uint32_t q_parts = (a.query_heads * ((a.c.rope_dims / 2 + 7) / 8 + (a.c.head_dim - a.c.rope_dims + 7) / 8) +
+                              kAppendThreads - 1) / kAppendThreads;
+    const dim3 grid(paged_units_most(a.b.sequences, a.b.tokens), kv_parts + q_parts);
     if (r->dtype == QWN_HIP_DTYPE_F32) {
-        hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(kAppendThreads), 0, s, a);
+        hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(kAppendThreads), 0, s, a, kv_parts);
     } else if (r->dtype == QWN_HIP_DTYPE_F16) {
-        hipLaunchKernelGGL(paged_append_kernel<f16>, grid, dim3(kAppendThreads), 0, s, a);
+        hipLaunchKernelGGL(paged_append_kernel<f16>, grid, dim3(kAppendThreads), 0, s, a, kv_parts);
     } else {
-        hipLaunchKernelGGL(paged_append_kernel<bf16>, grid, dim3(kAppendThreads), 0, s, a);
+        hipLaunchKernelGGL(paged_append_kernel<bf16>, grid, dim3(kAppendThreads), 0, s, a, kv_parts);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_fail("paged KV append launch", e);

@@ -52,40 +52,49 @@ __device__ __forceinline__ void range_of(const int32_t *starts, uint32_t r, uint
     to = ok ? static_cast<uint32_t>(b) : 0u;
 }
 
-// Entries [from, to) of a list, four to a load, f(index, entry) for each: every
-// thread's loads are issued together, four at a time.
-template <typename F>
-__device__ __forceinline__ void scan_list(const int32_t *list, uint32_t from, uint32_t to, F f) {
-    for (uint32_t i0 = from; i0 < to; i0 += 16 * kThreads) {
-        Vec<int32_t, 4> t[4];
+// Four entries of a list from i on, `none` past its end.
+template <typename E>
+__device__ __forceinline__ Vec<E, 4> load_entries(const E *list, uint32_t i, uint32_t to, E none) {
+    if (i + 4 <= to) return load_vec<E, 4>(list + i);
+    Vec<E, 4> t;
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            const uint32_t i = i0 + 4 * (threadIdx.x + kThreads * k);
-            if (i + 4 <= to) {
-                t[k] = load_vec<int32_t, 4>(list + i);
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) t[k].v[e] = i + e < to ? list[i + e] : -1;
-            }
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) f(i0 + 4 * (threadIdx.x + kThreads * k) + e, static_cast<uint32_t>(t[k].v[e]));
-    }
+    for (uint32_t e = 0; e < 4; ++e) t.v[e] = i + e < to ? list[i + e] : none;
+    return t;
 }
 
-// grid (slices of the vocabulary, rows).  A workgroup's slice of the logits is
-// loaded into registers; while it comes, the row's history is counted and its
-// biases are found among the slice's tokens in LDS (integer adds and ors: their
-// order does not matter).  Every slice reads the row's lists, from L2.  Touched
+// The biases of a token that has several, if `index` is its first entry: the
+// wave reads the list 64 entries a step and adds them in its order.
+__device__ __forceinline__ void add_biases(const LogitsArgs &a, uint32_t b0, uint32_t b1, uint32_t token, uint32_t index,
+                                           double *biases, uint32_t v0) {
+    const uint32_t lane = threadIdx.x % kWaveSize;
+    double sum = 0.0;
+    bool any = false;
+    for (uint32_t j0 = b0; j0 < b1; j0 += kWaveSize) {
+        const uint32_t j = j0 + lane;
+        const bool mine = j < b1 && static_cast<uint32_t>(a.bias_tokens[j]) == token;
+        const float v = mine ? a.bias_values[j] : 0.0f;
+        for (uint64_t left = __ballot(mine); left; left &= left - 1) {
+            const int l = __ffsll(static_cast<unsigned long long>(left)) - 1;
+            if (!any && j0 + l != index) return;  // another entry is the first
+            any = true;
+            sum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+        }
+    }
+    if (lane == 0) biases[token - v0] = sum;
+}
+
+// grid (slices of the vocabulary, rows).  The beginnings of the row's lists (up
+// to 4096 tokens and 1024 biases) and a workgroup's slice of the logits are
+// loaded into registers, in this order; while the logits come, the history is
+// counted and the biases are found among the slice's tokens in LDS (integer adds
+// and ors: their order does not matter).  Every slice reads the row's lists, from L2.  Touched
 // logits are computed in 64 bits and rounded once.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     constexpr int N = kSlice / (kThreads * VEC);  // vectors of a thread
     __shared__ __attribute__((aligned(16))) uint32_t counts[kSlice];
-    __shared__ float biases[kSlice];              // where kBias is set and kBiases is not
+    __shared__ double biases[kSlice];             // where kBias is set
     __shared__ uint64_t red[kThreads / kWaveSize];
     const uint32_t r = blockIdx.y, v0 = blockIdx.x * kSlice, v1 = min(a.vocab, v0 + kSlice), tid = threadIdx.x;
     const T *in = static_cast<const T *>(a.logits) + static_cast<size_t>(r) * a.in_stride;
@@ -98,32 +107,70 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
     const uint32_t prompt = a.prompt_counts ? static_cast<uint32_t>(max(0, a.prompt_counts[r])) : 0u;
     const double rep = a.repetition ? a.repetition[r] : 1.0f, pres = a.presence ? a.presence[r] : 0.0f,
                  freq = a.frequency ? a.frequency[r] : 0.0f;
+    constexpr uint32_t kHist = 4;  // vectors of the history that a thread loads first
+    const bool lists = h1 > h0 || b1 > b0;
+    Vec<int32_t, 4> hist[kHist], tokens;
+    Vec<float, 4> values;
+    if (lists) {
+        tokens = load_entries(a.bias_tokens, b0 + 4 * tid, b1, -1);
+        values = load_entries(a.bias_values, b0 + 4 * tid, b1, 0.0f);
+#pragma unroll
+        for (uint32_t k = 0; k < kHist; ++k) hist[k] = load_entries(a.history, h0 + 4 * (tid + kThreads * k), h1, -1);
+    }
     Vec<T, VEC> x[N];
     uint32_t allowed[N];  // the words that hold a vector's tokens: VEC divides 32
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const uint32_t v = v0 + (tid + kThreads * k) * VEC;
-        if (v + VEC <= v1) x[k] = load_vec<T, VEC>(in + v);
         allowed[k] = mask && v < v1 ? mask[v / 32] : 0xffffffffu;
+        if (v + VEC <= v1) x[k] = load_vec<T, VEC>(in + v);
     }
-    const bool lists = h1 > h0 || b1 > b0;
     if (lists) {
         for (uint32_t i = tid; i < kSlice / 4; i += kThreads) reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
         lds_barrier();
-        scan_list(a.history, h0, h1, [&](uint32_t i, uint32_t t) {
-            if (t < v0 || t >= v1) return;
-            atomicOr(&counts[t - v0], kSeen);
-            if (i - h0 >= prompt) atomicAdd(&counts[t - v0], 1u);
-        });
-        scan_list(a.bias_tokens, b0, b1, [&](uint32_t, uint32_t t) {
-            if (t < v0 || t >= v1) return;
-            if (atomicOr(&counts[t - v0], kBias) & kBias) atomicOr(&counts[t - v0], kBiases);
-        });
+        auto count = [&](uint32_t i, const Vec<int32_t, 4> &t4) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t t = static_cast<uint32_t>(t4.v[e]);
+                if (t < v0 || t >= v1) continue;
+                atomicOr(&counts[t - v0], kSeen);
+                if (i + e - h0 >= prompt) atomicAdd(&counts[t - v0], 1u);
+            }
+        };
+        auto find = [&](const Vec<int32_t, 4> &t4) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t t = static_cast<uint32_t>(t4.v[e]);
+                if (t < v0 || t >= v1) continue;
+                if (atomicOr(&counts[t - v0], kBias) & kBias) atomicOr(&counts[t - v0], kBiases);
+            }
+        };
+        // what comes once is put down; what comes several times is added up by the
+        // wave that has the token's first entry, in the list's order
+        auto put = [&](uint32_t i, const Vec<int32_t, 4> &t4, const Vec<float, 4> &v4) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t t = static_cast<uint32_t>(t4.v[e]);
+                const bool here = t >= v0 && t < v1, many = here && (counts[t - v0] & kBiases);
+                if (here && !many) biases[t - v0] = v4.v[e];
+                for (uint64_t left = __ballot(many); left; left &= left - 1) {
+                    const int lane = __ffsll(static_cast<unsigned long long>(left)) - 1;
+                    add_biases(a, b0, b1, __builtin_amdgcn_readlane(static_cast<int>(t), lane),
+                               __builtin_amdgcn_readlane(static_cast<int>(i + e), lane), biases, v0);
+                }
+            }
+        };
+        find(tokens);
+        for (uint32_t i = b0 + 4 * (tid + kThreads); i < b1; i += 4 * kThreads) find(load_entries(a.bias_tokens, i, b1, -1));
+#pragma unroll
+        for (uint32_t k = 0; k < kHist; ++k) count(h0 + 4 * (tid + kThreads * k), hist[k]);
+        for (uint32_t i = h0 + 4 * (tid + kThreads * kHist); i < h1; i += 4 * kThreads) count(i, load_entries(a.history, i, h1, -1));
         lds_barrier();
         if (b1 > b0) {
-            for (uint32_t i = b0 + tid; i < b1; i += kThreads) {
-                const uint32_t t = static_cast<uint32_t>(a.bias_tokens[i]);
-                if (t >= v0 && t < v1 && !(counts[t - v0] & kBiases)) biases[t - v0] = a.bias_values[i];
+            put(b0 + 4 * tid, tokens, values);
+            for (uint32_t i0 = b0 + 4 * kThreads; i0 < b1; i0 += 4 * kThreads) {
+                const uint32_t i = i0 + 4 * tid;
+                put(i, load_entries(a.bias_tokens, i, b1, -1), load_entries(a.bias_values, i, b1, 0.0f));
             }
             lds_barrier();
         }
@@ -135,14 +182,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
         if (n & kSeen) y *= y > 0.0 ? inv_rep : rep;
         const uint32_t made = n & kMostHistory;
         if (made) y = y - static_cast<double>(made) * freq - pres;
-        if (n & kBiases) {  // all of them, in the list's order
-            double bias = 0.0;
-            for (uint32_t i = b0; i < b1; ++i)
-                if (static_cast<uint32_t>(a.bias_tokens[i]) == v0 + k) bias += a.bias_values[i];
-            y += bias;
-        } else if (n & kBias) {
-            y += biases[k];
-        }
+        if (n & kBias) y += biases[k];
         return from_float<T>(static_cast<float>(y));
     };
     float best = -INFINITY;  // of the thread's tokens, in ascending order: NaN and -inf never win

@@ -148,6 +148,19 @@ def test_large_vocabulary(gpu_ctx):
     check(run(gpu_ctx, *c, "f32"), reference(*c), c[0])
 
 
+def test_biases_of_one_token(gpu_ctx):
+    """Lists that name one token often, across every step of the search for it, sums of very unlike
+    sizes among them: added in the list's order."""
+    vocab = 5000
+    g = sv.gen(9)
+    x = sv.normal(g, 3, vocab)
+    few = [(int(t), float(b)) for t, b in zip(torch.randint(0, 7, (900,), generator=g), sv.normal(g, 900))]
+    one = [(4321, 1e8 if i == 3 else -1e8 if i == 700 else 0.125) for i in range(800)]
+    nobody = [[], [], []]
+    args = (x, nobody, [0] * 3, [1.0] * 3, [0.0] * 3, [0.0] * 3, [few, one, [(0, 1.0), (2100, 2.0), (0, 3.0)]], [None] * 3)
+    check(run(gpu_ctx, *args, "f32"), reference(*args), x)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides_and_in_place(gpu_ctx, dtype):
     c = case(6, 4, 5001, dtype)

@@ -65,6 +65,7 @@ constexpr uint32_t kStart = 3;                    // pieces that a block's begin
 // merged; one of 512, 11 and 11.
 constexpr uint32_t kWholeSlots = 512, kWholeSlotsMany = 1024, kMany = 256;
 
+constexpr int kBlockQueryBits = 0;               // where keys are values: |query| < 1
 constexpr int kQueryBits = 15;                   // |query| < 2^15 in f16
 constexpr int kWeightBits = 11;                  // probability times step < 2^11 of the largest met,
 constexpr float kSlack = 4.0f;                   // and 2^4 more before the reference moves
@@ -227,17 +228,20 @@ __device__ __forceinline__ void load_words(uint32_t *dst, const uint8_t *src) {
         dst[0] = x[0], dst[1] = x[1];
     }
 }
-// s and token are the same in every lane.
+// The page of a slot, 0 and false where the table names none; s and slot are
+// the same in every lane.
+__device__ __forceinline__ bool page_at(const AttnArgs &a, uint32_t s, uint32_t slot, uint32_t &page) {
+    const uint32_t at = slot >> a.c.page_shift;
+    const bool in = at < a.b.table_stride;
+    const int32_t p = scalar_load(a.b.table + static_cast<size_t>(s) * a.b.table_stride + (in ? at : 0u));
+    const bool ok = in && p >= 0 && static_cast<uint32_t>(p) < a.c.pages;
+    page = ok ? static_cast<uint32_t>(p) : 0u;
+    return ok;
+}
 __device__ __forceinline__ Pages find_pages(const AttnArgs &a, uint32_t s, uint32_t token) {
     Pages p;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t at = (token + kPagedTile * i) >> a.c.page_shift;
-        const bool in = at < a.b.table_stride;
-        const int32_t page = scalar_load(a.b.table + static_cast<size_t>(s) * a.b.table_stride + (in ? at : 0u));
-        p.ok[i] = in && page >= 0 && static_cast<uint32_t>(page) < a.c.pages;
-        p.page[i] = p.ok[i] ? static_cast<uint32_t>(page) : 0u;
-    }
+    for (int i = 0; i < 2; ++i) p.ok[i] = page_at(a, s, token + kPagedTile * i, p.page[i]);
     return p;
 }
 // The keys' half of a step's tiles, or the values'.
@@ -610,12 +614,318 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
     }
 }
 
+// ---- many query rows ----------------------------------------------------------
+//
+// Prompts: a workgroup takes a block of RW x RT x 16 query rows of one KV head
+// and its whole context, in chunks of 64 tokens, every other chunk for each of
+// its two halves of RW waves; a wave has RT tiles of 16 rows.  Here the products
+// are as many as the reads are few, and unpacking per wave would cost more than
+// the products: a half's threads bring the chunk's codes to f16 values once,
+// step * code + minimum rounded once, in LDS and in the order of the matrix
+// cores' operands, and every wave reads them from there.  (f16 and bf16 rows
+// only: the rounding, 2^-12 of a value, is of the size of f16's own output.)
+// Bound by the vector ALU: exponentials, and the unpacking, which RW waves share.
+constexpr uint32_t kChunk = 64;
+constexpr uint32_t kChunkTiles = kChunk / kPagedTile;
+constexpr int kRowBits = 8;  // probabilities up to 2^8 of the largest met, and kSlack more
+
+// A lane's words of one tile's keys and values, and the scales that go with them.
+template <int W>
+struct TileWords {
+    uint32_t k[W / 32], v[W / 32], ks[W / 64], vs[W / 16];
+};
+template <int W>
+__device__ __forceinline__ void load_tile(const AttnArgs &a, uint32_t page, uint32_t slot, uint32_t head, uint32_t lane, TileWords<W> &t) {
+    constexpr int JW = W >= 128 ? 4 : 2;
+    const uint8_t *block = a.c.pool + paged_block_at(a.c, page, (slot & (a.c.page_tokens - 1)) / kPagedTile, head);
+#pragma unroll
+    for (int j = 0; j < W / 32; j += JW) {
+        load_words<JW>(t.k + j, block + 4 * paged_word(W, lane, j));
+        load_words<JW>(t.v + j, block + paged_values_at(W) + 4 * paged_word(W, lane, j));
+    }
+#pragma unroll
+    for (int j = 0; j < W / 64; ++j)
+        t.ks[j] = reinterpret_cast<const uint32_t *>(block + paged_key_scales_at(W))[lane % 16 * (W / 64) + j];
+    load_words<W / 16>(t.vs, block + paged_value_scales_at(W) + lane / 16 * (W / 4));
+}
+
+// Nibbles p and p + 4 of a word as step * code + minimum, of one or of two tokens.
+__device__ __forceinline__ v2h values2(uint32_t word, int p, v2h step, v2h least) {
+    const v2h base = {static_cast<_Float16>(1024.0f), static_cast<_Float16>(1024.0f)};
+    const v2h code = __builtin_bit_cast(v2h, ((word >> (4 * p)) & 0x000f000fu) | 0x64006400u) - base;
+    const v2h top = {static_cast<_Float16>(65504.0f), static_cast<_Float16>(65504.0f)};
+    return __builtin_elementwise_min(__builtin_elementwise_fma(code, step, least), top);  // a step rounded up may pass f16
+}
+__device__ __forceinline__ v2h both(uint32_t bits) { return __builtin_bit_cast(v2h, bits); }
+
+// The tile in LDS: keys [j][lane][8 halves], values [c][lane][half of a pair of
+// tiles][4 halves].
+template <int W>
+__device__ __forceinline__ void unpack_tile(const TileWords<W> &t, uint32_t tile, uint32_t lane, v4u *keys, v2u *values) {
+#pragma unroll
+    for (int j = 0; j < W / 32; ++j) {
+        const uint32_t w = t.ks[j / 2];
+        const v2h step = both(__builtin_amdgcn_perm(w, w, 0x03020302u)), least = both(__builtin_amdgcn_perm(w, w, 0x01000100u));
+        v4u o;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) o[p] = __builtin_bit_cast(uint32_t, values2(t.k[j], p, step, least));
+        keys[(tile * (W / 32) + j) * kWaveSize + lane] = o;
+    }
+#pragma unroll
+    for (int g = 0; g < W / 64; ++g) {
+        v2h step[2], least[2];  // of tokens 0, 1 and 2, 3
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t a = t.vs[2 * h * (W / 64) + g], b = t.vs[(2 * h + 1) * (W / 64) + g];
+            step[h] = both(__builtin_amdgcn_perm(b, a, 0x07060302u));
+            least[h] = both(__builtin_amdgcn_perm(b, a, 0x05040100u));
+        }
+#pragma unroll
+        for (int w = 2 * g; w < 2 * g + 2; ++w)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                v2u o;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) o[h] = __builtin_bit_cast(uint32_t, values2(t.v[w], 2 * c + h, step[h], least[h]));
+                values[((tile / 2 * (W / 16) + 2 * w + c) * kWaveSize + lane) * 2 + tile % 2] = o;
+            }
+    }
+}
+
+template <typename T, int W, int RW, int RT>
+__global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_kernel(AttnArgs a) {
+    constexpr int J = W / 32, C = W / 16;
+    constexpr uint32_t kBlockRows = RW * RT * 16;
+    constexpr uint32_t kTilesOfWave = kChunkTiles / RW;
+    // of each half: the chunk's keys, then its values
+    extern __shared__ v4u chunk[];
+    constexpr uint32_t kOperands = kChunkTiles * J * kWaveSize;  // 16-byte pieces of keys, and of values
+    const uint32_t lane = threadIdx.x % kWaveSize, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const uint32_t rw = wave % RW, half = wave / RW, n = lane % 16, g = lane / 16;
+    uint32_t s, at;
+    PagedSequence q;
+    if (!find_in(a.b, blockIdx.x, [&](const PagedSequence &x) { return (x.rows * a.group + kBlockRows - 1) / kBlockRows; }, s, at, q))
+        return;
+    const uint32_t all = q.rows * a.group, blocks = (all + kBlockRows - 1) / kBlockRows;
+    const uint32_t block = blocks - 1 - at, head = blockIdx.y;  // the longest contexts first
+    const uint32_t row0 = block * kBlockRows, last = min(row0 + kBlockRows, all) - 1;
+    const uint32_t most = min(q.past + last / a.group + 1, a.slots);
+    const uint32_t chunks = (most + kChunk - 1) / kChunk, rounds = (chunks + 1) / 2;
+    v4u *keys = chunk + half * 2 * kOperands, *values = keys + kOperands;
+
+    // the wave's rows and their queries
+    const uint32_t w_row0 = row0 + rw * RT * 16;
+    uint32_t visible[RT];
+    v8h qf[RT][J];
+    float mul[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const uint32_t r = w_row0 + t * 16 + n;
+        const bool real = r <= last;
+        const uint32_t rr = real ? r : last, tok = rr / a.group;
+        visible[t] = real ? min(q.past + tok + 1, a.slots) : 0u;
+        const T *qp = static_cast<const T *>(a.query) + static_cast<size_t>(q.row + tok) * a.query_stride +
+                      static_cast<size_t>(head * a.group + rr % a.group) * a.c.head_dim;
+        float x[J][8], top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) load_query(qp, 32 * j + 8 * g, a.c.head_dim, x[j]);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!real) x[j][i] = 0.0f;
+                top = fmaxf(top, fabsf(x[j][i]));
+            }
+        top = across_max(top);
+        int e = 0;
+        if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
+        e = max(e, -100);
+        // an infinite query makes the row NaN whatever the keys are
+        const float up = top == INFINITY ? __builtin_nanf("") : ldexpf(1.0f, kBlockQueryBits - e);
+        mul[t] = a.scale * 1.44269504088896340736f * ldexpf(1.0f, e - kBlockQueryBits);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[j][i] *= up;
+            qf[t][j] = halves<1>(x[j]).p[0];
+        }
+    }
+    const uint32_t w_last = min(w_row0 + RT * 16 - 1, last);
+    const bool idle = w_row0 > last;
+    const uint32_t w_most = idle ? 0u : min(q.past + w_last / a.group + 1, a.slots);   // slots any row of the wave sees
+    const uint32_t w_least = idle ? 0u : min(q.past + w_row0 / a.group + 1, a.slots);  // slots every one sees
+
+    v4f acc[RT][C];
+    float sum[RT], m[RT], ref[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        sum[t] = 0.0f, m[t] = -INFINITY, ref[t] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[t][c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // the tiles this wave brings: rw, rw + RW, ... of its half's chunk
+    TileWords<W> words[kTilesOfWave];
+    auto bring = [&](uint32_t t0) {
+#pragma unroll
+        for (uint32_t i = 0; i < kTilesOfWave; ++i) {
+            const uint32_t slot = min(t0, a.slots - 1) / kChunk * kChunk + (rw + RW * i) * kPagedTile;
+            uint32_t page;
+            page_at(a, s, slot, page);
+            load_tile<W>(a, page, slot, head, lane, words[i]);
+        }
+    };
+    bring(half * kChunk);
+    for (uint32_t round = 0; round < rounds; ++round) {
+        const uint32_t t0 = (2 * round + half) * kChunk;
+        lds_barrier();  // the chunk before is read
+#pragma unroll
+        for (uint32_t i = 0; i < kTilesOfWave; ++i)
+            unpack_tile<W>(words[i], rw + RW * i, lane, keys, reinterpret_cast<v2u *>(values));
+        lds_barrier();
+        if (round + 1 < rounds) bring(t0 + 2 * kChunk);
+        if (t0 >= w_most) continue;
+        bool ok[kChunkTiles], all_ok = true;
+#pragma unroll
+        for (uint32_t i = 0; i < kChunkTiles; ++i) {
+            uint32_t page;
+            ok[i] = page_at(a, s, t0 + i * kPagedTile, page);
+            all_ok = all_ok && ok[i];
+        }
+        v4f sc[RT][kChunkTiles];
+#pragma unroll
+        for (uint32_t i = 0; i < kChunkTiles; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const v8h kc = __builtin_bit_cast(v8h, keys[(i * J + j) * kWaveSize + lane]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        kc, qf[t][j], j == 0 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : sc[t][i], 0, 0, 0);
+            }
+        const bool masked = t0 + kChunk > w_least || !all_ok;
+        v8h pf[RT][kChunkTiles / 2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunkTiles; ++i) sc[t][i] *= mul[t];
+            if (masked) {
+#pragma unroll
+                for (uint32_t i = 0; i < kChunkTiles; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!ok[i] || t0 + i * kPagedTile + 4 * g + e >= visible[t]) sc[t][i][e] = -INFINITY;
+            }
+            float mx = sc[t][0][0];
+#pragma unroll
+            for (uint32_t i = 0; i < kChunkTiles; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][i][e]);
+            if (__any(mx > m[t] + kSlack)) {
+                mx = across_max(fmaxf(mx, m[t]));
+                const float moved = mx == -INFINITY ? 0.0f : mx - static_cast<float>(kRowBits);
+                const float alpha = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[t] - moved);
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[t][c] *= alpha;
+                sum[t] *= alpha;
+                m[t] = mx;
+                ref[t] = moved;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kChunkTiles / 2; ++i) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(sc[t][2 * i + e / 4][e % 4] - ref[t]);
+                    sum[t] += p[e];
+                }
+                pf[t][i] = halves<1>(p).p[0];
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kChunkTiles / 2; ++i)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const v8h vc = __builtin_bit_cast(v8h, values[(i * C + c) * kWaveSize + lane]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pf[t][i], acc[t][c], 0, 0, 0);
+            }
+    }
+
+    // the halves meet: the second one's sums through LDS, a wave's rows in its
+    // own part of it
+    lds_barrier();
+    constexpr uint32_t kPartLanes = kWaveSize + 1;  // float4s of a register quadruple, kept off one bank
+    v4f *parts = reinterpret_cast<v4f *>(chunk) + rw * RT * (C * kPartLanes + kWaveSize);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        sum[t] = across_sum(sum[t]);
+        if (half == 1) {
+            v4f *p = parts + t * (C * kPartLanes + kWaveSize);
+#pragma unroll
+            for (int c = 0; c < C; ++c) p[c * kPartLanes + lane] = acc[t][c];
+            p[C * kPartLanes + lane] = (v4f){m[t] == -INFINITY ? -INFINITY : ref[t], sum[t], 0.0f, 0.0f};
+        }
+    }
+    lds_barrier();
+    if (half == 1) return;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const v4f *p = parts + t * (C * kPartLanes + kWaveSize);
+        const v4f ml = p[C * kPartLanes + lane];
+        const float mine = m[t] == -INFINITY ? -INFINITY : ref[t];
+        const float top = fmaxf(mine, ml[0]), base = top == -INFINITY ? 0.0f : top;
+        const float f0 = __builtin_amdgcn_exp2f(mine - base), f1 = __builtin_amdgcn_exp2f(ml[0] - base);
+        const float l = sum[t] * f0 + ml[1] * f1, inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const uint32_t r = w_row0 + t * 16 + n;
+        if (r > last) continue;
+        T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + r / a.group) * a.output_stride +
+                 static_cast<size_t>(head * a.group + r % a.group) * a.c.head_dim;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const v4f o = (acc[t][c] * f0 + p[c * kPartLanes + lane] * f1) * inv;
+            const uint32_t ch = 16 * c + 4 * g;
+            Vec<T, 4> y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y.v[e] = from_float<T>(o[e]);
+            if (ch + 4 <= a.c.head_dim) {
+                store_vec<T, 4>(dst + ch, y);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (ch + e < a.c.head_dim) dst[ch + e] = y.v[e];
+            }
+        }
+    }
+}
+
 size_t partial_bytes(uint32_t width) {
     return static_cast<size_t>(kWorkers) * 2 * kRows * (width * sizeof(float) + sizeof(float2));
 }
 
+// Whether a batch's sequences have rows enough for the block kernel.
+bool block_rows(const AttnArgs &a) { return static_cast<uint64_t>(a.b.tokens) * a.group >= 64ull * a.b.sequences; }
+
+template <typename T, int W, int RW, int RT>
+hipError_t launch_block(const AttnArgs &a, hipStream_t stream) {
+    constexpr uint32_t kBlockRows = RW * RT * 16;
+    constexpr size_t chunks = 2 * 2 * kChunk * W * 2, parts = static_cast<size_t>(RW) * RT * (W / 16 * (kWaveSize + 1) + kWaveSize) * 16;
+    constexpr size_t lds = chunks > parts ? chunks : parts;
+    static_assert(lds <= 160 * 1024, "a workgroup's LDS");
+    const void *kernel = reinterpret_cast<const void *>(&paged_block_attention_kernel<T, W, RW, RT>);
+    hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+    if (e != hipSuccess) return e;
+    const uint32_t rows = a.b.tokens * a.group;
+    const uint32_t blocks = std::min(rows, rows / kBlockRows + std::min(a.b.sequences, a.b.tokens));
+    hipLaunchKernelGGL((paged_block_attention_kernel<T, W, RW, RT>), dim3(blocks, a.c.kv_heads), dim3(2 * RW * kWaveSize), lds, stream, a);
+    return hipGetLastError();
+}
+
 template <typename T, int W>
 hipError_t launch_width(AttnArgs a, uint32_t blocks, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        if (block_rows(a)) return launch_block<T, W, 2, W == 256 ? 1 : 2>(a, stream);
+    }
     a.whole = a.slots <= (blocks * a.c.kv_heads >= kMany ? kWholeSlotsMany : kWholeSlots);
     a.workers = a.whole ? blocks * a.c.kv_heads : W == 256 ? kWorkers / 3 : kWorkers;  // of 256 channels: one on each CU
     hipLaunchKernelGGL((paged_attention_kernel<T, W>), dim3(a.workers), dim3(kThreads), 0, stream, a);

@@ -184,7 +184,7 @@ def test_pages_that_the_table_does_not_name(gpu_ctx):
         c.close()
 
 
-def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None):
+def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None, block=False, gone=None):
     """64-bit attention over the cached values kv [2][tokens][..] (whole sequences, one after the
     other), and how far an output may be from it.
 
@@ -194,7 +194,9 @@ def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None):
     magnitudes |q| (15 step + |minimum|); its exponential has 2 more ulps and the argument's own
     rounding.  A relative error e of every probability moves the output by at most 2 e max|v|.
     Probabilities times step are halves with 2^-22 (one half: 2^-11) of themselves or 2^-25 of the
-    largest; the sums over the tokens round by 2^-24 each, in chains of at most `n` tokens / 32 + 64."""
+    largest; the sums over the tokens round by 2^-24 each, in chains of at most `n` tokens / 32 + 64.
+    Where sequences bring many rows (`block`), f16 and bf16 ones meet keys and values rounded to f16:
+    2^-11 of each."""
     group, out, tols = heads // kv_heads, [], []
     at = row = 0
     for p, n in zip(past, new):
@@ -207,11 +209,13 @@ def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None):
         see = torch.arange(p + n)[None] <= p + torch.arange(n)[:, None]
         if most is not None:
             see &= torch.arange(p + n)[None] < most
+        if gone is not None:
+            see &= ~gone
         o, t = torch.zeros(n, heads, d, dtype=torch.float64), torch.zeros(n, heads, d, dtype=torch.float64)
         for h in range(heads):
             kh, vh = k[:, h // group], v[:, h // group]
             s = (qs[:, h] @ kh.t() * scale).masked_fill(~see, -math.inf)
-            w = torch.softmax(s, dim=1)
+            w = torch.nan_to_num(torch.softmax(s, dim=1))        # a row that sees nothing: zeros
             o[:, h] = w @ vh
             # |minimum| + 15 step of any group is at most 3 times its largest magnitude
             kmag = 3 * kh.abs().amax()
@@ -220,6 +224,9 @@ def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None):
             lost = 2.0 ** -22 if dtype == "f32" else 2.0 ** -25
             e_s = abs(scale) * qs[:, h].abs().amax(1) * d * lost * kmag + size * 20 * 2.0 ** -24
             e_p = 2.0 ** -22 if dtype == "f32" else 2.0 ** -11
+            if block and dtype != "f32":
+                e_s = e_s + 2.0 ** -11 * abs(scale) * (qs[:, h].abs() @ kh.abs().t()).amax(1)
+                e_p += 2.0 ** -11
             chain = ((p + n) / 32 + 64) * 2.0 ** -24
             err = (2 * (e_s + 2.0 ** -22) + e_p + 2.0 ** -24 + chain) * vmag
             t[:, h] = err[:, None] + (sv.HALF[dtype] + 2.0 ** -23) * o[:, h].abs()
@@ -244,7 +251,8 @@ def attention_case(ctx, dtype, past, new, kv_heads, heads, d, page=16, scale=Non
         c.attend(c.batch(past, new, pad=pad), qd, out, dtype, heads, scale, query_stride=q.shape[1], output_stride=out.shape[1])
         got = out.cpu()
         assert bool((got[rows:] == 7.0).all()) and bool((got[:, heads * d:] == 7.0).all())
-        want, tol = reference(kv, q[:rows, :heads * d], past, new, kv_heads, heads, d, scale, dtype)
+        want, tol = reference(kv, q[:rows, :heads * d], past, new, kv_heads, heads, d, scale, dtype,
+                              block=rows * (heads // kv_heads) >= 64 * len(past))
         off = (got[:rows, :heads * d].double() - want).abs()
         assert bool((off <= tol).all()), f"off by {float((off / tol).max()):.2f} of the bound"
         return got
@@ -269,6 +277,61 @@ def attention_case(ctx, dtype, past, new, kv_heads, heads, d, page=16, scale=Non
 ])
 def test_attention(gpu_ctx, dtype, past, new, kv_heads, heads, d, page):
     attention_case(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, pad=3, seed=sum(past) + d)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("past,new,kv_heads,heads,d,page", [
+    ([0], [64], 1, 1, 64, 16),                                 # one block of rows, one chunk
+    ([0], [65], 1, 1, 128, 16),                                # a row, and a token, more
+    ([63, 64, 0, 0], [128, 63, 1, 200], 2, 2, 128, 32),        # chunks that begin and end inside
+    ([1000, 0], [40, 300], 2, 12, 128, 16),                    # a group of 6 heads: tokens across blocks
+    ([7, 500], [130, 90], 2, 4, 256, 64),
+    ([0, 33], [100, 77], 3, 6, 80, 16),
+    ([9], [200], 1, 5, 96, 128),
+    ([17, 0, 0], [150, 0, 1], 1, 4, 32, 16),
+    ([2000], [20], 1, 16, 128, 16),
+    ([5], [70], 1, 2, 65, 16),
+])
+def test_attention_of_prompts(gpu_ctx, dtype, past, new, kv_heads, heads, d, page):
+    attention_case(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, pad=2, seed=sum(past) + d + 1)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
+def test_attention_of_prompts_scales(gpu_ctx, scale):
+    attention_case(gpu_ctx, "f16", [90], [130], 2, 4, 64, scale=scale, seed=24, qs=3, os=5)
+
+
+def test_prompts_with_bad_pages_and_queries(gpu_ctx):
+    """In the kernel for many rows: pages that the table does not name are not attended to, rows before
+    them see nothing, and a row that is not finite is NaN by itself."""
+    hk, heads, d, n = 1, 2, 64, 130
+    k, v, _ = inputs(21, n, hk, d, "f32")
+    c = sv.Cache(gpu_ctx, [n], hk, d)
+    try:
+        b = c.batch([0], [n])
+        c.append(b, k.to(sv.DEV), v.to(sv.DEV), "f32")
+        kv = c.read(b)
+        table = c.table.clone()
+        table[0, 0], table[0, 1], table[0, 5] = -1, c.pages, -7          # slots 0 .. 31 and 80 .. 95
+        q = sv.normal(sv.gen(22), n, heads * d).to(torch.float16)
+        q[50, 3], q[60, d + 1] = math.nan, math.inf
+        out = torch.full((n, heads * d), 5.0, dtype=torch.float16, device=sv.DEV)
+        c.attend(c.batch([0], [n], table=table), q.to(sv.DEV), out, "f16", heads, d ** -0.5)
+        got = out.cpu()
+        assert not bool(got[:32].any())
+        clean = q.clone()
+        clean[50], clean[60] = 0.0, 0.0
+        gone = torch.zeros(n, dtype=torch.bool)
+        gone[:32] = gone[80:96] = True
+        want, tol = reference(kv, clean, [0], [n], hk, heads, d, d ** -0.5, "f16", block=True, gone=gone)
+        ok = (got.double() - want).abs() <= tol
+        ok[50, :d] = torch.isnan(got[50, :d])
+        ok[60, d:] = torch.isnan(got[60, d:])
+        ok[50, d:] = ~torch.isnan(got[50, d:])
+        ok[60, :d] = ~torch.isnan(got[60, :d])
+        assert bool(ok[32:].all())
+    finally:
+        c.close()
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.1, 3.0, 40.0])

@@ -624,9 +624,14 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
 // step * code + minimum rounded once, in LDS and in the order of the matrix
 // cores' operands, and every wave reads them from there.  (f16 and bf16 rows
 // only: the rounding, 2^-12 of a value, is of the size of f16's own output.)
-// Bound by the vector ALU: exponentials, and the unpacking, which RW waves share.
+// With two buffers a half unpacks the next chunk while it works on this one; of
+// the two waves that a SIMD holds, the first half's unpacks before its products
+// and the second's after them, so that one's vector instructions meet the
+// other's matrix ones.  Bound by the vector ALU: exponentials, and the
+// unpacking, which RW waves share.
 constexpr uint32_t kChunk = 64;
 constexpr uint32_t kChunkTiles = kChunk / kPagedTile;
+constexpr int kBlockWaves = 4;
 constexpr int kRowBits = 8;  // probabilities up to 2^8 of the largest met, and kSlack more
 
 // A lane's words of one tile's keys and values, and the scales that go with them.
@@ -692,7 +697,7 @@ __device__ __forceinline__ void unpack_tile(const TileWords<W> &t, uint32_t tile
     }
 }
 
-template <typename T, int W, int RW, int RT>
+template <typename T, int W, int RW, int RT, int BUFFERS>
 __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_kernel(AttnArgs a) {
     constexpr int J = W / 32, C = W / 16;
     constexpr uint32_t kBlockRows = RW * RT * 16;
@@ -711,7 +716,7 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     const uint32_t row0 = block * kBlockRows, last = min(row0 + kBlockRows, all) - 1;
     const uint32_t most = min(q.past + last / a.group + 1, a.slots);
     const uint32_t chunks = (most + kChunk - 1) / kChunk, rounds = (chunks + 1) / 2;
-    v4u *keys = chunk + half * 2 * kOperands, *values = keys + kOperands;
+    v4u *mine = chunk + half * BUFFERS * 2 * kOperands;  // this half's buffers: keys, then values
 
     // the wave's rows and their queries
     const uint32_t w_row0 = row0 + rw * RT * 16;
@@ -740,9 +745,10 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
         int e = 0;
         if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
         e = max(e, -100);
-        // an infinite query makes the row NaN whatever the keys are
-        const float up = top == INFINITY ? __builtin_nanf("") : ldexpf(1.0f, kBlockQueryBits - e);
-        mul[t] = a.scale * 1.44269504088896340736f * ldexpf(1.0f, e - kBlockQueryBits);
+        mul[t] = fabsf(a.scale) * 1.44269504088896340736f * ldexpf(1.0f, e - kBlockQueryBits);
+        float up = copysignf(ldexpf(1.0f, kBlockQueryBits - e), a.scale);
+        if (mul[t] == 0.0f) mul[t] = 1.0f, up = 0.0f;       // all scores alike
+        if (top == INFINITY) up = __builtin_nanf("");       // the row is NaN, whatever the keys are
 #pragma unroll
         for (int j = 0; j < J; ++j) {
 #pragma unroll
@@ -755,75 +761,79 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     const uint32_t w_most = idle ? 0u : min(q.past + w_last / a.group + 1, a.slots);   // slots any row of the wave sees
     const uint32_t w_least = idle ? 0u : min(q.past + w_row0 / a.group + 1, a.slots);  // slots every one sees
 
-    v4f acc[RT][C];
-    float sum[RT], m[RT], ref[RT];
+    // m and ref are of the products as they come, before mul (positive)
+    v4f acc[RT][C], sum[RT];
+    float m[RT], ref[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        sum[t] = 0.0f, m[t] = -INFINITY, ref[t] = 0.0f;
+        sum[t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f}, m[t] = -INFINITY, ref[t] = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[t][c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // the tiles this wave brings: rw, rw + RW, ... of its half's chunk
+    // the tiles this wave brings: rw, rw + RW, ... of its half's chunk.  Pages are
+    // looked up a round ahead, while the chunk before is unpacked: a scalar load
+    // under way would hold up every read of LDS
     TileWords<W> words[kTilesOfWave];
+    uint32_t pages[kChunkTiles], next_ok = 0;  // of the chunk to be brought next: bit i, its tile i has a page
+    constexpr uint32_t kAllTiles = (1u << kChunkTiles) - 1;
+    auto look_up = [&](uint32_t t0) {
+        next_ok = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kChunkTiles; ++i) next_ok |= page_at(a, s, t0 + i * kPagedTile, pages[i]) ? 1u << i : 0u;
+    };
     auto bring = [&](uint32_t t0) {
 #pragma unroll
         for (uint32_t i = 0; i < kTilesOfWave; ++i) {
-            const uint32_t slot = min(t0, a.slots - 1) / kChunk * kChunk + (rw + RW * i) * kPagedTile;
-            uint32_t page;
-            page_at(a, s, slot, page);
-            load_tile<W>(a, page, slot, head, lane, words[i]);
+            // pages[rw + RW i], by constant indexes
+            uint32_t page = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < kChunkTiles; ++k) page = k == rw + RW * i ? pages[k] : page;
+            load_tile<W>(a, page, t0 + (rw + RW * i) * kPagedTile, head, lane, words[i]);
         }
     };
-    bring(half * kChunk);
-    for (uint32_t round = 0; round < rounds; ++round) {
-        const uint32_t t0 = (2 * round + half) * kChunk;
-        lds_barrier();  // the chunk before is read
+    // chunk r of this half from the registers into LDS, chunk r + 1 on its way
+    auto unpack = [&](uint32_t r) {
+        v4u *keys = mine + (r % BUFFERS) * 2 * kOperands;
+        look_up((2 * (r + 1) + half) * kChunk);
 #pragma unroll
         for (uint32_t i = 0; i < kTilesOfWave; ++i)
-            unpack_tile<W>(words[i], rw + RW * i, lane, keys, reinterpret_cast<v2u *>(values));
-        lds_barrier();
-        if (round + 1 < rounds) bring(t0 + 2 * kChunk);
-        if (t0 >= w_most) continue;
-        bool ok[kChunkTiles], all_ok = true;
-#pragma unroll
-        for (uint32_t i = 0; i < kChunkTiles; ++i) {
-            uint32_t page;
-            ok[i] = page_at(a, s, t0 + i * kPagedTile, page);
-            all_ok = all_ok && ok[i];
-        }
+            unpack_tile<W>(words[i], rw + RW * i, lane, keys, reinterpret_cast<v2u *>(keys + kOperands));
+    };
+    auto work = [&](uint32_t r, uint32_t seen) {
+        const uint32_t t0 = (2 * r + half) * kChunk;
+        if (t0 >= w_most) return;
+        const v4u *keys = mine + (r % BUFFERS) * 2 * kOperands, *values = keys + kOperands;
         v4f sc[RT][kChunkTiles];
 #pragma unroll
-        for (uint32_t i = 0; i < kChunkTiles; ++i)
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
+            for (uint32_t i = 0; i < kChunkTiles; ++i) {
                 const v8h kc = __builtin_bit_cast(v8h, keys[(i * J + j) * kWaveSize + lane]);
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
                     sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                         kc, qf[t][j], j == 0 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : sc[t][i], 0, 0, 0);
             }
-        const bool masked = t0 + kChunk > w_least || !all_ok;
+        const bool masked = t0 + kChunk > w_least || seen != kAllTiles;
         v8h pf[RT][kChunkTiles / 2];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-#pragma unroll
-            for (uint32_t i = 0; i < kChunkTiles; ++i) sc[t][i] *= mul[t];
             if (masked) {
 #pragma unroll
                 for (uint32_t i = 0; i < kChunkTiles; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!ok[i] || t0 + i * kPagedTile + 4 * g + e >= visible[t]) sc[t][i][e] = -INFINITY;
+                        if (!((seen >> i) & 1u) || t0 + i * kPagedTile + 4 * g + e >= visible[t]) sc[t][i][e] = -INFINITY;
             }
             float mx = sc[t][0][0];
 #pragma unroll
             for (uint32_t i = 0; i < kChunkTiles; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][i][e]);
-            if (__any(mx > m[t] + kSlack)) {
+            if (__any((mx - m[t]) * mul[t] > kSlack)) {  // or nothing seen so far
                 mx = across_max(fmaxf(mx, m[t]));
-                const float moved = mx == -INFINITY ? 0.0f : mx - static_cast<float>(kRowBits);
+                const float moved = mx == -INFINITY ? 0.0f : fmaf(mx, mul[t], -static_cast<float>(kRowBits));
                 const float alpha = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[t] - moved);
 #pragma unroll
                 for (int c = 0; c < C; ++c) acc[t][c] *= alpha;
@@ -835,10 +845,8 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
             for (uint32_t i = 0; i < kChunkTiles / 2; ++i) {
                 float p[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(sc[t][2 * i + e / 4][e % 4] - ref[t]);
-                    sum[t] += p[e];
-                }
+                for (int e = 0; e < 8; ++e)
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(sc[t][2 * i + e / 4][e % 4], mul[t], -ref[t]));
                 pf[t][i] = halves<1>(p).p[0];
             }
         }
@@ -850,6 +858,45 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
 #pragma unroll
                 for (int t = 0; t < RT; ++t) acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pf[t][i], acc[t][c], 0, 0, 0);
             }
+        // the sum of the probabilities, as they were rounded: a product with ones
+        const _Float16 one = static_cast<_Float16>(1.0f);
+#pragma unroll
+        for (uint32_t i = 0; i < kChunkTiles / 2; ++i)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+                sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16((v8h){one, one, one, one, one, one, one, one}, pf[t][i], sum[t], 0, 0, 0);
+    };
+
+    look_up(half * kChunk);
+    uint32_t now = next_ok;  // of the chunk that is worked on
+    bring(half * kChunk);
+    if constexpr (BUFFERS == 2) {
+        unpack(0);
+        uint32_t next = next_ok;
+        bring((2 + half) * kChunk);
+        for (uint32_t r = 0; r < rounds; ++r) {
+            lds_barrier();  // chunk r is there, and the buffer of the one before is free
+            if (half == 0) {
+                unpack(r + 1);
+                bring((2 * (r + 2) + half) * kChunk);
+            }
+            work(r, now);
+            if (half == 1) {
+                unpack(r + 1);
+                bring((2 * (r + 2) + half) * kChunk);
+            }
+            now = next;
+            next = next_ok;
+        }
+    } else {
+        for (uint32_t r = 0; r < rounds; ++r) {
+            lds_barrier();
+            unpack(r);
+            lds_barrier();
+            bring((2 * (r + 1) + half) * kChunk);
+            work(r, now);
+            now = next_ok;
+        }
     }
 
     // the halves meet: the second one's sums through LDS, a wave's rows in its
@@ -859,12 +906,11 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     v4f *parts = reinterpret_cast<v4f *>(chunk) + rw * RT * (C * kPartLanes + kWaveSize);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        sum[t] = across_sum(sum[t]);
         if (half == 1) {
             v4f *p = parts + t * (C * kPartLanes + kWaveSize);
 #pragma unroll
             for (int c = 0; c < C; ++c) p[c * kPartLanes + lane] = acc[t][c];
-            p[C * kPartLanes + lane] = (v4f){m[t] == -INFINITY ? -INFINITY : ref[t], sum[t], 0.0f, 0.0f};
+            p[C * kPartLanes + lane] = (v4f){m[t] == -INFINITY ? -INFINITY : ref[t], sum[t][0], 0.0f, 0.0f};
         }
     }
     lds_barrier();
@@ -876,7 +922,7 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
         const float mine = m[t] == -INFINITY ? -INFINITY : ref[t];
         const float top = fmaxf(mine, ml[0]), base = top == -INFINITY ? 0.0f : top;
         const float f0 = __builtin_amdgcn_exp2f(mine - base), f1 = __builtin_amdgcn_exp2f(ml[0] - base);
-        const float l = sum[t] * f0 + ml[1] * f1, inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float l = sum[t][0] * f0 + ml[1] * f1, inv = l == 0.0f ? 0.0f : 1.0f / l;
         const uint32_t r = w_row0 + t * 16 + n;
         if (r > last) continue;
         T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + r / a.group) * a.output_stride +
@@ -906,25 +952,25 @@ size_t partial_bytes(uint32_t width) {
 // Whether a batch's sequences have rows enough for the block kernel.
 bool block_rows(const AttnArgs &a) { return static_cast<uint64_t>(a.b.tokens) * a.group >= 64ull * a.b.sequences; }
 
-template <typename T, int W, int RW, int RT>
+template <typename T, int W, int RW, int RT, int BUFFERS>
 hipError_t launch_block(const AttnArgs &a, hipStream_t stream) {
     constexpr uint32_t kBlockRows = RW * RT * 16;
-    constexpr size_t chunks = 2 * 2 * kChunk * W * 2, parts = static_cast<size_t>(RW) * RT * (W / 16 * (kWaveSize + 1) + kWaveSize) * 16;
+    constexpr size_t chunks = 2 * BUFFERS * 2 * kChunk * W * 2, parts = static_cast<size_t>(RW) * RT * (W / 16 * (kWaveSize + 1) + kWaveSize) * 16;
     constexpr size_t lds = chunks > parts ? chunks : parts;
     static_assert(lds <= 160 * 1024, "a workgroup's LDS");
-    const void *kernel = reinterpret_cast<const void *>(&paged_block_attention_kernel<T, W, RW, RT>);
+    const void *kernel = reinterpret_cast<const void *>(&paged_block_attention_kernel<T, W, RW, RT, BUFFERS>);
     hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     if (e != hipSuccess) return e;
     const uint32_t rows = a.b.tokens * a.group;
     const uint32_t blocks = std::min(rows, rows / kBlockRows + std::min(a.b.sequences, a.b.tokens));
-    hipLaunchKernelGGL((paged_block_attention_kernel<T, W, RW, RT>), dim3(blocks, a.c.kv_heads), dim3(2 * RW * kWaveSize), lds, stream, a);
+    hipLaunchKernelGGL((paged_block_attention_kernel<T, W, RW, RT, BUFFERS>), dim3(blocks, a.c.kv_heads), dim3(2 * RW * kWaveSize), lds, stream, a);
     return hipGetLastError();
 }
 
 template <typename T, int W>
 hipError_t launch_width(AttnArgs a, uint32_t blocks, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
-        if (block_rows(a)) return launch_block<T, W, 2, W == 256 ? 1 : 2>(a, stream);
+        if (block_rows(a)) return launch_block<T, W, kBlockWaves, W == 256 ? 1 : 2, W == 256 ? 1 : 2>(a, stream);
     }
     a.whole = a.slots <= (blocks * a.c.kv_heads >= kMany ? kWholeSlotsMany : kWholeSlots);
     a.workers = a.whole ? blocks * a.c.kv_heads : W == 256 ? kWorkers / 3 : kWorkers;  // of 256 channels: one on each CU

@@ -65,7 +65,6 @@ constexpr uint32_t kStart = 3;                    // pieces that a block's begin
 // merged; one of 512, 11 and 11.
 constexpr uint32_t kWholeSlots = 512, kWholeSlotsMany = 1024, kMany = 256;
 
-constexpr int kBlockQueryBits = 0;               // where keys are values: |query| < 1
 constexpr int kQueryBits = 15;                   // |query| < 2^15 in f16
 constexpr int kWeightBits = 11;                  // probability times step < 2^11 of the largest met,
 constexpr float kSlack = 4.0f;                   // and 2^4 more before the reference moves
@@ -81,6 +80,7 @@ struct AttnArgs {
     uint32_t slots;      // of a sequence's row of the table
     uint32_t workers;    // workgroups of the launch
     bool whole;
+    uint32_t parts;      // of a block's context in the block kernel, at most
     float scale;
 };
 
@@ -631,6 +631,14 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
 // unpacking, which RW waves share.
 constexpr uint32_t kChunk = 64;
 constexpr uint32_t kChunkTiles = kChunk / kPagedTile;
+constexpr uint32_t kNoPage = 0xffffffffu;
+// Where a launch has fewer blocks than half the CUs, a block's context is split
+// among several workgroups, each with kPartRounds rounds at least, and merged
+// after (32 heads of 128: 64 tokens behind 4032 25 us, 89 whole; 512 behind 7680
+// 103 us, 169 whole).  Workgroups that follow each other on a CU do not pay for
+// the merge: with twice kBlockGroups the second takes 116 us and eight prompts of
+// 152 blocks 70, 59 whole.  Eight rounds at least: the first takes 33 us.
+constexpr uint32_t kBlockGroups = 256, kBlockPartsMost = 8, kPartRounds = 4;
 constexpr int kBlockWaves = 4;
 constexpr int kRowBits = 8;  // probabilities up to 2^8 of the largest met, and kSlack more
 
@@ -697,6 +705,10 @@ __device__ __forceinline__ void unpack_tile(const TileWords<W> &t, uint32_t tile
     }
 }
 
+__device__ __forceinline__ uint32_t block_parts(const AttnArgs &a, uint32_t rounds) {
+    return min(a.parts, (rounds + kPartRounds - 1) / kPartRounds);
+}
+
 template <typename T, int W, int RW, int RT, int BUFFERS>
 __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_kernel(AttnArgs a) {
     constexpr int J = W / 32, C = W / 16;
@@ -715,45 +727,98 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     const uint32_t block = blocks - 1 - at, head = blockIdx.y;  // the longest contexts first
     const uint32_t row0 = block * kBlockRows, last = min(row0 + kBlockRows, all) - 1;
     const uint32_t most = min(q.past + last / a.group + 1, a.slots);
-    const uint32_t chunks = (most + kChunk - 1) / kChunk, rounds = (chunks + 1) / 2;
+    const uint32_t chunks = (most + kChunk - 1) / kChunk, all_rounds = (chunks + 1) / 2;
+    const uint32_t parts = block_parts(a, all_rounds);
+    if (blockIdx.z >= parts) return;
+    const uint32_t from = all_rounds * blockIdx.z / parts, rounds = all_rounds * (blockIdx.z + 1) / parts;
     v4u *mine = chunk + half * BUFFERS * 2 * kOperands;  // this half's buffers: keys, then values
 
-    // the wave's rows and their queries
+    // the tiles this wave brings: rw, rw + RW, ... of its half's chunk.  A lane
+    // holds the page of one tile of 64, and the next 64 are on their way: looking
+    // a chunk's pages up in the table, a round's wait each, was a fifth of the time
+    TileWords<W> words[kTilesOfWave];
+    uint32_t pages[kChunkTiles], next_ok = 0;  // of the chunk to be brought next: bit i, its tile i has a page
+    constexpr uint32_t kAllTiles = (1u << kChunkTiles) - 1;
+    auto load_window = [&](uint32_t tile) {
+        const uint32_t i = ((tile + lane) * kPagedTile) >> a.c.page_shift;
+        const int32_t p = i < a.b.table_stride ? a.b.table[static_cast<size_t>(s) * a.b.table_stride + i] : -1;
+        return p >= 0 && static_cast<uint32_t>(p) < a.c.pages ? static_cast<uint32_t>(p) : kNoPage;
+    };
+    uint32_t window_tile = 2 * from * kChunkTiles / kWaveSize * kWaveSize;
+    uint32_t window = load_window(window_tile), next_window = load_window(window_tile + kWaveSize);
+    // the wave's rows and their queries, on their way while the first pages are
+    // looked up
     const uint32_t w_row0 = row0 + rw * RT * 16;
     uint32_t visible[RT];
+    Vec<T, 8> raw[RT][J];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const uint32_t r = w_row0 + t * 16 + n;
+        const uint32_t rr = min(r, last), tok = rr / a.group;
+        visible[t] = r <= last ? min(q.past + tok + 1, a.slots) : 0u;
+        const T *qp = static_cast<const T *>(a.query) + static_cast<size_t>(q.row + tok) * a.query_stride +
+                      static_cast<size_t>(head * a.group + rr % a.group) * a.c.head_dim;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const uint32_t c0 = 32 * j + 8 * g;
+            if (a.c.head_dim == W || c0 + 8 <= a.c.head_dim) {
+                raw[t][j] = load_vec<T, 8>(qp + c0);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) raw[t][j].v[e] = c0 + e < a.c.head_dim ? qp[c0 + e] : from_float<T>(0.0f);
+            }
+        }
+    }
+    auto look_up = [&](uint32_t t0) {
+        if (t0 / kPagedTile >= window_tile + kWaveSize) {
+            window = next_window;
+            window_tile += kWaveSize;
+            next_window = load_window(window_tile + kWaveSize);
+        }
+        next_ok = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kChunkTiles; ++i) {
+            const uint32_t p = lane_of(window, (t0 / kPagedTile + i) % kWaveSize);
+            next_ok |= p != kNoPage ? 1u << i : 0u;
+            pages[i] = p != kNoPage ? p : 0u;
+        }
+    };
+    auto bring = [&](uint32_t t0) {
+#pragma unroll
+        for (uint32_t i = 0; i < kTilesOfWave; ++i) {
+            // pages[rw + RW i], by constant indexes
+            uint32_t page = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < kChunkTiles; ++k) page = k == rw + RW * i ? pages[k] : page;
+            load_tile<W>(a, page, t0 + (rw + RW * i) * kPagedTile, head, lane, words[i]);
+        }
+    };
+    look_up((2 * from + half) * kChunk);
+    uint32_t now = next_ok;  // of the chunk that is worked on
+    bring((2 * from + half) * kChunk);
     v8h qf[RT][J];
     float mul[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const uint32_t r = w_row0 + t * 16 + n;
-        const bool real = r <= last;
-        const uint32_t rr = real ? r : last, tok = rr / a.group;
-        visible[t] = real ? min(q.past + tok + 1, a.slots) : 0u;
-        const T *qp = static_cast<const T *>(a.query) + static_cast<size_t>(q.row + tok) * a.query_stride +
-                      static_cast<size_t>(head * a.group + rr % a.group) * a.c.head_dim;
-        float x[J][8], top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) load_query(qp, 32 * j + 8 * g, a.c.head_dim, x[j]);
+        float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!real) x[j][i] = 0.0f;
-                top = fmaxf(top, fabsf(x[j][i]));
-            }
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_float(raw[t][j].v[e])));
         top = across_max(top);
         int e = 0;
         if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
         e = max(e, -100);
-        mul[t] = fabsf(a.scale) * 1.44269504088896340736f * ldexpf(1.0f, e - kBlockQueryBits);
-        float up = copysignf(ldexpf(1.0f, kBlockQueryBits - e), a.scale);
+        mul[t] = fabsf(a.scale) * 1.44269504088896340736f * ldexpf(1.0f, e);
+        float up = copysignf(ldexpf(1.0f, -e), a.scale);   // |query| < 1
         if (mul[t] == 0.0f) mul[t] = 1.0f, up = 0.0f;       // all scores alike
         if (top == INFINITY) up = __builtin_nanf("");       // the row is NaN, whatever the keys are
 #pragma unroll
         for (int j = 0; j < J; ++j) {
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[j][i] *= up;
-            qf[t][j] = halves<1>(x[j]).p[0];
+            for (int k = 0; k < 8; ++k) x[k] = to_float(raw[t][j].v[k]) * up;
+            qf[t][j] = halves<1>(x).p[0];
         }
     }
     const uint32_t w_last = min(w_row0 + RT * 16 - 1, last);
@@ -771,27 +836,6 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
         for (int c = 0; c < C; ++c) acc[t][c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // the tiles this wave brings: rw, rw + RW, ... of its half's chunk.  Pages are
-    // looked up a round ahead, while the chunk before is unpacked: a scalar load
-    // under way would hold up every read of LDS
-    TileWords<W> words[kTilesOfWave];
-    uint32_t pages[kChunkTiles], next_ok = 0;  // of the chunk to be brought next: bit i, its tile i has a page
-    constexpr uint32_t kAllTiles = (1u << kChunkTiles) - 1;
-    auto look_up = [&](uint32_t t0) {
-        next_ok = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kChunkTiles; ++i) next_ok |= page_at(a, s, t0 + i * kPagedTile, pages[i]) ? 1u << i : 0u;
-    };
-    auto bring = [&](uint32_t t0) {
-#pragma unroll
-        for (uint32_t i = 0; i < kTilesOfWave; ++i) {
-            // pages[rw + RW i], by constant indexes
-            uint32_t page = 0;
-#pragma unroll
-            for (uint32_t k = 0; k < kChunkTiles; ++k) page = k == rw + RW * i ? pages[k] : page;
-            load_tile<W>(a, page, t0 + (rw + RW * i) * kPagedTile, head, lane, words[i]);
-        }
-    };
     // chunk r of this half from the registers into LDS, chunk r + 1 on its way
     auto unpack = [&](uint32_t r) {
         v4u *keys = mine + (r % BUFFERS) * 2 * kOperands;
@@ -867,14 +911,11 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
                 sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16((v8h){one, one, one, one, one, one, one, one}, pf[t][i], sum[t], 0, 0, 0);
     };
 
-    look_up(half * kChunk);
-    uint32_t now = next_ok;  // of the chunk that is worked on
-    bring(half * kChunk);
     if constexpr (BUFFERS == 2) {
-        unpack(0);
+        unpack(from);
         uint32_t next = next_ok;
-        bring((2 + half) * kChunk);
-        for (uint32_t r = 0; r < rounds; ++r) {
+        bring((2 * (from + 1) + half) * kChunk);
+        for (uint32_t r = from; r < rounds; ++r) {
             lds_barrier();  // chunk r is there, and the buffer of the one before is free
             if (half == 0) {
                 unpack(r + 1);
@@ -889,7 +930,7 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
             next = next_ok;
         }
     } else {
-        for (uint32_t r = 0; r < rounds; ++r) {
+        for (uint32_t r = from; r < rounds; ++r) {
             lds_barrier();
             unpack(r);
             lds_barrier();
@@ -902,39 +943,44 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     // the halves meet: the second one's sums through LDS, a wave's rows in its
     // own part of it
     lds_barrier();
-    constexpr uint32_t kPartLanes = kWaveSize + 1;  // float4s of a register quadruple, kept off one bank
-    v4f *parts = reinterpret_cast<v4f *>(chunk) + rw * RT * (C * kPartLanes + kWaveSize);
+    constexpr uint32_t kSumLanes = kWaveSize + 1;  // float4s of a register quadruple, kept off one bank
+    constexpr uint32_t kSums = C * kSumLanes + kWaveSize;
+    v4f *sums = reinterpret_cast<v4f *>(chunk) + rw * RT * kSums;
+    if (half == 1) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        if (half == 1) {
-            v4f *p = parts + t * (C * kPartLanes + kWaveSize);
+        for (int t = 0; t < RT; ++t) {
 #pragma unroll
-            for (int c = 0; c < C; ++c) p[c * kPartLanes + lane] = acc[t][c];
-            p[C * kPartLanes + lane] = (v4f){m[t] == -INFINITY ? -INFINITY : ref[t], sum[t][0], 0.0f, 0.0f};
+            for (int c = 0; c < C; ++c) sums[t * kSums + c * kSumLanes + lane] = acc[t][c];
+            sums[t * kSums + C * kSumLanes + lane] = (v4f){m[t] == -INFINITY ? -INFINITY : ref[t], sum[t][0], 0.0f, 0.0f};
         }
     }
     lds_barrier();
     if (half == 1) return;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const v4f *p = parts + t * (C * kPartLanes + kWaveSize);
-        const v4f ml = p[C * kPartLanes + lane];
-        const float mine = m[t] == -INFINITY ? -INFINITY : ref[t];
-        const float top = fmaxf(mine, ml[0]), base = top == -INFINITY ? 0.0f : top;
-        const float f0 = __builtin_amdgcn_exp2f(mine - base), f1 = __builtin_amdgcn_exp2f(ml[0] - base);
-        const float l = sum[t][0] * f0 + ml[1] * f1, inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const v4f other = sums[t * kSums + C * kSumLanes + lane];
+        const float own = m[t] == -INFINITY ? -INFINITY : ref[t];
+        const float top = fmaxf(own, other[0]), base = top == -INFINITY ? 0.0f : top;
+        const float f0 = __builtin_amdgcn_exp2f(own - base), f1 = __builtin_amdgcn_exp2f(other[0] - base);
+        const float l = sum[t][0] * f0 + other[1] * f1, inv = l == 0.0f ? 0.0f : 1.0f / l;
         const uint32_t r = w_row0 + t * 16 + n;
         if (r > last) continue;
         T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + r / a.group) * a.output_stride +
                  static_cast<size_t>(head * a.group + r % a.group) * a.c.head_dim;
+        const size_t at_part = ((static_cast<size_t>(blockIdx.x) * a.c.kv_heads + head) * a.parts + blockIdx.z) * kBlockRows + r - row0;
+        if (parts > 1 && g == 0) a.part_ml[at_part] = make_float2(top, l);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const v4f o = (acc[t][c] * f0 + p[c * kPartLanes + lane] * f1) * inv;
+            const v4f o = acc[t][c] * f0 + sums[t * kSums + c * kSumLanes + lane] * f1;
             const uint32_t ch = 16 * c + 4 * g;
+            if (parts > 1) {
+                *reinterpret_cast<v4f *>(a.part_o + at_part * W + ch) = o;
+                continue;
+            }
             Vec<T, 4> y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y.v[e] = from_float<T>(o[e]);
-            if (ch + 4 <= a.c.head_dim) {
+            for (int e = 0; e < 4; ++e) y.v[e] = from_float<T>(o[e] * inv);
+            if (a.c.head_dim == W || ch + 4 <= a.c.head_dim) {
                 store_vec<T, 4>(dst + ch, y);
             } else {
 #pragma unroll
@@ -945,25 +991,83 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     }
 }
 
-size_t partial_bytes(uint32_t width) {
-    return static_cast<size_t>(kWorkers) * 2 * kRows * (width * sizeof(float) + sizeof(float2));
+// The parts of the blocks whose contexts were split.  grid (blocks at most, KV
+// heads, row groups): W / 4 threads a row.
+template <typename T, int W, uint32_t ROWS>
+__global__ __launch_bounds__(kThreads) void paged_block_merge_kernel(AttnArgs a) {
+    constexpr uint32_t kLanes = W / 4, kGroups = kThreads / kLanes;
+    uint32_t s, at;
+    PagedSequence q;
+    if (!find_in(a.b, blockIdx.x, [&](const PagedSequence &x) { return (x.rows * a.group + ROWS - 1) / ROWS; }, s, at, q)) return;
+    const uint32_t all = q.rows * a.group, block = (all + ROWS - 1) / ROWS - 1 - at, head = blockIdx.y;
+    const uint32_t row0 = block * ROWS, last = min(row0 + ROWS, all) - 1;
+    const uint32_t most = min(q.past + last / a.group + 1, a.slots);
+    const uint32_t parts = block_parts(a, ((most + kChunk - 1) / kChunk + 1) / 2);
+    if (parts == 1) return;
+    const uint32_t lane = threadIdx.x % kLanes, r = blockIdx.z * kGroups + threadIdx.x / kLanes, row = row0 + r;
+    if (row > last) return;
+    const size_t first = (static_cast<size_t>(blockIdx.x) * a.c.kv_heads + head) * a.parts * ROWS + r;
+    float2 ml[kBlockPartsMost];
+    v4f x[kBlockPartsMost];
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t i = 0; i < kBlockPartsMost; ++i)
+        if (i < parts) {
+            ml[i] = a.part_ml[first + i * ROWS];
+            x[i] = *reinterpret_cast<const v4f *>(a.part_o + (first + i * ROWS) * W + 4 * lane);
+            top = fmaxf(top, ml[i].x);
+        }
+    const float base = top == -INFINITY ? 0.0f : top;
+    v4f o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kBlockPartsMost; ++i)
+        if (i < parts) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - base);
+            o += x[i] * f;
+            l += ml[i].y * f;
+        }
+    T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + row / a.group) * a.output_stride +
+             static_cast<size_t>(head * a.group + row % a.group) * a.c.head_dim;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (4 * lane + e < a.c.head_dim) dst[4 * lane + e] = from_float<T>(l == 0.0f ? 0.0f : o[e] / l);
 }
+
+// Rows of the block kernel's blocks.
+constexpr uint32_t block_rows_of(uint32_t width) { return kBlockWaves * (width == 256 ? 1u : 2u) * 16; }
+
+// Partial rows that a workspace holds: two blocks of each worker, or a part of a
+// block of each of the block kernel's workgroups.
+size_t partial_rows(uint32_t width) {
+    return std::max<size_t>(static_cast<size_t>(kWorkers) * 2 * kRows, static_cast<size_t>(kBlockGroups) * block_rows_of(width));
+}
+size_t partial_bytes(uint32_t width) { return partial_rows(width) * (width * sizeof(float) + sizeof(float2)); }
 
 // Whether a batch's sequences have rows enough for the block kernel.
 bool block_rows(const AttnArgs &a) { return static_cast<uint64_t>(a.b.tokens) * a.group >= 64ull * a.b.sequences; }
 
 template <typename T, int W, int RW, int RT, int BUFFERS>
-hipError_t launch_block(const AttnArgs &a, hipStream_t stream) {
+hipError_t launch_block(AttnArgs a, hipStream_t stream) {
     constexpr uint32_t kBlockRows = RW * RT * 16;
-    constexpr size_t chunks = 2 * BUFFERS * 2 * kChunk * W * 2, parts = static_cast<size_t>(RW) * RT * (W / 16 * (kWaveSize + 1) + kWaveSize) * 16;
-    constexpr size_t lds = chunks > parts ? chunks : parts;
+    static_assert(kBlockRows == block_rows_of(W), "the workspace is sized by it");
+    constexpr size_t chunks = 2 * BUFFERS * 2 * kChunk * W * 2;
+    constexpr size_t sums = static_cast<size_t>(RW) * RT * (W / 16 * (kWaveSize + 1) + kWaveSize) * 16;
+    constexpr size_t lds = chunks > sums ? chunks : sums;
     static_assert(lds <= 160 * 1024, "a workgroup's LDS");
     const void *kernel = reinterpret_cast<const void *>(&paged_block_attention_kernel<T, W, RW, RT, BUFFERS>);
     hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     if (e != hipSuccess) return e;
-    const uint32_t rows = a.b.tokens * a.group;
-    const uint32_t blocks = std::min(rows, rows / kBlockRows + std::min(a.b.sequences, a.b.tokens));
-    hipLaunchKernelGGL((paged_block_attention_kernel<T, W, RW, RT, BUFFERS>), dim3(blocks, a.c.kv_heads), dim3(2 * RW * kWaveSize), lds, stream, a);
+    // at most one block of each sequence is not full; of one sequence no workgroup is
+    // without work, as one is enough to send two others to the same CU
+    const uint64_t rows = static_cast<uint64_t>(a.b.tokens) * a.group, used = std::min(a.b.sequences, a.b.tokens);
+    const uint32_t blocks = static_cast<uint32_t>((rows + used * (kBlockRows - 1)) / kBlockRows);
+    a.parts = std::max(1u, std::min(kBlockPartsMost, kBlockGroups / (blocks * a.c.kv_heads)));
+    hipLaunchKernelGGL((paged_block_attention_kernel<T, W, RW, RT, BUFFERS>), dim3(blocks, a.c.kv_heads, a.parts),
+                       dim3(2 * RW * kWaveSize), lds, stream, a);
+    if ((e = hipGetLastError()) != hipSuccess || a.parts == 1 || a.slots <= 2 * kPartRounds * kChunk) return e;
+    hipLaunchKernelGGL((paged_block_merge_kernel<T, W, kBlockRows>), dim3(blocks, a.c.kv_heads, kBlockRows / (kThreads / (W / 4))),
+                       dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -1052,7 +1156,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_attention_device(QwnCudaContextHandle 
     a.output = r->output;
     a.scale = r->scale;
     a.part_ml = static_cast<float2 *>(r->workspace);
-    a.part_o = reinterpret_cast<float *>(a.part_ml + static_cast<size_t>(kWorkers) * 2 * kRows);
+    a.part_o = reinterpret_cast<float *>(a.part_ml + partial_rows(a.c.width));
     hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
     const hipError_t e = r->dtype == QWN_HIP_DTYPE_F32   ? launch_paged_attention<float>(a, static_cast<uint32_t>(blocks), s)
                          : r->dtype == QWN_HIP_DTYPE_F16 ? launch_paged_attention<f16>(a, static_cast<uint32_t>(blocks), s)

@@ -296,6 +296,51 @@ def test_attention_of_prompts(gpu_ctx, dtype, past, new, kv_heads, heads, d, pag
     attention_case(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, pad=2, seed=sum(past) + d + 1)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("past,new,kv_heads,heads,d,page", [
+    ([1500], [130], 1, 2, 64, 16),                             # blocks whose context several workgroups share
+    ([3000], [20], 2, 8, 128, 32),
+    ([900, 0, 1300], [33, 128, 40], 1, 4, 256, 64),            # and others beside them that one does
+    ([2100], [64], 1, 1, 80, 16),
+    ([700, 1200], [70, 3], 1, 2, 32, 16),
+    ([511], [65], 1, 1, 128, 16),                              # from four rounds to a fifth
+    ([9000], [33], 1, 2, 128, 1024),
+])
+def test_attention_of_few_blocks(gpu_ctx, dtype, past, new, kv_heads, heads, d, page):
+    attention_case(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, pad=2, seed=sum(past) + d + 2)
+
+
+def test_few_blocks_with_bad_pages_and_queries(gpu_ctx):
+    """Parts of a context that hold nothing to attend to; a row that is not finite."""
+    hk, heads, d, past, n = 1, 2, 64, 2000, 64
+    k, v, _ = inputs(31, past + n, hk, d, "f32")
+    c = sv.Cache(gpu_ctx, [past + n], hk, d)
+    try:
+        b = c.batch([0], [past + n])
+        c.append(b, k.to(sv.DEV), v.to(sv.DEV), "f32")
+        kv = c.read(b)
+        q = sv.normal(sv.gen(32), n, heads * d).to(torch.bfloat16)
+        q[7, 3] = math.nan
+        clean = q.clone()
+        clean[7] = 0.0
+        for first, last in ((0, 700 // 16), (1024 // 16, 2064 // 16), (0, 2064 // 16)):
+            table = c.table.clone()
+            table[0, first:last] = -1
+            gone = torch.zeros(past + n, dtype=torch.bool)
+            gone[first * 16:last * 16] = True
+            out = torch.full((n, heads * d), 5.0, dtype=torch.bfloat16, device=sv.DEV)
+            c.attend(c.batch([past], [n], table=table), q.to(sv.DEV), out, "bf16", heads, d ** -0.5)
+            got = out.cpu()
+            want, tol = reference(kv, clean, [past], [n], hk, heads, d, d ** -0.5, "bf16", block=True, gone=gone)
+            ok = (got.double() - want).abs() <= tol
+            ok[7, :d] = torch.isnan(got[7, :d]) if not gone.all() else True
+            ok[7, d:] = ~torch.isnan(got[7, d:])
+            assert bool(ok.all())
+            assert not gone.all() or not bool(torch.nan_to_num(got).any())
+    finally:
+        c.close()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
 def test_attention_of_prompts_scales(gpu_ctx, scale):
     attention_case(gpu_ctx, "f16", [90], [130], 2, 4, 64, scale=scale, seed=24, qs=3, os=5)

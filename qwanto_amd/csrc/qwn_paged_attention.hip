@@ -23,7 +23,7 @@
 // 11.  The elements that meet the larger ones are divided by 16 beforehand, the
 // sums multiplied by 2^24 at the end.  (The matrix cores sum such operands to
 // 2e-7 of their magnitudes, integers to 5e-8: fp32 takes integers, less 8 to
-// halve what cancels.)  A probability that f16 rounds would count its error
+// halve what cancels, and so do f16's values.)  A probability that f16 rounds would count its error
 // times the code, although codes are 7.5 +- 5 and the values they make around
 // zero; the sum of the rounded weights, one more product with a row of ones,
 // takes 8 times that error out again.
@@ -41,6 +41,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -286,7 +287,12 @@ __device__ __forceinline__ void load_query(const T *row, uint32_t c0, uint32_t n
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_kernel(AttnArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
-    constexpr bool WHOLE = NP == 2;
+    // Keys meet a few large products, in whole codes only for fp32.  Values meet
+    // many: the sum of p * code as it lies less that of p * 8 leaves 2e-4 of an
+    // output that 131000 tokens average to near nothing (2.9e-4 of error become
+    // 3.7e-4, output's own rounding 2.1e-4), nothing next to bf16's rounding;
+    // f16's in whole codes 49 us for 48.
+    constexpr bool WHOLE = NP == 2, WHOLE_V = !std::is_same_v<T, bf16>;
     constexpr int J = W / 32, G = W / 64, C = W / 16;
     constexpr int kPad = W + 4;
     __shared__ float merge_o[kWaves][kRows][kPad];
@@ -467,10 +473,10 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t w = vs[i / 4][(i % 4) * G + gg];
                     low[gg] = fmaf(p[i], fmaf(8.0f, step_of(w), least_of(w)), low[gg]);
-                    x[i] = fmaf(p[i] * balance<WHOLE>(i), step_of(w), 0.0f);
+                    x[i] = fmaf(p[i] * balance<WHOLE_V>(i), step_of(w), 0.0f);
                 }
                 pf[gg] = halves<NP>(x);
-                if constexpr (!WHOLE) {
+                if constexpr (!WHOLE_V) {
                     const _Float16 one = static_cast<_Float16>(1.0f), more = static_cast<_Float16>(16.0f);
                     weights[gg] = __builtin_amdgcn_mfma_f32_16x16x32_f16((v8h){one, one, more, more, one, one, more, more},
                                                                         pf[gg].p[0], weights[gg], 0, 0, 0);
@@ -479,8 +485,8 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int w = c / 2, b = (c % 2) * 2;
-                const v2h x0 = codes2<WHOLE>(v[0][w], b), x1 = codes2<WHOLE>(v[0][w], b + 1);
-                const v2h x2 = codes2<WHOLE>(v[1][w], b), x3 = codes2<WHOLE>(v[1][w], b + 1);
+                const v2h x0 = codes2<WHOLE_V>(v[0][w], b), x1 = codes2<WHOLE_V>(v[0][w], b + 1);
+                const v2h x2 = codes2<WHOLE_V>(v[1][w], b), x3 = codes2<WHOLE_V>(v[1][w], b + 1);
                 const v8h vc = {x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 #pragma unroll
                 for (int kk = 0; kk < NP; ++kk)
@@ -499,7 +505,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
         if (real) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const v4f o = WHOLE ? acc[c] + low[c / 4] : acc[c] * 0x1p24f - 8.0f * weights[c / 4] + low[c / 4];
+                const v4f o = WHOLE_V ? acc[c] + low[c / 4] : acc[c] * 0x1p24f - 8.0f * weights[c / 4] + low[c / 4];
                 *reinterpret_cast<v4f *>(&merge_o[wave][n][16 * c + 4 * g]) = o;
             }
             if (g == 0) merge_ml[wave][n] = make_float2(m == -INFINITY ? -INFINITY : ref, sum);

@@ -79,20 +79,44 @@ __device__ __forceinline__ void store8(T *row, uint32_t c0, uint32_t n, const fl
     }
 }
 
+// Where the angle of pair f stands in LDS: threads that take 8 pairs each read
+// next to each other.
+__device__ __forceinline__ uint32_t angle_at(uint32_t f) { return f % 8 * 16 + f / 8; }
+
 // v, of channels [c0, c0 + 8), rotated with their partners o; cs: cos and sin
-// [half] of the position.
+// of the position, at angle_at(pair).
 template <typename T>
 __device__ __forceinline__ void rotate8(float v[8], const Eight<T> &o, uint32_t c0, uint32_t rope, const double2 *cs) {
     const uint32_t half = rope / 2;
+    if (half % 8 == 0) {  // all 8 are first channels of their pairs, or second ones, or not rotated
+        if (c0 >= rope) return;
+        const double2 *t = cs + (c0 < half ? c0 : c0 - half) / 8;
+        const uint32_t flip = c0 < half ? 0x80000000u : 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, o.at(i)) ^ flip);
+            v[i] = static_cast<float>(static_cast<double>(v[i]) * t[16 * i].x + static_cast<double>(w) * t[16 * i].y);
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t c = c0 + i;
         if (c < rope) {
-            const double2 t = cs[c < half ? c : c - half];
+            const double2 t = cs[angle_at(c < half ? c : c - half)];
             const double s = c < half ? -t.y : t.y;
             v[i] = static_cast<float>(static_cast<double>(v[i]) * t.x + static_cast<double>(o.at(i)) * s);
         }
     }
+}
+
+// The lanes' values 1, 2 and 7 - i apart within 8: after all three every lane
+// has met all 8.
+template <int STEP>
+__device__ __forceinline__ float lane_near(float v) {
+    constexpr int kCtrl = STEP == 0 ? 0xb1 : STEP == 1 ? 0x4e : 0x141;  // quad_perm [1, 0, 3, 2], [2, 3, 0, 1]; row_half_mirror
+    const int x = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, kCtrl, 0xf, 0xf, true));
 }
 
 // The 4-bit codes (nibble i: channel c0 + i) of a lane's 8 channels of a
@@ -100,36 +124,58 @@ __device__ __forceinline__ void rotate8(float v[8], const Eight<T> &o, uint32_t 
 // Channels past n count for nothing.  A code is the 64-bit quotient rounded,
 // halves to even: f16 and bf16 inputs lie on borders between two codes.  The
 // fp32 quotient is off by less than 2^-18 (three roundings of a number up to
-// 16), so only next to a border does the 64-bit one decide.
-__device__ __forceinline__ uint32_t quantize8(const float *x, uint32_t c0, uint32_t n, f16 &step, f16 &least) {
+// 16), so only next to a border does a lane compare in 64 bits what the border
+// (of at most 16 bits) and the value are.
+__device__ __forceinline__ uint32_t quantize8(float v[8], uint32_t c0, uint32_t n, f16 &step, f16 &least) {
     constexpr float kMax = 65504.0f;  // the largest f16
-    float v[8], lo = kMax, hi = -kMax;
+    float lo = v[0], hi = v[0];
+    bool odd = c0 + 8 > n;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        v[i] = isfinite(x[i]) ? fminf(kMax, fmaxf(-kMax, x[i])) : 0.0f;
-        if (c0 + i < n) {
-            lo = fminf(lo, v[i]);
-            hi = fmaxf(hi, v[i]);
+        lo = fminf(lo, v[i]);
+        hi = fmaxf(hi, v[i]);
+        if (i % 2) odd |= __builtin_isunordered(v[i - 1], v[i]);
+    }
+    if (__any(odd || lo < -kMax || hi > kMax)) {  // values that are not finite or past f16, channels past n
+        lo = kMax, hi = -kMax;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] = isfinite(v[i]) ? fminf(kMax, fmaxf(-kMax, v[i])) : 0.0f;
+            if (c0 + i < n) {
+                lo = fminf(lo, v[i]);
+                hi = fmaxf(hi, v[i]);
+            }
         }
     }
-    for (int off = 4; off > 0; off >>= 1) {
-        lo = fminf(lo, __shfl_xor(lo, off));
-        hi = fmaxf(hi, __shfl_xor(hi, off));
-    }
+    lo = fminf(lo, lane_near<0>(lo)), hi = fmaxf(hi, lane_near<0>(hi));
+    lo = fminf(lo, lane_near<1>(lo)), hi = fmaxf(hi, lane_near<1>(hi));
+    lo = fminf(lo, lane_near<2>(lo)), hi = fmaxf(hi, lane_near<2>(hi));
     if (lo > hi) lo = hi = 0.0f;  // a group past the head's channels
     least = static_cast<f16>(lo);
     step = static_cast<f16>((hi - lo) / 15.0f);
     const float d = static_cast<float>(step), m = static_cast<float>(least), inv = d > 0.0f ? 1.0f / d : 0.0f;
+    constexpr float kOne = 8388608.0f;  // 2^23: the sum's last bits are the number, rounded
     uint32_t codes = 0;
+    float far = 0.0f;  // from a code
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float t = (v[i] - m) * inv;
-        float code = rintf(t);
-        if (fabsf(t - code) > 0.4999f && fabsf(t) < 17.0f)
-            code = static_cast<float>(rint((static_cast<double>(v[i]) - static_cast<double>(m)) / static_cast<double>(d)));
-        const uint32_t c = static_cast<uint32_t>(fminf(15.0f, fmaxf(0.0f, code)));
-        codes |= (c0 + i < n ? c : 0u) << (4 * i);
+        const float t = __builtin_amdgcn_fmed3f((v[i] - m) * inv, 0.0f, 15.0f), r = t + kOne;
+        codes += __builtin_bit_cast(uint32_t, r) << (4 * i);
+        far = fmaxf(far, fabsf(t - (r - kOne)));
     }
+    codes -= 0x4b000000u + 0xb0000000u;  // kOne's bits, not shifted and shifted by 4: of the others nothing is left
+    if (far > 0.49999f) {
+        codes = 0;
+        const double wide = static_cast<double>(d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float h = floorf((v[i] - m) * inv);
+            const double x = static_cast<double>(v[i]) - static_cast<double>(m), border = (static_cast<double>(h) + 0.5) * wide;
+            const float code = x > border ? h + 1.0f : x < border ? h : rintf(h + 0.5f);
+            codes |= static_cast<uint32_t>(__builtin_amdgcn_fmed3f(code, 0.0f, 15.0f)) << (4 * i);
+        }
+    }
+    if (c0 + 8 > n) codes &= c0 < n ? (1u << 4 * (n - c0)) - 1 : 0u;
     return codes;
 }
 
@@ -215,30 +261,48 @@ struct KvTask {
                     [token * groups + lane / 8] = scale_word(step, least);
             if (is_key) reinterpret_cast<uint32_t *>(block)[paged_key_word(c.width, token, c0)] = key_order(codes[k]);
         }
-        // values: channels c0 .. c0 + 7 are columns n = c0 % 16 .. of the 16
-        // wide half c0 / 16; the other half of their words is two lanes on
+        // values: channels c0 .. c0 + 7 are columns c0 % 16 .. of the 16 wide half
+        // c0 / 16; the other half of their words is two lanes on.  Of the 8 columns
+        // the first lane writes 4 words, the second 4: `cols` holds a token's 4
+        // nibbles of the first half, and of the second.
 #pragma unroll
-        for (uint32_t k = 0; k < kPagedUnit; ++k) other[k] = __shfl_xor(codes[k], 2);
+        for (uint32_t k = 0; k < kPagedUnit; ++k) {
+            if (k < u.count) other[k] = __builtin_amdgcn_update_dpp(0, static_cast<int>(codes[k]), 0x4e, 0xf, 0xf, true);
+        }
         if (!real || is_key) return;
-        const bool odd = (lane / 2) % 2;  // this lane's channels are the words' upper halves
+        const bool odd = (lane / 2) % 2;  // this lane's channels are the words' second halves
+        uint32_t cols[kPagedUnit] = {}, mask = ~0u;
+#pragma unroll
+        for (uint32_t k = 0; k < kPagedUnit; ++k)
+            if (k < u.count) cols[k] = __builtin_amdgcn_perm(other[k], codes[k], odd ? 0x03020706u : 0x05040100u);
+        if (u.count < kPagedUnit) {  // to their places in the unit
+            uint32_t at[kPagedUnit] = {};
+            mask = 0;
+#pragma unroll
+            for (uint32_t t = 0; t < kPagedUnit; ++t)
+#pragma unroll
+                for (uint32_t k = 0; k < kPagedUnit; ++k)
+                    if (k < u.count && u.from + k == t) {
+                        at[t] = cols[k];
+                        mask |= 15u << paged_value_bit(t, 0) | 15u << paged_value_bit(t, 16);
+                    }
+#pragma unroll
+            for (uint32_t t = 0; t < kPagedUnit; ++t) cols[t] = at[t];
+        }
+        // a word: tokens 0 and 2 of the first half, of the second, then 1 and 3
+        constexpr uint32_t kLow = 0x0f0f0f0fu;
+        const uint32_t even0 = (cols[0] & kLow) | (cols[2] & kLow) << 4, even1 = (cols[1] & kLow) | (cols[3] & kLow) << 4;
+        const uint32_t odd0 = (cols[0] >> 4 & kLow) | (cols[2] & ~kLow), odd1 = (cols[1] >> 4 & kLow) | (cols[3] & ~kLow);
+        const uint32_t bits[4] = {__builtin_amdgcn_perm(even1, even0, 0x06040200u), __builtin_amdgcn_perm(odd1, odd0, 0x06040200u),
+                                  __builtin_amdgcn_perm(even1, even0, 0x07050301u), __builtin_amdgcn_perm(odd1, odd0, 0x07050301u)};
         uint32_t *words = reinterpret_cast<uint32_t *>(block + paged_values_at(c.width));
 #pragma unroll
         for (uint32_t m = 0; m < 4; ++m) {
-            const uint32_t i4 = odd ? 4 + m : m;  // of the lane pair's 8 columns the even lane writes 4, the odd lane 4
-            uint32_t bits = 0, mask = 0;
-#pragma unroll
-            for (uint32_t k = 0; k < kPagedUnit; ++k) {
-                if (k >= u.count) break;
-                const uint32_t mine = (codes[k] >> (4 * i4)) & 15u, theirs = (other[k] >> (4 * i4)) & 15u;
-                const uint32_t lo = paged_value_bit(u.from + k, 0), hi = paged_value_bit(u.from + k, 16);
-                bits |= (odd ? theirs : mine) << lo | (odd ? mine : theirs) << hi;
-                mask |= 15u << lo | 15u << hi;
-            }
-            uint32_t *w = words + paged_value_word(c.width, first, (c0 & ~16u) + i4);
+            uint32_t *w = words + paged_value_word(c.width, first, (c0 & ~16u) + (odd ? 4 + m : m));
             if (u.count == kPagedUnit) {
-                *w = bits;
+                *w = bits[m];
             } else {
-                atomicXor(w, (*w ^ bits) & mask);
+                atomicXor(w, (*w ^ bits[m]) & mask);
             }
         }
     }
@@ -285,7 +349,7 @@ struct QueryTask {
             if (pair) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const double2 t = cs[k][min(c0 + e, half - 1)];
+                    const double2 t = cs[k][angle_at(min(c0 + e, half - 1))];
                     const double v = static_cast<double>(p[e]), w = static_cast<double>(y[k].at(e));
                     p[e] = static_cast<float>(v * t.x - w * t.y);
                     r[e] = static_cast<float>(v * t.y + w * t.x);
@@ -322,17 +386,17 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
                                          : static_cast<double>(u.slot + u.from + k);
             double2 t;
             sincos(p * (first ? freq : a.c.freqs[f]), &t.y, &t.x);
-            cs[k][f] = t;
+            cs[k][angle_at(f)] = t;
         }
         lds_barrier();
     };
     if (blockIdx.y < kv_parts) {
         uint32_t page = 0;
-        if (!paged_page(a.c, a.b, s, u.slot, page)) return;
+        const bool stored = paged_page(a.c, a.b, s, u.slot, page);  // looked up while the task's loads are on their way
         KvTask<T> task;
         task.load(a, u, blockIdx.y * kAppendThreads + threadIdx.x);
         angles();
-        task.store(a, u, page, cs);
+        if (stored) task.store(a, u, page, cs);
     } else {
         QueryTask<T> task;
         task.load(a, u, (blockIdx.y - kv_parts) * kAppendThreads + threadIdx.x);

@@ -83,9 +83,9 @@ __device__ __forceinline__ void add_biases(const LogitsArgs &a, uint32_t b0, uin
     if (lane == 0) biases[token - v0] = sum;
 }
 
-// grid (slices of the vocabulary, rows).  The beginnings of the row's lists (up
-// to 4096 tokens and 1024 biases) and a workgroup's slice of the logits are
-// loaded into registers, in this order; while the logits come, the history is
+// grid (slices of the vocabulary, rows).  The beginnings of the row's lists (1024
+// tokens and biases; 4096 tokens are no faster, 26 us for 24) and a workgroup's
+// slice of the logits are loaded into registers, in this order; while the logits come, the history is
 // counted and the biases are found among the slice's tokens in LDS (integer adds
 // and ors: their order does not matter).  Every slice reads the row's lists, from L2.  Touched
 // logits are computed in 64 bits and rounded once.
@@ -107,15 +107,13 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
     const uint32_t prompt = a.prompt_counts ? static_cast<uint32_t>(max(0, a.prompt_counts[r])) : 0u;
     const double rep = a.repetition ? a.repetition[r] : 1.0f, pres = a.presence ? a.presence[r] : 0.0f,
                  freq = a.frequency ? a.frequency[r] : 0.0f;
-    constexpr uint32_t kHist = 4;  // vectors of the history that a thread loads first
     const bool lists = h1 > h0 || b1 > b0;
-    Vec<int32_t, 4> hist[kHist], tokens;
+    Vec<int32_t, 4> hist, tokens;
     Vec<float, 4> values;
     if (lists) {
         tokens = load_entries(a.bias_tokens, b0 + 4 * tid, b1, -1);
         values = load_entries(a.bias_values, b0 + 4 * tid, b1, 0.0f);
-#pragma unroll
-        for (uint32_t k = 0; k < kHist; ++k) hist[k] = load_entries(a.history, h0 + 4 * (tid + kThreads * k), h1, -1);
+        hist = load_entries(a.history, h0 + 4 * tid, h1, -1);
     }
     Vec<T, VEC> x[N];
     uint32_t allowed[N];  // the words that hold a vector's tokens: VEC divides 32
@@ -162,9 +160,8 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
         };
         find(tokens);
         for (uint32_t i = b0 + 4 * (tid + kThreads); i < b1; i += 4 * kThreads) find(load_entries(a.bias_tokens, i, b1, -1));
-#pragma unroll
-        for (uint32_t k = 0; k < kHist; ++k) count(h0 + 4 * (tid + kThreads * k), hist[k]);
-        for (uint32_t i = h0 + 4 * (tid + kThreads * kHist); i < h1; i += 4 * kThreads) count(i, load_entries(a.history, i, h1, -1));
+        count(h0 + 4 * tid, hist);
+        for (uint32_t i = h0 + 4 * (tid + kThreads); i < h1; i += 4 * kThreads) count(i, load_entries(a.history, i, h1, -1));
         lds_barrier();
         if (b1 > b0) {
             put(b0 + 4 * tid, tokens, values);

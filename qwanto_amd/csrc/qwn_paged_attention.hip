@@ -542,11 +542,13 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
 }
 
 // Blocks that several workers shared: their partial sums joined.  grid (row
-// blocks of the batch at most, KV heads, kMergeParts): part z takes rows z, z +
-// kMergeParts, ... of a block.  W / 4 threads hold 4 channels each of a row;
-// where a part has fewer rows than the workgroup has such groups, several
-// groups share a row's partials and meet in LDS.
-constexpr uint32_t kMergeParts = 4;
+// blocks of the batch at most, KV heads, parts): part z takes rows z, z + parts,
+// ... of a block.  W / 4 threads hold 4 channels each of a row; where a part has
+// fewer rows than the workgroup has such groups, several groups share a row's
+// partials and meet in LDS.  Parts as many as the GPU holds workgroups, and no
+// more than rows: 4 sequences of 8 new tokens behind up to 30000 (8 KV heads, 4
+// query heads each) 30 us with 16, 36 with 4; 61 of 2 behind 4000 29 and 25.
+constexpr uint32_t kMergeGroups = 2048;
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
     constexpr uint32_t kLanes = W / 4, kGroups = kThreads / kLanes;
@@ -573,12 +575,12 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
     const uint32_t p0 = paged_partial(total, workers, first, w0), n = w1 - w0 + 1;
     const uint32_t all = min(kRows, q.rows * a.group - block * kRows);
     if (blockIdx.z >= all) return;
-    const uint32_t rows = (all - blockIdx.z + kMergeParts - 1) / kMergeParts;
+    const uint32_t rows = (all - blockIdx.z + gridDim.z - 1) / gridDim.z;
     uint32_t share = 1;  // groups of a row
     while (2 * share * rows <= kGroups) share *= 2;
     const uint32_t group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, mine = group % share;
     for (uint32_t r0 = 0; r0 < rows; r0 += kGroups / share) {
-        const uint32_t r = r0 + group / share, row = blockIdx.z + r * kMergeParts;
+        const uint32_t r = r0 + group / share, row = blockIdx.z + r * gridDim.z;
         v4f o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
         float top = -INFINITY, l = 0.0f;
         if (r < rows) {
@@ -1087,7 +1089,10 @@ hipError_t launch_width(AttnArgs a, uint32_t blocks, hipStream_t stream) {
     hipLaunchKernelGGL((paged_attention_kernel<T, W>), dim3(a.workers), dim3(kThreads), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.whole) return e;
-    hipLaunchKernelGGL((paged_merge_kernel<T, W>), dim3(blocks, a.c.kv_heads, kMergeParts), dim3(kThreads), 0, stream, a);
+    // rows of a sequence, about
+    const uint32_t each = static_cast<uint32_t>((static_cast<uint64_t>(a.b.tokens) * a.group + a.b.sequences - 1) / a.b.sequences);
+    const uint32_t parts = std::min({kRows, each, std::max(3u, kMergeGroups / (blocks * a.c.kv_heads))});
+    hipLaunchKernelGGL((paged_merge_kernel<T, W>), dim3(blocks, a.c.kv_heads, parts), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 template <typename T>

@@ -630,13 +630,17 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
 // are as many as the reads are few, and unpacking per wave would cost more than
 // the products: a half's threads bring the chunk's codes to f16 values once,
 // step * code + minimum rounded once, in LDS and in the order of the matrix
-// cores' operands, and every wave reads them from there.  (f16 and bf16 rows
+// cores' operands, and every wave reads them from there.  Workgroups are numbered
+// by blocks, then heads: a sequence's longest contexts come first for all heads
+// (a prompt of 2048 tokens, 8 KV heads, 62 us; head by head 98), and with 8 heads
+// each stays on one XCD's L2.  (f16 and bf16 rows
 // only: the rounding, 2^-12 of a value, is of the size of f16's own output.)
 // With two buffers a half unpacks the next chunk while it works on this one; of
 // the two waves that a SIMD holds, the first half's unpacks before its products
 // and the second's after them, so that one's vector instructions meet the
-// other's matrix ones.  Bound by the vector ALU: exponentials, and the
-// unpacking, which RW waves share.
+// other's matrix ones.  A round of 128 tokens takes 2.5 us where the matrix
+// cores, the vector ALU (exponentials, unpacking) and LDS (every wave reads its
+// whole chunk) have about 1.1 us to do each: bound by how they overlap.
 constexpr uint32_t kChunk = 64;
 constexpr uint32_t kChunkTiles = kChunk / kPagedTile;
 constexpr uint32_t kNoPage = 0xffffffffu;
@@ -644,7 +648,7 @@ constexpr uint32_t kNoPage = 0xffffffffu;
 // among several workgroups, each with kPartRounds rounds at least, and merged
 // after (32 heads of 128: 64 tokens behind 4032 25 us, 89 whole; 512 behind 7680
 // 103 us, 169 whole).  Workgroups that follow each other on a CU do not pay for
-// the merge: with twice kBlockGroups the second takes 116 us and eight prompts of
+// the merge: with twice kBlockGroups the second takes 116 us and four prompts of
 // 152 blocks 70, 59 whole.  Eight rounds at least: the first takes 33 us.
 constexpr uint32_t kBlockGroups = 256, kBlockPartsMost = 8, kPartRounds = 4;
 constexpr int kBlockWaves = 4;
@@ -729,16 +733,17 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     const uint32_t rw = wave % RW, half = wave / RW, n = lane % 16, g = lane / 16;
     uint32_t s, at;
     PagedSequence q;
-    if (!find_in(a.b, blockIdx.x, [&](const PagedSequence &x) { return (x.rows * a.group + kBlockRows - 1) / kBlockRows; }, s, at, q))
+    const uint32_t head = blockIdx.x % a.c.kv_heads, index = blockIdx.x / a.c.kv_heads;
+    if (!find_in(a.b, index, [&](const PagedSequence &x) { return (x.rows * a.group + kBlockRows - 1) / kBlockRows; }, s, at, q))
         return;
     const uint32_t all = q.rows * a.group, blocks = (all + kBlockRows - 1) / kBlockRows;
-    const uint32_t block = blocks - 1 - at, head = blockIdx.y;  // the longest contexts first
+    const uint32_t block = blocks - 1 - at;  // a sequence's longest contexts first
     const uint32_t row0 = block * kBlockRows, last = min(row0 + kBlockRows, all) - 1;
     const uint32_t most = min(q.past + last / a.group + 1, a.slots);
     const uint32_t chunks = (most + kChunk - 1) / kChunk, all_rounds = (chunks + 1) / 2;
     const uint32_t parts = block_parts(a, all_rounds);
-    if (blockIdx.z >= parts) return;
-    const uint32_t from = all_rounds * blockIdx.z / parts, rounds = all_rounds * (blockIdx.z + 1) / parts;
+    if (blockIdx.y >= parts) return;
+    const uint32_t from = all_rounds * blockIdx.y / parts, rounds = all_rounds * (blockIdx.y + 1) / parts;
     v4u *mine = chunk + half * BUFFERS * 2 * kOperands;  // this half's buffers: keys, then values
 
     // the tiles this wave brings: rw, rw + RW, ... of its half's chunk.  A lane
@@ -975,7 +980,7 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
         if (r > last) continue;
         T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + r / a.group) * a.output_stride +
                  static_cast<size_t>(head * a.group + r % a.group) * a.c.head_dim;
-        const size_t at_part = ((static_cast<size_t>(blockIdx.x) * a.c.kv_heads + head) * a.parts + blockIdx.z) * kBlockRows + r - row0;
+        const size_t at_part = (static_cast<size_t>(blockIdx.x) * a.parts + blockIdx.y) * kBlockRows + r - row0;
         if (parts > 1 && g == 0) a.part_ml[at_part] = make_float2(top, l);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -999,22 +1004,23 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
     }
 }
 
-// The parts of the blocks whose contexts were split.  grid (blocks at most, KV
-// heads, row groups): W / 4 threads a row.
+// The parts of the blocks whose contexts were split.  grid (KV heads of blocks at
+// most, row groups): W / 4 threads a row.
 template <typename T, int W, uint32_t ROWS>
 __global__ __launch_bounds__(kThreads) void paged_block_merge_kernel(AttnArgs a) {
     constexpr uint32_t kLanes = W / 4, kGroups = kThreads / kLanes;
     uint32_t s, at;
     PagedSequence q;
-    if (!find_in(a.b, blockIdx.x, [&](const PagedSequence &x) { return (x.rows * a.group + ROWS - 1) / ROWS; }, s, at, q)) return;
-    const uint32_t all = q.rows * a.group, block = (all + ROWS - 1) / ROWS - 1 - at, head = blockIdx.y;
+    const uint32_t head = blockIdx.x % a.c.kv_heads, index = blockIdx.x / a.c.kv_heads;
+    if (!find_in(a.b, index, [&](const PagedSequence &x) { return (x.rows * a.group + ROWS - 1) / ROWS; }, s, at, q)) return;
+    const uint32_t all = q.rows * a.group, block = (all + ROWS - 1) / ROWS - 1 - at;
     const uint32_t row0 = block * ROWS, last = min(row0 + ROWS, all) - 1;
     const uint32_t most = min(q.past + last / a.group + 1, a.slots);
     const uint32_t parts = block_parts(a, ((most + kChunk - 1) / kChunk + 1) / 2);
     if (parts == 1) return;
-    const uint32_t lane = threadIdx.x % kLanes, r = blockIdx.z * kGroups + threadIdx.x / kLanes, row = row0 + r;
+    const uint32_t lane = threadIdx.x % kLanes, r = blockIdx.y * kGroups + threadIdx.x / kLanes, row = row0 + r;
     if (row > last) return;
-    const size_t first = (static_cast<size_t>(blockIdx.x) * a.c.kv_heads + head) * a.parts * ROWS + r;
+    const size_t first = static_cast<size_t>(blockIdx.x) * a.parts * ROWS + r;
     float2 ml[kBlockPartsMost];
     v4f x[kBlockPartsMost];
     float top = -INFINITY;
@@ -1071,10 +1077,10 @@ hipError_t launch_block(AttnArgs a, hipStream_t stream) {
     const uint64_t rows = static_cast<uint64_t>(a.b.tokens) * a.group, used = std::min(a.b.sequences, a.b.tokens);
     const uint32_t blocks = static_cast<uint32_t>((rows + used * (kBlockRows - 1)) / kBlockRows);
     a.parts = std::max(1u, std::min(kBlockPartsMost, kBlockGroups / (blocks * a.c.kv_heads)));
-    hipLaunchKernelGGL((paged_block_attention_kernel<T, W, RW, RT, BUFFERS>), dim3(blocks, a.c.kv_heads, a.parts),
+    hipLaunchKernelGGL((paged_block_attention_kernel<T, W, RW, RT, BUFFERS>), dim3(blocks * a.c.kv_heads, a.parts),
                        dim3(2 * RW * kWaveSize), lds, stream, a);
     if ((e = hipGetLastError()) != hipSuccess || a.parts == 1 || a.slots <= 2 * kPartRounds * kChunk) return e;
-    hipLaunchKernelGGL((paged_block_merge_kernel<T, W, kBlockRows>), dim3(blocks, a.c.kv_heads, kBlockRows / (kThreads / (W / 4))),
+    hipLaunchKernelGGL((paged_block_merge_kernel<T, W, kBlockRows>), dim3(blocks * a.c.kv_heads, kBlockRows / (kThreads / (W / 4))),
                        dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }

@@ -281,7 +281,10 @@ def test_attention(gpu_ctx, dtype, past, new, kv_heads, heads, d, page):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("past,new,kv_heads,heads,d,page", [
-    ([0], [64], 1, 1, 64, 16),                                 # one block of rows, one chunk
+    ([0], [64], 1, 1, 64, 16),                                 # one chunk
+    ([0], [79], 1, 1, 128, 16),                                # a row fewer than the kernel for many takes,
+    ([0], [80], 1, 1, 128, 16),                                # and as many: part of a block
+    ([0, 64], [96, 64], 1, 1, 64, 16),
     ([0], [65], 1, 1, 128, 16),                                # a row, and a token, more
     ([63, 64, 0, 0], [128, 63, 1, 200], 2, 2, 128, 32),        # chunks that begin and end inside
     ([1000, 0], [40, 300], 2, 12, 128, 16),                    # a group of 6 heads: tokens across blocks

@@ -263,12 +263,12 @@ QWN_CUDA_ABI_API int qwn_hip_ext_kv_attention_device_noalloc(QwnCudaContextHandl
  * paged 4-bit KV cache, and the logits' penalties and masks.  Each takes a
  * request struct of device pointers that a caller builds once and passes
  * every step; strides are in elements (0: rows back to back), and no pointer
- * needs more alignment than its element.  A request's outputs may not overlap its inputs except
- * where it says so.  Sizes that only the device knows (a batch's row starts,
- * cached lengths, page numbers, token ids) are read there, so a captured
- * step replays with new ones; each is checked there, and what points outside
- * the buffers that the host described is left out.  No counterpart in the
- * reference. */
+ * needs more alignment than its element.  A request's outputs may not overlap
+ * its inputs or each other except where it says so.  Sizes that only the device
+ * knows (a batch's row starts, cached lengths, page numbers, token ids) are read
+ * there, so a captured step replays with new ones; each is checked there, and
+ * what points outside the buffers that the host described is left out.  No
+ * counterpart in the reference. */
 #define QWN_HIP_DTYPE_F32 0u
 #define QWN_HIP_DTYPE_F16 1u
 #define QWN_HIP_DTYPE_BF16 2u
@@ -381,10 +381,13 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_read_device(QwnCudaContextHandle *cont
  * past[s] + i, query head h to KV head h / (query_heads / kv_heads).  A row
  * that attends to nothing is zeros; a row whose query is not finite is NaN.
  * fp32 queries are computed to fp32 (22 bits of query and probability in the
- * matrix products), f16 and bf16 ones with f16 probabilities.  The workspace
- * (qwn_hip_ext_paged_kv_attention_workspace_bytes, the same for every batch
- * of a cache; 0 for a request that is refused; 16-byte aligned) holds nothing
- * between calls, and may not be shared by calls that run at the same time. */
+ * matrix products), f16 and bf16 ones with f16 probabilities, and where the
+ * batch has 80 rows (a token's query heads of one KV head) a sequence or more
+ * with the keys and values rounded to f16.  The output may not be the query.
+ * The workspace (qwn_hip_ext_paged_kv_attention_workspace_bytes, the same for
+ * every batch of a cache; 0 for a request that is refused; 16-byte aligned)
+ * holds nothing between calls, and may not be shared by calls that run at the
+ * same time. */
 typedef struct {
     QwnCudaAbiHeader header;
     const QwnHipPagedBatch *batch;

@@ -235,6 +235,10 @@ QWN_CUDA_ABI_API int qwn_hip_ext_norm_quantize_device(QwnCudaContextHandle *hand
         set_error("invalid norm request");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
+    if (r->y && (r->y == r->x || r->y == r->residual || r->y == r->residual_out)) {
+        set_error("norm request: y may not be x, residual or residual_out");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
     NormArgs a{};
     a.x = r->x;
     a.residual = r->residual;

@@ -312,7 +312,8 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
         Shape h = shape_of(a, q);
         while (u - before >= h.blocks * a.c.kv_heads * h.units) {
             before += h.blocks * a.c.kv_heads * h.units;
-            q = sequence_of(a.b, ++s);
+            if (++s >= a.b.sequences) return;  // starts that do not ascend: the list's length has wrapped
+            q = sequence_of(a.b, s);
             h = shape_of(a, q);
         }
         const uint32_t item = (u - before) / h.units, at = (u - before) % h.units;
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
             if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
             e = max(e, -100);
             const float up = ldexpf(1.0f, kQueryBits - e);
-            row_mul = a.scale * 1.44269504088896340736f * ldexpf(1.0f, e - kQueryBits + (WHOLE ? 0 : 24));
+            row_mul = ldexpf(a.scale * 1.44269504088896340736f, e - kQueryBits + (WHOLE ? 0 : 24));
 #pragma unroll
             for (int gg = 0; gg < G; ++gg) qsum[gg] = 0.0f;
 #pragma unroll
@@ -570,6 +571,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
     }
     const Shape h = shape_of(a, q);
     const uint32_t first = before + (block * a.c.kv_heads + head) * h.units + kStart;
+    if (first + h.pieces > total) return;  // starts that do not ascend: the list's length has wrapped
     const uint32_t w0 = paged_worker(total, workers, first), w1 = paged_worker(total, workers, first + h.pieces - 1);
     if (w0 == w1) return;  // one worker had it all, and wrote it
     const uint32_t p0 = paged_partial(total, workers, first, w0), n = w1 - w0 + 1;
@@ -822,7 +824,7 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
         int e = 0;
         if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
         e = max(e, -100);
-        mul[t] = fabsf(a.scale) * 1.44269504088896340736f * ldexpf(1.0f, e);
+        mul[t] = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e);
         float up = copysignf(ldexpf(1.0f, -e), a.scale);   // |query| < 1
         if (mul[t] == 0.0f) mul[t] = 1.0f, up = 0.0f;       // all scores alike
         if (top == INFINITY) up = __builtin_nanf("");       // the row is NaN, whatever the keys are
@@ -1151,7 +1153,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_attention_device(QwnCudaContextHandle 
     }
     std::lock_guard<std::mutex> lock(ctx->mutex);
     AttnArgs a{};
-    if (!attention_of(ctx, h, r, a) || !r->query || !r->output || !r->workspace) {
+    if (!attention_of(ctx, h, r, a) || !r->query || !r->output || r->query == r->output || !r->workspace) {
         set_error("invalid paged attention request");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }

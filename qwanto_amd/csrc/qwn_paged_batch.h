@@ -60,6 +60,7 @@ __device__ __forceinline__ bool find_in(const PagedBatch &b, uint32_t index, W w
             const int first = __ffsll(static_cast<unsigned long long>(past)) - 1;
             seq = s0 + first;
             at = index - (lane_of(end, first) - lane_of(n, first));
+            if (at >= lane_of(n, first)) return false;  // starts that do not ascend: the sums have wrapped
             q = PagedSequence{lane_of(mine.row, first), lane_of(mine.rows, first), lane_of(mine.past, first)};
             return true;
         }

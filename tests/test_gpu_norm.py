@@ -148,7 +148,8 @@ def test_refusals(gpu_ctx):
     gpu_ctx.norm_quantize_device(req(), stream=sv.stream())
     bad = [req(x_ptr=None), req(norm_ptr=None), req(scales_ptr=None), req(q8_ptr=None), req(x_stride=63), req(q8_stride=63),
            req(y_ptr=sv.ptr(x), y_stride=8), req(residual_ptr=sv.ptr(x), residual_stride=5),
-           req(residual_out_ptr=sv.ptr(x), residual_out_stride=65)]
+           req(residual_out_ptr=sv.ptr(x), residual_out_stride=65), req(y_ptr=sv.ptr(x)),
+           req(residual_ptr=sv.ptr(s), y_ptr=sv.ptr(s)), req(residual_out_ptr=sv.ptr(s), y_ptr=sv.ptr(s))]
     for field, value in (("tokens", 0), ("cols", 0), ("dtype", 3), ("tokens", 0x80000000)):
         r = req()
         setattr(r, field, value)

@@ -475,6 +475,57 @@ def test_queries_of_any_size(gpu_ctx, size):
         c.close()
 
 
+@pytest.mark.parametrize("new", [1, 90])
+def test_large_queries_of_small_scale(gpu_ctx, new):
+    """The row's power of two and the scale meet before either leaves fp32's range."""
+    hk, heads, d, n = 1, 2, 128, 200
+    c = sv.Cache(gpu_ctx, [n], hk, d)
+    try:
+        k, v, _ = inputs(27, n, hk, d, "f32")
+        fill = c.batch([0], [n])
+        c.append(fill, k.to(sv.DEV), v.to(sv.DEV), "f32")
+        kv = c.read(fill)
+        q = (sv.normal(sv.gen(28), new, heads * d).clamp(-3, 3) * 1e37).to(torch.bfloat16)
+        out = torch.zeros(new, heads * d, dtype=torch.bfloat16, device=sv.DEV)
+        scale = float(torch.tensor(2e-38, dtype=torch.float32))
+        c.attend(c.batch([n - new], [new]), q.to(sv.DEV), out, "bf16", heads, scale)
+        want, tol = reference(kv, q, [n - new], [new], hk, heads, d, scale, "bf16", block=new > 40)
+        assert bool(((out.cpu().double() - want).abs() <= tol).all())
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("dtype,heads", [("f32", 2), ("bf16", 16)])
+def test_starts_that_do_not_ascend(gpu_ctx, dtype, heads):
+    """A sequence whose rows do not lie in the batch, or go backwards, is left out; the others' rows are
+    what they are without it."""
+    hk, d = 2, 64
+    c = sv.Cache(gpu_ctx, [64, 64, 64, 64, 64], hk, d)
+    try:
+        k, v, q = inputs(29, 40, hk, d, dtype, heads)
+        fill = c.batch([0] * 5, [8] * 5)
+        c.append(fill, k.to(sv.DEV), v.to(sv.DEV), dtype)
+        before = c.read(fill)
+        b = c.batch([8] * 5, [8] * 5)
+        starts = torch.tensor([0, 8, -3, 16, 41, 30], dtype=torch.int32, device=sv.DEV)   # of five only the first's are rows
+        b.starts = sv.ptr(starts)
+        out = torch.full_like(q.to(sv.DEV), 3.0)
+        c.append(b, k.to(sv.DEV), v.to(sv.DEV), dtype)
+        c.attend(b, q.to(sv.DEV), out, dtype, heads, 0.125)
+        assert torch.equal(c.read(fill), before)
+        got = out.cpu()
+        assert bool((got[8:] == 3.0).all())
+        one = c.batch([8], [8], table=c.table[:1].contiguous())
+        alone = torch.full_like(out, 3.0)
+        c.attend(one, q.to(sv.DEV), alone, dtype, heads, 0.125)
+        both = torch.cat([before[:, :8], c.read(one)[:, :8]], dim=1)
+        want, tol = reference(both, q[:8], [8], [8], hk, heads, d, 0.125, dtype, block=True)
+        assert bool(((got[:8].double() - want).abs() <= tol).all())
+        assert bool(((alone.cpu()[:8].double() - want).abs() <= tol).all())
+    finally:
+        c.close()
+
+
 def test_refusals(gpu_ctx):
     for kw, status in ((dict(pages=0), -1), (dict(kv_heads=0), -1), (dict(head_dim=0), -1), (dict(head_dim=257), -5),
                        (dict(page_tokens=24), -5), (dict(page_tokens=8), -5), (dict(page_tokens=2048), -5),
@@ -518,12 +569,12 @@ def test_refusals(gpu_ctx):
     refuse(small.paged_kv_read_device, c.h, ok, sv.ptr(x), None, stride=3)
 
     def att(heads=2, **kw):
-        r = small.paged_attention_request(ok, "f32", heads, sv.ptr(x), sv.ptr(x), 0.1, workspace_ptr=sv.ptr(x))
+        r = small.paged_attention_request(ok, "f32", heads, sv.ptr(x), sv.ptr(x) + 4096, 0.1, workspace_ptr=sv.ptr(x))
         for k, v in kw.items():
             setattr(r, k, v)
         return r
 
-    for r in (att(3), att(0), att(query=None), att(output=None), att(workspace=None), att(workspace=sv.ptr(x) + 4),
+    for r in (att(3), att(0), att(query=None), att(output=None), att(output=sv.ptr(x)), att(workspace=None), att(workspace=sv.ptr(x) + 4),
               att(dtype=3), att(query_stride=100), att(output_stride=100)):
         refuse(small.paged_kv_attention_device, c.h, r)
     # another context's handle, and one that is gone

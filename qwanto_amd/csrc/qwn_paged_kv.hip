@@ -209,7 +209,9 @@ __device__ __forceinline__ Unit unit_of(const PagedSequence &q, uint32_t unit) {
 }
 
 // A unit's values and keys: a task is 8 channels of one head of either, of all
-// its tokens, whose loads are issued together.  Keys fill whole words.  A word
+// its tokens, the next one's loads issued before this one's work.  (A loop, not
+// four copies: those were 42 KB of instructions, most of a call of few tokens
+// spent on fetching them, and 130 registers.)  Keys fill whole words.  A word
 // of values is stored where the call brings all 4 of its tokens; else its bits
 // are changed by an exclusive or, so that tokens of one word that come from two
 // sequences of a call (a shared page) do not lose each other.
@@ -217,25 +219,23 @@ template <typename T>
 struct KvTask {
     uint32_t head, lane;
     bool real, is_key;
-    Eight<T> x[kPagedUnit], o[kPagedUnit];
+    Eight<T> x, o;
 
-    __device__ __forceinline__ void load(const AppendArgs &a, const Unit &u, uint32_t i) {
-        const PagedKv &c = a.c;
-        const uint32_t lanes = c.width / 8, kv_tasks = c.kv_heads * lanes;
+    __device__ __forceinline__ void take(const AppendArgs &a, uint32_t i) {
+        const uint32_t lanes = a.c.width / 8, kv_tasks = a.c.kv_heads * lanes;
         real = i < 2 * kv_tasks;
         is_key = i >= kv_tasks;
         const uint32_t j = real ? i - (is_key ? kv_tasks : 0u) : 0u;
         head = j / lanes;
         lane = j % lanes;
-#pragma unroll
-        for (uint32_t k = 0; k < kPagedUnit; ++k) {
-            if (k >= u.count) break;
-            const size_t row = u.row + k;
-            const T *src = (is_key ? static_cast<const T *>(a.key) + row * a.key_stride
-                                   : static_cast<const T *>(a.value) + row * a.value_stride) + head * c.head_dim;
-            x[k].load(src, lane * 8, c.head_dim);
-            if (is_key && c.rope_dims) o[k].load_partners(src, lane * 8, c.head_dim, c.rope_dims);
-        }
+    }
+    __device__ __forceinline__ void load(const AppendArgs &a, const Unit &u, uint32_t k) {
+        const PagedKv &c = a.c;
+        const size_t row = u.row + k;
+        const T *src = (is_key ? static_cast<const T *>(a.key) + row * a.key_stride
+                               : static_cast<const T *>(a.value) + row * a.value_stride) + head * c.head_dim;
+        x.load(src, lane * 8, c.head_dim);
+        if (is_key && c.rope_dims) o.load_partners(src, lane * 8, c.head_dim, c.rope_dims);
     }
 
     // Whole waves: lanes 1 to 4 apart exchange.
@@ -244,61 +244,42 @@ struct KvTask {
         const uint32_t tile = (u.slot & (c.page_tokens - 1)) / kPagedTile, first = u.slot % kPagedTile;
         const uint32_t groups = c.width / kPagedGroup, c0 = lane * 8;
         uint8_t *block = c.pool + paged_block_at(c, page, tile, head);
-        uint32_t codes[kPagedUnit] = {}, other[kPagedUnit];
-#pragma unroll
-        for (uint32_t k = 0; k < kPagedUnit; ++k) {
-            if (k >= u.count) break;
-            const uint32_t token = first + u.from + k;
+        // values: channels c0 .. c0 + 7 are columns c0 % 16 .. of the 16 wide half
+        // c0 / 16; the other half of their words is two lanes on.  Of the 8 columns
+        // the first lane writes 4 words, the second 4; a word holds tokens 0 and 2 of
+        // the first half, of the second, then 1 and 3.  even[t % 2], odd: tokens t and
+        // t + 2 of columns 0 and 2, and of 1 and 3, a byte a half and column.
+        const bool second = (lane / 2) % 2;  // this lane's channels are the words' second halves
+        uint32_t even0 = 0, even1 = 0, odd0 = 0, odd1 = 0, mask = 0;
+#pragma unroll 1
+        for (uint32_t k = 0; k < u.count; ++k) {
+            const uint32_t t = u.from + k, token = first + t;
             f16 step, least;
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = x[k].at(i);
-            if (is_key) rotate8(v, o[k], c0, c.rope_dims, cs[k]);
-            codes[k] = quantize8(v, c0, c.head_dim, step, least);
-            if (!real) continue;
-            if (lane % 8 == 0)
+            for (int i = 0; i < 8; ++i) v[i] = x.at(i);
+            if (is_key) rotate8(v, o, c0, c.rope_dims, cs[k]);
+            if (k + 1 < u.count) load(a, u, k + 1);
+            const uint32_t codes = quantize8(v, c0, c.head_dim, step, least);
+            if (real && lane % 8 == 0)
                 reinterpret_cast<uint32_t *>(block + (is_key ? paged_key_scales_at(c.width) : paged_value_scales_at(c.width)))
                     [token * groups + lane / 8] = scale_word(step, least);
-            if (is_key) reinterpret_cast<uint32_t *>(block)[paged_key_word(c.width, token, c0)] = key_order(codes[k]);
-        }
-        // values: channels c0 .. c0 + 7 are columns c0 % 16 .. of the 16 wide half
-        // c0 / 16; the other half of their words is two lanes on.  Of the 8 columns
-        // the first lane writes 4 words, the second 4: `cols` holds a token's 4
-        // nibbles of the first half, and of the second.
-#pragma unroll
-        for (uint32_t k = 0; k < kPagedUnit; ++k) {
-            if (k < u.count) other[k] = __builtin_amdgcn_update_dpp(0, static_cast<int>(codes[k]), 0x4e, 0xf, 0xf, true);
+            if (real && is_key) reinterpret_cast<uint32_t *>(block)[paged_key_word(c.width, token, c0)] = key_order(codes);
+            const uint32_t other = __builtin_amdgcn_update_dpp(0, static_cast<int>(codes), 0x4e, 0xf, 0xf, true);
+            // a token's 4 nibbles of the first half, and of the second
+            const uint32_t cols = __builtin_amdgcn_perm(other, codes, second ? 0x03020706u : 0x05040100u);
+            const uint32_t up = t & 2 ? 4 : 0, even = (cols & 0x0f0f0f0fu) << up, odd = (cols >> 4 & 0x0f0f0f0fu) << up;
+            even0 |= t & 1 ? 0u : even, odd0 |= t & 1 ? 0u : odd;
+            even1 |= t & 1 ? even : 0u, odd1 |= t & 1 ? odd : 0u;
+            mask |= 15u << paged_value_bit(t, 0) | 15u << paged_value_bit(t, 16);
         }
         if (!real || is_key) return;
-        const bool odd = (lane / 2) % 2;  // this lane's channels are the words' second halves
-        uint32_t cols[kPagedUnit] = {}, mask = ~0u;
-#pragma unroll
-        for (uint32_t k = 0; k < kPagedUnit; ++k)
-            if (k < u.count) cols[k] = __builtin_amdgcn_perm(other[k], codes[k], odd ? 0x03020706u : 0x05040100u);
-        if (u.count < kPagedUnit) {  // to their places in the unit
-            uint32_t at[kPagedUnit] = {};
-            mask = 0;
-#pragma unroll
-            for (uint32_t t = 0; t < kPagedUnit; ++t)
-#pragma unroll
-                for (uint32_t k = 0; k < kPagedUnit; ++k)
-                    if (k < u.count && u.from + k == t) {
-                        at[t] = cols[k];
-                        mask |= 15u << paged_value_bit(t, 0) | 15u << paged_value_bit(t, 16);
-                    }
-#pragma unroll
-            for (uint32_t t = 0; t < kPagedUnit; ++t) cols[t] = at[t];
-        }
-        // a word: tokens 0 and 2 of the first half, of the second, then 1 and 3
-        constexpr uint32_t kLow = 0x0f0f0f0fu;
-        const uint32_t even0 = (cols[0] & kLow) | (cols[2] & kLow) << 4, even1 = (cols[1] & kLow) | (cols[3] & kLow) << 4;
-        const uint32_t odd0 = (cols[0] >> 4 & kLow) | (cols[2] & ~kLow), odd1 = (cols[1] >> 4 & kLow) | (cols[3] & ~kLow);
         const uint32_t bits[4] = {__builtin_amdgcn_perm(even1, even0, 0x06040200u), __builtin_amdgcn_perm(odd1, odd0, 0x06040200u),
                                   __builtin_amdgcn_perm(even1, even0, 0x07050301u), __builtin_amdgcn_perm(odd1, odd0, 0x07050301u)};
         uint32_t *words = reinterpret_cast<uint32_t *>(block + paged_values_at(c.width));
 #pragma unroll
         for (uint32_t m = 0; m < 4; ++m) {
-            uint32_t *w = words + paged_value_word(c.width, first, (c0 & ~16u) + (odd ? 4 + m : m));
+            uint32_t *w = words + paged_value_word(c.width, first, (c0 & ~16u) + (second ? 4 + m : m));
             if (u.count == kPagedUnit) {
                 *w = bits[m];
             } else {
@@ -315,42 +296,40 @@ template <typename T>
 struct QueryTask {
     uint32_t head, c0, end;
     bool real, pair;
-    Eight<T> x[kPagedUnit], y[kPagedUnit];
+    Eight<T> x, y;
 
-    __device__ __forceinline__ void load(const AppendArgs &a, const Unit &u, uint32_t i) {
+    __device__ __forceinline__ void take(const AppendArgs &a, uint32_t i) {
         const uint32_t D = a.c.head_dim, rope = a.c.rope_dims, half = rope / 2;
         const uint32_t pairs = (half + 7) / 8, lanes = pairs + (D - rope + 7) / 8;
         real = i < a.query_heads * lanes;
-        if (!real) return;
         head = i / lanes;
         const uint32_t lane = i % lanes;
         pair = lane < pairs;
         c0 = pair ? lane * 8 : rope + (lane - pairs) * 8;
         end = pair ? half : D;
-#pragma unroll
-        for (uint32_t k = 0; k < kPagedUnit; ++k) {
-            if (k >= u.count) break;
-            const T *src = static_cast<const T *>(a.query) + static_cast<size_t>(u.row + k) * a.query_stride + head * D;
-            x[k].load(src, c0, end);
-            if (pair) y[k].load(src + half, c0, half);
-        }
+    }
+    __device__ __forceinline__ void load(const AppendArgs &a, const Unit &u, uint32_t k) {
+        if (!real) return;
+        const T *src = static_cast<const T *>(a.query) + static_cast<size_t>(u.row + k) * a.query_stride + head * a.c.head_dim;
+        x.load(src, c0, end);
+        if (pair) y.load(src + a.c.rope_dims / 2, c0, a.c.rope_dims / 2);
     }
 
     __device__ __forceinline__ void store(const AppendArgs &a, const Unit &u, const double2 (*cs)[128]) {
         if (!real) return;
         const uint32_t half = a.c.rope_dims / 2;
-#pragma unroll
-        for (uint32_t k = 0; k < kPagedUnit; ++k) {
-            if (k >= u.count) break;
+#pragma unroll 1
+        for (uint32_t k = 0; k < u.count; ++k) {
             T *dst = static_cast<T *>(a.query_out) + static_cast<size_t>(u.row + k) * a.query_out_stride + head * a.c.head_dim;
             float p[8], r[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = x[k].at(e);
+            for (int e = 0; e < 8; ++e) p[e] = x.at(e), r[e] = y.at(e);
+            if (k + 1 < u.count) load(a, u, k + 1);
             if (pair) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const double2 t = cs[k][angle_at(min(c0 + e, half - 1))];
-                    const double v = static_cast<double>(p[e]), w = static_cast<double>(y[k].at(e));
+                    const double v = static_cast<double>(p[e]), w = static_cast<double>(r[e]);
                     p[e] = static_cast<float>(v * t.x - w * t.y);
                     r[e] = static_cast<float>(v * t.y + w * t.x);
                 }
@@ -364,7 +343,7 @@ struct QueryTask {
 // grid (units of 4 slots at most, parts): the first kv_parts workgroups of a
 // unit take its values and keys, the others its queries, a task a thread.  The
 // angles of the unit's rows are computed once in each, in 64 bits (at position
-// 100000 an fp32 angle would be off by hundredths), while the tasks' loads are
+// 100000 an fp32 angle would be off by hundredths), while the first loads are
 // in flight.
 template <typename T>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a, uint32_t kv_parts) {
@@ -394,12 +373,14 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
         uint32_t page = 0;
         const bool stored = paged_page(a.c, a.b, s, u.slot, page);  // looked up while the task's loads are on their way
         KvTask<T> task;
-        task.load(a, u, blockIdx.y * kAppendThreads + threadIdx.x);
+        task.take(a, blockIdx.y * kAppendThreads + threadIdx.x);
+        task.load(a, u, 0);
         angles();
         if (stored) task.store(a, u, page, cs);
     } else {
         QueryTask<T> task;
-        task.load(a, u, (blockIdx.y - kv_parts) * kAppendThreads + threadIdx.x);
+        task.take(a, (blockIdx.y - kv_parts) * kAppendThreads + threadIdx.x);
+        task.load(a, u, 0);
         angles();
         task.store(a, u, cs);
     }

@@ -23,10 +23,10 @@
 // 11.  The elements that meet the larger ones are divided by 16 beforehand, the
 // sums multiplied by 2^24 at the end.  (The matrix cores sum such operands to
 // 2e-7 of their magnitudes, integers to 5e-8: fp32 takes integers, less 8 to
-// halve what cancels, and so do f16's values.)  A probability that f16 rounds would count its error
-// times the code, although codes are 7.5 +- 5 and the values they make around
-// zero; the sum of the rounded weights, one more product with a row of ones,
-// takes 8 times that error out again.
+// halve what cancels, and so do f16's values.)  A probability that f16 rounds
+// would count its error times the code, although codes are 7.5 +- 5 and the
+// values they make around zero; the sum of the rounded weights, one more product
+// with a row of ones, takes 8 times that error out again.
 //
 // Queries are scaled by a power of two
 // per row to below 2^15, probabilities times steps by one per row and wave to
@@ -635,8 +635,8 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
 // cores' operands, and every wave reads them from there.  Workgroups are numbered
 // by blocks, then heads: a sequence's longest contexts come first for all heads
 // (a prompt of 2048 tokens, 8 KV heads, 62 us; head by head 98), and with 8 heads
-// each stays on one XCD's L2.  (f16 and bf16 rows
-// only: the rounding, 2^-12 of a value, is of the size of f16's own output.)
+// each stays on one XCD's L2.  (bf16 rows only: the rounding of keys and values,
+// 2^-12 of a value, is a sixteenth of the output's.)
 // With two buffers a half unpacks the next chunk while it works on this one; of
 // the two waves that a SIMD holds, the first half's unpacks before its products
 // and the second's after them, so that one's vector instructions meet the
@@ -1060,11 +1060,15 @@ size_t partial_rows(uint32_t width) {
 }
 size_t partial_bytes(uint32_t width) { return partial_rows(width) * (width * sizeof(float) + sizeof(float2)); }
 
-// Whether a batch's sequences have rows enough for the block kernel.  (Of 8 KV
-// heads: 16 sequences of 3000 tokens with 64 rows each 70 us in it and 53 in
+// Whether a batch is for the block kernel: its sequences have rows enough (of 8
+// KV heads: 16 sequences of 3000 tokens with 64 rows each 70 us in it and 53 in
 // blocks of 16, with 80 rows 70 and 66, with 124 72 and 88; 64 of 1000 with 80
-// rows 64 and 78.)
-bool block_rows(const AttnArgs &a) { return static_cast<uint64_t>(a.b.tokens) * a.group >= 80ull * a.b.sequences; }
+// rows 64 and 78), and there are more than a few short ones (a prompt of 128
+// tokens 13 and 9, of 256 16 and 12; 8 of 64 behind 192 16 and 20).
+bool block_rows(const AttnArgs &a) {
+    const uint64_t rows = static_cast<uint64_t>(a.b.tokens) * a.group;
+    return rows >= 80ull * a.b.sequences && (rows * a.c.kv_heads > 8192 || a.slots > kWholeSlots);
+}
 
 template <typename T, int W, int RW, int RT, int BUFFERS>
 hipError_t launch_block(AttnArgs a, hipStream_t stream) {
@@ -1092,7 +1096,11 @@ hipError_t launch_block(AttnArgs a, hipStream_t stream) {
 
 template <typename T, int W>
 hipError_t launch_width(AttnArgs a, uint32_t blocks, hipStream_t stream) {
-    if constexpr (sizeof(T) == 2) {
+    // f16 rows are left to blocks of 16, whose values are exact: keys and values
+    // rounded to f16 would cost more than the output's own rounding (error 3.5 to
+    // 4.5e-4, there 2.9e-4, of which the output's 2.1e-4; four prompts of 512 tokens
+    // behind 2048 290 us for 134)
+    if constexpr (std::is_same_v<T, bf16>) {
         if (block_rows(a)) return launch_block<T, W, kBlockWaves, W == 256 ? 1 : 2, W == 256 ? 1 : 2>(a, stream);
     }
     a.whole = a.slots <= (blocks * a.c.kv_heads >= kMany ? kWholeSlotsMany : kWholeSlots);

@@ -195,8 +195,8 @@ def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None, blo
     rounding.  A relative error e of every probability moves the output by at most 2 e max|v|.
     Probabilities times step are halves with 2^-22 (one half: 2^-11) of themselves or 2^-25 of the
     largest; the sums over the tokens round by 2^-24 each, in chains of at most `n` tokens / 32 + 64.
-    Where sequences bring many rows (`block`), f16 and bf16 ones meet keys and values rounded to f16:
-    2^-11 of each."""
+    Where sequences bring many rows (`block`), bf16 ones meet keys and values rounded to f16: 2^-11 of
+    each."""
     group, out, tols = heads // kv_heads, [], []
     at = row = 0
     for p, n in zip(past, new):
@@ -224,7 +224,7 @@ def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None, blo
             lost = 2.0 ** -22 if dtype == "f32" else 2.0 ** -25
             e_s = abs(scale) * qs[:, h].abs().amax(1) * d * lost * kmag + size * 20 * 2.0 ** -24
             e_p = 2.0 ** -22 if dtype == "f32" else 2.0 ** -11
-            if block and dtype != "f32":
+            if block and dtype == "bf16":
                 e_s = e_s + 2.0 ** -11 * abs(scale) * (qs[:, h].abs() @ kh.abs().t()).amax(1)
                 e_p += 2.0 ** -11
             chain = ((p + n) / 32 + 64) * 2.0 ** -24
@@ -235,10 +235,11 @@ def reference(kv, q, past, new, kv_heads, heads, d, scale, dtype, most=None, blo
     return torch.cat(out), torch.cat(tols)
 
 
-def attention_case(ctx, dtype, past, new, kv_heads, heads, d, page=16, scale=None, pad=0, seed=0, qs=0, os=0):
+def attention_case(ctx, dtype, past, new, kv_heads, heads, d, page=16, scale=None, pad=0, seed=0, qs=0, os=0, slots=0):
+    """`slots`: of a table row at least; a table for long contexts takes other kernels."""
     scale = d ** -0.5 if scale is None else scale
     total = [p + n for p, n in zip(past, new)]
-    c = sv.Cache(ctx, total, kv_heads, d, page, seed=seed)
+    c = sv.Cache(ctx, total, kv_heads, d, page, seed=seed, width=max(-(-max(total) // page), -(-slots // page)))
     try:
         k, v, _ = inputs(seed + 1, sum(total), kv_heads, d, "f32")
         fill = c.batch([0] * len(total), total)
@@ -296,7 +297,13 @@ def test_attention(gpu_ctx, dtype, past, new, kv_heads, heads, d, page):
     ([5], [70], 1, 2, 65, 16),
 ])
 def test_attention_of_prompts(gpu_ctx, dtype, past, new, kv_heads, heads, d, page):
-    attention_case(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, pad=2, seed=sum(past) + d + 1)
+    for slots in (0, 2048):
+        attention_case(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, pad=2, seed=sum(past) + d + 1, slots=slots)
+
+
+def test_attention_of_many_prompts(gpu_ctx):
+    """Enough rows for blocks, whatever the contexts may be."""
+    attention_case(gpu_ctx, "bf16", [0] * 9, [130, 128, 200, 64, 300, 127, 129, 1, 150], 2, 16, 64, page=64, seed=41)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -344,34 +351,36 @@ def test_few_blocks_with_bad_pages_and_queries(gpu_ctx):
         c.close()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
-def test_attention_of_prompts_scales(gpu_ctx, scale):
-    attention_case(gpu_ctx, "f16", [90], [130], 2, 4, 64, scale=scale, seed=24, qs=3, os=5)
+def test_attention_of_prompts_scales(gpu_ctx, scale, dtype):
+    attention_case(gpu_ctx, dtype, [90], [130], 2, 4, 64, scale=scale, seed=24, qs=3, os=5, slots=1024)
 
 
-def test_prompts_with_bad_pages_and_queries(gpu_ctx):
+@pytest.mark.parametrize("dtype,slots", [("f16", 0), ("bf16", 0), ("bf16", 2048)])
+def test_prompts_with_bad_pages_and_queries(gpu_ctx, dtype, slots):
     """In the kernel for many rows: pages that the table does not name are not attended to, rows before
     them see nothing, and a row that is not finite is NaN by itself."""
     hk, heads, d, n = 1, 2, 64, 130
     k, v, _ = inputs(21, n, hk, d, "f32")
-    c = sv.Cache(gpu_ctx, [n], hk, d)
+    c = sv.Cache(gpu_ctx, [n], hk, d, width=max(-(-n // 16), slots // 16))
     try:
         b = c.batch([0], [n])
         c.append(b, k.to(sv.DEV), v.to(sv.DEV), "f32")
         kv = c.read(b)
         table = c.table.clone()
         table[0, 0], table[0, 1], table[0, 5] = -1, c.pages, -7          # slots 0 .. 31 and 80 .. 95
-        q = sv.normal(sv.gen(22), n, heads * d).to(torch.float16)
+        q = sv.normal(sv.gen(22), n, heads * d).to(sv.DTYPES[dtype])
         q[50, 3], q[60, d + 1] = math.nan, math.inf
-        out = torch.full((n, heads * d), 5.0, dtype=torch.float16, device=sv.DEV)
-        c.attend(c.batch([0], [n], table=table), q.to(sv.DEV), out, "f16", heads, d ** -0.5)
+        out = torch.full((n, heads * d), 5.0, dtype=sv.DTYPES[dtype], device=sv.DEV)
+        c.attend(c.batch([0], [n], table=table), q.to(sv.DEV), out, dtype, heads, d ** -0.5)
         got = out.cpu()
         assert not bool(got[:32].any())
         clean = q.clone()
         clean[50], clean[60] = 0.0, 0.0
         gone = torch.zeros(n, dtype=torch.bool)
         gone[:32] = gone[80:96] = True
-        want, tol = reference(kv, clean, [0], [n], hk, heads, d, d ** -0.5, "f16", block=True, gone=gone)
+        want, tol = reference(kv, clean, [0], [n], hk, heads, d, d ** -0.5, dtype, block=True, gone=gone)
         ok = (got.double() - want).abs() <= tol
         ok[50, :d] = torch.isnan(got[50, :d])
         ok[60, d:] = torch.isnan(got[60, d:])
@@ -479,7 +488,7 @@ def test_queries_of_any_size(gpu_ctx, size):
 def test_large_queries_of_small_scale(gpu_ctx, new):
     """The row's power of two and the scale meet before either leaves fp32's range."""
     hk, heads, d, n = 1, 2, 128, 200
-    c = sv.Cache(gpu_ctx, [n], hk, d)
+    c = sv.Cache(gpu_ctx, [n], hk, d, width=64)
     try:
         k, v, _ = inputs(27, n, hk, d, "f32")
         fill = c.batch([0], [n])
@@ -495,12 +504,12 @@ def test_large_queries_of_small_scale(gpu_ctx, new):
         c.close()
 
 
-@pytest.mark.parametrize("dtype,heads", [("f32", 2), ("bf16", 16)])
+@pytest.mark.parametrize("dtype,heads", [("f32", 2), ("f16", 16), ("bf16", 32)])
 def test_starts_that_do_not_ascend(gpu_ctx, dtype, heads):
     """A sequence whose rows do not lie in the batch, or go backwards, is left out; the others' rows are
     what they are without it."""
     hk, d = 2, 64
-    c = sv.Cache(gpu_ctx, [64, 64, 64, 64, 64], hk, d)
+    c = sv.Cache(gpu_ctx, [64, 64, 64, 64, 64], hk, d, width=64)
     try:
         k, v, q = inputs(29, 40, hk, d, dtype, heads)
         fill = c.batch([0] * 5, [8] * 5)

@@ -148,6 +148,21 @@ def test_large_vocabulary(gpu_ctx):
     check(run(gpu_ctx, *c, "f32"), reference(*c), c[0])
 
 
+@pytest.mark.parametrize("lengths", [(1023, 1024), (1025, 1028), (6001, 2500)])
+def test_long_lists(gpu_ctx, lengths):
+    """Histories and biases past what a workgroup loads ahead, and at its ends."""
+    vocab, rows = 9001, 2
+    x, hist, prompts, rep, pres, freq, biases, masks = case(11, rows, vocab, "f32", masked=False)
+    g = sv.gen(12)
+    for r in range(rows):
+        hist[r] = torch.randint(0, vocab, (lengths[r],), generator=g).tolist()
+        prompts[r] = lengths[r] // 3
+        n = lengths[1 - r]
+        biases[r] = list(zip(torch.randint(0, vocab, (n,), generator=g).tolist(), sv.normal(g, n).tolist()))
+    c = (x, hist, prompts, rep, pres, freq, biases, masks)
+    check(run(gpu_ctx, *c, "f32"), reference(*c), x)
+
+
 def test_biases_of_one_token(gpu_ctx):
     """Lists that name one token often, across every step of the search for it, sums of very unlike
     sizes among them: added in the list's order."""

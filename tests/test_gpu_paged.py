@@ -79,6 +79,38 @@ def test_append_and_read(gpu_ctx, dtype, kv_heads, head_dim, page, rope):
         c.close()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kv_heads,head_dim,rope,odd", [(2, 128, 128, 0), (2, 64, 32, 3), (1, 80, 40, 1), (3, 65, 10, 5)])
+def test_append_from_one_buffer(gpu_ctx, dtype, kv_heads, head_dim, rope, odd):
+    """Queries, keys and values side by side in a projection's rows, at any alignment: the same codes
+    and queries as from tensors of their own."""
+    heads, past, new = 3 * kv_heads, [3, 0, 17], [6, 1, 30]
+    rows = sum(new)
+    k, v, q = inputs(head_dim, rows, kv_heads, head_dim, dtype, heads)
+    c = sv.Cache(gpu_ctx, [p + n for p, n in zip(past, new)], kv_heads, head_dim, 16, rope)
+    try:
+        b = c.batch(past, new)
+        qo = torch.zeros(rows, heads * head_dim, dtype=q.dtype, device=sv.DEV)
+        c.append(b, k.to(sv.DEV), v.to(sv.DEV), dtype, q=q.to(sv.DEV), q_out=qo, heads=heads)
+        want = c.read(b)
+        zero = torch.zeros_like(k).to(sv.DEV)
+        c.append(b, zero, zero, dtype)
+        assert not bool(c.read(b).any())
+        buf = torch.cat([torch.full((rows, odd), 9.0).to(q.dtype), q, k, v, torch.full((rows, odd), 9.0).to(q.dtype)], dim=1)
+        dev = buf.to(sv.DEV).contiguous()
+        w, qc, kc = dev.shape[1], heads * head_dim, kv_heads * head_dim
+        at = lambda n: dev[:, n:]  # noqa: E731
+        c.append(b, at(odd + qc), at(odd + qc + kc), dtype, q=at(odd), q_out=at(odd), heads=heads, key_stride=w, value_stride=w,
+                 query_stride=w, query_out_stride=w)
+        assert torch.equal(c.read(b), want)
+        got = dev.cpu()
+        assert torch.equal(got[:, odd:odd + qc], qo.cpu())                       # in place,
+        got[:, odd:odd + qc] = q
+        assert torch.equal(got, buf)                                             # and nothing beside it
+    finally:
+        c.close()
+
+
 def test_tokens_one_by_one_equal_a_prompt(gpu_ctx):
     """The same slots written a token at a time, in runs of 3 and at once; neighbours in a word keep
     their codes, and other slots of the pool stay as they were."""

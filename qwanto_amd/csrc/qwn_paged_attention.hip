@@ -103,6 +103,31 @@ __device__ __forceinline__ Shape shape_of(const AttnArgs &a, const PagedSequence
     r.units = a.whole ? 1u : kStart + r.pieces;
     return r;
 }
+// Where a block and head stand among a sequence's items of the list.  Heads next
+// to each other, on XCDs of their own, are best where blocks hardly differ.  In
+// prompts, without cuts the longest contexts come first; where they are cut and a
+// prompt has little before it, its first rows see little of the context and its
+// last ones all: a share of several blocks has of both, the blocks of each head
+// in turn from both ends (2048 tokens, fp32: 213 us, 253 in the rows' order; four
+// of 512 behind 2048 407, and 393 with heads next to each other).
+template <bool PROMPT>
+__device__ __forceinline__ uint32_t item_of(const AttnArgs &a, const PagedSequence &q, uint32_t blocks, uint32_t block, uint32_t head) {
+    if (PROMPT && !a.whole && q.past < q.rows)
+        return head * blocks + (2 * block < blocks ? 2 * block : 2 * (blocks - 1 - block) + 1);
+    return (PROMPT && a.whole ? blocks - 1 - block : block) * a.c.kv_heads + head;
+}
+template <bool PROMPT>
+__device__ __forceinline__ void place_of(const AttnArgs &a, const PagedSequence &q, uint32_t blocks, uint32_t item, uint32_t &block,
+                                         uint32_t &head) {
+    if (PROMPT && !a.whole && q.past < q.rows) {
+        const uint32_t place = item % blocks;
+        head = item / blocks;
+        block = place % 2 ? blocks - 1 - place / 2 : place / 2;
+    } else {
+        head = item % a.c.kv_heads;
+        block = PROMPT && a.whole ? blocks - 1 - item / a.c.kv_heads : item / a.c.kv_heads;
+    }
+}
 __device__ __forceinline__ PagedSequence lane_sequence(const AttnArgs &a, uint32_t s) {
     return s < a.b.sequences ? paged_sequence(a.b, s) : PagedSequence{};
 }
@@ -284,7 +309,7 @@ __device__ __forceinline__ void load_query(const T *row, uint32_t c0, uint32_t n
 // are there, its values once they are used: the other half of the step's work
 // hides each, in one set of registers.  Bound by HBM in the long run, by the
 // searches and loads that a block starts with where contexts are short.
-template <typename T, int W>
+template <typename T, int W, bool PROMPT>
 __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_kernel(AttnArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     // Keys meet a few large products, in whole codes only for fp32.  Values meet
@@ -320,12 +345,19 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
         const uint32_t first = u - at + (a.whole ? 0u : kStart);  // the unit of its first piece
         if (u < first) u = min(first, end);
         if (u == end) break;
-        const uint32_t block = item / a.c.kv_heads, head = item % a.c.kv_heads;
+        uint32_t block, head;
+        place_of<PROMPT>(a, q, h.blocks, item, block, head);
         const uint32_t piece0 = u - first;
         const uint32_t count = a.whole ? h.pieces : min(h.pieces - piece0, end - u);
         const uint32_t rows = min(kRows, q.rows * a.group - block * kRows);
         const uint32_t most = min(q.past + (block * kRows + rows - 1) / a.group + 1, a.slots);  // slots any row sees
         const uint32_t least_seen = q.past + block * kRows / a.group + 1;                        // slots every row sees
+        // of this block's rows: a prompt's first ones see nothing of the sequence's others
+        const uint32_t pieces = PROMPT ? (most + kPiece - 1) / kPiece : h.pieces;
+        if (PROMPT && piece0 >= pieces) {
+            u += count;
+            continue;
+        }
         const uint32_t t_end = min(most, (piece0 + count) * kPiece);
         uint32_t t0 = piece0 * kPiece + wave * kStep;
         uint32_t k[2][J], v[2][J], ks[2][4 * G], vs[2][4 * G];
@@ -512,7 +544,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
             if (g == 0) merge_ml[wave][n] = make_float2(m == -INFINITY ? -INFINITY : ref, sum);
         }
         __syncthreads();
-        const bool whole = count == h.pieces;
+        const bool whole = piece0 == 0 && count >= pieces;
         const uint32_t part = paged_partial(list.total, workers, first, blockIdx.x);
         for (uint32_t i = threadIdx.x; i < rows * W; i += kThreads) {
             const uint32_t row = i / W, ch = i % W;
@@ -550,7 +582,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
 // more than rows: 4 sequences of 8 new tokens behind up to 30000 (8 KV heads, 4
 // query heads each) 30 us with 16, 36 with 4; 61 of 2 behind 4000 29 and 25.
 constexpr uint32_t kMergeGroups = 2048;
-template <typename T, int W>
+template <typename T, int W, bool PROMPT>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
     constexpr uint32_t kLanes = W / 4, kGroups = kThreads / kLanes;
     __shared__ v4f part_o[kGroups][kLanes];
@@ -570,12 +602,14 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
         }
     }
     const Shape h = shape_of(a, q);
-    const uint32_t first = before + (block * a.c.kv_heads + head) * h.units + kStart;
+    const uint32_t first = before + item_of<PROMPT>(a, q, h.blocks, block, head) * h.units + kStart;
+    const uint32_t all = min(kRows, q.rows * a.group - block * kRows);
+    const uint32_t most = min(q.past + (block * kRows + all - 1) / a.group + 1, a.slots);
+    const uint32_t pieces = PROMPT ? (most + kPiece - 1) / kPiece : h.pieces;
     if (first + h.pieces > total) return;  // starts that do not ascend: the list's length has wrapped
-    const uint32_t w0 = paged_worker(total, workers, first), w1 = paged_worker(total, workers, first + h.pieces - 1);
+    const uint32_t w0 = paged_worker(total, workers, first), w1 = paged_worker(total, workers, first + pieces - 1);
     if (w0 == w1) return;  // one worker had it all, and wrote it
     const uint32_t p0 = paged_partial(total, workers, first, w0), n = w1 - w0 + 1;
-    const uint32_t all = min(kRows, q.rows * a.group - block * kRows);
     if (blockIdx.z >= all) return;
     const uint32_t rows = (all - blockIdx.z + gridDim.z - 1) / gridDim.z;
     uint32_t share = 1;  // groups of a row
@@ -1060,14 +1094,14 @@ size_t partial_rows(uint32_t width) {
 }
 size_t partial_bytes(uint32_t width) { return partial_rows(width) * (width * sizeof(float) + sizeof(float2)); }
 
-// Whether a batch is for the block kernel: its sequences have rows enough (of 8
-// KV heads: 16 sequences of 3000 tokens with 64 rows each 70 us in it and 53 in
+// Whether a batch's sequences bring rows as prompts do (of 8 KV heads: 16
+// sequences of 3000 tokens with 64 rows each 70 us in the block kernel and 53 in
 // blocks of 16, with 80 rows 70 and 66, with 124 72 and 88; 64 of 1000 with 80
-// rows 64 and 78), and there are more than a few short ones (a prompt of 128
-// tokens 13 and 9, of 256 16 and 12; 8 of 64 behind 192 16 and 20).
+// rows 64 and 78), and is for the block kernel: more than a few short ones (a
+// prompt of 128 tokens 13 and 9, of 256 16 and 12; 8 of 64 behind 192 16 and 20).
+bool many_rows(const AttnArgs &a) { return static_cast<uint64_t>(a.b.tokens) * a.group >= 80ull * a.b.sequences; }
 bool block_rows(const AttnArgs &a) {
-    const uint64_t rows = static_cast<uint64_t>(a.b.tokens) * a.group;
-    return rows >= 80ull * a.b.sequences && (rows * a.c.kv_heads > 8192 || a.slots > kWholeSlots);
+    return many_rows(a) && (static_cast<uint64_t>(a.b.tokens) * a.group * a.c.kv_heads > 8192 || a.slots > kWholeSlots);
 }
 
 template <typename T, int W, int RW, int RT, int BUFFERS>
@@ -1094,25 +1128,30 @@ hipError_t launch_block(AttnArgs a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <typename T, int W>
-hipError_t launch_width(AttnArgs a, uint32_t blocks, hipStream_t stream) {
-    // f16 rows are left to blocks of 16, whose values are exact: keys and values
-    // rounded to f16 would cost more than the output's own rounding (error 3.5 to
-    // 4.5e-4, there 2.9e-4, of which the output's 2.1e-4; four prompts of 512 tokens
-    // behind 2048 290 us for 134)
-    if constexpr (std::is_same_v<T, bf16>) {
-        if (block_rows(a)) return launch_block<T, W, kBlockWaves, W == 256 ? 1 : 2, W == 256 ? 1 : 2>(a, stream);
-    }
+template <typename T, int W, bool PROMPT>
+hipError_t launch_blocks(AttnArgs a, uint32_t blocks, hipStream_t stream) {
     a.whole = a.slots <= (blocks * a.c.kv_heads >= kMany ? kWholeSlotsMany : kWholeSlots);
     a.workers = a.whole ? blocks * a.c.kv_heads : W == 256 ? kWorkers / 3 : kWorkers;  // of 256 channels: one on each CU
-    hipLaunchKernelGGL((paged_attention_kernel<T, W>), dim3(a.workers), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<T, W, PROMPT>), dim3(a.workers), dim3(kThreads), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.whole) return e;
     // rows of a sequence, about
     const uint32_t each = static_cast<uint32_t>((static_cast<uint64_t>(a.b.tokens) * a.group + a.b.sequences - 1) / a.b.sequences);
     const uint32_t parts = std::min({kRows, each, std::max(3u, kMergeGroups / (blocks * a.c.kv_heads))});
-    hipLaunchKernelGGL((paged_merge_kernel<T, W>), dim3(blocks, a.c.kv_heads, parts), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_merge_kernel<T, W, PROMPT>), dim3(blocks, a.c.kv_heads, parts), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
+}
+
+template <typename T, int W>
+hipError_t launch_width(AttnArgs a, uint32_t blocks, hipStream_t stream) {
+    // f16 rows are left to blocks of 16, whose values are exact: keys and values
+    // rounded to f16 would cost more than the output's own rounding (error 3.5 to
+    // 4.5e-4, there 2.9e-4, of which the output's 2.1e-4; four prompts of 512 tokens
+    // behind 2048 276 us for 134)
+    if constexpr (std::is_same_v<T, bf16>) {
+        if (block_rows(a)) return launch_block<T, W, kBlockWaves, W == 256 ? 1 : 2, W == 256 ? 1 : 2>(a, stream);
+    }
+    return many_rows(a) ? launch_blocks<T, W, true>(a, blocks, stream) : launch_blocks<T, W, false>(a, blocks, stream);
 }
 template <typename T>
 hipError_t launch_paged_attention(const AttnArgs &a, uint32_t blocks, hipStream_t stream) {

@@ -287,3 +287,43 @@ def test_a_page_that_comes_twice(gpu_ctx):
         assert bool(((out.cpu().double() - want).abs() <= tol).all())
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prompt_attention_captured(gpu_ctx, dtype):
+    """The kernels of many rows, their contexts cut and joined, recorded once and replayed with other
+    lengths, rows and pages."""
+    slots = [3000, 700, 400]
+    c = sv.Cache(gpu_ctx, slots, 2, 128)
+    try:
+        g = sv.gen(8)
+        k, v = sv.normal(g, sum(slots), 256).to(sv.DEV), sv.normal(g, sum(slots), 256).to(sv.DEV)
+        c.append(c.batch([0, 0, 0], slots), k, v, "f32")
+        rows = 128
+        q = sv.normal(g, rows, 8 * 128).to(sv.DTYPES[dtype]).to(sv.DEV)
+        out, want = torch.zeros_like(q), torch.zeros_like(q)
+        b = c.batch([0, 0, 0], [rows, 0, 0])
+        r, e = c.request(b, q, out, dtype, 8, 0.1), c.request(b, q, want, dtype, 8, 0.1)
+        starts, past, table = (torch.zeros(4, dtype=torch.int32, device=sv.DEV), torch.zeros(3, dtype=torch.int32, device=sv.DEV),
+                               c.table.clone())
+        b.starts, b.past, b.page_table = sv.ptr(starts), sv.ptr(past), sv.ptr(table)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            gpu_ctx.paged_kv_attention_device(c.h, r, stream=sv.stream())
+        for ps, ns, flip in (([2900, 600, 300], [100, 20, 8], False), ([0, 0, 0], [128, 0, 0], False), ([10, 650, 390], [1, 50, 10], True),
+                             ([2872, 0, 0], [128, 0, 0], False), ([5, 5, 5], [40, 40, 40], True)):
+            starts.copy_(torch.tensor([0, ns[0], ns[0] + ns[1], sum(ns)], dtype=torch.int32))
+            past.copy_(torch.tensor(ps, dtype=torch.int32))
+            table.copy_(c.table.flip(0) if flip else c.table)
+            for o in (out, want):
+                o.fill_(2.0)
+            graph.replay()
+            gpu_ctx.paged_kv_attention_device(c.h, e, stream=sv.stream())
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), (ps, ns)
+            assert bool((out[sum(ns):] == 2.0).all())
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), (ps, ns)
+    finally:
+        c.close()

@@ -61,10 +61,12 @@ constexpr uint32_t kStep = 32;                    // tokens of a wave's step
 constexpr uint32_t kPiece = kStep * kWaves;       // tokens of a workgroup's step: the unit work is split in
 constexpr uint32_t kWorkers = 768;                // workgroups at most: three of four waves on each CU
 constexpr uint32_t kStart = 3;                    // pieces that a block's beginning and end cost as much as
-// Contexts are not split up to so many slots, where there are few blocks or
-// many: 64 sequences of 1024 tokens, 8 KV heads, 20 us whole and 28 split and
-// merged; one of 512, 11 and 11.
-constexpr uint32_t kWholeSlots = 512, kWholeSlotsMany = 1024, kMany = 256;
+// Contexts are not split up to so many slots, the second where blocks are many
+// (64 sequences of 1024 tokens, 8 KV heads, 20 us whole and 28 split and merged),
+// or fewer with eight waves each (8 of 1000 bf16 11.5 and 14.5, fp32 14.8 and
+// 15.7), for 16-bit rows down to one sequence (of 700, 10.0 and 10.9; fp32 12.4
+// and 11.2).
+constexpr uint32_t kWholeSlots = 512, kWholeSlotsMany = 1024, kMany = 256, kSome = 16;
 
 constexpr int kQueryBits = 15;                   // |query| < 2^15 in f16
 constexpr int kWeightBits = 11;                  // probability times step < 2^11 of the largest met,
@@ -309,8 +311,8 @@ __device__ __forceinline__ void load_query(const T *row, uint32_t c0, uint32_t n
 // are there, its values once they are used: the other half of the step's work
 // hides each, in one set of registers.  Bound by HBM in the long run, by the
 // searches and loads that a block starts with where contexts are short.
-template <typename T, int W, bool PROMPT>
-__global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_kernel(AttnArgs a) {
+template <typename T, int W, bool PROMPT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 2) void paged_attention_kernel(AttnArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     // Keys meet a few large products, in whole codes only for fp32.  Values meet
     // many: the sum of p * code as it lies less that of p * 8 leaves 2e-4 of an
@@ -320,8 +322,9 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
     constexpr bool WHOLE = NP == 2, WHOLE_V = !std::is_same_v<T, bf16>;
     constexpr int J = W / 32, G = W / 64, C = W / 16;
     constexpr int kPad = W + 4;
-    __shared__ float merge_o[kWaves][kRows][kPad];
-    __shared__ float2 merge_ml[kWaves][kRows];
+    constexpr uint32_t kStride = WAVES * kStep;  // tokens of the workgroup's step: a piece, but where nothing is cut
+    __shared__ float merge_o[WAVES][kRows][kPad];
+    __shared__ float2 merge_ml[WAVES][kRows];
     const uint32_t lane = threadIdx.x % kWaveSize;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const uint32_t n = lane % 16, g = lane / 16;
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
         load_tiles<W, false>(a, pv, head, t0, lane, v, vs);
         // where nothing follows a step's loads are issued again: how many are in
         // flight does not depend on a branch, and no wait is for more than it needs
-        uint32_t next = t0 + kPiece < t_end ? t0 + kPiece : t0;
+        uint32_t next = t0 + kStride < t_end ? t0 + kStride : t0;
         Pages pn = find_pages(a, s, next);
 
         // this lane's query row (column n): token and head, its visible slots
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
 #pragma unroll
         for (int gg = 0; gg < G; ++gg) low[gg] = 0.0f, weights[gg] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 
-        for (; t0 < t_end; t0 += kPiece) {
+        for (; t0 < t_end; t0 += kStride) {
             float sc[8];
 #pragma unroll
             for (int i2 = 0; i2 < 2; ++i2) {
@@ -451,7 +454,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
             const uint32_t now = next;
             pk = pn;
             load_tiles<W, true>(a, pk, head, now, lane, k, ks);
-            next = t0 + 2 * kPiece < t_end ? t0 + 2 * kPiece : now;
+            next = t0 + 2 * kStride < t_end ? t0 + 2 * kStride : now;
             pn = find_pages(a, s, next);
             uint32_t top = 0;
             if (t0 + kStep > least_seen || !pg.ok[0] || !pg.ok[1]) {  // not all tokens for all rows
@@ -546,15 +549,15 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 3) void paged_attention_ke
         __syncthreads();
         const bool whole = piece0 == 0 && count >= pieces;
         const uint32_t part = paged_partial(list.total, workers, first, blockIdx.x);
-        for (uint32_t i = threadIdx.x; i < rows * W; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < rows * W; i += WAVES * kWaveSize) {
             const uint32_t row = i / W, ch = i % W;
             float top = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, merge_ml[w][row].x);
+            for (int w = 0; w < WAVES; ++w) top = fmaxf(top, merge_ml[w][row].x);
             const float base = top == -INFINITY ? 0.0f : top;
             float o = 0.0f, l = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 const float f = __builtin_amdgcn_exp2f(merge_ml[w][row].x - base);
                 o = fmaf(merge_o[w][row][ch], f, o);
                 l = fmaf(merge_ml[w][row].y, f, l);
@@ -1130,9 +1133,21 @@ hipError_t launch_block(AttnArgs a, hipStream_t stream) {
 
 template <typename T, int W, bool PROMPT>
 hipError_t launch_blocks(AttnArgs a, uint32_t blocks, hipStream_t stream) {
-    a.whole = a.slots <= (blocks * a.c.kv_heads >= kMany ? kWholeSlotsMany : kWholeSlots);
-    a.workers = a.whole ? blocks * a.c.kv_heads : W == 256 ? kWorkers / 3 : kWorkers;  // of 256 channels: one on each CU
-    hipLaunchKernelGGL((paged_attention_kernel<T, W, PROMPT>), dim3(a.workers), dim3(kThreads), 0, stream, a);
+    const uint32_t groups = blocks * a.c.kv_heads;
+    constexpr bool kEight = !PROMPT && W != 256;  // of 256 channels they would not have the registers
+    const bool eight = kEight && groups < kMany;
+    const bool longer = groups >= kMany || (eight && (sizeof(T) == 2 || groups >= kSome));
+    a.whole = a.slots <= (longer ? kWholeSlotsMany : kWholeSlots);
+    a.workers = a.whole ? groups : W == 256 ? kWorkers / 3 : kWorkers;  // of 256 channels: one on each CU
+    if constexpr (kEight) {
+        // few blocks that are not cut: eight waves each (one sequence of 334 tokens,
+        // 2 KV heads, bf16 7.9 us, with four 8.4; fp32 9.4 and 9.7)
+        if (a.whole && eight) {
+            hipLaunchKernelGGL((paged_attention_kernel<T, W, false, 8>), dim3(a.workers), dim3(8 * kWaveSize), 0, stream, a);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((paged_attention_kernel<T, W, PROMPT, kWaves>), dim3(a.workers), dim3(kThreads), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.whole) return e;
     // rows of a sequence, about

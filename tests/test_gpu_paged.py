@@ -307,6 +307,9 @@ def attention_case(ctx, dtype, past, new, kv_heads, heads, d, page=16, scale=Non
     ([77], [4], 5, 15, 96, 32),
     ([50], [3], 2, 2, 65, 16),
     ([5000, 20, 2600], [1, 1, 4], 1, 4, 128, 16),              # one sequence split over many workgroups
+    ([1500, 3, 127, 128, 700], [1, 1, 1, 1, 2], 8, 32, 128, 64),
+    ([2000, 40, 1029], [3, 1, 1], 2, 8, 64, 16),
+    ([1020, 511], [4, 1], 2, 12, 128, 16),                     # as long as contexts get that are not split
 ])
 def test_attention(gpu_ctx, dtype, past, new, kv_heads, heads, d, page):
     attention_case(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, pad=3, seed=sum(past) + d)

@@ -31,7 +31,9 @@
 // Queries are scaled by a power of two
 // per row to below 2^15, probabilities times steps by one per row and wave to
 // below 2^11 where their largest was met (2^15 a little past it): f16 then has
-// 25 binades and more below the largest, for the second halves as well.
+// 25 binades and more below the largest, for the second halves as well.  The
+// largest product is taken off before products become exponents: rounded, its
+// exponent would be off by more than f16 holds where scores pass 2^27.
 #include "qwn_context.h"
 #include "qwn_device.h"
 #include "qwn_hip_ext.h"
@@ -71,6 +73,7 @@ constexpr uint32_t kWholeSlots = 512, kWholeSlotsMany = 1024, kMany = 256, kSome
 constexpr int kQueryBits = 15;                   // |query| < 2^15 in f16
 constexpr int kWeightBits = 11;                  // probability times step < 2^11 of the largest met,
 constexpr float kSlack = 4.0f;                   // and 2^4 more before the reference moves
+constexpr float kNothing = -3.402823466e38f;     // the largest product where none was seen: finite, what is taken off it too
 
 struct AttnArgs {
     PagedKv c;
@@ -78,7 +81,7 @@ struct AttnArgs {
     const void *query;
     void *output;
     float *part_o;       // [worker][2][kRows][width]
-    float2 *part_ml;     // [worker][2][kRows]: reference exponent, sum
+    float4 *part_ml;     // [worker][2][kRows]: largest product, sum, what makes products exponents
     uint32_t query_stride, output_stride, query_heads, group;
     uint32_t slots;      // of a sequence's row of the table
     uint32_t workers;    // workgroups of the launch
@@ -288,6 +291,18 @@ __device__ __forceinline__ void load_tiles(const AttnArgs &a, const Pages &p, ui
     }
 }
 
+// What a row's products, of queries times `up` = 2^(bits it is divided by), are
+// multiplied by to be exponents of 2: positive, the scale's sign is the queries'.
+// Where nothing is left of it all scores are alike.  Where it passes fp32, two
+// products that differ (by 2^-100 at least: minima, steps and the largest query
+// have no smaller bits) are further apart than any exponent, with the largest
+// fp32 in its place as well.
+__device__ __forceinline__ float exponents_of(float scale, int bits, float &up) {
+    const float mul = fminf(ldexpf(fabsf(scale), bits) * 1.44269504088896340736f, 3.402823466e38f);
+    up = mul > 0.0f ? copysignf(up, scale) : 0.0f;
+    return mul > 0.0f ? mul : 1.0f;
+}
+
 // The 8 channels of a query row from c0, zeros past the head's.
 template <typename T>
 __device__ __forceinline__ void load_query(const T *row, uint32_t c0, uint32_t n, float x[8]) {
@@ -324,7 +339,8 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
     constexpr int kPad = W + 4;
     constexpr uint32_t kStride = WAVES * kStep;  // tokens of the workgroup's step: a piece, but where nothing is cut
     __shared__ float merge_o[WAVES][kRows][kPad];
-    __shared__ float2 merge_ml[WAVES][kRows];
+    __shared__ float2 merge_ml[WAVES][kRows];  // largest product, sum
+    __shared__ float merge_mul[kRows];
     const uint32_t lane = threadIdx.x % kWaveSize;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const uint32_t n = lane % 16, g = lane / 16;
@@ -395,8 +411,8 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
             int e = 0;  // top < 2^e
             if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);
             e = max(e, -100);
-            const float up = ldexpf(1.0f, kQueryBits - e);
-            row_mul = ldexpf(a.scale * 1.44269504088896340736f, e - kQueryBits + (WHOLE ? 0 : 24));
+            float up = ldexpf(1.0f, kQueryBits - e);
+            row_mul = exponents_of(a.scale, e - kQueryBits + (WHOLE ? 0 : 24), up);
 #pragma unroll
             for (int gg = 0; gg < G; ++gg) qsum[gg] = 0.0f;
 #pragma unroll
@@ -412,12 +428,13 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
 #pragma unroll
             for (int gg = 0; gg < G; ++gg) {
                 qsum[gg] = across_sum(qsum[gg]) * (WHOLE ? 1.0f : 0x1p-24f);
-                if (top == INFINITY) qsum[gg] = __builtin_nanf("");  // not finite: NaN, whatever the codes are
+                if (top == INFINITY || !isfinite(a.scale)) qsum[gg] = __builtin_nanf("");  // the row is NaN, whatever the codes are
             }
         }
 
         v4f acc[C], weights[G];
-        float low[G], sum = 0.0f, m = -INFINITY, ref = 0.0f;
+        // m is of the products as they come, before row_mul: below 2^40
+        float low[G], sum = 0.0f, m = kNothing, up_bits = 0.0f;
         uint32_t steps = 0;  // no step of a value met so far is larger: f16 bits above, 0xffff below
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
@@ -447,7 +464,7 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
                         x = fmaf(step_of(w), d[gg][i], x);
                         x = fmaf(WHOLE ? fmaf(8.0f, step_of(w), least_of(w)) : least_of(w), qsum[gg], x);
                     }
-                    sc[4 * i2 + i] = x * row_mul;
+                    sc[4 * i2 + i] = x;
                 }
             }
             const Pages pg = pv;
@@ -476,7 +493,7 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
             for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i]);
             // a new reference only where a score is well past the last one's or a
             // step larger: rare once a few steps are done
-            if (__any(mx > m + kSlack || top > steps)) {
+            if (__any((mx - m) * row_mul > kSlack || top > steps)) {
                 mx = across_max(fmaxf(mx, m));
                 top = max(top, steps);
                 top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
@@ -484,21 +501,20 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
                 steps = top | 0xffffu;
                 // steps < 2^e; 2^-24 is the smallest that is not zero
                 const int e = max(-24, static_cast<int>(__builtin_bit_cast(uint32_t, step_of(top)) >> 23) - 126);
-                const float moved = mx == -INFINITY ? 0.0f : mx + static_cast<float>(e - kWeightBits);
-                // nothing seen yet: sums of zeros, whatever the reference was
-                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - moved);
+                const float bits = static_cast<float>(kWeightBits - e);
+                const float alpha = __builtin_amdgcn_exp2f(fmaf(m - mx, row_mul, bits - up_bits));
 #pragma unroll
                 for (int c = 0; c < C; ++c) acc[c] *= alpha;
 #pragma unroll
                 for (int gg = 0; gg < G; ++gg) low[gg] *= alpha, weights[gg] *= alpha;
                 sum *= alpha;
                 m = mx;
-                ref = moved;
+                up_bits = bits;
             }
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(sc[i] - ref);
+                p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i] - m, row_mul, up_bits));
                 sum += p[i];
             }
             Halves<NP> pf[G];
@@ -537,28 +553,30 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
         sum = across_sum(sum);
 #pragma unroll
         for (int gg = 0; gg < G; ++gg) low[gg] = across_sum(low[gg]);
+        const float down = ldexpf(1.0f, -static_cast<int>(up_bits));  // the largest probability is 1 again
         __syncthreads();  // the previous block's results are read
         if (real) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const v4f o = WHOLE_V ? acc[c] + low[c / 4] : acc[c] * 0x1p24f - 8.0f * weights[c / 4] + low[c / 4];
-                *reinterpret_cast<v4f *>(&merge_o[wave][n][16 * c + 4 * g]) = o;
+                *reinterpret_cast<v4f *>(&merge_o[wave][n][16 * c + 4 * g]) = o * down;
             }
-            if (g == 0) merge_ml[wave][n] = make_float2(m == -INFINITY ? -INFINITY : ref, sum);
+            if (g == 0) merge_ml[wave][n] = make_float2(m, sum * down);
+            if (g == 0 && wave == 0) merge_mul[n] = row_mul;
         }
         __syncthreads();
         const bool whole = piece0 == 0 && count >= pieces;
         const uint32_t part = paged_partial(list.total, workers, first, blockIdx.x);
         for (uint32_t i = threadIdx.x; i < rows * W; i += WAVES * kWaveSize) {
             const uint32_t row = i / W, ch = i % W;
-            float top = -INFINITY;
+            float top = kNothing;
+            const float mul = merge_mul[row];
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) top = fmaxf(top, merge_ml[w][row].x);
-            const float base = top == -INFINITY ? 0.0f : top;
             float o = 0.0f, l = 0.0f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(merge_ml[w][row].x - base);
+                const float f = __builtin_amdgcn_exp2f((merge_ml[w][row].x - top) * mul);
                 o = fmaf(merge_o[w][row][ch], f, o);
                 l = fmaf(merge_ml[w][row].y, f, l);
             }
@@ -570,7 +588,7 @@ __global__ __launch_bounds__(WAVES * kWaveSize, W == 256 ? 1 : WAVES == 4 ? 3 : 
             } else {
                 const size_t at_part = static_cast<size_t>(part) * kRows + row;
                 a.part_o[at_part * W + ch] = o;
-                if (ch == 0) a.part_ml[at_part] = make_float2(top, l);
+                if (ch == 0) a.part_ml[at_part] = make_float4(top, l, mul, 0.0f);
             }
         }
         u += a.whole ? 1u : count;
@@ -621,16 +639,17 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
     for (uint32_t r0 = 0; r0 < rows; r0 += kGroups / share) {
         const uint32_t r = r0 + group / share, row = blockIdx.z + r * gridDim.z;
         v4f o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-        float top = -INFINITY, l = 0.0f;
+        float top = kNothing, l = 0.0f, mul = 1.0f;
         if (r < rows) {
 #pragma unroll 4
             for (uint32_t i = mine; i < n; i += share) {
                 // the first worker's partial may be its second, the others' are their first
                 const size_t at = static_cast<size_t>(i ? 2 * (w0 + i) : p0) * kRows + row;
-                const float2 ml = a.part_ml[at];
+                const float4 ml = a.part_ml[at];
                 const v4f x = *reinterpret_cast<const v4f *>(a.part_o + at * W + 4 * lane);
-                const float next = fmaxf(top, ml.x), base = next == -INFINITY ? 0.0f : next;
-                const float f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(ml.x - base);
+                const float next = fmaxf(top, ml.x);
+                mul = ml.z;
+                const float f0 = __builtin_amdgcn_exp2f((top - next) * mul), f1 = __builtin_amdgcn_exp2f((ml.x - next) * mul);
                 o = o * f0 + x * f1;
                 l = l * f0 + ml.y * f1;
                 top = next;
@@ -642,11 +661,10 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(AttnArgs a) {
             __syncthreads();
             if (mine != 0) continue;
             for (uint32_t i = 1; i < share; ++i) top = fmaxf(top, part_ml[group + i].x);
-            const float base = top == -INFINITY ? 0.0f : top;
             o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
             l = 0.0f;
             for (uint32_t i = 0; i < share; ++i) {
-                const float f = __builtin_amdgcn_exp2f(part_ml[group + i].x - base);
+                const float f = __builtin_amdgcn_exp2f((part_ml[group + i].x - top) * mul);
                 o += part_o[group + i][lane] * f;
                 l += part_ml[group + i].y * f;
             }
@@ -1020,7 +1038,7 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
         T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + r / a.group) * a.output_stride +
                  static_cast<size_t>(head * a.group + r % a.group) * a.c.head_dim;
         const size_t at_part = (static_cast<size_t>(blockIdx.x) * a.parts + blockIdx.y) * kBlockRows + r - row0;
-        if (parts > 1 && g == 0) a.part_ml[at_part] = make_float2(top, l);
+        if (parts > 1 && g == 0) a.part_ml[at_part] = make_float4(top, l, 1.0f, 0.0f);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const v4f o = acc[t][c] * f0 + sums[t * kSums + c * kSumLanes + lane] * f1;
@@ -1066,7 +1084,8 @@ __global__ __launch_bounds__(kThreads) void paged_block_merge_kernel(AttnArgs a)
 #pragma unroll
     for (uint32_t i = 0; i < kBlockPartsMost; ++i)
         if (i < parts) {
-            ml[i] = a.part_ml[first + i * ROWS];
+            const float4 part = a.part_ml[first + i * ROWS];
+            ml[i] = make_float2(part.x, part.y);
             x[i] = *reinterpret_cast<const v4f *>(a.part_o + (first + i * ROWS) * W + 4 * lane);
             top = fmaxf(top, ml[i].x);
         }
@@ -1095,7 +1114,7 @@ constexpr uint32_t block_rows_of(uint32_t width) { return kBlockWaves * (width =
 size_t partial_rows(uint32_t width) {
     return std::max<size_t>(static_cast<size_t>(kWorkers) * 2 * kRows, static_cast<size_t>(kBlockGroups) * block_rows_of(width));
 }
-size_t partial_bytes(uint32_t width) { return partial_rows(width) * (width * sizeof(float) + sizeof(float2)); }
+size_t partial_bytes(uint32_t width) { return partial_rows(width) * (width * sizeof(float) + sizeof(float4)); }
 
 // Whether a batch's sequences bring rows as prompts do (of 8 KV heads: 16
 // sequences of 3000 tokens with 64 rows each 70 us in the block kernel and 53 in
@@ -1239,7 +1258,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_attention_device(QwnCudaContextHandle 
     a.query = r->query;
     a.output = r->output;
     a.scale = r->scale;
-    a.part_ml = static_cast<float2 *>(r->workspace);
+    a.part_ml = static_cast<float4 *>(r->workspace);
     a.part_o = reinterpret_cast<float *>(a.part_ml + partial_rows(a.c.width));
     hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
     const hipError_t e = r->dtype == QWN_HIP_DTYPE_F32   ? launch_paged_attention<float>(a, static_cast<uint32_t>(blocks), s)

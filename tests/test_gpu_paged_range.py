@@ -102,3 +102,8 @@ PROMPTS = [
 @pytest.mark.parametrize("past,new,kv_heads,heads,d,slots", PROMPTS)
 def test_scores_of_any_size_in_prompts(gpu_ctx, dtype, past, new, kv_heads, heads, d, slots):
     check_sizes(gpu_ctx, dtype, past, new, kv_heads, heads, d, slots)
+
+
+@pytest.mark.parametrize("past,new,kv_heads,heads,d,slots", PROMPTS)
+def test_scores_of_any_size_in_blocks_of_many_rows(gpu_ctx, past, new, kv_heads, heads, d, slots):
+    check_sizes(gpu_ctx, "bf16", past, new, kv_heads, heads, d, slots)

@@ -123,3 +123,67 @@ class Cache:
     def close(self):
         torch.cuda.synchronize()
         self.ctx.paged_kv_destroy(self.h)
+
+
+# ---- attention: how far a row may be off -------------------------------------------
+
+
+def attention_rows(kv, q, past, new, kv_heads, heads, d, scale, dtype, kernel, gone=()):
+    """64-bit attention over the cached values kv [2][tokens][..], [rows][heads][d], and how far a row
+    of it may be off in the 2-norm, [rows][heads].  `gone`: slots that are left out.
+
+    With scores off by e_t, weights by w_t of themselves and values by y_t, a row o = sum p_t v_t moves
+    by sum p_t ((e_t + w_t) (v_t - o) + y_t).  These are roundings: of zero mean and independent from
+    token to token, the largest r (r / sqrt 3 in the root mean square), so the sum is held to 6 times
+    the root of its squares' sum.  r is
+    - of a score: about 20 fp32 sums, 2^-24 each of the magnitudes |q| (|k| + 16 steps) (the matrix
+      cores' sums of subnormal codes, 16-bit rows, 2^-22), and fp32's queries in two halves 2^-22 of
+      each product; in "block" the keys' rounding to f16, 2^-11 of each product;
+    - of a weight: 2^-20 for the exponential and its argument; in "block" 2^-11, f16;
+    - of a value: weight times step rounded, 2^-11 (two halves: 2^-22) of what it multiplies, the value
+      less the middle of its group; in "block" 2^-11 of the value.
+    The sums over n tokens are chains of n / 16 + 64 fp32 sums of magnitudes that grow as the root of
+    the squares' sum and as the output; subnormal codes' are off by 2^-22 of a sum of 8 steps.  On top
+    of it the output's own rounding."""
+    group, half = heads // kv_heads, HALF[dtype]
+    out, lim = [], []
+    at = row = 0
+    for p0, n in zip(past, new):
+        total = p0 + n
+        k, v = (kv[i, at:at + total].double().reshape(total, kv_heads, d) for i in range(2))
+        at += total
+        if not n:
+            continue
+        qs = q[row:row + n].double().reshape(n, heads, d)
+        row += n
+        see = torch.arange(total)[None] <= p0 + torch.arange(n)[:, None]
+        for s in gone:
+            see[:, s] = False
+        for h in range(heads):
+            kh, vh, qh = k[:, h // group], v[:, h // group], qs[:, h]
+            s = (qh @ kh.t() * scale).masked_fill(~see, -float("inf"))
+            p = torch.nan_to_num(torch.softmax(s, dim=1))
+            o = p @ vh
+            steps, middle = [], []
+            for x in (kh, vh):
+                lo = torch.cat([g.amin(1, keepdim=True).expand_as(g) for g in x.split(GROUP, 1)], 1)
+                hi = torch.cat([g.amax(1, keepdim=True).expand_as(g) for g in x.split(GROUP, 1)], 1)
+                steps.append((hi - lo) / 15)
+                middle.append(lo + 8 * (hi - lo) / 15)
+            products = ((qh ** 2) @ (kh ** 2).t()).sqrt()
+            sums = qh.abs() @ (kh.abs() + 16 * steps[0]).t()
+            e = (20 / 3) ** 0.5 * (2.0 ** -24 if dtype == "f32" else 2.0 ** -22) * sums
+            e = e + 3 ** -0.5 * (2.0 ** -22 if dtype == "f32" else 2.0 ** -11 if kernel == "block" else 0.0) * products
+            e = abs(scale) * e + 3 ** -0.5 * (2.0 ** -11 if kernel == "block" else 2.0 ** -20)
+            away = ((vh ** 2).sum(1)[None] - 2 * o @ vh.t() + (o ** 2).sum(1)[:, None]).clamp_min(0)
+            value = vh if kernel == "block" else vh - middle[1]
+            y = 3 ** -0.5 * (2.0 ** -22 if dtype == "f32" else 2.0 ** -11) * (value ** 2).sum(1).sqrt()
+            moved = ((p * e) ** 2 * away).sum(1).sqrt() + ((p * y[None]) ** 2).sum(1).sqrt()
+            length = (o ** 2).sum(1).sqrt()
+            chain = 2.0 ** -24 * (total / 16 + 64) ** 0.5 * (((p ** 2) @ (vh ** 2).sum(1)).sqrt() + length)
+            if dtype != "f32":
+                chain = chain + 2.0 ** -22 * p @ (8 * steps[1]).square().sum(1).sqrt()
+            out.append(o)
+            lim.append((half + 2.0 ** -23) * length + 6 * (moved + chain))
+    rows = lambda x, *s: torch.cat([torch.stack(x[i:i + heads], 1) for i in range(0, len(x), heads)])  # noqa: E731
+    return rows(out), rows(lim)

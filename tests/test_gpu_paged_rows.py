@@ -1,0 +1,98 @@
+"""Attention over the paged cache held row by row to what its roundings can do (the bound's own test:
+test_paged_bounds.py)."""
+import pytest
+import torch
+
+import serving as sv
+from test_gpu_paged import inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def check(ctx, kernel, dtype, past, new, kv_heads, heads, d, page=16, slots=0, pad=0, sharp=1.0, seed=0):
+    scale = sharp * d ** -0.5
+    total = [p + n for p, n in zip(past, new)]
+    width = max(-(-max(total) // page), -(-slots // page))
+    c = sv.Cache(ctx, total, kv_heads, d, page, seed=seed, width=width)
+    try:
+        k, v, _ = inputs(seed + 1, sum(total), kv_heads, d, "f32")
+        fill = c.batch([0] * len(total), total)
+        c.append(fill, k.to(sv.DEV), v.to(sv.DEV), "f32")
+        kv = c.read(fill)
+        rows = sum(new)
+        q = (1.2 * sv.normal(sv.gen(seed + 2), rows + pad, heads * d)).to(sv.DTYPES[dtype])
+        want, limit = sv.attention_rows(kv, q, past, new, kv_heads, heads, d, scale, dtype, kernel)
+        b, first = c.batch(past, new, pad=pad), None
+        for _ in range(3):          # the same every time, bit for bit
+            out = torch.full((rows + pad, heads * d), 7.0, dtype=sv.DTYPES[dtype], device=sv.DEV)
+            c.attend(b, q.to(sv.DEV), out, dtype, heads, scale)
+            out = out.cpu()
+            assert bool((out[rows:] == 7.0).all())
+            first = out if first is None else first
+            assert torch.equal(out, first)
+        off = ((first[:rows].reshape(want.shape).double() - want) ** 2).sum(2).sqrt() / limit
+        assert bool((off <= 1).all()), f"off by {float(off.max()):.2f} of the bound"
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("past,new,kv_heads,heads,d,page,slots,sharp", [
+    ([0], [1], 1, 1, 64, 16, 0, 1.0),
+    ([15, 16, 17, 0, 31, 300], [1, 1, 1, 0, 1, 1], 2, 12, 128, 16, 0, 1.0),
+    ([15, 16, 17, 0, 31, 300], [1, 1, 1, 0, 1, 1], 2, 12, 128, 16, 4096, 1.0),
+    ([1000, 3, 127, 128, 129], [1, 1, 1, 1, 1], 8, 32, 128, 64, 0, 1.0),
+    ([700, 0, 12], [5, 9, 2], 2, 8, 80, 32, 0, 2.0),
+    ([40, 700], [1, 3], 1, 16, 256, 16, 0, 1.0),
+    ([333], [1], 1, 40, 32, 128, 0, 1.0),
+    ([2000], [20], 4, 8, 128, 16, 0, 1.0),
+    ([5000, 20, 2600], [1, 1, 4], 1, 4, 128, 16, 0, 1.0),
+    ([9000], [33], 1, 2, 128, 1024, 0, 1.0),
+    ([511], [65], 1, 1, 128, 16, 0, 1.0),
+    ([300], [79], 1, 1, 96, 16, 2048, 1.0),          # a row fewer than a prompt has
+])
+def test_decode(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, slots, sharp):
+    check(gpu_ctx, "decode", dtype, past, new, kv_heads, heads, d, page, slots, sharp=sharp, seed=sum(past) + d)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("past,new,kv_heads,heads,d,page,slots,sharp", [
+    ([0], [80], 1, 1, 128, 16, 0, 1.0),
+    ([63, 64, 0, 0], [128, 63, 1, 200], 2, 2, 128, 32, 0, 1.0),
+    ([63, 64, 0, 0], [128, 63, 1, 200], 2, 2, 128, 32, 2048, 1.0),
+    ([1500], [130], 1, 2, 64, 16, 0, 1.0),
+    ([2000], [40], 1, 16, 128, 16, 0, 2.0),
+    ([900, 0, 1300], [90, 128, 40], 1, 4, 256, 64, 0, 1.0),
+    ([0, 33], [100, 77], 3, 6, 80, 16, 0, 1.0),
+])
+def test_prompts(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, slots, sharp):
+    check(gpu_ctx, "prompt", dtype, past, new, kv_heads, heads, d, page, slots, sharp=sharp, seed=sum(past) + d + 1, pad=2)
+
+
+@pytest.mark.parametrize("dtype,kernel", [("f32", "decode"), ("f16", "decode"), ("bf16", "decode"), ("f32", "prompt"), ("f16", "prompt"),
+                                          ("bf16", "block")])
+def test_every_slot_is_read(gpu_ctx, dtype, kernel):
+    """Keys of one direction, each larger than all before it by more than rounding: row i is slot i's
+    value, whatever page, tile, piece or part the slot lies in."""
+    n, d = 600, 64
+    step = 60 if kernel == "decode" else n          # rows of a call
+    c = sv.Cache(gpu_ctx, [n], 1, d, 16, width=128)
+    try:
+        g = sv.gen(5)
+        u = torch.where(torch.rand(d, generator=g) < 0.5, -1.0, 1.0)
+        u[0], u[1] = 1.0, -1.0
+        k = 2.0 ** (-8 + 20 * torch.arange(n) / n)[:, None] * u
+        v = sv.normal(g, n, d)
+        fill = c.batch([0], [n])
+        c.append(fill, k.to(sv.DEV), v.to(sv.DEV), "f32")
+        kv = c.read(fill)
+        # scores 64 * 2^-8 * 2^14 and up, 2.3 % apart
+        q = (u * 2.0 ** 7).repeat(step, 1).to(sv.DTYPES[dtype])
+        for first in range(0, n, step):
+            out = torch.zeros(step, d, dtype=sv.DTYPES[dtype], device=sv.DEV)
+            c.attend(c.batch([first], [step]), q.to(sv.DEV), out, dtype, 1, 128.0)
+            want = kv[1, first:first + step].double()
+            tol = (sv.HALF[dtype] + 2.0 ** -11 + 2.0 ** -20) * want.abs() + 2.0 ** -20 * 3 * v.abs().max()
+            assert bool(((out.cpu().double() - want).abs() <= tol).all())
+    finally:
+        c.close()

@@ -125,7 +125,26 @@ class Cache:
         self.ctx.paged_kv_destroy(self.h)
 
 
-# ---- attention: how far a row may be off -------------------------------------------
+# ---- attention: which kernel takes a batch, and how far a row may be off -----------
+
+
+def attention_path(dtype, past, new, kv_heads, heads, d, slots, pad=0):
+    """(kernel, split) that the library's rules on sizes give a batch whose table rows hold `slots`
+    slots: "block" (many bf16 rows), "prompt" or "decode" (16 rows), and whether a context may be
+    shared among workgroups."""
+    group, tokens, seqs = heads // kv_heads, max(1, sum(new) + pad), len(past)
+    width = 64 if d <= 64 else 128 if d <= 128 else 256
+    rows, used = tokens * group, min(seqs, tokens)
+    many = rows >= 80 * seqs
+    if many and dtype == "bf16" and (rows * kv_heads > 8192 or slots > 512):
+        block = 64 if width == 256 else 128
+        parts = max(1, min(8, 256 // ((rows + used * (block - 1)) // block * kv_heads)))
+        longest = max(min(p + n, slots) for p, n in zip(past, new) if n)
+        return "block", parts > 1 and -(-(-(-longest // 64)) // 2) > 4
+    groups = min(rows, rows // 16 + used) * kv_heads
+    eight = not many and width != 256 and groups < 256
+    longer = groups >= 256 or (eight and (dtype != "f32" or groups >= 16))
+    return "prompt" if many else "decode", slots > (1024 if longer else 512)
 
 
 def attention_rows(kv, q, past, new, kv_heads, heads, d, scale, dtype, kernel, gone=()):

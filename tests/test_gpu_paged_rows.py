@@ -1,5 +1,5 @@
 """Attention over the paged cache held row by row to what its roundings can do (the bound's own test:
-test_paged_bounds.py)."""
+test_paged_bounds.py), each case in the kernel that it names."""
 import pytest
 import torch
 
@@ -9,10 +9,12 @@ from test_gpu_paged import inputs
 pytestmark = pytest.mark.gpu
 
 
-def check(ctx, kernel, dtype, past, new, kv_heads, heads, d, page=16, slots=0, pad=0, sharp=1.0, seed=0):
+def check(ctx, kernel, dtype, past, new, kv_heads, heads, d, page=16, slots=0, pad=0, sharp=1.0, seed=0, split=None):
     scale = sharp * d ** -0.5
     total = [p + n for p, n in zip(past, new)]
     width = max(-(-max(total) // page), -(-slots // page))
+    got = sv.attention_path(dtype, past, new, kv_heads, heads, d, width * page, pad)
+    assert got[0] == kernel and (split is None or got[1] == split), got
     c = sv.Cache(ctx, total, kv_heads, d, page, seed=seed, width=width)
     try:
         k, v, _ = inputs(seed + 1, sum(total), kv_heads, d, "f32")
@@ -69,6 +71,35 @@ def test_prompts(gpu_ctx, dtype, past, new, kv_heads, heads, d, page, slots, sha
     check(gpu_ctx, "prompt", dtype, past, new, kv_heads, heads, d, page, slots, sharp=sharp, seed=sum(past) + d + 1, pad=2)
 
 
+def test_short_prompts_of_bf16(gpu_ctx):
+    """Few rows of short contexts stay in blocks of 16."""
+    for past, new, kv_heads, heads, d in (([0], [80], 1, 1, 128), ([63, 64, 0], [128, 100, 40], 2, 2, 128), ([7], [200], 1, 4, 256)):
+        check(gpu_ctx, "prompt", "bf16", past, new, kv_heads, heads, d, seed=d + new[0])
+
+
+@pytest.mark.parametrize("past,new,kv_heads,heads,d,page,slots,split", [
+    ([0], [80], 1, 1, 128, 16, 2048, False),                 # as many rows as the kernel takes: part of a block
+    ([0], [81], 1, 1, 96, 16, 2048, False),
+    ([0, 64], [96, 70], 1, 1, 64, 16, 1024, False),
+    ([63, 64, 0, 0], [128, 63, 1, 200], 2, 2, 128, 32, 1024, False),
+    ([700, 1200], [150, 30], 1, 2, 32, 16, 0, True),         # contexts that several workgroups share,
+    ([2100], [90], 1, 1, 80, 16, 0, True),
+    ([1500], [130], 1, 2, 64, 16, 0, True),
+    ([900, 0, 1300], [90, 128, 40], 1, 4, 256, 64, 0, True),
+    ([9000], [90], 1, 2, 128, 1024, 0, True),
+    ([3000], [40], 2, 8, 128, 32, 0, True),
+    ([511], [81], 1, 1, 128, 16, 0, True),                   # from five rounds on,
+    ([430], [82], 1, 1, 128, 16, 592, False),                # not of four
+    ([5], [85], 1, 2, 65, 16, 640, False),
+    ([0] * 9, [130, 128, 200, 64, 300, 127, 129, 1, 150], 2, 16, 64, 64, 0, False),
+    ([2000], [45], 1, 16, 128, 16, 0, True),
+    ([600], [1024], 8, 32, 128, 16, 0, False),               # as many blocks as the GPU has units for
+])
+def test_blocks_of_many_rows(gpu_ctx, past, new, kv_heads, heads, d, page, slots, split):
+    for pad, sharp in ((0, 1.0), (2, 1.0)):
+        check(gpu_ctx, "block", "bf16", past, new, kv_heads, heads, d, page, slots, pad, sharp, sum(past) + d + 2, split)
+
+
 @pytest.mark.parametrize("dtype,kernel", [("f32", "decode"), ("f16", "decode"), ("bf16", "decode"), ("f32", "prompt"), ("f16", "prompt"),
                                           ("bf16", "block")])
 def test_every_slot_is_read(gpu_ctx, dtype, kernel):
@@ -89,6 +120,7 @@ def test_every_slot_is_read(gpu_ctx, dtype, kernel):
         # scores 64 * 2^-8 * 2^14 and up, 2.3 % apart
         q = (u * 2.0 ** 7).repeat(step, 1).to(sv.DTYPES[dtype])
         for first in range(0, n, step):
+            assert sv.attention_path(dtype, [first], [step], 1, 1, d, 2048)[0] == kernel
             out = torch.zeros(step, d, dtype=sv.DTYPES[dtype], device=sv.DEV)
             c.attend(c.batch([first], [step]), q.to(sv.DEV), out, dtype, 1, 128.0)
             want = kv[1, first:first + step].double()

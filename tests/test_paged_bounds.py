@@ -80,3 +80,13 @@ def test_what_a_row_may_be_off(dtype, kernel, past, new, kv_heads, heads, d, sha
         for to in (torch.float16, torch.bfloat16):
             assert float(off(of=to).double().mean()) > 0.8, to
             assert sharp > 1 or float(off(weights=to).double().mean()) > 0.8, to
+
+
+def test_rows_are_told_apart():
+    """The kernels' sides as the cases of the GPU tests name them."""
+    path = sv.attention_path
+    assert path("bf16", [0], [79], 1, 1, 128, 2048) == ("decode", True)
+    assert path("bf16", [0], [80], 1, 1, 128, 2048)[0] == "block"
+    assert path("bf16", [0], [80], 1, 1, 128, 512)[0] == "prompt"
+    assert path("f16", [0], [80], 1, 1, 128, 2048) == ("prompt", True)
+    assert path("bf16", [511], [81], 1, 1, 128, 592) == ("block", True) and path("bf16", [430], [81], 1, 1, 128, 592) == ("block", False)

@@ -264,7 +264,8 @@ QWN_CUDA_ABI_API int qwn_hip_ext_kv_attention_device_noalloc(QwnCudaContextHandl
  * request struct of device pointers that a caller builds once and passes
  * every step; strides are in elements (0: rows back to back), and no pointer
  * needs more alignment than its element.  A request's outputs may not overlap
- * its inputs or each other except where it says so.  Sizes that only the device
+ * its inputs, the workspace or each other except where it says so: such a request
+ * is refused (columns of one wider buffer do not overlap).  Sizes that only the device
  * knows (a batch's row starts, cached lengths, page numbers, token ids) are read
  * there, so a captured step replays with new ones; each is checked there, and
  * what points outside the buffers that the host described is left out.  No
@@ -379,7 +380,8 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_read_device(QwnCudaContextHandle *cont
 /* Causal attention of the batch's rows over the cache, the batch's own tokens
  * appended before: token past[s] + i of sequence s attends to its slots 0 ..
  * past[s] + i, query head h to KV head h / (query_heads / kv_heads).  A row
- * that attends to nothing is zeros; a row whose query is not finite is NaN.
+ * that attends to nothing is zeros; a row whose query (or the scale) is not
+ * finite is NaN.  Scores may be of any size, past fp32's too.
  * fp32 queries are computed to fp32 (22 bits of query and probability in the
  * matrix products), f16 and bf16 ones with f16 probabilities, and bf16 batches
  * of many rows (80 of a KV head a sequence and more) with the keys and values

@@ -130,6 +130,9 @@ inline uint32_t stride_or(uint32_t stride, uint64_t row) {
     return stride ? stride : static_cast<uint32_t>(std::min<uint64_t>(row, UINT32_MAX));
 }
 
+// Bytes of an element of QWN_HIP_DTYPE_*.
+inline uint64_t dtype_bytes(uint32_t dtype) { return dtype == 0 ? 4 : 2; }
+
 // Makes `device` current for one call and the caller's device current again
 // after it.
 class DeviceScope {

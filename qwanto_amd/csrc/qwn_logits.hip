@@ -3,6 +3,7 @@
 #include "qwn_context.h"
 #include "qwn_device.h"
 #include "qwn_hip_ext.h"
+#include "qwn_overlap.h"
 #include "qwn_types.h"
 
 #include <algorithm>
@@ -276,6 +277,25 @@ QWN_CUDA_ABI_API int qwn_hip_ext_logits_process_device(QwnCudaContextHandle *han
         (r->mask && (a.mask_stride < (r->vocab + 31) / 32 || r->mask_rows == 0 || (!r->mask_index && r->mask_rows < r->rows))) ||
         (r->ids && (!r->workspace || (reinterpret_cast<uintptr_t>(r->workspace) & 7u)))) {
         set_error("invalid logits request: a history, biases, mask or workspace without what it needs");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    const uint64_t size = dtype_bytes(r->dtype), rows = r->rows;
+    const Rows in = row_block(r->logits, rows, r->vocab, a.in_stride, size), out = row_block(r->out, rows, r->vocab, a.out_stride, size);
+    const auto list = [](bool used, const void *p, uint64_t n) { return list_of_bytes(used ? p : nullptr, 4 * n); };
+    const bool history = r->history, biases = r->bias_tokens;
+    const Rows ids = list(true, r->ids, rows),
+               work = list_of_bytes(r->ids ? r->workspace : nullptr, qwn_hip_ext_logits_workspace_bytes(r->rows, r->vocab)),
+               mask = row_block(r->mask, r->mask_rows, (r->vocab + 31) / 32, a.mask_stride, 4);
+    const auto written = [&](const Rows &w) {
+        return overlaps_any(w, {list(true, r->history, r->history_capacity), list(history, r->history_starts, rows + 1),
+                                list(true, r->prompt_counts, rows), list(true, r->repetition, rows), list(true, r->presence, rows),
+                                list(true, r->frequency, rows), list(true, r->bias_tokens, r->bias_capacity),
+                                list(biases, r->bias_values, r->bias_capacity), list(biases, r->bias_starts, rows + 1), mask,
+                                list(r->mask, r->mask_index, rows)});
+    };
+    if ((!in_place(out, in) && overlap(out, in)) || overlaps_any(ids, {in, out, work}) || overlaps_any(work, {in, out}) || written(out) ||
+        written(ids) || written(work)) {
+        set_error("logits request: an output or the workspace overlaps an input or another output");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
     std::lock_guard<std::mutex> lock(ctx->mutex);

@@ -3,6 +3,7 @@
 #include "qwn_context.h"
 #include "qwn_device.h"
 #include "qwn_hip_ext.h"
+#include "qwn_overlap.h"
 #include "qwn_types.h"
 
 namespace {
@@ -235,10 +236,6 @@ QWN_CUDA_ABI_API int qwn_hip_ext_norm_quantize_device(QwnCudaContextHandle *hand
         set_error("invalid norm request");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
-    if (r->y && (r->y == r->x || r->y == r->residual || r->y == r->residual_out)) {
-        set_error("norm request: y may not be x, residual or residual_out");
-        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
-    }
     NormArgs a{};
     a.x = r->x;
     a.residual = r->residual;
@@ -258,6 +255,19 @@ QWN_CUDA_ABI_API int qwn_hip_ext_norm_quantize_device(QwnCudaContextHandle *hand
         a.q8_stride < a.cols || (a.residual_out == a.x && a.residual_out_stride != a.x_stride) ||
         (a.residual_out && a.residual_out == a.residual && a.residual_out_stride != a.residual_stride)) {
         set_error("norm request: a row stride is shorter than its row, or differs in place");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    const uint64_t size = dtype_bytes(r->dtype);
+    const Rows x = row_block(a.x, r->tokens, a.cols, a.x_stride, size), res = row_block(a.residual, r->tokens, a.cols, a.residual_stride, size),
+               out = row_block(a.residual_out, r->tokens, a.cols, a.residual_out_stride, size),
+               y = row_block(a.y, r->tokens, a.cols, a.y_stride, size),
+               q8 = row_block(a.q8, r->tokens, a.q8_stride, a.q8_stride, 1),
+               scales = list_of_bytes(a.q8 ? a.scales : nullptr, r->tokens * sizeof(float)),
+               norm = list_of_bytes(a.norm, a.cols * sizeof(float));
+    if ((!in_place(out, x) && overlap(out, x)) || (!in_place(out, res) && overlap(out, res)) ||
+        overlaps_any(y, {x, res, out, norm, q8, scales}) || overlaps_any(q8, {x, res, out, norm, scales}) ||
+        overlaps_any(scales, {x, res, out, norm}) || overlap(out, norm)) {
+        set_error("norm request: an output overlaps an input or another output");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
     std::lock_guard<std::mutex> lock(ctx->mutex);

@@ -1241,12 +1241,20 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_attention_device(QwnCudaContextHandle 
     }
     std::lock_guard<std::mutex> lock(ctx->mutex);
     AttnArgs a{};
-    if (!attention_of(ctx, h, r, a) || !r->query || !r->output || r->query == r->output || !r->workspace) {
+    if (!attention_of(ctx, h, r, a) || !r->query || !r->output || !r->workspace) {
         set_error("invalid paged attention request");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
     if (reinterpret_cast<uintptr_t>(r->workspace) & 15u) {
         set_error("paged attention workspace must be 16-byte aligned");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    const uint64_t channels = static_cast<uint64_t>(r->query_heads) * a.c.head_dim, size = dtype_bytes(r->dtype);
+    const Rows in = row_block(r->query, a.b.tokens, channels, a.query_stride, size),
+               out = row_block(r->output, a.b.tokens, channels, a.output_stride, size),
+               work = list_of_bytes(r->workspace, partial_bytes(a.c.width));
+    if (overlaps_any(out, {in, work}) || overlap(work, in) || overlaps_batch(out, a.b) || overlaps_batch(work, a.b)) {
+        set_error("paged attention: the output or the workspace overlaps an input or each other");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
     // row blocks and pieces of the batch at most: counted in 32 bits

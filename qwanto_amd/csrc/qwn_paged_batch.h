@@ -5,6 +5,7 @@
 #include "qwn_context.h"
 #include "qwn_hip_ext.h"
 #include "qwn_internal.h"
+#include "qwn_overlap.h"
 #include "qwn_paged.h"
 
 namespace qwn {
@@ -14,6 +15,13 @@ ResidentPaged *paged_of(Context *ctx, const QwnHipPagedKvHandle &h);
 
 // A caller's batch as kernels take it; false where it is not one.
 bool batch_of(const QwnHipPagedBatch *b, PagedBatch &out);
+
+// Whether what a call writes would change the batch that it reads.
+inline bool overlaps_batch(const Rows &out, const PagedBatch &b) {
+    const uint64_t n = b.sequences;
+    return overlaps_any(out, {list_of_bytes(b.starts, 4 * (n + 1)), list_of_bytes(b.past, 4 * n),
+                              list_of_bytes(b.table, 4 * n * b.table_stride)});
+}
 
 // A read of what no kernel of the call writes, at an address that every lane
 // shares: through the scalar cache, apart from the vector loads in flight.

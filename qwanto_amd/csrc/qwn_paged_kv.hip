@@ -609,6 +609,15 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_append_device(QwnCudaContextHandle *ha
         set_error("paged KV append request: a row stride is shorter than its row, or differs in place");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
+    const uint64_t size = dtype_bytes(r->dtype), rows = a.b.tokens;
+    const Rows in = row_block(r->query, rows, q_channels, a.query_stride, size),
+               out = row_block(r->query ? r->query_out : nullptr, rows, q_channels, a.query_out_stride, size);
+    if ((!in_place(out, in) && overlap(out, in)) || overlaps_batch(out, a.b) ||
+        overlaps_any(out, {row_block(r->key, rows, channels, a.key_stride, size), row_block(r->value, rows, channels, a.value_stride, size),
+                           list_of_bytes(r->positions, 4 * rows)})) {
+        set_error("paged KV append request: the rotated queries overlap an input");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
     DeviceScope device(ctx->device);
     if (device.error() != hipSuccess) return hip_fail("paged KV append device", device.error());
     a.c = rp->c;
@@ -651,6 +660,12 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_read_device(QwnCudaContextHandle *hand
     if (rp) a.stride = stride_or(stride, rp->c.kv_heads * rp->c.head_dim);
     if (!rp || a.stride < rp->c.kv_heads * rp->c.head_dim) {
         set_error("invalid paged KV read request");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    const uint32_t channels = rp->c.kv_heads * rp->c.head_dim;
+    const Rows k = row_block(keys, a.b.tokens, channels, a.stride, 4), v = row_block(values, a.b.tokens, channels, a.stride, 4);
+    if (overlap(k, v) || overlaps_batch(k, a.b) || overlaps_batch(v, a.b)) {
+        set_error("paged KV read: the keys, the values and the batch overlap");
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
     DeviceScope device(ctx->device);

@@ -128,3 +128,33 @@ def test_every_slot_is_read(gpu_ctx, dtype, kernel):
             assert bool(((out.cpu().double() - want).abs() <= tol).all())
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("dtype,kernel", [("f32", "prompt"), ("f16", "prompt"), ("bf16", "block")])
+def test_single_tokens_beside_a_prompt(gpu_ctx, dtype, kernel):
+    """Single tokens behind long contexts and a prompt's rows: in one call, and in a call each over the
+    same tensors."""
+    past, new, kv_heads, heads, d = [3000, 700, 5, 40], [1, 1, 1, 300], 2, 8, 128
+    check(gpu_ctx, kernel, dtype, past, new, kv_heads, heads, d, seed=71, pad=1)
+    total = [p + n for p, n in zip(past, new)]
+    c = sv.Cache(gpu_ctx, total, kv_heads, d)
+    try:
+        k, v, _ = inputs(72, sum(total), kv_heads, d, "f32")
+        fill = c.batch([0] * 4, total)
+        c.append(fill, k.to(sv.DEV), v.to(sv.DEV), "f32")
+        kv = c.read(fill)
+        rows, one = sum(new), 3
+        q = (1.2 * sv.normal(sv.gen(73), rows, heads * d)).to(sv.DTYPES[dtype])
+        qd, out = q.to(sv.DEV), torch.full((rows, heads * d), 7.0, dtype=sv.DTYPES[dtype], device=sv.DEV)
+        b = c.batch(past, new)
+        singles = gpu_ctx.paged_batch(one, one, b.starts, b.past, b.page_table, b.table_stride)
+        prompt = gpu_ctx.paged_batch(1, rows, b.starts + 4 * one, b.past + 4 * one, b.page_table + 4 * one * b.table_stride, b.table_stride)
+        c.attend(singles, qd, out, dtype, heads, d ** -0.5)
+        assert bool((out[one:] == 7.0).all()) and not bool((out[:one] == 7.0).all())
+        c.attend(prompt, qd, out, dtype, heads, d ** -0.5)
+        want, limit = (torch.cat(x) for x in zip(
+            sv.attention_rows(kv, q, past, new[:3] + [0], kv_heads, heads, d, d ** -0.5, dtype, "decode"),
+            sv.attention_rows(kv[:, sum(total[:3]):], q[3:], past[3:], new[3:], kv_heads, heads, d, d ** -0.5, dtype, kernel)))
+        assert bool((((out.cpu().reshape(want.shape).double() - want) ** 2).sum(2).sqrt() <= limit).all())
+    finally:
+        c.close()

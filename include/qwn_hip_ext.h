@@ -384,8 +384,9 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_read_device(QwnCudaContextHandle *cont
  * finite is NaN.  Scores may be of any size, past fp32's too.
  * fp32 queries are computed to fp32 (22 bits of query and probability in the
  * matrix products), f16 and bf16 ones with f16 probabilities, and bf16 batches
- * of many rows (80 of a KV head a sequence and more) with the keys and values
- * rounded to f16.  The output may not be the query.
+ * of many rows (80 of a KV head a sequence and more on average) with the keys and
+ * values rounded to f16.  The kernels are chosen by `tokens`, `sequences` and
+ * table_stride: prompts go best in a call apart from single tokens.  The output may not be the query.
  * The workspace (qwn_hip_ext_paged_kv_attention_workspace_bytes, the same for
  * every batch of a cache; 0 for a request that is refused; 16-byte aligned)
  * holds nothing between calls, and may not be shared by calls that run at the

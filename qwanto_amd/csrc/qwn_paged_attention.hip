@@ -73,7 +73,9 @@ constexpr uint32_t kWholeSlots = 512, kWholeSlotsMany = 1024, kMany = 256, kSome
 constexpr int kQueryBits = 15;                   // |query| < 2^15 in f16
 constexpr int kWeightBits = 11;                  // probability times step < 2^11 of the largest met,
 constexpr float kSlack = 4.0f;                   // and 2^4 more before the reference moves
-constexpr float kNothing = -3.402823466e38f;     // the largest product where none was seen: finite, what is taken off it too
+// The largest product where none was seen: finite, and any exponents' factor
+// (2^-100 and more) takes it past kSlack from every product.
+constexpr float kNothing = -3.402823466e38f;
 
 struct AttnArgs {
     PagedKv c;
@@ -291,16 +293,17 @@ __device__ __forceinline__ void load_tiles(const AttnArgs &a, const Pages &p, ui
     }
 }
 
-// What a row's products, of queries times `up` = 2^(bits it is divided by), are
-// multiplied by to be exponents of 2: positive, the scale's sign is the queries'.
-// Where nothing is left of it all scores are alike.  Where it passes fp32, two
-// products that differ (by 2^-100 at least: minima, steps and the largest query
-// have no smaller bits) are further apart than any exponent, with the largest
-// fp32 in its place as well.
+// What a row's products, of queries times the power of two `up`, are multiplied
+// by to be exponents of 2: positive, the scale's sign is the queries'.  Below
+// 2^-100 all scores are alike, as products are below 2^40.  Past fp32 the largest
+// fp32 stands in its place: products that differ (by far more than 2^-120, of
+// f16 minima and steps and a row's largest query) are further apart than any
+// exponent with either.
 __device__ __forceinline__ float exponents_of(float scale, int bits, float &up) {
     const float mul = fminf(ldexpf(fabsf(scale), bits) * 1.44269504088896340736f, 3.402823466e38f);
-    up = mul > 0.0f ? copysignf(up, scale) : 0.0f;
-    return mul > 0.0f ? mul : 1.0f;
+    const bool alike = mul < 0x1p-100f;
+    up = alike ? 0.0f : copysignf(up, scale);
+    return alike ? 1.0f : mul;
 }
 
 // The 8 channels of a query row from c0, zeros past the head's.
@@ -957,18 +960,18 @@ __global__ __launch_bounds__(2 * RW * kWaveSize, 2) void paged_block_attention_k
             }
             // a far reference is rounded by more than f16 has room for: then the
             // largest product is taken off first (for all rows 60.8 us for 58.2)
-            float from = ref[t];
-            if (__any(fabsf(from) > kFarRef)) {
+            float less = ref[t];
+            if (__any(fabsf(less) > kFarRef)) {
 #pragma unroll
                 for (uint32_t i = 0; i < kChunkTiles; ++i) sc[t][i] -= m[t];
-                from = -static_cast<float>(kRowBits);
+                less = -static_cast<float>(kRowBits);
             }
 #pragma unroll
             for (uint32_t i = 0; i < kChunkTiles / 2; ++i) {
                 float p[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(sc[t][2 * i + e / 4][e % 4], mul[t], -from));
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(sc[t][2 * i + e / 4][e % 4], mul[t], -less));
                 pf[t][i] = halves<1>(p).p[0];
             }
         }

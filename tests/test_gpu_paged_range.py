@@ -104,6 +104,43 @@ def test_scores_of_any_size_in_prompts(gpu_ctx, dtype, past, new, kv_heads, head
     check_sizes(gpu_ctx, dtype, past, new, kv_heads, heads, d, slots)
 
 
+@pytest.mark.parametrize("dtype,new", [("f32", 1), ("f16", 3), ("bf16", 2), ("f32", 90), ("f16", 90), ("bf16", 90)])
+def test_scales_next_to_nothing_and_not_finite(gpu_ctx, dtype, new):
+    """Rows with queries of all sizes, in one block: a scale that leaves nothing of the scores is a mean,
+    one that is not finite makes rows NaN, but for a row that attends to nothing."""
+    n, heads, d = 300, 2, 64
+    c = sv.Cache(gpu_ctx, [n], 1, d, width=128)
+    try:
+        k, v = (sv.normal(sv.gen(i), n, d) for i in (1, 2))
+        fill = c.batch([0], [n])
+        c.append(fill, k.to(sv.DEV), v.to(sv.DEV), "f32")
+        kv = c.read(fill)
+        dt = sv.DTYPES[dtype]
+        sizes = torch.tensor([1.0, 0.0, 2.0 ** -20, 2.0 ** 12] if dtype == "f16" else [1.0, 0.0, 2.0 ** -125, 2.0 ** 100, 2.0 ** -60])
+        q = (sv.normal(sv.gen(3), new, heads, d) * sizes[torch.arange(new * heads) % len(sizes)].reshape(new, heads, 1)).reshape(new, -1).to(dt)
+        path = sv.attention_path(dtype, [n - new], [new], 1, heads, d, 2048)[0]
+        b = c.batch([n - new], [new])
+        for scale in (0.0, 1e-45, -1e-40, 1e-36, 2.0 ** -103, 0.125, float("inf"), float("-inf"), float("nan")):
+            out = torch.full((new, heads * d), 7.0, dtype=dt, device=sv.DEV)
+            c.attend(b, q.to(sv.DEV), out, dtype, heads, scale)
+            got = out.cpu().double().reshape(new, heads, d)
+            if not math.isfinite(scale):
+                assert bool(torch.isnan(got).all()), scale
+                continue
+            want, limit = sv.attention_rows(kv, q, [n - new], [new], 1, heads, d, scale, dtype, path)
+            # rows whose scores are past what the bound's first order holds for are another test's
+            held = (scale * q.double().reshape(new, heads, d).abs().amax(2)).abs() < 3
+            off = ((got - want) ** 2).sum(2).sqrt() / limit
+            assert bool((off[held] <= 1).all()) and bool(torch.isfinite(got).all()), (scale, float(off[held].max()))
+        none = c.batch([n - new], [new], table=torch.full_like(c.table, -1))
+        for scale in (0.125, float("inf"), float("nan")):
+            out = torch.full((new, heads * d), 7.0, dtype=dt, device=sv.DEV)
+            c.attend(none, q.to(sv.DEV), out, dtype, heads, scale)
+            assert not bool(out.any())
+    finally:
+        c.close()
+
+
 @pytest.mark.parametrize("past,new,kv_heads,heads,d,slots", PROMPTS)
 def test_scores_of_any_size_in_blocks_of_many_rows(gpu_ctx, past, new, kv_heads, heads, d, slots):
     check_sizes(gpu_ctx, "bf16", past, new, kv_heads, heads, d, slots)

@@ -453,6 +453,163 @@ QWN_CUDA_ABI_API uint64_t qwn_hip_ext_logits_workspace_bytes(uint32_t rows, uint
 QWN_CUDA_ABI_API int qwn_hip_ext_logits_process_device(QwnCudaContextHandle *context,
                                                        const QwnHipLogitsRequest *request, void *stream);
 
+/* ---- operators of packed prompts and of beams ------------------------------
+ * Requests and their rules are those of a batched serving step (above). */
+
+/* Queries and keys of a step's tokens: each head normed where weights are given,
+ *   y = x * norm / sqrt(mean(x^2) + eps)
+ * then its first rope_dims (even, 0: none) channels rotated as pairs (i, i +
+ * rope_dims / 2) by positions[axis][token] * rope_theta^(-2 i / rope_dims).  Of
+ * the pairs, sections[0] belong to axis 0, sections[1] to axis 1, ... (they add
+ * up to rope_dims / 2): one section after the other, or, with in_turn not 0,
+ * dealt to the axes in turn, past those that have all of theirs.  Axes 0, 1 and 2
+ * may be time, height and width; text has the same position in all.  In 64 bits,
+ * rounded to fp32 and to dtype.  An output may be its input with that one's
+ * stride. */
+#define QWN_HIP_ROTARY_AXES 4u
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t tokens;
+    uint32_t dtype;
+    uint32_t query_heads;          /* 0: no queries */
+    uint32_t key_heads;            /* 0: no keys */
+    uint32_t head_dim;             /* up to 256 */
+    uint32_t rope_dims;
+    uint32_t sections[4];
+    uint32_t in_turn;
+    uint32_t query_stride;
+    uint32_t key_stride;
+    uint32_t query_out_stride;
+    uint32_t key_out_stride;
+    uint32_t position_stride;      /* 0: tokens */
+    float rope_theta;
+    float eps;
+    const void *query;             /* [tokens][query_stride]: [query_heads][head_dim] */
+    const void *key;               /* [tokens][key_stride]: [key_heads][head_dim] */
+    void *query_out;
+    void *key_out;
+    const float *query_norm;       /* NULL, or [head_dim] */
+    const float *key_norm;
+    const int32_t *positions;      /* [axes with a section][position_stride] */
+} QwnHipRotaryRequest;
+QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *context, const QwnHipRotaryRequest *request, void *stream);
+
+/* Causal attention of packed sequences over their own keys and values: row
+ * starts[s] + i of sequence s attends to the rows starts[s] .. starts[s] + i,
+ * query head h to KV head h / (query_heads / kv_heads).  Rows behind
+ * starts[sequences] belong to no sequence: they are not read, and the output
+ * keeps what it held there; a sequence whose rows do not lie in 0 .. tokens is
+ * left out.  Scores and sums are fp32, probabilities are rounded to dtype; fp32 is
+ * fp32 throughout.  Scores may be of any size, past fp32's too (of fp32 and bf16, a
+ * channel counts as zero where the key is below 2^-100, or the query below 2^-100 of
+ * its row's largest).  A row with a score that is NaN or infinite, or with a
+ * scale that is, is NaN; a value that is not finite makes its channel so in the
+ * rows that attend to it, and in no other.  For single tokens behind a cache:
+ * qwn_hip_ext_paged_kv_attention_device. */
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t sequences;
+    uint32_t tokens;               /* rows of the tensors */
+    uint32_t dtype;
+    uint32_t query_heads;          /* a multiple of kv_heads */
+    uint32_t kv_heads;
+    uint32_t head_dim;             /* up to 256 */
+    uint32_t query_stride;
+    uint32_t key_stride;
+    uint32_t value_stride;
+    uint32_t output_stride;
+    float scale;
+    uint32_t reserved;
+    const int32_t *starts;         /* device [sequences + 1], ascending */
+    const void *query;             /* [tokens][query_stride]: [query_heads][head_dim] */
+    const void *key;               /* [tokens][key_stride]: [kv_heads][head_dim] */
+    const void *value;             /* [tokens][value_stride] */
+    void *output;                  /* [tokens][output_stride] */
+} QwnHipPromptAttentionRequest;
+QWN_CUDA_ABI_API int qwn_hip_ext_prompt_attention_device(QwnCudaContextHandle *context,
+                                                         const QwnHipPromptAttentionRequest *request, void *stream);
+
+/* The best continuations of each sequence's beams.  Row s * beams + b of the
+ * logits is beam b of sequence s, whose log probabilities so far add up to
+ * scores[s][b]; token t continues it to
+ *   scores[s][b] + logits[t] - log(sum of exp(logits))
+ * Of a sequence's beams and tokens the `count` largest, in order (ties: the lower
+ * beam, then the lower token), as value, row and token: -inf, -1, -1 past the
+ * last.  next_*: of those the first `beams` whose token is none of end_tokens, the
+ * same way.  No candidates come from a beam whose score is not finite, from
+ * logits that are -inf or NaN (they do not count in the sum), or from a row with a
+ * logit of +inf.  The order is that of 64-bit values; `values` are rounded to fp32.
+ * The workspace (qwn_hip_ext_beam_select_workspace_bytes, 0 for sizes that are
+ * refused; 16-byte aligned) holds nothing between calls, and may not be shared by
+ * calls that run at the same time. */
+#define QWN_HIP_BEAM_MAX_BEAMS 32u
+#define QWN_HIP_BEAM_MAX_COUNT 64u
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t sequences;
+    uint32_t beams;                /* 1..32 */
+    uint32_t vocab;
+    uint32_t count;                /* candidates of a sequence, 1..64 */
+    uint32_t dtype;                /* of logits */
+    uint32_t in_stride;
+    uint32_t end_count;            /* of end_tokens, up to 4 */
+    int32_t end_tokens[4];
+    uint32_t reserved;
+    const void *logits;            /* [sequences * beams][in_stride] */
+    const float *scores;           /* [sequences][beams] */
+    float *values;                 /* [sequences][count] */
+    int32_t *parents;              /* [sequences][count]: rows of the logits */
+    int32_t *tokens;               /* [sequences][count] */
+    float *next_scores;            /* NULL (then all three), or [sequences][beams]; may be scores */
+    int32_t *next_parents;
+    int32_t *next_tokens;
+    void *workspace;
+} QwnHipBeamSelectRequest;
+QWN_CUDA_ABI_API uint64_t qwn_hip_ext_beam_select_workspace_bytes(uint32_t sequences, uint32_t beams, uint32_t vocab,
+                                                                  uint32_t count);
+QWN_CUDA_ABI_API int qwn_hip_ext_beam_select_device(QwnCudaContextHandle *context, const QwnHipBeamSelectRequest *request,
+                                                    void *stream);
+
+/* What the beams keep follows them: row r (of sequence r / beams) goes on from
+ * row parents[r] of its sequence, with that one's length past[p] + added, its
+ * history, to which tokens[r] comes as entry past[p] + added, and its pages.  Pages
+ * that are full are shared; the one in use goes on with the first row that has
+ * this parent, and each further one takes the page `spare` that it holds, to
+ * which the slots are copied in every cache given, and in exchange the page in
+ * use of a row that nothing goes on from becomes its spare.  Where the page in
+ * use has just become full, every row takes its spare as the next one, and has
+ * none (-1) until the caller hands it another.  So a row owns two pages, one in
+ * use and one spare, and no row's table names another's; the caller takes back
+ * full pages that no table names any more.  Table entries past the page in use are
+ * -1.  A row whose parent is none of its sequence (-1) goes on from itself, with no
+ * token; one whose parent's length is negative, too (its own negative: nothing of
+ * it changes).  Pages that are not the caches' are not copied to or from.  Tables and histories may be in
+ * place, lengths and spares may not. */
+#define QWN_HIP_BEAM_MAX_CACHES 256u
+typedef struct {
+    QwnCudaAbiHeader header;
+    uint32_t sequences;
+    uint32_t beams;                /* 1..32 */
+    uint32_t page_tokens;          /* of the caches */
+    uint32_t table_stride;         /* pages of a row of the tables */
+    uint32_t added;                /* tokens the step brought to each row */
+    uint32_t history_length;       /* entries of a row's history */
+    const int32_t *parents;        /* [rows] */
+    const int32_t *past;           /* [rows] */
+    int32_t *past_out;             /* [rows] */
+    const int32_t *page_table;     /* [rows][table_stride] */
+    int32_t *page_table_out;       /* may be page_table */
+    const int32_t *spare;          /* [rows] */
+    int32_t *spare_out;            /* [rows] */
+    const int32_t *tokens;         /* NULL, or [rows] */
+    const int32_t *history;        /* NULL, or [rows][history_length] */
+    int32_t *history_out;          /* may be history */
+} QwnHipBeamAdvanceRequest;
+/* `caches`: count handles of one shape (up to 256; 0: no pages are copied). */
+QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_beam_advance_device(QwnCudaContextHandle *context, const QwnHipPagedKvHandle *caches,
+                                                              uint32_t count, const QwnHipBeamAdvanceRequest *request,
+                                                              void *stream);
+
 /* Debug: the integer sums of the GEMV for one token, computed by the same
  * device code as the GEMV (host pointers, synchronous).  HyperVSQ-2:
  * out[row][block*8 + octant] = sum (code-1)*a; Q4_0: out[row][block] =

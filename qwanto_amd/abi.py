@@ -64,6 +64,8 @@ EXT_EXPORTS = (
     "qwn_hip_ext_paged_kv_append_device", "qwn_hip_ext_paged_kv_read_device",
     "qwn_hip_ext_paged_kv_attention_workspace_bytes", "qwn_hip_ext_paged_kv_attention_device",
     "qwn_hip_ext_logits_workspace_bytes", "qwn_hip_ext_logits_process_device",
+    "qwn_hip_ext_rotary_device", "qwn_hip_ext_prompt_attention_device", "qwn_hip_ext_beam_select_workspace_bytes",
+    "qwn_hip_ext_beam_select_device", "qwn_hip_ext_paged_kv_beam_advance_device",
 )
 DECODER_EXPORTS = (
     "qwn_hip_decoder_create", "qwn_hip_decoder_destroy", "qwn_hip_decoder_reset",
@@ -259,6 +261,39 @@ class LogitsRequest(_Versioned):
                 "workspace")
 
 
+class RotaryRequest(_Versioned):
+    _fields_ = [("header", Header)] + \
+        _fields(ctypes.c_uint32, "tokens", "dtype", "query_heads", "key_heads", "head_dim", "rope_dims") + \
+        [("sections", ctypes.c_uint32 * 4)] + \
+        _fields(ctypes.c_uint32, "in_turn", "query_stride", "key_stride", "query_out_stride", "key_out_stride",
+                "position_stride") + \
+        _fields(ctypes.c_float, "rope_theta", "eps") + \
+        _fields(ctypes.c_void_p, "query", "key", "query_out", "key_out", "query_norm", "key_norm", "positions")
+
+
+class PromptAttentionRequest(_Versioned):
+    _fields_ = [("header", Header)] + \
+        _fields(ctypes.c_uint32, "sequences", "tokens", "dtype", "query_heads", "kv_heads", "head_dim", "query_stride",
+                "key_stride", "value_stride", "output_stride") + \
+        [("scale", ctypes.c_float), ("reserved", ctypes.c_uint32)] + \
+        _fields(ctypes.c_void_p, "starts", "query", "key", "value", "output")
+
+
+class BeamSelectRequest(_Versioned):
+    _fields_ = [("header", Header)] + \
+        _fields(ctypes.c_uint32, "sequences", "beams", "vocab", "count", "dtype", "in_stride", "end_count") + \
+        [("end_tokens", ctypes.c_int32 * 4), ("reserved", ctypes.c_uint32)] + \
+        _fields(ctypes.c_void_p, "logits", "scores", "values", "parents", "tokens", "next_scores", "next_parents",
+                "next_tokens", "workspace")
+
+
+class BeamAdvanceRequest(_Versioned):
+    _fields_ = [("header", Header)] + \
+        _fields(ctypes.c_uint32, "sequences", "beams", "page_tokens", "table_stride", "added", "history_length") + \
+        _fields(ctypes.c_void_p, "parents", "past", "past_out", "page_table", "page_table_out", "spare", "spare_out",
+                "tokens", "history", "history_out")
+
+
 class Placement(ctypes.Structure):
     """QwnHipPlacement (the reference's QwnPlacement layout)."""
     _fields_ = [("name_hash", ctypes.c_uint64), ("byte_offset", ctypes.c_uint64),
@@ -394,6 +429,12 @@ class Library:
         lib.qwn_hip_ext_logits_workspace_bytes.argtypes = [U32, U32]
         lib.qwn_hip_ext_logits_workspace_bytes.restype = ctypes.c_uint64
         lib.qwn_hip_ext_logits_process_device.argtypes = [P(Handle), P(LogitsRequest), V]
+        lib.qwn_hip_ext_rotary_device.argtypes = [P(Handle), P(RotaryRequest), V]
+        lib.qwn_hip_ext_prompt_attention_device.argtypes = [P(Handle), P(PromptAttentionRequest), V]
+        lib.qwn_hip_ext_beam_select_workspace_bytes.argtypes = [U32, U32, U32, U32]
+        lib.qwn_hip_ext_beam_select_workspace_bytes.restype = ctypes.c_uint64
+        lib.qwn_hip_ext_beam_select_device.argtypes = [P(Handle), P(BeamSelectRequest), V]
+        lib.qwn_hip_ext_paged_kv_beam_advance_device.argtypes = [P(Handle), P(Handle), U32, P(BeamAdvanceRequest), V]
         lib.qwn_hip_ext_plan_residency.argtypes = [V, V, V, V, U32, ctypes.c_uint64, ctypes.c_uint64, V, V]
         lib.qwn_hip_decoder_create.argtypes = [P(Handle), P(DecoderDesc), P(Handle)]
         lib.qwn_hip_decoder_destroy.argtypes = [P(Handle), P(Handle)]
@@ -769,6 +810,73 @@ class Context:
     def logits_process_device(self, req: LogitsRequest, stream: int | None = None) -> None:
         self.lib.check("logits_process_device",
                        self.lib.lib.qwn_hip_ext_logits_process_device(self._h, ctypes.byref(req), stream))
+
+    # -- packed prompts and beams -------------------------------------------------
+    def rotary_request(self, tokens: int, dtype: str, head_dim: int, rope_dims: int, rope_theta: float,
+                       positions_ptr: int | None, sections=None, in_turn: bool = False, query_heads: int = 0,
+                       q_ptr: int | None = None, q_out_ptr: int | None = None, key_heads: int = 0,
+                       k_ptr: int | None = None, k_out_ptr: int | None = None, q_norm_ptr: int | None = None,
+                       k_norm_ptr: int | None = None, eps: float = 0.0, query_stride: int = 0, key_stride: int = 0,
+                       query_out_stride: int = 0, key_out_stride: int = 0, position_stride: int = 0) -> RotaryRequest:
+        """`sections`: pairs of each axis, up to 4 (None: all of them the first axis')."""
+        sections = [rope_dims // 2] if sections is None else list(sections)
+        return RotaryRequest(tokens=tokens, dtype=ACTIVATION[dtype], query_heads=query_heads, key_heads=key_heads,
+                             head_dim=head_dim, rope_dims=rope_dims, sections=(ctypes.c_uint32 * 4)(*sections),
+                             in_turn=int(in_turn), query_stride=query_stride, key_stride=key_stride,
+                             query_out_stride=query_out_stride, key_out_stride=key_out_stride,
+                             position_stride=position_stride, rope_theta=rope_theta, eps=eps, query=q_ptr, key=k_ptr,
+                             query_out=q_out_ptr, key_out=k_out_ptr, query_norm=q_norm_ptr, key_norm=k_norm_ptr,
+                             positions=positions_ptr)
+
+    def rotary_device(self, req: RotaryRequest, stream: int | None = None) -> None:
+        self.lib.check("rotary_device", self.lib.lib.qwn_hip_ext_rotary_device(self._h, ctypes.byref(req), stream))
+
+    def prompt_attention_request(self, sequences: int, tokens: int, starts_ptr: int, dtype: str, query_heads: int,
+                                 kv_heads: int, head_dim: int, q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int,
+                                 scale: float, query_stride: int = 0, key_stride: int = 0, value_stride: int = 0,
+                                 output_stride: int = 0) -> PromptAttentionRequest:
+        return PromptAttentionRequest(sequences=sequences, tokens=tokens, dtype=ACTIVATION[dtype], query_heads=query_heads,
+                                      kv_heads=kv_heads, head_dim=head_dim, query_stride=query_stride,
+                                      key_stride=key_stride, value_stride=value_stride, output_stride=output_stride,
+                                      scale=scale, starts=starts_ptr, query=q_ptr, key=k_ptr, value=v_ptr, output=out_ptr)
+
+    def prompt_attention_device(self, req: PromptAttentionRequest, stream: int | None = None) -> None:
+        self.lib.check("prompt_attention_device",
+                       self.lib.lib.qwn_hip_ext_prompt_attention_device(self._h, ctypes.byref(req), stream))
+
+    def beam_select_workspace_bytes(self, sequences: int, beams: int, vocab: int, count: int) -> int:
+        return int(self.lib.lib.qwn_hip_ext_beam_select_workspace_bytes(sequences, beams, vocab, count))
+
+    def beam_select_request(self, sequences: int, beams: int, vocab: int, count: int, dtype: str, logits_ptr: int,
+                            scores_ptr: int, values_ptr: int, parents_ptr: int, tokens_ptr: int, workspace_ptr: int,
+                            in_stride: int = 0, end_tokens=(), next_scores_ptr: int | None = None,
+                            next_parents_ptr: int | None = None, next_tokens_ptr: int | None = None) -> BeamSelectRequest:
+        return BeamSelectRequest(sequences=sequences, beams=beams, vocab=vocab, count=count, dtype=ACTIVATION[dtype],
+                                 in_stride=in_stride, end_count=len(end_tokens), end_tokens=(ctypes.c_int32 * 4)(*end_tokens),
+                                 logits=logits_ptr, scores=scores_ptr, values=values_ptr, parents=parents_ptr,
+                                 tokens=tokens_ptr, next_scores=next_scores_ptr, next_parents=next_parents_ptr,
+                                 next_tokens=next_tokens_ptr, workspace=workspace_ptr)
+
+    def beam_select_device(self, req: BeamSelectRequest, stream: int | None = None) -> None:
+        self.lib.check("beam_select_device",
+                       self.lib.lib.qwn_hip_ext_beam_select_device(self._h, ctypes.byref(req), stream))
+
+    def beam_advance_request(self, sequences: int, beams: int, page_tokens: int, table_stride: int, parents_ptr: int,
+                             past_ptr: int, past_out_ptr: int, table_ptr: int, table_out_ptr: int, spare_ptr: int,
+                             spare_out_ptr: int, added: int = 1, tokens_ptr: int | None = None,
+                             history_ptr: int | None = None, history_out_ptr: int | None = None,
+                             history_length: int = 0) -> BeamAdvanceRequest:
+        return BeamAdvanceRequest(sequences=sequences, beams=beams, page_tokens=page_tokens, table_stride=table_stride,
+                                  added=added, history_length=history_length, parents=parents_ptr, past=past_ptr,
+                                  past_out=past_out_ptr, page_table=table_ptr, page_table_out=table_out_ptr,
+                                  spare=spare_ptr, spare_out=spare_out_ptr, tokens=tokens_ptr, history=history_ptr,
+                                  history_out=history_out_ptr)
+
+    def paged_kv_beam_advance_device(self, caches, req: BeamAdvanceRequest, stream: int | None = None) -> None:
+        """`caches`: the layers' paged caches, all of one shape."""
+        arr = (Handle * max(1, len(caches)))(*caches)
+        self.lib.check("paged_kv_beam_advance_device", self.lib.lib.qwn_hip_ext_paged_kv_beam_advance_device(
+            self._h, arr, len(caches), ctypes.byref(req), stream))
 
     # -- misc -----------------------------------------------------------------
     def telemetry(self) -> Telemetry:

@@ -21,7 +21,7 @@ LIB = os.path.join(LIBDIR, "libqwn_hip.so")
 LOADER_NAME = os.path.join(LIBDIR, "qwn_cuda.so")
 SOURCES = ["qwn_runtime.hip", "qwn_gemv.hip", "qwn_attention.hip", "qwn_decoder.hip", "qwn_noalloc.hip",
            "qwn_head.hip", "qwn_block_attention.hip", "qwn_wide_gemm.hip", "qwn_norm.hip", "qwn_paged_kv.hip",
-           "qwn_paged_attention.hip", "qwn_logits.hip"]
+           "qwn_paged_attention.hip", "qwn_logits.hip", "qwn_rotary.hip", "qwn_prompt_attention.hip", "qwn_beam.hip"]
 ARCH = os.environ.get("QWN_HIP_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

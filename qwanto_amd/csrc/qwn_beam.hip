@@ -1,0 +1,552 @@
+// Beams: the best continuations of each sequence's beams over the vocabulary
+// (qwn_hip_ext_beam_select_device), and what the beams keep following them
+// (qwn_hip_ext_paged_kv_beam_advance_device).
+#include "qwn_context.h"
+#include "qwn_device.h"
+#include "qwn_hip_ext.h"
+#include "qwn_overlap.h"
+#include "qwn_paged.h"
+#include "qwn_paged_batch.h"
+#include "qwn_types.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace qwn;
+
+// ---- selection --------------------------------------------------------------
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kBeamsMost = QWN_HIP_BEAM_MAX_BEAMS, kCountMost = QWN_HIP_BEAM_MAX_COUNT;
+constexpr uint32_t kNone = 0xffffffffu;
+constexpr int kLoads = 4;               // vectors of 16 bytes that a thread takes of a row
+template <typename T>
+constexpr uint32_t kSlice = kThreads * kLoads * (16 / sizeof(T));  // tokens of the vocabulary a workgroup takes
+
+// Candidates in order: a larger value, then the smaller place, is the larger key;
+// 0 is none.  Of a row, places are tokens and values fp32 logits; of a sequence,
+// places are beams and tokens and values 64 bits.
+__device__ __forceinline__ uint64_t row_key(float v, uint32_t token) {
+    if (!(v > -INFINITY)) return 0;  // -inf and NaN are no candidates
+    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // -0 is 0
+    const uint32_t ord = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    return (static_cast<uint64_t>(ord) << 32) | (kNone - token);
+}
+__device__ __forceinline__ float row_value(uint64_t key) {
+    const uint32_t ord = static_cast<uint32_t>(key >> 32);
+    return __builtin_bit_cast(float, (ord & 0x80000000u) ? ord & 0x7fffffffu : ~ord);
+}
+__device__ __forceinline__ uint32_t row_token(uint64_t key) { return kNone - static_cast<uint32_t>(key); }
+
+struct BeamKey {
+    uint64_t value, place;  // ordered bits of the value; ~(beam, token)
+};
+__device__ __forceinline__ bool larger(uint64_t a, uint64_t b) { return a > b; }
+__device__ __forceinline__ bool larger(const BeamKey &a, const BeamKey &b) {
+    return a.value > b.value || (a.value == b.value && a.place > b.place);
+}
+__device__ __forceinline__ void clear(uint64_t &k) { k = 0; }
+__device__ __forceinline__ void clear(BeamKey &k) { k.value = k.place = 0; }
+__device__ __forceinline__ bool some(uint64_t k) { return k != 0; }
+__device__ __forceinline__ bool some(const BeamKey &k) { return k.value != 0; }
+
+// The `count` largest of the workgroup's keys, N a thread, largest first, in
+// list[0 .. count); none where there are fewer.  The result does not fall below the
+// count-th largest of the threads' own largest keys, and no more than count * N
+// keys are as large; of those, each one's place is the number that are larger.
+// found: room for kCountMost * N keys.
+template <typename K>
+struct Held {
+    K bound;
+    uint32_t count;
+};
+template <int N, typename K>
+__device__ __forceinline__ void select_keys(const K (&keys)[N], uint32_t count, K *tops, K *found, Held<K> *held, K *list) {
+    const uint32_t tid = threadIdx.x;
+    K top = keys[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+        if (larger(keys[i], top)) top = keys[i];
+    tops[tid] = top;
+    if (tid == 0) {
+        held->count = 0;
+        clear(held->bound);
+    }
+    for (uint32_t i = tid; i < count; i += kThreads) clear(list[i]);
+    lds_barrier();
+    uint32_t rank = 0;
+    for (uint32_t i = 0; i < kThreads; ++i) rank += larger(tops[i], top) ? 1u : 0u;
+    if (rank == count - 1 && some(top)) held->bound = top;  // one thread's: keys differ, unless they are none
+    lds_barrier();
+    if (rank < count) {
+        const K bound = held->bound;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (some(keys[i]) && !larger(bound, keys[i])) found[atomicAdd(&held->count, 1u)] = keys[i];
+    }
+    lds_barrier();
+    const uint32_t n = held->count;
+    for (uint32_t e = tid; e < n; e += kThreads) {
+        const K mine = found[e];
+        uint32_t place = 0;
+        for (uint32_t i = 0; i < n; ++i) place += larger(found[i], mine) ? 1u : 0u;
+        if (place < count) list[place] = mine;
+    }
+    lds_barrier();
+}
+
+struct SelectArgs {
+    const void *logits;
+    const float *scores;
+    float *values, *next_scores;
+    int32_t *parents, *tokens, *next_parents, *next_tokens;
+    float2 *sums;        // [rows][parts]: the largest logit of a part, the sum of exp(logit - it)
+    uint64_t *keys;      // [rows][parts][count]
+    uint32_t beams, vocab, count, in_stride, parts, end_count;
+    int32_t end_tokens[4];
+};
+
+// grid (parts of the vocabulary, rows): a part's largest logits and its share of
+// the sum, in one pass over them.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void beam_rows_kernel(SelectArgs a) {
+    constexpr int VEC = 16 / sizeof(T), N = kLoads * VEC;
+    __shared__ uint64_t tops[kThreads], found[kCountMost * N], list[kCountMost];
+    __shared__ Held<uint64_t> held;
+    __shared__ float2 red[kThreads / kWaveSize];
+    const uint32_t r = blockIdx.y, v0 = blockIdx.x * kSlice<T>, tid = threadIdx.x;
+    const T *in = static_cast<const T *>(a.logits) + static_cast<size_t>(r) * a.in_stride;
+    float x[N];
+    uint64_t keys[N];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+        const uint32_t v = v0 + (tid + kThreads * k) * VEC;
+        if (v + VEC <= a.vocab) {
+            const Vec<T, VEC> t = load_vec<T, VEC>(in + v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[k * VEC + i] = to_float(t.v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[k * VEC + i] = v + i < a.vocab ? to_float(in[v + i]) : -INFINITY;
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    m = wave_max_all(m);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t v = v0 + (tid + kThreads * (i / VEC)) * VEC + i % VEC;
+        keys[i] = row_key(x[i], v);
+        s += x[i] > -INFINITY ? expf(x[i] - m) : 0.0f;
+    }
+    s = wave_sum_all(s);
+    if (tid % kWaveSize == 0) red[tid / kWaveSize] = make_float2(m, s);
+    select_keys(keys, a.count, tops, found, &held, list);
+    const size_t part = static_cast<size_t>(r) * a.parts + blockIdx.x;
+    for (uint32_t i = tid; i < a.count; i += kThreads) a.keys[part * a.count + i] = list[i];
+    if (tid == 0) {
+        float top = red[0].x, sum = 0.0f;
+        for (uint32_t w = 1; w < kThreads / kWaveSize; ++w) top = fmaxf(top, red[w].x);
+        for (uint32_t w = 0; w < kThreads / kWaveSize; ++w) sum += red[w].x > -INFINITY ? red[w].y * expf(red[w].x - top) : 0.0f;
+        a.sums[part] = make_float2(top, sum);
+    }
+}
+
+// grid (sequences): the rows' sums, and the largest of their parts' candidates.
+__global__ __launch_bounds__(kThreads) void beam_sequences_kernel(SelectArgs a) {
+    constexpr int N = 4;
+    __shared__ BeamKey tops[kThreads], found[kCountMost * N], list[kCountMost];
+    __shared__ double base[kBeamsMost], most[kBeamsMost];  // of a beam: its score less the logarithm of its sum, -inf: no
+                                                           // candidates; its largest logit
+    __shared__ Held<BeamKey> held;
+    const uint32_t tid = threadIdx.x, lane = tid % kWaveSize, wave = tid / kWaveSize, row0 = blockIdx.x * a.beams;
+    for (uint32_t b = wave; b < a.beams; b += kThreads / kWaveSize) {
+        const float2 *sums = a.sums + static_cast<size_t>(row0 + b) * a.parts;
+        const float score = a.scores[row0 + b];
+        float m = -INFINITY;
+        for (uint32_t i = lane; i < a.parts; i += kWaveSize) m = fmaxf(m, sums[i].x);
+        m = wave_max_all(m);
+        double s = 0.0;
+        for (uint32_t i = lane; i < a.parts; i += kWaveSize)
+            if (sums[i].x > -INFINITY) s += static_cast<double>(sums[i].y) * exp(static_cast<double>(sums[i].x) - static_cast<double>(m));
+        s = wave_sum_f64(s);
+        if (lane == 0) {
+            base[b] = isfinite(m) && isfinite(score) ? static_cast<double>(score) - log(s) : -INFINITY;
+            most[b] = m;
+        }
+    }
+    lds_barrier();
+    const uint32_t of_row = a.parts * a.count, all = a.beams * of_row;
+    const uint64_t *keys = a.keys + static_cast<size_t>(row0) * of_row;
+    for (uint32_t i0 = 0; i0 == 0 || i0 < all;) {
+        // what is left of the round before, and the next keys
+        BeamKey k[N];
+        const bool first = i0 == 0;
+        const uint32_t step = first ? N * kThreads : (N - 1) * kThreads;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            clear(k[e]);
+            if (!first && e == N - 1) {
+                if (tid < a.count) k[e] = list[tid];
+                continue;
+            }
+            const uint32_t i = i0 + tid + kThreads * e;
+            if (i >= all) continue;
+            const uint64_t key = keys[i];
+            const uint32_t b = i / of_row;
+            if (key == 0 || !(base[b] > -INFINITY)) continue;
+            const uint64_t v = __builtin_bit_cast(uint64_t, base[b] + (static_cast<double>(row_value(key)) - most[b]) + 0.0);
+            k[e].value = (v >> 63) ? ~v : (v | 1ull << 63);
+            k[e].place = ~(static_cast<uint64_t>(b) << 32 | row_token(key));
+        }
+        i0 += step;
+        lds_barrier();  // the list is read
+        select_keys(k, a.count, tops, found, &held, list);
+    }
+    // the list is one wave's: place, and place among those that go on
+    if (wave > 0) return;
+    const size_t out = static_cast<size_t>(blockIdx.x) * a.count, next = static_cast<size_t>(blockIdx.x) * a.beams;
+    float value = -INFINITY;
+    int32_t parent = -1, token = -1;
+    const bool real = lane < a.count && some(list[lane]);
+    if (real) {
+        const uint64_t o = list[lane].value, place = ~list[lane].place;
+        value = static_cast<float>(__builtin_bit_cast(double, (o >> 63) ? o & ~(1ull << 63) : ~o));
+        parent = static_cast<int32_t>(row0 + static_cast<uint32_t>(place >> 32));
+        token = static_cast<int32_t>(static_cast<uint32_t>(place));
+    }
+    if (lane < a.count) {
+        a.values[out + lane] = value;
+        a.parents[out + lane] = parent;
+        a.tokens[out + lane] = token;
+    }
+    if (!a.next_scores) return;
+    bool goes = real;
+    for (uint32_t i = 0; i < a.end_count; ++i) goes = goes && token != a.end_tokens[i];
+    const uint64_t on = __ballot(goes);
+    const uint32_t place = __popcll(on & ((1ull << lane) - 1)), n = __popcll(on);
+    if (goes && place < a.beams) {
+        a.next_scores[next + place] = value;
+        a.next_parents[next + place] = parent;
+        a.next_tokens[next + place] = token;
+    }
+    if (lane >= n && lane < a.beams) {
+        a.next_scores[next + lane] = -INFINITY;
+        a.next_parents[next + lane] = -1;
+        a.next_tokens[next + lane] = -1;
+    }
+}
+
+uint32_t parts_of(uint32_t vocab, uint32_t slice) { return (vocab + slice - 1) / slice; }
+// sums, then keys: of the type with the most parts
+uint64_t sums_bytes(uint64_t rows, uint64_t parts) { return (rows * parts * sizeof(float2) + 15) / 16 * 16; }
+
+template <typename T>
+hipError_t launch_select(SelectArgs a, uint32_t sequences, void *workspace, hipStream_t stream) {
+    const uint32_t rows = sequences * a.beams;
+    a.parts = parts_of(a.vocab, kSlice<T>);
+    a.sums = static_cast<float2 *>(workspace);
+    a.keys = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + sums_bytes(rows, a.parts));
+    hipLaunchKernelGGL(beam_rows_kernel<T>, dim3(a.parts, rows), dim3(kThreads), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(beam_sequences_kernel, dim3(sequences), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+bool select_sizes(uint32_t sequences, uint32_t beams, uint32_t vocab, uint32_t count) {
+    return sequences > 0 && beams > 0 && beams <= kBeamsMost && static_cast<uint64_t>(sequences) * beams <= 65535 && vocab > 0 &&
+           vocab <= 1u << 24 && count > 0 && count <= kCountMost;
+}
+
+// ---- what the beams keep ------------------------------------------------------
+
+constexpr uint32_t kCachesMost = QWN_HIP_BEAM_MAX_CACHES;
+
+struct AdvanceArgs {
+    const int32_t *parents, *past, *table, *spare, *tokens, *history;
+    int32_t *past_out, *table_out, *spare_out, *history_out;
+    uint32_t beams, page_shift, table_stride, added, history_length;
+};
+struct CopyArgs {
+    AdvanceArgs a;
+    PagedKv c;
+    uint8_t *pools[kCachesMost];
+};
+
+// Where row r of its sequence goes on from, and its length then; false: from
+// none, nothing of it changes.
+struct Goes {
+    uint32_t parent;   // row
+    uint32_t length;
+    bool token;        // not from itself for want of a parent
+};
+__device__ __forceinline__ bool goes_on(const AdvanceArgs &a, uint32_t row0, uint32_t r, Goes &g) {
+    const int32_t p = a.parents[r];
+    g.token = p >= static_cast<int32_t>(row0) && p < static_cast<int32_t>(row0 + a.beams) && a.past[p] >= 0;
+    g.parent = g.token ? static_cast<uint32_t>(p) : r;
+    const int32_t past = a.past[g.parent];
+    if (past < 0) return false;
+    g.length = static_cast<uint32_t>(min(static_cast<int64_t>(past) + a.added, static_cast<int64_t>(0x7fffffff)));
+    return true;
+}
+__device__ __forceinline__ int32_t page_of(const AdvanceArgs &a, uint32_t row, uint32_t at) {
+    return at < a.table_stride ? a.table[static_cast<size_t>(row) * a.table_stride + at] : -1;
+}
+
+// What the rows of a sequence are to each other: a lane a row (lanes past them: none).
+struct Kin {
+    bool goes;        // the lane's row is one, and goes on
+    bool later;       // not its parent's first child
+    Goes g;
+    uint64_t laters, childless;
+};
+__device__ __forceinline__ Kin kin_of(const AdvanceArgs &a, uint32_t row0, uint32_t lane) {
+    Kin k{};
+    const bool row = lane < a.beams;
+    k.goes = row && goes_on(a, row0, row0 + lane, k.g);
+    const uint32_t mine = k.goes ? k.g.parent - row0 : kNone;
+    uint64_t parents = 0;
+    for (uint32_t b = 0; b < a.beams; ++b) {
+        const uint32_t p = lane_of(mine, static_cast<int>(b));
+        if (b < lane && p == mine) k.later = k.goes;
+        if (p != kNone) parents |= 1ull << p;
+    }
+    k.laters = __ballot(k.later);
+    k.childless = __ballot(row && !((parents >> lane) & 1ull));
+    return k;
+}
+
+// grid (rows, caches, at least one): the slots of the parent's page in use to the
+// row's spare, in one cache; the first of a row's workgroups writes its length
+// and the spare it gets.  Bytes bound it.
+__global__ __launch_bounds__(kThreads) void beam_copy_kernel(CopyArgs args) {
+    const AdvanceArgs &a = args.a;
+    const uint32_t r = blockIdx.x, row0 = r / a.beams * a.beams, lane = threadIdx.x % kWaveSize;
+    const Kin k = kin_of(a, row0, lane);
+    const int b = static_cast<int>(r - row0);
+    const bool goes = lane_of(k.goes, b), later = lane_of(k.later, b);
+    const uint32_t parent = lane_of(k.g.parent, b), length = lane_of(k.g.length, b);
+    const uint32_t full = length >> a.page_shift, used = length & ((1u << a.page_shift) - 1);
+    const int32_t spare = a.spare[r];
+    if (blockIdx.y == 0 && threadIdx.x == 0) {
+        int32_t next = spare;
+        if (goes && used == 0) {
+            next = -1;
+        } else if (goes && later) {
+            // of the rows that nothing goes on from, the one with this row's place among those that copy
+            uint64_t left = k.childless;
+            for (uint64_t before = k.laters & ((1ull << b) - 1); before; before &= before - 1) left &= left - 1;
+            next = -1;
+            if (left) {
+                const uint32_t q = row0 + __ffsll(static_cast<unsigned long long>(left)) - 1;
+                const int64_t past = static_cast<int64_t>(a.past[q]) + a.added;
+                if (a.past[q] >= 0 && (past & ((1 << a.page_shift) - 1)))
+                    next = page_of(a, q, static_cast<uint32_t>(min(past >> a.page_shift, static_cast<int64_t>(a.table_stride))));
+            }
+        }
+        a.past_out[r] = goes ? static_cast<int32_t>(length) : a.past[r];
+        a.spare_out[r] = next;
+    }
+    if (!goes || !later || used == 0 || !args.pools[blockIdx.y]) return;
+    const PagedKv &c = args.c;
+    const int32_t from = page_of(a, parent, full);
+    if (from < 0 || static_cast<uint32_t>(from) >= c.pages || spare < 0 || static_cast<uint32_t>(spare) >= c.pages || from == spare) return;
+    const uint32_t tiles = (used + kPagedTile - 1) / kPagedTile, words = tiles * (paged_block_bytes(c.width) / 16);
+    for (uint32_t i = threadIdx.x; i < c.kv_heads * words; i += kThreads) {
+        const uint32_t head = i / words, w = i % words;
+        uint8_t *pool = args.pools[blockIdx.y];
+        reinterpret_cast<uint4 *>(pool + paged_block_at(c, static_cast<uint32_t>(spare), 0, head))[w] =
+            reinterpret_cast<const uint4 *>(pool + paged_block_at(c, static_cast<uint32_t>(from), 0, head))[w];
+    }
+}
+
+// grid (columns, sequences): a thread moves a column of the table or of the
+// histories in all of the sequence's rows, reading all of them first, so that they
+// may be in place.
+__global__ __launch_bounds__(kThreads) void beam_rows_move_kernel(AdvanceArgs a, uint32_t table_groups) {
+    const uint32_t row0 = blockIdx.y * a.beams, lane = threadIdx.x % kWaveSize;
+    const Kin k = kin_of(a, row0, lane);
+    const bool table = blockIdx.x < table_groups;
+    const uint32_t column = (table ? blockIdx.x : blockIdx.x - table_groups) * kThreads + threadIdx.x;
+    const uint32_t stride = table ? a.table_stride : a.history_length;
+    const bool in = column < stride;
+    const int32_t *from = table ? a.table : a.history;
+    int32_t *to = table ? a.table_out : a.history_out;
+    int32_t v[kBeamsMost];
+#pragma unroll
+    for (uint32_t b = 0; b < kBeamsMost; ++b) {
+        v[b] = 0;
+        if (b >= a.beams) continue;
+        const bool goes = lane_of(k.goes, b), later = lane_of(k.later, b), token = lane_of(k.g.token, b);
+        const uint32_t parent = goes ? lane_of(k.g.parent, b) : row0 + b, length = lane_of(k.g.length, b);
+        if (in) v[b] = from[static_cast<size_t>(parent) * stride + column];
+        if (!goes) continue;
+        if (table) {
+            const uint32_t full = length >> a.page_shift, used = length & ((1u << a.page_shift) - 1);
+            if (column == full && (used == 0 || later)) v[b] = a.spare[row0 + b];
+            if (column > full) v[b] = -1;
+        } else if (token && a.tokens && column == length) {
+            v[b] = a.tokens[row0 + b];
+        }
+    }
+    if (!in) return;
+#pragma unroll
+    for (uint32_t b = 0; b < kBeamsMost; ++b)
+        if (b < a.beams) to[static_cast<size_t>(row0 + b) * stride + column] = v[b];
+}
+
+}  // namespace
+
+extern "C" {
+
+QWN_CUDA_ABI_API uint64_t qwn_hip_ext_beam_select_workspace_bytes(uint32_t sequences, uint32_t beams, uint32_t vocab,
+                                                                  uint32_t count) {
+    if (!select_sizes(sequences, beams, vocab, count)) return 0;
+    const uint64_t rows = static_cast<uint64_t>(sequences) * beams, parts = parts_of(vocab, kSlice<float>);
+    return sums_bytes(rows, parts) + rows * parts * count * sizeof(uint64_t);
+}
+
+QWN_CUDA_ABI_API int qwn_hip_ext_beam_select_device(QwnCudaContextHandle *handle, const QwnHipBeamSelectRequest *r, void *stream) {
+    Context *ctx = context_of(handle);
+    if (!ctx || !r || !header_ok(*r) || r->sequences == 0 || r->beams == 0 || r->vocab == 0 || r->count == 0 || !r->logits || !r->scores ||
+        !r->values || !r->parents || !r->tokens || !r->workspace || (reinterpret_cast<uintptr_t>(r->workspace) & 15u) ||
+        r->dtype > QWN_HIP_DTYPE_BF16 || r->end_count > 4 || !r->next_scores != !r->next_parents || !r->next_scores != !r->next_tokens) {
+        set_error("invalid beam selection request");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    if (!select_sizes(r->sequences, r->beams, r->vocab, r->count)) {
+        set_error("unsupported beam selection: %u sequences of %u beams, %u candidates of %u tokens", r->sequences, r->beams, r->count,
+                  r->vocab);
+        return QWN_CUDA_STATUS_UNSUPPORTED;
+    }
+    SelectArgs a{};
+    a.in_stride = stride_or(r->in_stride, r->vocab);
+    if (a.in_stride < r->vocab) {
+        set_error("beam selection request: a row stride is shorter than its row");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    const uint64_t rows = static_cast<uint64_t>(r->sequences) * r->beams, found = static_cast<uint64_t>(r->sequences) * r->count;
+    const Rows logits = row_block(r->logits, rows, r->vocab, a.in_stride, dtype_bytes(r->dtype)), scores = list_of_bytes(r->scores, 4 * rows);
+    const Rows outs[7] = {list_of_bytes(r->workspace, qwn_hip_ext_beam_select_workspace_bytes(r->sequences, r->beams, r->vocab, r->count)),
+                          list_of_bytes(r->values, 4 * found),      list_of_bytes(r->parents, 4 * found),
+                          list_of_bytes(r->tokens, 4 * found),      list_of_bytes(r->next_parents, 4 * rows),
+                          list_of_bytes(r->next_tokens, 4 * rows),  list_of_bytes(r->next_scores, 4 * rows)};
+    bool bad = false;
+    for (int i = 0; i < 7; ++i) {
+        bad = bad || overlap(outs[i], logits) || (overlap(outs[i], scores) && !(i == 6 && in_place(outs[i], scores)));
+        for (int k = 0; k < i; ++k) bad = bad || overlap(outs[i], outs[k]);
+    }
+    if (bad) {
+        set_error("beam selection request: an output or the workspace overlaps an input or another output");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    std::lock_guard<std::mutex> lock(ctx->mutex);
+    DeviceScope device(ctx->device);
+    if (device.error() != hipSuccess) return hip_fail("beam selection device", device.error());
+    a.logits = r->logits;
+    a.scores = r->scores;
+    a.values = r->values;
+    a.parents = r->parents;
+    a.tokens = r->tokens;
+    a.next_scores = r->next_scores;
+    a.next_parents = r->next_parents;
+    a.next_tokens = r->next_tokens;
+    a.beams = r->beams;
+    a.vocab = r->vocab;
+    a.count = r->count;
+    a.end_count = r->end_count;
+    std::copy(r->end_tokens, r->end_tokens + 4, a.end_tokens);
+    hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
+    const hipError_t e = r->dtype == QWN_HIP_DTYPE_F32   ? launch_select<float>(a, r->sequences, r->workspace, s)
+                         : r->dtype == QWN_HIP_DTYPE_F16 ? launch_select<f16>(a, r->sequences, r->workspace, s)
+                                                         : launch_select<bf16>(a, r->sequences, r->workspace, s);
+    return e == hipSuccess ? QWN_CUDA_STATUS_OK : hip_fail("beam selection launch", e);
+}
+
+QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_beam_advance_device(QwnCudaContextHandle *handle, const QwnHipPagedKvHandle *caches,
+                                                              uint32_t count, const QwnHipBeamAdvanceRequest *r, void *stream) {
+    Context *ctx = context_of(handle);
+    if (!ctx || (count && !caches) || !r || !header_ok(*r) || r->sequences == 0 || r->beams == 0 || r->table_stride == 0 || !r->parents ||
+        !r->past || !r->past_out || !r->page_table || !r->page_table_out || !r->spare || !r->spare_out || !r->history != !r->history_out ||
+        (r->history && r->history_length == 0) || r->page_tokens < kPagedTile || r->page_tokens > 1024 ||
+        (r->page_tokens & (r->page_tokens - 1)) || r->added > 0x7fffffffu) {
+        set_error("invalid beam advance request");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    const uint64_t rows = static_cast<uint64_t>(r->sequences) * r->beams;
+    const uint64_t table_groups = (static_cast<uint64_t>(r->table_stride) + kThreads - 1) / kThreads;
+    const uint64_t history_groups = r->history ? (static_cast<uint64_t>(r->history_length) + kThreads - 1) / kThreads : 0;
+    if (r->beams > kBeamsMost || rows > 65535 || count > kCachesMost) {
+        set_error("unsupported beam advance: %u sequences of %u beams, %u caches", r->sequences, r->beams, count);
+        return QWN_CUDA_STATUS_UNSUPPORTED;
+    }
+    const Rows table = row_block(r->page_table, rows, r->table_stride, r->table_stride, 4),
+               history = row_block(r->history, rows, r->history_length, r->history_length, 4);
+    const Rows lists[4] = {list_of_bytes(r->parents, 4 * rows), list_of_bytes(r->past, 4 * rows), list_of_bytes(r->spare, 4 * rows),
+                           list_of_bytes(r->tokens, 4 * rows)};
+    const Rows outs[4] = {row_block(r->page_table_out, rows, r->table_stride, r->table_stride, 4),
+                          row_block(r->history_out, rows, r->history_length, r->history_length, 4), list_of_bytes(r->past_out, 4 * rows),
+                          list_of_bytes(r->spare_out, 4 * rows)};
+    bool bad = false;
+    for (int i = 0; i < 4; ++i) {
+        for (const Rows &x : lists) bad = bad || overlap(outs[i], x);
+        for (int k = 0; k < i; ++k) bad = bad || overlap(outs[i], outs[k]);
+        bad = bad || (overlap(outs[i], table) && !(i == 0 && in_place(outs[i], table))) ||
+              (overlap(outs[i], history) && !(i == 1 && in_place(outs[i], history)));
+    }
+    if (bad) {
+        set_error("beam advance request: an output overlaps an input or another output");
+        return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+    }
+    std::lock_guard<std::mutex> lock(ctx->mutex);
+    CopyArgs c{};
+    for (uint32_t i = 0; i < count; ++i) {
+        ResidentPaged *rp = paged_of(ctx, caches[i]);
+        if (!rp) {
+            set_error("paged KV-cache handle is not resident in this context");
+            return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+        }
+        if (i == 0) c.c = rp->c;
+        if (rp->c.page_tokens != r->page_tokens || rp->c.pages != c.c.pages || rp->c.kv_heads != c.c.kv_heads || rp->c.width != c.c.width) {
+            set_error("beam advance request: the caches are not of one shape, or not of pages of %u tokens", r->page_tokens);
+            return QWN_CUDA_STATUS_INVALID_ARGUMENT;
+        }
+        c.pools[i] = rp->c.pool;
+    }
+    DeviceScope device(ctx->device);
+    if (device.error() != hipSuccess) return hip_fail("beam advance device", device.error());
+    AdvanceArgs &a = c.a;
+    a.parents = r->parents;
+    a.past = r->past;
+    a.past_out = r->past_out;
+    a.table = r->page_table;
+    a.table_out = r->page_table_out;
+    a.spare = r->spare;
+    a.spare_out = r->spare_out;
+    a.tokens = r->tokens;
+    a.history = r->history;
+    a.history_out = r->history_out;
+    a.beams = r->beams;
+    while ((1u << a.page_shift) < r->page_tokens) ++a.page_shift;
+    a.table_stride = r->table_stride;
+    a.added = r->added;
+    a.history_length = r->history_length;
+    hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
+    // the copies read the tables as they were: a launch of their own
+    hipLaunchKernelGGL(beam_copy_kernel, dim3(static_cast<uint32_t>(rows), std::max(1u, count)), dim3(kThreads), 0, s, c);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) {
+        hipLaunchKernelGGL(beam_rows_move_kernel, dim3(static_cast<uint32_t>(table_groups + history_groups), r->sequences), dim3(kThreads), 0,
+                           s, a, static_cast<uint32_t>(table_groups));
+        e = hipGetLastError();
+    }
+    if (e != hipSuccess) return hip_fail("beam advance launch", e);
+    ctx->telemetry.kv_cache_kernel_count++;
+    return QWN_CUDA_STATUS_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,336 @@
+"""Causal attention of packed sequences (qwn_hip_ext_prompt_attention_device), each row against the
+definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import serving as sv
+from qwanto_amd import abi
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_of(q, k, v, lengths, heads, kv_heads, d, scale, dtype):
+    """64-bit attention of packed q, k, v, and how far each row and head may be off in the 2-norm:
+    ([rows][heads][d], [rows][heads]).
+
+    With scores off by e_t and weights by w_t of themselves, a row o = sum p_t v_t moves by
+    sum p_t (e_t + w_t) (v_t - o); a weight that is rounded only where it meets a value, by r_t, moves
+    it by sum p_t r_t v_t.  These are roundings, of zero mean and independent from token to token, the
+    largest r (r / sqrt 3 in the root mean square): the sum is held to 6 times the root of its squares'.
+    - a score is a chain of at most d / 2 fp32 sums, 2^-24 each of the magnitudes |q| |k|;
+    - an exponent is rounded to fp32: 2^-24 of |log2 p_t|, at most 2^-19 where p_t counts; its
+      power of 2 by 2^-23;
+    - a probability that meets a value is rounded to the type (fp32's is not).
+    The sums over n tokens are chains of n / 2 + 64 fp32 sums of magnitudes that grow as the root of
+    the squares' sum and as the output.  On top the output's own rounding."""
+    half, group = sv.HALF[dtype], heads // kv_heads
+    out, lim, at = [], [], 0
+    for n in lengths:
+        if not n:
+            continue
+        qs, ks, vs = (x[at:at + n].double().reshape(n, -1, d) for x in (q, k, v))
+        at += n
+        later = torch.ones(n, n).triu(1) > 0
+        for h in range(heads):
+            kh, vh, qh = ks[:, h // group], vs[:, h // group], qs[:, h]
+            p = torch.softmax((qh @ kh.t() * scale).masked_fill(later, -math.inf), dim=1)
+            o = p @ vh
+            e = abs(scale) * (d / 6) ** 0.5 * 2.0 ** -24 * (qh.abs() @ kh.abs().t()) + 2.0 ** -19
+            away = ((vh ** 2).sum(1)[None] - 2 * o @ vh.t() + (o ** 2).sum(1)[:, None]).clamp_min(0)
+            moved = ((p * e) ** 2 * away).sum(1).sqrt()
+            length = (o ** 2).sum(1).sqrt()
+            squares = ((p ** 2) @ (vh ** 2).sum(1)).sqrt()
+            if dtype != "f32":
+                moved = moved + 3 ** -0.5 * half * squares
+            chain = 2.0 ** -24 * (n / 2 + 64) ** 0.5 * (squares + length)
+            out.append(o)
+            lim.append((half + 2.0 ** -23) * length + 6 * (moved + chain))
+    rows = lambda x: torch.cat([torch.stack(x[i:i + heads], 1) for i in range(0, len(x), heads)])  # noqa: E731
+    return rows(out), rows(lim)
+
+
+def inputs(seed, rows, heads, kv_heads, d, dtype):
+    g = sv.gen(seed)
+    scale = 0.3 + 1.2 * torch.rand(kv_heads * d, generator=g)
+    dt = sv.DTYPES[dtype]
+    return ((1.2 * sv.normal(g, rows, heads * d)).to(dt), (sv.normal(g, rows, kv_heads * d) * scale + 0.3).to(dt),
+            (sv.normal(g, rows, kv_heads * d) * scale.flip(0)).to(dt))
+
+
+def starts_of(lengths):
+    return torch.tensor([sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=torch.int32)
+
+
+def attend(ctx, q, k, v, lengths, heads, kv_heads, d, scale, dtype, out=None, starts=None, rows=None, **strides):
+    """The output of tensors on the host or the GPU; rows that no sequence has keep 5."""
+    dev = [x.to(sv.DEV) for x in (q, k, v)]
+    if out is None:
+        out = torch.full(dev[0].shape, 5.0, dtype=dev[0].dtype, device=sv.DEV)
+    st = (starts if starts is not None else starts_of(lengths)).to(sv.DEV)
+    r = ctx.prompt_attention_request(st.numel() - 1, rows or q.shape[0], sv.ptr(st), dtype, heads, kv_heads, d, *(sv.ptr(x) for x in dev),
+                                     sv.ptr(out), scale, **strides)
+    ctx.prompt_attention_device(r, stream=sv.stream())
+    torch.cuda.synchronize()
+    return out
+
+
+def check(got, q, k, v, lengths, heads, kv_heads, d, scale, dtype):
+    n = sum(lengths)
+    want, lim = rows_of(q, k, v, lengths, heads, kv_heads, d, scale, dtype)
+    off = (got[:n].cpu().double().reshape(n, heads, d) - want).square().sum(-1).sqrt()
+    assert bool((off <= lim).all()), float((off / lim).max())
+    assert bool((got[n:] == 5.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d,lengths,pad", [
+    (1, 1, 64, [1], 0),
+    (12, 2, 128, [1, 2, 3], 2),
+    (2, 2, 128, [31, 0, 32, 33], 1),
+    (4, 2, 64, [63, 64, 65], 0),
+    (3, 1, 128, [127, 128, 129, 0], 3),
+    (32, 8, 128, [200, 1, 17], 0),
+    (4, 1, 32, [150, 9], 0),
+    (2, 1, 80, [100, 40], 1),
+    (6, 2, 96, [70, 71], 0),
+    (2, 1, 256, [90, 161], 0),
+    (5, 5, 1, [40], 0),
+    (2, 1, 33, [77, 5], 0),
+    (2, 1, 200, [65], 0),
+    (129, 1, 64, [3, 70], 0),
+    (8, 1, 128, [600], 0),
+    (2, 2, 64, [1000, 300], 0),
+    (1, 1, 128, [2500], 0),
+])
+def test_sizes(gpu_ctx, dtype, heads, kv_heads, d, lengths, pad):
+    q, k, v = inputs(d + sum(lengths), sum(lengths) + pad, heads, kv_heads, d, dtype)
+    got = attend(gpu_ctx, q, k, v, lengths, heads, kv_heads, d, d ** -0.5, dtype)
+    check(got, q, k, v, lengths, heads, kv_heads, d, d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_sequences(gpu_ctx, dtype):
+    """More sequences than a wave has lanes, most of one token and some of none."""
+    lengths = [(i * 7) % 5 for i in range(200)] + [130] + [1] * 70
+    q, k, v = inputs(3, sum(lengths), 4, 2, 64, dtype)
+    got = attend(gpu_ctx, q, k, v, lengths, 4, 2, 64, 0.125, dtype)
+    check(got, q, k, v, lengths, 4, 2, 64, 0.125, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d,odd", [(4, 2, 128, 0), (6, 2, 64, 1), (2, 1, 80, 3), (2, 1, 33, 0)])
+def test_columns_of_one_buffer(gpu_ctx, dtype, heads, kv_heads, d, odd):
+    """Queries, keys and values side by side in a projection's rows, at any alignment, the output in
+    a wider one: the same to the bit, and nothing beside it is touched."""
+    lengths = [90, 41]
+    n = sum(lengths)
+    q, k, v = inputs(odd + d, n, heads, kv_heads, d, dtype)
+    want = attend(gpu_ctx, q, k, v, lengths, heads, kv_heads, d, 0.1, dtype)
+    edge = torch.full((n, odd), float("nan")).to(q.dtype)
+    buf = torch.cat([edge, q, k, v, edge], dim=1).to(sv.DEV).contiguous()
+    out = torch.full((n, heads * d + 2 * odd + 5), 5.0, dtype=q.dtype, device=sv.DEV)
+    w, a, b = buf.shape[1], odd + heads * d, odd + (heads + kv_heads) * d
+    attend(gpu_ctx, buf[:, odd:], buf[:, a:], buf[:, b:], lengths, heads, kv_heads, d, 0.1, dtype, out=out[:, odd:], query_stride=w,
+           key_stride=w, value_stride=w, output_stride=out.shape[1])
+    assert torch.equal(out[:, odd:odd + heads * d], want)
+    assert bool((out[:, :odd] == 5.0).all()) and bool((out[:, odd + heads * d:] == 5.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_what_is_masked_does_not_count(gpu_ctx, dtype, d):
+    """Keys and values that are not finite, or the type's largest, behind a row and in other sequences
+    leave it as it was to the bit; in front of it they show in it, values in their channel alone."""
+    heads, kv_heads, lengths = 4, 2, [150, 70]
+    q, k, v = inputs(d, 221, heads, kv_heads, d, dtype)
+    k[220], v[220] = float("nan"), float("nan")                  # of no sequence
+    clean = attend(gpu_ctx, q, k, v, lengths, heads, kv_heads, d, 0.1, dtype)
+    top = torch.finfo(q.dtype).max
+    for t, bad in ((149, float("nan")), (100, float("inf")), (128, -float("inf")), (37, float("nan")), (149, top), (0, float("nan"))):
+        kb, vb = k.clone(), v.clone()
+        kb[t, :d] = bad
+        vb[t, d + 3] = bad
+        rows = torch.arange(221)
+        before = (rows < t) | (rows >= 150)
+        got = attend(gpu_ctx, q, k, vb, lengths, heads, kv_heads, d, 0.1, dtype).cpu()
+        assert torch.equal(got[before], clean.cpu()[before]), (t, bad)
+        after = got[t:150].reshape(150 - t, heads, d)
+        others = torch.ones(heads, d, dtype=torch.bool)
+        others[2:, 3] = False
+        assert torch.equal(after[:, others], clean[t:150].cpu().reshape(150 - t, heads, d)[:, others]), (t, bad)
+        if bad != top:
+            assert not bool(torch.isfinite(after[:, 2:, 3]).any()), (t, bad)
+            if not math.isnan(bad):
+                assert bool((after[:, 2:, 3] == bad).all()), (t, bad)
+        got = attend(gpu_ctx, q, kb, v, lengths, heads, kv_heads, d, 0.1, dtype).cpu()
+        assert torch.equal(got[before], clean.cpu()[before]), (t, bad)
+        assert torch.equal(got[:, 2 * d:], clean[:, 2 * d:].cpu()), (t, bad)      # the other KV head
+        if math.isnan(bad):
+            assert bool(torch.isnan(got[t:150, :2 * d]).all()), (t, bad)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_values_of_both_infinities(gpu_ctx, dtype):
+    q, k, v = inputs(1, 40, 1, 1, 64, dtype)
+    v[10, 7], v[20, 7], v[15, 9] = math.inf, -math.inf, -math.inf
+    got = attend(gpu_ctx, q, k, v, [40], 1, 1, 64, 0.125, dtype).cpu()
+    assert bool(torch.isfinite(got[:10]).all())
+    assert bool((got[10:20, 7] == math.inf).all()) and bool(torch.isnan(got[20:, 7]).all())
+    assert bool((got[15:, 9] == -math.inf).all())
+    rest = [c for c in range(64) if c not in (7, 9)]
+    assert bool(torch.isfinite(got[:, rest]).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_size,k_size,scale", [(1.0, 1.0, -0.3), (1.0, 1.0, 0.0), (60.0, 60.0, 1.0), (3e4, 3e4, 1.0), (3e4, 3e4, -1e30),
+                                                 (1e-4, 1.0, 1e4), (1.0, 1.0, 1e-40), (1.0, 1.0, 3e38)])
+def test_scores_of_any_size(gpu_ctx, dtype, q_size, k_size, scale):
+    """Against the definition in 64 bits: softmax of scores whose largest is far from the next is the
+    value of one token."""
+    lengths, d = [70, 33], 64
+    g = sv.gen(5)
+    dt = sv.DTYPES[dtype]
+    q, k, v = ((s * (2 * torch.rand(103, d, generator=g) - 1)).to(dt) for s in (q_size, k_size, 1.0))
+    got = attend(gpu_ctx, q, k, v, lengths, 1, 1, d, scale, dtype)
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    want, lim = rows_of(q, k, v, lengths, 1, 1, d, scale, dtype)
+    off = (got.cpu().double().reshape(103, 1, d) - want).square().sum(-1).sqrt()
+    # where scores are so large that their own roundings decide between tokens, the row is one or the other
+    clear = []
+    at = 0
+    for n in lengths:
+        s = (q[at:at + n].double() @ k[at:at + n].double().t() * scale).masked_fill(torch.ones(n, n).triu(1) > 0, -math.inf)
+        e = abs(scale) * (d / 2) * 2.0 ** -24 * (q[at:at + n].double().abs() @ k[at:at + n].double().abs().t())
+        best = s.topk(min(2, n), dim=1).values
+        gap = best[:, 0] - best[:, -1] if n > 1 else torch.full((n,), math.inf, dtype=torch.float64)
+        clear.append((gap > 2 * e.max(dim=1).values + 40) | (e.max(dim=1).values < 1e-3))
+        at += n
+    clear = torch.cat(clear)
+    assert bool(clear.float().mean() > 0.9)
+    assert bool((off[clear] <= lim[clear] + 1e-9).all())
+    assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scores_past_fp32(gpu_ctx, dtype):
+    """Products past fp32's largest: the row is the value of its best token."""
+    d = 64
+    g = sv.gen(6)
+    dt = sv.DTYPES[dtype]
+    q, k, v = ((s * (2 * torch.rand(50, d, generator=g) - 1)).to(dt) for s in (1e37, 1e38, 1.0))
+    for scale in (1.0, -1e20, 1e-30):
+        got = attend(gpu_ctx, q, k, v, [50], 1, 1, d, scale, dtype).cpu().double()
+        s = (q.double() @ k.double().t() * scale).masked_fill(torch.ones(50, 50).triu(1) > 0, -math.inf)
+        want = v.double()[s.argmax(dim=1)]
+        assert bool(((got - want).abs() <= (sv.HALF[dtype] + 2.0 ** -22) * want.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_queries_and_scales_that_are_not_finite(gpu_ctx, dtype):
+    q, k, v = inputs(2, 40, 2, 1, 64, dtype)
+    clean = attend(gpu_ctx, q, k, v, [40], 2, 1, 64, 0.125, dtype).cpu()
+    for bad in (math.nan, math.inf, -math.inf):
+        b = q.clone()
+        b[7, 64 + 5] = bad
+        got = attend(gpu_ctx, b, k, v, [40], 2, 1, 64, 0.125, dtype).cpu()
+        assert bool(torch.isnan(got[7, 64:]).all())
+        got[7, 64:] = clean[7, 64:]
+        assert torch.equal(got, clean)
+        assert bool(torch.isnan(attend(gpu_ctx, q, k, v, [40], 2, 1, 64, bad, dtype)).all())
+
+
+def test_starts_that_are_none(gpu_ctx):
+    """Sequences whose rows do not lie in the batch are left out, the others are not."""
+    q, k, v = inputs(4, 100, 2, 1, 64, "bf16")
+    for starts, good in (([0, 30, 101], [(0, 30)]), ([-1, 30, 60], [(30, 60)]), ([40, 10, 60], [(10, 60)]), ([0, 0, 0], []),
+                         ([5, 2 ** 31 - 1, 7], []), ([20, 100, 100], [(20, 100)]), ([0, -2 ** 31, 9], [])):
+        got = attend(gpu_ctx, q, k, v, None, 2, 1, 64, 0.125, "bf16", starts=torch.tensor(starts, dtype=torch.int32))
+        kept = torch.ones(100, dtype=torch.bool)
+        for a, b in good:
+            part = got[a:b]
+            check(part, q[a:b], k[a:b], v[a:b], [b - a], 2, 1, 64, 0.125, "bf16")
+            kept[a:b] = False
+        assert bool((got.cpu()[kept] == 5.0).all()), starts
+
+
+def test_rows_far_apart(gpu_ctx):
+    """Row offsets past 32 bits."""
+    stride, n, d = 2 ** 31 + 8, 5, 64
+    q, k, v = inputs(9, n, 1, 1, d, "bf16")
+    want = attend(gpu_ctx, q, k, v, [n], 1, 1, d, 0.125, "bf16")
+    buf = torch.empty((n - 1) * stride + 4 * d, dtype=torch.bfloat16, device=sv.DEV)
+    wide = torch.as_strided(buf, (n, 4 * d), (stride, 1))
+    wide.copy_(torch.cat([q, k, v, torch.full_like(q, 5.0)], dim=1))
+    cols = [wide[:, i * d:(i + 1) * d] for i in range(4)]
+    attend(gpu_ctx, *cols[:3], [n], 1, 1, d, 0.125, "bf16", out=cols[3], query_stride=stride, key_stride=stride, value_stride=stride,
+           output_stride=stride)
+    assert torch.equal(cols[3], want)
+
+
+def test_refusals(gpu_ctx):
+    n, d = 6, 64
+    buf = torch.zeros(n + 1, 6 * d, device=sv.DEV)
+    st = torch.tensor([0, n], dtype=torch.int32, device=sv.DEV)
+    at = lambda row, col: sv.ptr(buf) + (row * 6 * d + col) * 4  # noqa: E731
+
+    def req(**kw):
+        base = dict(sequences=1, tokens=n, starts_ptr=sv.ptr(st), dtype="f32", query_heads=2, kv_heads=1, head_dim=d, q_ptr=at(0, 0),
+                    k_ptr=at(0, 2 * d), v_ptr=at(0, 3 * d), out_ptr=at(0, 4 * d), scale=0.1, query_stride=6 * d, key_stride=6 * d,
+                    value_stride=6 * d, output_stride=6 * d)
+        base.update(kw)
+        return gpu_ctx.prompt_attention_request(**base)
+
+    def status(r):
+        with pytest.raises(abi.AbiError) as e:
+            gpu_ctx.prompt_attention_device(r, stream=sv.stream())
+        return e.value.status
+
+    for good in (req(), req(v_ptr=at(0, 2 * d)), req(k_ptr=at(0, 0))):
+        gpu_ctx.prompt_attention_device(good, stream=sv.stream())
+    for bad in (dict(sequences=0), dict(tokens=0), dict(starts_ptr=None), dict(query_heads=0), dict(kv_heads=0), dict(head_dim=0),
+                dict(q_ptr=None), dict(k_ptr=None), dict(v_ptr=None), dict(out_ptr=None), dict(query_stride=d), dict(key_stride=d - 1),
+                dict(value_stride=1), dict(output_stride=2 * d - 1), dict(out_ptr=at(0, 0)), dict(out_ptr=at(0, 1)), dict(out_ptr=at(1, d)),
+                dict(out_ptr=at(0, 3 * d + 1)), dict(out_ptr=at(0, 2 * d - 1)), dict(out_ptr=sv.ptr(st) - 4, output_stride=2 * d)):
+        assert status(req(**bad)) == -1, bad
+    for bad in (dict(head_dim=257, query_stride=0, key_stride=0, value_stride=0, output_stride=0), dict(query_heads=3, kv_heads=2, head_dim=16),
+                dict(tokens=2 ** 31 - 1, out_ptr=at(0, 0) + 2 ** 50)):
+        assert status(req(**bad)) == -5, bad
+    r = req()
+    r.dtype = 3
+    assert status(r) == -1
+    r = req()
+    r.header.abi_version = 2
+    assert status(r) == -1
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_captured_and_on_two_streams(gpu_ctx, dtype):
+    """Recorded once and replayed with other sequences, eager calls on another stream between: the same
+    to the bit, and rows of no sequence stay."""
+    n, heads, kv_heads, d = 400, 4, 2, 128
+    q, k, v = (x.to(sv.DEV) for x in inputs(7, n, heads, kv_heads, d, dtype))
+    st = torch.zeros(4, dtype=torch.int32, device=sv.DEV)
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    req = lambda o: gpu_ctx.prompt_attention_request(3, n, sv.ptr(st), dtype, heads, kv_heads, d, sv.ptr(q), sv.ptr(k), sv.ptr(v),  # noqa: E731
+                                                     sv.ptr(o), 0.1)
+    r, e = req(out), req(want)
+    gpu_ctx.prompt_attention_device(e, stream=sv.stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu_ctx.prompt_attention_device(r, stream=sv.stream())
+    side = torch.cuda.Stream()
+    for starts in ([0, 400, 400, 400], [0, 1, 200, 333], [0, 0, 130, 260], [0, 399, 399, 400]):
+        st.copy_(torch.tensor(starts, dtype=torch.int32))
+        out.fill_(2.0)
+        want.fill_(2.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            gpu_ctx.prompt_attention_device(e, stream=sv.stream())
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), starts
+        assert bool((out[starts[-1]:] == 2.0).all())

@@ -37,9 +37,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kWaves = 4, kThreads = kWaves * kWaveSize;
 constexpr uint32_t kWaveRows = 32, kBlockRows = kWaves * kWaveRows;
-constexpr float kSlack = 8.0f;               // exponents of 2 that a row's products may pass the reference by
 constexpr float kFar = 0x1p20f;               // of references: past it their rounding would be more than 2^-4 of an exponent
-constexpr float kNothing = -3.402823466e38f; // the largest product where none was seen
 
 struct PromptArgs {
     const void *query, *key, *value;
@@ -59,6 +57,7 @@ struct Matrix<f16> {
     typedef _Float16 pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ v16f mul(frag a, frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static constexpr int kQueryBits = 15;  // |query| < 2^15: products below 2^40
+    static constexpr float kMost = 0x1p15f;  // what a lane's probabilities of a tile may add up to: none passes f16
 };
 template <>
 struct Matrix<bf16> {
@@ -66,12 +65,14 @@ struct Matrix<bf16> {
     typedef __bf16 pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ v16f mul(frag a, frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static constexpr int kQueryBits = -9;  // |query| < 2^-9: products with any finite key below 2^127
+    static constexpr float kMost = 0x1p40f;
 };
 template <>
 struct Matrix<float> {
     typedef float frag __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ v16f mul(float a, float b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
     static constexpr int kQueryBits = -9;
+    static constexpr float kMost = 0x1p40f;
 };
 
 struct Span {
@@ -158,6 +159,13 @@ __device__ __forceinline__ v4u load_chunk(const T *row, uint32_t c, uint32_t n) 
     for (uint32_t e = 0; e < CE; ++e) x.v[e] = c + e < n ? row[c + e] : from_float<T>(0.0f);
     return __builtin_bit_cast(v4u, x);
 }
+// 16 bytes a lane into LDS, the wave's next to each other from `to` on.  In
+// assembly, as the compiler would wait for all such loads before the transposing reads
+// of the other buffer; it does not count them: wait_vmcnt does.
+__device__ __forceinline__ void load_to_lds(const void *from, v4u *to) {
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)to));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
+}
 template <typename T>
 __device__ __forceinline__ bool finite(T v) {
     if constexpr (sizeof(T) == 4) {
@@ -168,12 +176,18 @@ __device__ __forceinline__ bool finite(T v) {
     }
 }
 
+__device__ const uint4 kZeros = {0, 0, 0, 0};  // what channels past the head's are loaded from
+
 // A workgroup takes 128 rows of a KV head, 32 a wave, and goes through the tiles
-// of its context; two buffers of LDS, the next tile's loads in registers
-// meanwhile.  Masked tokens have probability 0; so that 0 times a value that is
-// not finite does not reach rows that do not see it, such values are taken
-// as 0 in the tiles that are masked and added to the rows that see them.
-template <typename T, int W, int KT>
+// of its context; two buffers of LDS, one worked on while the other is filled
+// (DIRECT, of whole aligned chunks: by loads that go to LDS; else through registers).
+// Exponents are taken from a reference, the row's largest product in its first
+// tile: where a later tile's probabilities add up to more than kMost, the
+// reference is moved to what is largest then, so other tiles need no maximum.  Masked
+// tokens have probability 0; so that 0 times a value that is not finite does
+// not reach rows that do not see it, such values are taken as 0 in the tiles that
+// are masked and added to the rows that see them.
+template <typename T, int W, int KT, bool DIRECT>
 __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_kernel(PromptArgs a) {
     using M = Matrix<T>;
     using L = Tile<T, W>;
@@ -199,34 +213,57 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
     const T *keys = static_cast<const T *>(a.key) + static_cast<size_t>(q.row) * a.key_stride + head * a.head_dim;
     const T *values = static_cast<const T *>(a.value) + static_cast<size_t>(q.row) * a.value_stride + head * a.head_dim;
 
+    // chunk x of a tile in LDS: its token and place; tokens past the last are the last
     v4u kr[kOfThread], vr[kOfThread];
-    auto load = [&](uint32_t i) {
-#pragma unroll
-        for (uint32_t e = 0; e < kOfThread; ++e) {
-            const uint32_t x = tid + kThreads * e, t = min(i * KT + x / NC, most - 1), c = x % NC * CE;
-            kr[e] = load_chunk(keys + static_cast<size_t>(t) * a.key_stride, c, a.head_dim);
-            vr[e] = load_chunk(values + static_cast<size_t>(t) * a.value_stride, c, a.head_dim);
-        }
-    };
-    auto put = [&](uint32_t i) {
+    auto bring = [&](uint32_t i) {
         v4u *buf = tiles + i % 2 * 2 * kChunks;
 #pragma unroll
         for (uint32_t e = 0; e < kOfThread; ++e) {
-            const uint32_t x = tid + kThreads * e, to = L::at(x / NC, x % NC);
-            buf[to] = kr[e];
-            if (i >= masked) {
-                Vec<T, CE> v = __builtin_bit_cast(Vec<T, CE>, vr[e]);
-                bool bad = false;
-#pragma unroll
-                for (uint32_t k = 0; k < CE; ++k)
-                    if (!finite(v.v[k])) bad = true, v.v[k] = from_float<T>(0.0f);
-                if (bad) atomicOr(&odd[i - masked][x / NC / 32], 1u << x / NC % 32);
-                vr[e] = __builtin_bit_cast(v4u, v);
+            const uint32_t x = tid + kThreads * e, t = min(i * KT + x / NC, most - 1), c = (x % NC ^ L::spread(x / NC)) * CE;
+            const T *k = keys + static_cast<size_t>(t) * a.key_stride, *v = values + static_cast<size_t>(t) * a.value_stride;
+            if constexpr (DIRECT) {
+                const bool in = c < a.head_dim;
+                v4u *to = buf + kThreads * e + wave * kWaveSize;
+                const void *kp = in ? static_cast<const void *>(k + c) : &kZeros, *vp = in ? static_cast<const void *>(v + c) : &kZeros;
+                load_to_lds(kp, to);
+                load_to_lds(vp, to + kChunks);
+            } else {
+                kr[e] = load_chunk(k, c, a.head_dim);
+                vr[e] = load_chunk(v, c, a.head_dim);
             }
-            buf[kChunks + to] = vr[e];
         }
     };
-    load(0);
+    // what was brought is in LDS
+    auto settle = [&](uint32_t i) {
+        if constexpr (DIRECT) {
+            wait_vmcnt<0>();
+        } else {
+            v4u *buf = tiles + i % 2 * 2 * kChunks;
+#pragma unroll
+            for (uint32_t e = 0; e < kOfThread; ++e) {
+                buf[tid + kThreads * e] = kr[e];
+                buf[kChunks + tid + kThreads * e] = vr[e];
+            }
+        }
+        lds_barrier();
+    };
+    auto clean = [&](uint32_t i) {
+        v4u *vt = tiles + (i % 2 * 2 + 1) * kChunks;
+#pragma unroll 1
+        for (uint32_t x = tid; x < kChunks; x += kThreads) {
+            Vec<T, CE> v = __builtin_bit_cast(Vec<T, CE>, vt[x]);
+            bool bad = false;
+#pragma unroll
+            for (uint32_t k = 0; k < CE; ++k)
+                if (!finite(v.v[k])) bad = true, v.v[k] = from_float<T>(0.0f);
+            if (bad) {
+                vt[x] = __builtin_bit_cast(v4u, v);
+                atomicOr(&odd[i - masked][x / NC / 32], 1u << x / NC % 32);
+            }
+        }
+        lds_barrier();
+    };
+    bring(0);
 
     // this lane's row, as a column of the products
     const uint32_t w_row0 = row0 + wave * kWaveRows, r = w_row0 + n;
@@ -263,34 +300,32 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         }
     }
     if (tid < kMasked * (KT / 32)) odd[tid / (KT / 32)][tid % (KT / 32)] = 0;
-    lds_barrier();
-    put(0);
-    if (count > 1) load(1);
 
     v16f acc[C];
-    float m = real ? kNothing : 0.0f, ref = m, sum = 0.0f;  // the largest product, and times mul: what exponents are taken from
+    // the reference as a product, and times mul; far: some row's is too far to be rounded
+    float m = 0.0f, ref = 0.0f, sum = 0.0f;
+    bool far = false;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[c][e] = 0.0f;
 
     for (uint32_t i = 0; i < count; ++i) {
-        lds_barrier();  // tile i is there, and the other buffer is free
-        if (i + 1 < count) {
-            put(i + 1);
-            if (i + 2 < count) load(i + 2);
-        }
+        settle(i);  // tile i is there, and the other buffer is free
+        if (i >= masked) clean(i);
+        if (i + 1 < count) bring(i + 1);
         const uint32_t t0 = i * KT;
         if (t0 >= w_most) continue;
         const v4u *kt = tiles + i % 2 * 2 * kChunks, *vt = kt + kChunks;
         v16f sc[S];
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[s][e] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
+            for (int s = 0; s < S; ++s) {
                 const typename M::frag kf = __builtin_bit_cast(typename M::frag, kt[L::at(32 * s + n, 2 * j + h)]);
+                if (j == 0)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sc[s][e] = 0.0f;
                 if constexpr (sizeof(T) == 4) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sc[s] = M::mul(kf[e], qf[j][e], sc[s]);
@@ -298,7 +333,6 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
                     sc[s] = M::mul(kf, qf[j], sc[s]);
                 }
             }
-        }
         // element e of sc[s]: token 32 s + 8 (e / 4) + 4 h + e % 4 of the tile
         if (t0 + KT > w_least) {
             const int32_t seen = static_cast<int32_t>(visible) - static_cast<int32_t>(t0 + 4 * h);
@@ -308,17 +342,49 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
                 for (int e = 0; e < 16; ++e)
                     if (32 * s + 8 * (e / 4) + e % 4 >= seen) sc[s][e] = -INFINITY;
         }
-        float mx = sc[0][0];
+        auto largest = [&] {
+            float mx = sc[0][0];
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[s][e]);
-        if (__any((mx - m) * mul > kSlack)) {  // or nothing seen so far
-            mx = halves_max(fmaxf(mx, m));
-            mx = (mx - m) * mul > kSlack ? mx : m;  // a row's sums do not depend on other rows
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[s][e]);
+            return halves_max(mx);
+        };
+        if (i == 0) {
+            m = real ? largest() : 0.0f;
+            ref = mul_rounded(m, mul);
+            far = __any(!(fabsf(ref) < kFar));
+        }
+        float p[S][16], add;
+        auto weigh = [&] {
+            add = 0.0f;
+            if (far) {  // of rows with a far reference the product is taken off first
+                const bool mine = !(fabsf(ref) < kFar);
+                const float off = mine ? m : 0.0f, less = mine ? 0.0f : ref;
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        p[s][e] = __builtin_amdgcn_exp2f(fmaf(sc[s][e] - off, mul, -less));
+                        add += p[s][e];
+                    }
+            } else {
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        p[s][e] = __builtin_amdgcn_exp2f(fmaf(sc[s][e], mul, -ref));
+                        add += p[s][e];
+                    }
+            }
+        };
+        weigh();
+        if (__any(!(add < M::kMost))) {
+            // of the rows that pass it, which does not depend on other rows
+            const bool over = halves_max(add < M::kMost ? 0.0f : 1.0f) > 0.0f;
+            const float mx = over ? fmaxf(m, largest()) : m, to = mul_rounded(mx, mul);
             // what exponents were taken from, and are now: of near references
-            // themselves, else the largest product times mul, as it is
-            const float to = mul_rounded(mx, mul);
+            // themselves, else the product times mul, as it is
             const bool was = fabsf(ref) < kFar, is = fabsf(to) < kFar;
             const float alpha = __builtin_amdgcn_exp2f(was ? (is ? ref - to : fmaf(-mx, mul, ref)) : is ? fmaf(m, mul, -to) : (m - mx) * mul);
 #pragma unroll
@@ -326,23 +392,10 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
             sum *= alpha;
             m = mx;
             ref = to;
+            far = __any(!is);
+            weigh();
         }
-        float less = ref;
-        if (__any(!(fabsf(ref) < kFar))) {  // of such rows the largest product is taken off first
-            const bool far = !(fabsf(ref) < kFar);
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sc[s][e] -= far ? m : 0.0f;
-            less = far ? 0.0f : ref;
-        }
-#pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[s][e] = __builtin_amdgcn_exp2f(fmaf(sc[s][e], mul, -less));
-                sum += sc[s][e];
-            }
+        sum += add;
         if constexpr (sizeof(T) == 4) {
             const float *v = reinterpret_cast<const float *>(vt);
 #pragma unroll
@@ -352,7 +405,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
                     const uint32_t t = 32 * s + 8 * (e / 4) + e % 4 + 4 * h;
 #pragma unroll
                     for (int c = 0; c < C; ++c)
-                        acc[c] = M::mul(v[4 * L::at(t, (32 * c + n) / 4) + n % 4], sc[s][e], acc[c]);
+                        acc[c] = M::mul(v[4 * L::at(t, (32 * c + n) / 4) + n % 4], p[s][e], acc[c]);
                 }
         } else {
 #pragma unroll
@@ -362,7 +415,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
                     typename M::frag pf;
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
-                        const auto p2 = __builtin_convertvector((v2f){sc[s][8 * u + e], sc[s][8 * u + e + 1]}, typename M::pair);
+                        const auto p2 = __builtin_convertvector((v2f){p[s][8 * u + e], p[s][8 * u + e + 1]}, typename M::pair);
                         pf[e] = p2[0], pf[e + 1] = p2[1];
                     }
                     // rows of V^T: of 16 lanes each, 4 tokens of 16 channels
@@ -385,18 +438,20 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
                 }
         }
         if (i >= masked) {
-#pragma unroll
+#pragma unroll 1
             for (int s = 0; s < S; ++s)
                 for (uint32_t left = odd[i - masked][s]; left; left &= left - 1) {
                     const uint32_t t = t0 + 32 * s + __ffs(static_cast<int>(left)) - 1;
                     if (t >= visible) continue;
                     const T *row = values + static_cast<size_t>(t) * a.value_stride;
+                    uint32_t d = a.head_dim;
+                    asm("" : "+s"(d));  // compared here: 16 C masks kept over the loop would not have the registers
 #pragma unroll
                     for (int c = 0; c < C; ++c)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const uint32_t ch = 32 * c + 8 * (e / 4) + 4 * h + e % 4;
-                            if (ch < a.head_dim && !finite(row[ch])) acc[c][e] += to_float(row[ch]);
+                            if (ch < d && !finite(row[ch])) acc[c][e] += to_float(row[ch]);
                         }
                 }
         }
@@ -424,18 +479,25 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         }
 }
 
-template <typename T, int W, int KT>
-hipError_t launch_tile(const PromptArgs &a, hipStream_t stream) {
+template <typename T, int W, int KT, bool DIRECT>
+hipError_t launch_loads(const PromptArgs &a, hipStream_t stream) {
     constexpr size_t lds = 2 * 2 * KT * W * sizeof(T);
     static_assert(lds <= 128 * 1024, "a workgroup's LDS");
-    const void *kernel = reinterpret_cast<const void *>(&prompt_attention_kernel<T, W, KT>);
+    const void *kernel = reinterpret_cast<const void *>(&prompt_attention_kernel<T, W, KT, DIRECT>);
     const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     if (e != hipSuccess) return e;
     // at most one block of each sequence is not full
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, used = std::min(a.sequences, a.tokens);
     const uint32_t blocks = static_cast<uint32_t>((rows + used * (kBlockRows - 1)) / kBlockRows);
-    hipLaunchKernelGGL((prompt_attention_kernel<T, W, KT>), dim3(blocks * a.kv_heads), dim3(kThreads), lds, stream, a);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, W, KT, DIRECT>), dim3(blocks * a.kv_heads), dim3(kThreads), lds, stream, a);
     return hipGetLastError();
+}
+template <typename T, int W, int KT>
+hipError_t launch_tile(const PromptArgs &a, hipStream_t stream) {
+    // loads to LDS take whole chunks of 16 bytes, aligned
+    const uint64_t sizes = (static_cast<uint64_t>(a.head_dim) | a.key_stride | a.value_stride) * sizeof(T) |
+                           reinterpret_cast<uintptr_t>(a.key) | reinterpret_cast<uintptr_t>(a.value);
+    return sizes % 16 == 0 ? launch_loads<T, W, KT, true>(a, stream) : launch_loads<T, W, KT, false>(a, stream);
 }
 template <typename T>
 hipError_t launch_prompt(const PromptArgs &a, hipStream_t stream) {

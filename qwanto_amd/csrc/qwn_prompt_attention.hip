@@ -22,6 +22,7 @@
 #include "qwn_types.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -35,9 +36,14 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kWaves = 4, kThreads = kWaves * kWaveSize;
-constexpr uint32_t kWaveRows = 32, kBlockRows = kWaves * kWaveRows;
+constexpr uint32_t kWaves = 4, kThreads = kWaves * kWaveSize, kWaveRows = 32;
+constexpr float kLowest = -3.402823466e38f;
 constexpr float kFar = 0x1p20f;               // of references: past it their rounding would be more than 2^-4 of an exponent
+
+// Workgroups from which on blocks of 128 rows are best (bf16, 32 heads of 128: one
+// prompt of 512 tokens, 128 groups, 18 us and in blocks of 64 14; of 1777 and eight
+// shorter, 728 groups, 52 and 59).
+constexpr uint64_t kManyGroups = 320;
 
 struct PromptArgs {
     const void *query, *key, *value;
@@ -48,7 +54,7 @@ struct PromptArgs {
     float scale;
 };
 
-// The two 16-bit types' operands and products; of fp32 a lane's operand is one number.
+// The two 16-bit types' operands and products.
 template <typename T>
 struct Matrix;
 template <>
@@ -56,24 +62,20 @@ struct Matrix<f16> {
     typedef _Float16 frag __attribute__((ext_vector_type(8)));
     typedef _Float16 pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ v16f mul(frag a, frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-    static constexpr int kQueryBits = 15;  // |query| < 2^15: products below 2^40
-    static constexpr float kMost = 0x1p15f;  // what a lane's probabilities of a tile may add up to: none passes f16
 };
 template <>
 struct Matrix<bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
     typedef __bf16 pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ v16f mul(frag a, frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-    static constexpr int kQueryBits = -9;  // |query| < 2^-9: products with any finite key below 2^127
-    static constexpr float kMost = 0x1p40f;
 };
-template <>
-struct Matrix<float> {
-    typedef float frag __attribute__((ext_vector_type(4)));
-    static __device__ __forceinline__ v16f mul(float a, float b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
-    static constexpr int kQueryBits = -9;
-    static constexpr float kMost = 0x1p40f;
-};
+// Queries are scaled to below 2^kQueryBits: of f16 products are then below 2^40, of
+// the others, with any finite key, below 2^127.
+template <typename T>
+constexpr int kQueryBits = std::is_same_v<T, f16> ? 15 : -9;
+// What a lane's probabilities of a tile may add up to: of f16 none passes it.
+template <typename T>
+constexpr float kMost = std::is_same_v<T, f16> ? 0x1p15f : 0x1p40f;
 
 struct Span {
     uint32_t row = 0, rows = 0;  // of a sequence; none where its starts do not lie in the batch
@@ -89,10 +91,10 @@ __device__ __forceinline__ Span span_of(const PromptArgs &a, uint32_t s) {
 }
 // The sequence that holds block `index` of the batch, and its number there;
 // false past the last.  Every wave searches for itself, 64 sequences a step.
-__device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t index, Span &q, uint32_t &at) {
+__device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t block_rows, uint32_t index, Span &q, uint32_t &at) {
     for (uint32_t s0 = 0; s0 < a.sequences; s0 += kWaveSize) {
         const Span mine = span_of(a, s0 + threadIdx.x % kWaveSize);
-        const uint32_t n = (mine.rows * a.group + kBlockRows - 1) / kBlockRows, end = wave_scan(n);
+        const uint32_t n = (mine.rows * a.group + block_rows - 1) / block_rows, end = wave_scan(n);
         const uint64_t past = __ballot(end > index);
         if (past) {
             const int first = __ffsll(static_cast<unsigned long long>(past)) - 1;
@@ -136,6 +138,165 @@ __device__ __forceinline__ float halves_sum(float v) {
     return b.low + b.high;
 }
 
+// What sums are multiplied by as the reference goes from (m, ref) to (mx, to):
+// exponents were taken from ref itself where it is near, else from m times mul as it is.
+__device__ __forceinline__ float moved(float m, float ref, float mx, float to, float mul) {
+    const bool was = fabsf(ref) < kFar, is = fabsf(to) < kFar;
+    return __builtin_amdgcn_exp2f(was ? (is ? ref - to : fmaf(-mx, mul, ref)) : is ? fmaf(m, mul, -to) : (m - mx) * mul);
+}
+
+// A row's softmax so far: the reference as a product, and times mul; far: some row of
+// the wave has one too far to be rounded.  m is 0 of a row that has seen nothing.
+struct Softmax {
+    float m = 0.0f, ref = 0.0f, sum = 0.0f, mul = 0.0f;
+    bool far = false;
+};
+template <int S>
+__device__ __forceinline__ float largest_of(const v16f (&sc)[S]) {
+    float mx = sc[0][0];
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[s][e]);
+    return halves_max(mx);
+}
+// The probabilities of products sc, and their sum.
+template <int S>
+__device__ __forceinline__ float weigh(const v16f (&sc)[S], const Softmax &x, float (&p)[S][16]) {
+    float add = 0.0f;
+    if (x.far) {  // of rows with a far reference the product is taken off first
+        const bool mine = !(fabsf(x.ref) < kFar);
+        const float off = mine ? x.m : 0.0f, less = mine ? 0.0f : x.ref;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                p[s][e] = __builtin_amdgcn_exp2f(fmaf(sc[s][e] - off, x.mul, -less));
+                add += p[s][e];
+            }
+    } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                p[s][e] = __builtin_amdgcn_exp2f(fmaf(sc[s][e], x.mul, -x.ref));
+                add += p[s][e];
+            }
+    }
+    return add;
+}
+// A tile's probabilities, the sums moved to another reference where they would pass
+// `top`.  first: the wave's first tile; sees: the row sees some of it.
+template <int S, int C>
+__device__ __forceinline__ void softmax_tile(const v16f (&sc)[S], Softmax &x, float (&p)[S][16], v16f (&acc)[C], bool first, bool sees,
+                                             float top) {
+    if (first) {
+        x.m = sees ? fmaxf(largest_of(sc), kLowest) : 0.0f;
+        x.ref = mul_rounded(x.m, x.mul);
+        x.far = __any(!(fabsf(x.ref) < kFar));
+    }
+    float add = weigh(sc, x, p);
+    if (__any(!(add < top))) {
+        // of the rows that pass it, which does not depend on other rows
+        const bool over = halves_max(add < top ? 0.0f : 1.0f) > 0.0f;
+        const float mx = over ? fmaxf(x.m, largest_of(sc)) : x.m, to = mul_rounded(mx, x.mul);
+        const float alpha = moved(x.m, x.ref, mx, to, x.mul);
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= alpha;
+        x.sum *= alpha;
+        x.m = mx;
+        x.ref = to;
+        x.far = __any(!(fabsf(to) < kFar));
+        add = weigh(sc, x, p);
+    }
+    x.sum += add;
+}
+
+// The sums of the waves that took parts of the same rows' tokens, RW waves a part,
+// in those of part 0; false in the others.  A row that has seen none of a part's
+// tokens has the sum 0 there, and no reference.
+template <int C, int RW, int NW>
+constexpr size_t join_bytes = RW == NW ? 0 : NW * kWaveSize * 16 + (NW - RW) * C * 16 * kWaveSize * 4;
+template <int C, int RW, int NW>
+__device__ __forceinline__ bool join_parts(v4u *lds, uint32_t wave, uint32_t lane, bool sees, Softmax &x, v16f (&acc)[C]) {
+    constexpr int KW = NW / RW;
+    x.sum = halves_sum(x.sum);
+    if constexpr (KW > 1) {
+        lds_barrier();
+        float4 *state = reinterpret_cast<float4 *>(lds);                     // [wave][lane]
+        float *sums = reinterpret_cast<float *>(state + NW * kWaveSize);     // [wave past part 0][element][lane]
+        state[wave * kWaveSize + lane] = make_float4(x.m, x.ref, x.sum, sees ? 1.0f : 0.0f);
+        if (wave >= RW) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sums[((wave - RW) * C * 16 + c * 16 + e) * kWaveSize + lane] = acc[c][e];
+        }
+        lds_barrier();
+        if (wave >= RW) return false;
+        float mx = x.m;
+#pragma unroll
+        for (int k = 1; k < KW; ++k) {
+            const float4 o = state[(wave + k * RW) * kWaveSize + lane];
+            if (o.w > 0.0f) mx = fmaxf(mx, o.x);
+        }
+        const float to = mul_rounded(mx, x.mul), mine = moved(x.m, x.ref, mx, to, x.mul);
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= mine;
+        x.sum *= mine;
+#pragma unroll
+        for (int k = 1; k < KW; ++k) {
+            const float4 o = state[(wave + k * RW) * kWaveSize + lane];
+            const bool any = o.w > 0.0f;
+            const float f = any ? moved(o.x, o.y, mx, to, x.mul) : 0.0f;
+            x.sum += any ? o.z * f : 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float o2 = sums[((wave + (k - 1) * RW) * C * 16 + c * 16 + e) * kWaveSize + lane];
+                    acc[c][e] += any ? o2 * f : 0.0f;
+                }
+        }
+    }
+    return true;
+}
+
+// A block of rows of a KV head, and a lane's row of it.
+struct Block {
+    Span q;
+    uint32_t head, row0, last;   // of the sequence's rows: the first, and the last real one
+    uint32_t most, least;        // tokens that any row sees, and every one
+};
+template <uint32_t ROWS>
+__device__ __forceinline__ bool block_of(const PromptArgs &a, Block &b) {
+    uint32_t at;
+    b.head = blockIdx.x % a.kv_heads;
+    if (!find_block(a, ROWS, blockIdx.x / a.kv_heads, b.q, at)) return false;
+    const uint32_t all = b.q.rows * a.group, blocks = (all + ROWS - 1) / ROWS;
+    b.row0 = (blocks - 1 - at) * ROWS;  // a sequence's longest contexts first
+    b.last = min(b.row0 + ROWS, all) - 1;
+    b.most = b.last / a.group + 1;
+    b.least = b.row0 / a.group + 1;
+    return true;
+}
+struct Row {
+    uint32_t token, at;          // of the sequence; elements from the token's first query channel
+    uint32_t visible;            // tokens it sees; none where it is no row
+    uint32_t w_most, w_least;    // tokens that any row of the wave sees, and every one
+};
+__device__ __forceinline__ Row row_of(const PromptArgs &a, const Block &b, uint32_t w_row0, uint32_t n) {
+    Row r;
+    const uint32_t rr = min(w_row0 + n, b.last);
+    r.token = rr / a.group;
+    r.at = (b.head * a.group + rr % a.group) * a.head_dim;
+    r.visible = w_row0 + n <= b.last ? r.token + 1 : 0u;
+    const bool idle = w_row0 > b.last;
+    r.w_most = idle ? 0u : min(w_row0 + kWaveRows - 1, b.last) / a.group + 1;
+    r.w_least = idle ? 0u : w_row0 / a.group + 1;
+    return r;
+}
+
 // A tile of `KT` tokens of W channels in LDS, 16 bytes (CE channels) a chunk.
 // Chunk c of token t lies in place c ^ spread(t) of its row: reads of one chunk
 // of 16 tokens, and of 4 chunks of 4 tokens, both reach each bank once.
@@ -176,42 +337,69 @@ __device__ __forceinline__ bool finite(T v) {
     }
 }
 
+// Keys and values of a tile, and how many tiles LDS is given room for.
+template <typename T, int W, int KT>
+constexpr size_t tile_bytes = 2 * KT * W * sizeof(T);
+
 __device__ const uint4 kZeros = {0, 0, 0, 0};  // what channels past the head's are loaded from
 
-// A workgroup takes 128 rows of a KV head, 32 a wave, and goes through the tiles
-// of its context; two buffers of LDS, one worked on while the other is filled
-// (DIRECT, of whole aligned chunks: by loads that go to LDS; else through registers).
+// A lane's 16-byte pieces of its query, CE channels each, scaled; pieces 2 j + h.
+template <typename T, int J>
+__device__ __forceinline__ void load_query(const PromptArgs &a, const Block &b, const Row &r, uint32_t h, v4u (&qf)[J], float &mul) {
+    constexpr uint32_t CE = 16 / sizeof(T);
+    const T *qp = static_cast<const T *>(a.query) + static_cast<size_t>(b.q.row + r.token) * a.query_stride + r.at;
+    Vec<T, CE> raw[J];
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) raw[j] = __builtin_bit_cast(Vec<T, CE>, load_chunk(qp, (2 * j + h) * CE, a.head_dim));
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (uint32_t e = 0; e < CE; ++e) top = fmaxf(top, fabsf(to_float(raw[j].v[e])));
+    top = halves_max(top);
+    int e2 = 0;  // top < 2^e2
+    if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e2);
+    e2 = max(e2, -100);
+    float up = ldexpf(1.0f, kQueryBits<T> - e2);
+    mul = exponents_of(a.scale, e2 - kQueryBits<T>, up);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        Vec<T, CE> x;
+#pragma unroll
+        for (uint32_t e = 0; e < CE; ++e) x.v[e] = from_float<T>(to_float(raw[j].v[e]) * up);
+        qf[j] = __builtin_bit_cast(v4u, x);
+    }
+}
+
+// f16 and bf16.  A workgroup takes RW blocks of 32 rows of a KV head, a wave's
+// each, and goes through the tiles of its context; of a tile's tokens, 4 / RW waves
+// with the same rows take a part each, and their sums meet at the end.  Two
+// buffers of LDS, one worked on while the other is filled (DIRECT, of whole aligned
+// chunks: by loads that go to LDS; else through registers).
 // Exponents are taken from a reference, the row's largest product in its first
 // tile: where a later tile's probabilities add up to more than kMost, the
 // reference is moved to what is largest then, so other tiles need no maximum.  Masked
 // tokens have probability 0; so that 0 times a value that is not finite does
 // not reach rows that do not see it, such values are taken as 0 in the tiles that
 // are masked and added to the rows that see them.
-template <typename T, int W, int KT, bool DIRECT>
+template <typename T, int W, int KT, int RW, bool DIRECT>
 __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_kernel(PromptArgs a) {
     using M = Matrix<T>;
     using L = Tile<T, W>;
     constexpr uint32_t CE = L::CE, NC = L::NC;
-    constexpr uint32_t kChunks = KT * NC, kOfThread = kChunks / kThreads;
-    constexpr int C = W / 32, S = KT / 32, J = NC / 2;
-    static_assert(kChunks % kThreads == 0, "whole rounds of loads");
-    extern __shared__ v4u tiles[];          // two buffers of keys, then values
+    constexpr uint32_t kChunks = KT * NC, kOfThread = kChunks / kThreads, kBlockRows = RW * kWaveRows;
+    constexpr int KW = kWaves / RW, C = W / 32, S = KT / 32 / KW, J = NC / 2;
+    static_assert(kChunks % kThreads == 0 && S > 0, "whole rounds of loads, a part for each wave");
+    extern __shared__ v4u tiles[];          // two times keys, then values
     constexpr uint32_t kMasked = kBlockRows / KT + 2;
     __shared__ uint32_t odd[kMasked][KT / 32];  // of the masked tiles: tokens with values that are not finite
     const uint32_t tid = threadIdx.x, lane = tid % kWaveSize, wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
-    const uint32_t n = lane % 32, h = lane / 32;
-    const uint32_t head = blockIdx.x % a.kv_heads;
-    Span q;
-    uint32_t at;
-    if (!find_block(a, blockIdx.x / a.kv_heads, q, at)) return;
-    const uint32_t all = q.rows * a.group, blocks = (all + kBlockRows - 1) / kBlockRows;
-    const uint32_t row0 = (blocks - 1 - at) * kBlockRows;  // a sequence's longest contexts first
-    const uint32_t last = min(row0 + kBlockRows, all) - 1;
-    const uint32_t most = last / a.group + 1;              // tokens that any row sees
-    const uint32_t least = row0 / a.group + 1;             // and every one
-    const uint32_t count = (most + KT - 1) / KT, masked = least / KT;  // tiles, and the first that not every row sees all of
-    const T *keys = static_cast<const T *>(a.key) + static_cast<size_t>(q.row) * a.key_stride + head * a.head_dim;
-    const T *values = static_cast<const T *>(a.value) + static_cast<size_t>(q.row) * a.value_stride + head * a.head_dim;
+    const uint32_t n = lane % 32, h = lane / 32, part = wave / RW;  // of a tile's tokens
+    Block b;
+    if (!block_of<kBlockRows>(a, b)) return;
+    const uint32_t count = (b.most + KT - 1) / KT, masked = b.least / KT;  // tiles, and the first that not every row sees all of
+    const T *keys = static_cast<const T *>(a.key) + static_cast<size_t>(b.q.row) * a.key_stride + b.head * a.head_dim;
+    const T *values = static_cast<const T *>(a.value) + static_cast<size_t>(b.q.row) * a.value_stride + b.head * a.head_dim;
 
     // chunk x of a tile in LDS: its token and place; tokens past the last are the last
     v4u kr[kOfThread], vr[kOfThread];
@@ -219,14 +407,13 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         v4u *buf = tiles + i % 2 * 2 * kChunks;
 #pragma unroll
         for (uint32_t e = 0; e < kOfThread; ++e) {
-            const uint32_t x = tid + kThreads * e, t = min(i * KT + x / NC, most - 1), c = (x % NC ^ L::spread(x / NC)) * CE;
+            const uint32_t x = tid + kThreads * e, t = min(i * KT + x / NC, b.most - 1), c = (x % NC ^ L::spread(x / NC)) * CE;
             const T *k = keys + static_cast<size_t>(t) * a.key_stride, *v = values + static_cast<size_t>(t) * a.value_stride;
             if constexpr (DIRECT) {
                 const bool in = c < a.head_dim;
                 v4u *to = buf + kThreads * e + wave * kWaveSize;
-                const void *kp = in ? static_cast<const void *>(k + c) : &kZeros, *vp = in ? static_cast<const void *>(v + c) : &kZeros;
-                load_to_lds(kp, to);
-                load_to_lds(vp, to + kChunks);
+                load_to_lds(in ? static_cast<const void *>(k + c) : &kZeros, to);
+                load_to_lds(in ? static_cast<const void *>(v + c) : &kZeros, to + kChunks);
             } else {
                 kr[e] = load_chunk(k, c, a.head_dim);
                 vr[e] = load_chunk(v, c, a.head_dim);
@@ -266,45 +453,13 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
     bring(0);
 
     // this lane's row, as a column of the products
-    const uint32_t w_row0 = row0 + wave * kWaveRows, r = w_row0 + n;
-    const bool real = r <= last;
-    const uint32_t rr = min(r, last), tok = rr / a.group;
-    const uint32_t visible = real ? tok + 1 : 0u;
-    const bool idle = w_row0 > last;
-    const uint32_t w_most = idle ? 0u : min(w_row0 + kWaveRows - 1, last) / a.group + 1, w_least = idle ? 0u : w_row0 / a.group + 1;
-    typename M::frag qf[J];
-    float mul;
-    {
-        const T *qp = static_cast<const T *>(a.query) + static_cast<size_t>(q.row + tok) * a.query_stride +
-                      static_cast<size_t>(head * a.group + rr % a.group) * a.head_dim;
-        Vec<T, CE> raw[J];
-        float top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) raw[j] = __builtin_bit_cast(Vec<T, CE>, load_chunk(qp, (2 * j + h) * CE, a.head_dim));
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (uint32_t e = 0; e < CE; ++e) top = fmaxf(top, fabsf(to_float(raw[j].v[e])));
-        top = halves_max(top);
-        int e2 = 0;  // top < 2^e2
-        if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e2);
-        e2 = max(e2, -100);
-        float up = ldexpf(1.0f, M::kQueryBits - e2);
-        mul = exponents_of(a.scale, e2 - M::kQueryBits, up);
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            Vec<T, CE> x;
-#pragma unroll
-            for (uint32_t e = 0; e < CE; ++e) x.v[e] = from_float<T>(to_float(raw[j].v[e]) * up);
-            qf[j] = __builtin_bit_cast(typename M::frag, x);
-        }
-    }
+    const Row r = row_of(a, b, b.row0 + wave % RW * kWaveRows, n);
+    v4u qf[J];
+    Softmax soft;
+    load_query<T>(a, b, r, h, qf, soft.mul);
     if (tid < kMasked * (KT / 32)) odd[tid / (KT / 32)][tid % (KT / 32)] = 0;
 
     v16f acc[C];
-    // the reference as a product, and times mul; far: some row's is too far to be rounded
-    float m = 0.0f, ref = 0.0f, sum = 0.0f;
-    bool far = false;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -314,135 +469,65 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         settle(i);  // tile i is there, and the other buffer is free
         if (i >= masked) clean(i);
         if (i + 1 < count) bring(i + 1);
-        const uint32_t t0 = i * KT;
-        if (t0 >= w_most) continue;
-        const v4u *kt = tiles + i % 2 * 2 * kChunks, *vt = kt + kChunks;
+        const uint32_t t0 = i * KT + part * S * 32;  // the wave's part, and where it lies in the tile
+        if (t0 >= r.w_most) continue;
+        const v4u *kt = tiles + i % 2 * 2 * kChunks + part * S * 32 * NC, *vt = kt + kChunks;
         v16f sc[S];
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const typename M::frag kf = __builtin_bit_cast(typename M::frag, kt[L::at(32 * s + n, 2 * j + h)]);
+                const auto kf = __builtin_bit_cast(typename M::frag, kt[L::at(32 * s + n, 2 * j + h)]);
                 if (j == 0)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sc[s][e] = 0.0f;
-                if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[s] = M::mul(kf[e], qf[j][e], sc[s]);
-                } else {
-                    sc[s] = M::mul(kf, qf[j], sc[s]);
-                }
+                sc[s] = M::mul(kf, __builtin_bit_cast(typename M::frag, qf[j]), sc[s]);
             }
-        // element e of sc[s]: token 32 s + 8 (e / 4) + 4 h + e % 4 of the tile
-        if (t0 + KT > w_least) {
-            const int32_t seen = static_cast<int32_t>(visible) - static_cast<int32_t>(t0 + 4 * h);
+        // element e of sc[s]: token t0 + 32 s + 8 (e / 4) + 4 h + e % 4
+        if (t0 + S * 32 > r.w_least) {
+            const int32_t seen = static_cast<int32_t>(r.visible) - static_cast<int32_t>(t0 + 4 * h);
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (32 * s + 8 * (e / 4) + e % 4 >= seen) sc[s][e] = -INFINITY;
         }
-        auto largest = [&] {
-            float mx = sc[0][0];
+        float p[S][16];
+        softmax_tile(sc, soft, p, acc, i == 0, r.visible > t0, kMost<T>);
 #pragma unroll
-            for (int s = 0; s < S; ++s)
+        for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[s][e]);
-            return halves_max(mx);
-        };
-        if (i == 0) {
-            m = real ? largest() : 0.0f;
-            ref = mul_rounded(m, mul);
-            far = __any(!(fabsf(ref) < kFar));
-        }
-        float p[S][16], add;
-        auto weigh = [&] {
-            add = 0.0f;
-            if (far) {  // of rows with a far reference the product is taken off first
-                const bool mine = !(fabsf(ref) < kFar);
-                const float off = mine ? m : 0.0f, less = mine ? 0.0f : ref;
+            for (int u = 0; u < 2; ++u) {
+                typename M::frag pf;
 #pragma unroll
-                for (int s = 0; s < S; ++s)
+                for (int e = 0; e < 8; e += 2) {
+                    const auto p2 = __builtin_convertvector((v2f){p[s][8 * u + e], p[s][8 * u + e + 1]}, typename M::pair);
+                    pf[e] = p2[0], pf[e + 1] = p2[1];
+                }
+                // rows of V^T: of 16 lanes each, 4 tokens of 16 channels
+                const uint32_t t = 32 * s + 16 * u + 4 * h + lane % 16 / 4;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        p[s][e] = __builtin_amdgcn_exp2f(fmaf(sc[s][e] - off, mul, -less));
-                        add += p[s][e];
+                for (int c = 0; c < C; ++c) {
+                    const uint32_t ch = 4 * c + 2 * (lane / 16 % 2) + lane % 4 / 2;
+                    typedef __attribute__((address_space(3))) v4s lds_v4s;
+                    union {
+                        v4s part[2];
+                        typename M::frag whole;
+                    } x;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint16_t *from = reinterpret_cast<const uint16_t *>(vt + L::at(t + 8 * k, ch)) + 4 * (lane % 2);
+                        x.part[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(from));
                     }
-            } else {
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        p[s][e] = __builtin_amdgcn_exp2f(fmaf(sc[s][e], mul, -ref));
-                        add += p[s][e];
-                    }
+                    acc[c] = M::mul(x.whole, pf, acc[c]);
+                }
             }
-        };
-        weigh();
-        if (__any(!(add < M::kMost))) {
-            // of the rows that pass it, which does not depend on other rows
-            const bool over = halves_max(add < M::kMost ? 0.0f : 1.0f) > 0.0f;
-            const float mx = over ? fmaxf(m, largest()) : m, to = mul_rounded(mx, mul);
-            // what exponents were taken from, and are now: of near references
-            // themselves, else the product times mul, as it is
-            const bool was = fabsf(ref) < kFar, is = fabsf(to) < kFar;
-            const float alpha = __builtin_amdgcn_exp2f(was ? (is ? ref - to : fmaf(-mx, mul, ref)) : is ? fmaf(m, mul, -to) : (m - mx) * mul);
-#pragma unroll
-            for (int c = 0; c < C; ++c) acc[c] *= alpha;
-            sum *= alpha;
-            m = mx;
-            ref = to;
-            far = __any(!is);
-            weigh();
-        }
-        sum += add;
-        if constexpr (sizeof(T) == 4) {
-            const float *v = reinterpret_cast<const float *>(vt);
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const uint32_t t = 32 * s + 8 * (e / 4) + e % 4 + 4 * h;
-#pragma unroll
-                    for (int c = 0; c < C; ++c)
-                        acc[c] = M::mul(v[4 * L::at(t, (32 * c + n) / 4) + n % 4], p[s][e], acc[c]);
-                }
-        } else {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    typename M::frag pf;
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        const auto p2 = __builtin_convertvector((v2f){p[s][8 * u + e], p[s][8 * u + e + 1]}, typename M::pair);
-                        pf[e] = p2[0], pf[e + 1] = p2[1];
-                    }
-                    // rows of V^T: of 16 lanes each, 4 tokens of 16 channels
-                    const uint32_t t = 32 * s + 16 * u + 4 * h + lane % 16 / 4;
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const uint32_t ch = 4 * c + 2 * (lane / 16 % 2) + lane % 4 / 2;
-                        typedef __attribute__((address_space(3))) v4s lds_v4s;
-                        union {
-                            v4s part[2];
-                            typename M::frag whole;
-                        } x;
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const uint16_t *from = reinterpret_cast<const uint16_t *>(vt + L::at(t + 8 * k, ch)) + 4 * (lane % 2);
-                            x.part[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(from));
-                        }
-                        acc[c] = M::mul(x.whole, pf, acc[c]);
-                    }
-                }
-        }
         if (i >= masked) {
 #pragma unroll 1
             for (int s = 0; s < S; ++s)
-                for (uint32_t left = odd[i - masked][s]; left; left &= left - 1) {
+                for (uint32_t left = odd[i - masked][part * S + s]; left; left &= left - 1) {
                     const uint32_t t = t0 + 32 * s + __ffs(static_cast<int>(left)) - 1;
-                    if (t >= visible) continue;
+                    if (t >= r.visible) continue;
                     const T *row = values + static_cast<size_t>(t) * a.value_stride;
                     uint32_t d = a.head_dim;
                     asm("" : "+s"(d));  // compared here: 16 C masks kept over the loop would not have the registers
@@ -457,10 +542,9 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         }
     }
 
-    if (!real) return;
-    const float inv = 1.0f / halves_sum(sum);
-    T *dst = static_cast<T *>(a.output) + static_cast<size_t>(q.row + tok) * a.output_stride +
-             static_cast<size_t>(head * a.group + rr % a.group) * a.head_dim;
+    if (!join_parts<C, RW, kWaves>(tiles, wave, lane, r.visible > part * S * 32, soft, acc) || r.visible == 0) return;
+    const float inv = 1.0f / soft.sum;
+    T *dst = static_cast<T *>(a.output) + static_cast<size_t>(b.q.row + r.token) * a.output_stride + r.at;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -479,31 +563,209 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         }
 }
 
-template <typename T, int W, int KT, bool DIRECT>
-hipError_t launch_loads(const PromptArgs &a, hipStream_t stream) {
-    constexpr size_t lds = 2 * 2 * KT * W * sizeof(T);
-    static_assert(lds <= 128 * 1024, "a workgroup's LDS");
-    const void *kernel = reinterpret_cast<const void *>(&prompt_attention_kernel<T, W, KT, DIRECT>);
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+// fp32.  A product of two fp32 operands (v_mfma_f32_32x32x2_f32) takes 64 cycles for
+// an operand of 4 bytes a lane, 16 times as long as the 16-bit ones for theirs: L2
+// brings a wave's operands in the time, so there is no LDS and no barrier.  The four
+// waves of a workgroup take the same 32 rows and every fourth tile of 32 tokens; a tile's values come
+// while its scores are computed, the next tile's keys from then on, in one set of
+// registers each.  A lane's values are W / 32 channels next to each other: block
+// c of the output's rows are channels c, c + W / 32, ...  WHOLE: heads of W channels.
+// Of 256 channels the output, keys and values have 384 registers: the lane's query
+// stays in LDS.
+template <int W>
+constexpr bool kQueryInLds = W == 256;
+template <int W, bool WHOLE>
+__global__ __launch_bounds__(kThreads, W == 64 ? 2 : 1) void prompt_attention_f32_kernel(PromptArgs a) {
+    constexpr uint32_t KT = 32, KW = kWaves;
+    constexpr int C = W / 32, J = W / 8;
+    extern __shared__ v4u lds[];
+    const uint32_t tid = threadIdx.x, lane = tid % kWaveSize, wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
+    const uint32_t n = lane % 32, h = lane / 32, part = wave;
+    Block b;
+    if (!block_of<kWaveRows>(a, b)) return;
+    const Row r = row_of(a, b, b.row0, n);
+    const uint32_t count = (r.w_most + KT - 1) / KT;
+    const float *keys = static_cast<const float *>(a.key) + static_cast<size_t>(b.q.row) * a.key_stride + b.head * a.head_dim;
+    const float *values = static_cast<const float *>(a.value) + static_cast<size_t>(b.q.row) * a.value_stride + b.head * a.head_dim;
+    auto piece = [&](const float *row, uint32_t c) {
+        if constexpr (WHOLE) {
+            return load_vec<float, 4>(row + c);
+        } else {
+            return __builtin_bit_cast(Vec<float, 4>, load_chunk(row, c, a.head_dim));
+        }
+    };
+    Vec<float, 4> kf[J];
+    Vec<float, C> vf[16];
+    auto load_keys = [&](uint32_t i) {
+        const float *row = keys + static_cast<size_t>(min(i * KT + n, b.most - 1)) * a.key_stride;
+#pragma unroll
+        for (int j = 0; j < J; ++j) kf[j] = piece(row, (2 * j + h) * 4);
+    };
+    auto load_values = [&](uint32_t i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float *row = values + static_cast<size_t>(min(i * KT + 8 * (e / 4) + 4 * h + e % 4, b.most - 1)) * a.value_stride;
+            if constexpr (C >= 4) {
+#pragma unroll
+                for (int x = 0; x < C / 4; ++x) {
+                    const Vec<float, 4> v = piece(row, C * n + 4 * x);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) vf[e].v[4 * x + k] = v.v[k];
+                }
+            } else if constexpr (WHOLE) {
+                vf[e] = load_vec<float, C>(row + C * n);
+            } else {
+#pragma unroll
+                for (int k = 0; k < C; ++k) vf[e].v[k] = C * n + k < a.head_dim ? row[C * n + k] : 0.0f;
+            }
+        }
+    };
+    if (part < count) load_keys(part);
+    v4u qf[J];
+    Softmax soft;
+    load_query<float>(a, b, r, h, qf, soft.mul);
+    v4u *own = lds + wave * J * kWaveSize + lane;
+    if constexpr (kQueryInLds<W>) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) own[j * kWaveSize] = qf[j];
+    }
+    v16f acc[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[c][e] = 0.0f;
+
+    for (uint32_t i = part; i < count; i += KW) {
+        if constexpr (!kQueryInLds<W>) {
+            load_values(i);
+            __builtin_amdgcn_sched_barrier(0);  // or they are put off until they are needed
+        }
+        const uint32_t t0 = i * KT;
+        v16f sc[1], odd;  // two chains of products
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[0][e] = odd[e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const v4f q4 = __builtin_bit_cast(v4f, kQueryInLds<W> ? own[j * kWaveSize] : qf[j]);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j].v[e], q4[e], sc[0], 0, 0, 0);
+                odd = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j].v[e + 1], q4[e + 1], odd, 0, 0, 0);
+            }
+        }
+        if constexpr (kQueryInLds<W>) load_values(i);
+        load_keys(min(i + KW, count - 1));  // past the last tile too: how many loads are in flight does not depend on a branch
+        __builtin_amdgcn_sched_barrier(0);
+        sc[0] += odd;
+        uint32_t bad = 0;  // tokens of a masked tile with values that are not finite
+        if (t0 + KT > r.w_least) {
+            const int32_t seen = static_cast<int32_t>(r.visible) - static_cast<int32_t>(t0 + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t t = 8 * (e / 4) + e % 4;
+                if (static_cast<int32_t>(t) >= seen) sc[0][e] = -INFINITY;
+                bool f = true;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    f = f && finite(vf[e].v[c]);
+                    vf[e].v[c] = finite(vf[e].v[c]) ? vf[e].v[c] : 0.0f;
+                }
+                const uint64_t not_f = __ballot(!f);
+                bad |= (static_cast<uint32_t>(not_f) ? 1u << t : 0u) | (not_f >> 32 ? 1u << (t + 4) : 0u);
+            }
+        }
+        float p[1][16];
+        softmax_tile(sc, soft, p, acc, i == part, r.visible > t0, kMost<float>);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[e].v[c], p[0][e], acc[c], 0, 0, 0);
+        for (; bad; bad &= bad - 1) {
+            const uint32_t t = t0 + __ffs(static_cast<int>(bad)) - 1;
+            if (t >= r.visible) continue;
+            const float *row = values + static_cast<size_t>(t) * a.value_stride;
+            uint32_t d = a.head_dim;
+            asm("" : "+s"(d));
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const uint32_t ch = C * (8 * (e / 4) + 4 * h + e % 4) + c;
+                    if (ch < d && !finite(row[ch])) acc[c][e] += row[ch];
+                }
+        }
+    }
+
+    if (!join_parts<C, 1, kWaves>(lds, wave, lane, r.visible > part * KT, soft, acc) || r.visible == 0) return;
+    const float inv = 1.0f / soft.sum;
+    float *dst = static_cast<float *>(a.output) + static_cast<size_t>(b.q.row + r.token) * a.output_stride + r.at;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const uint32_t ch = C * (8 * (e / 4) + 4 * h + e % 4);
+        Vec<float, C> y;
+#pragma unroll
+        for (int c = 0; c < C; ++c) y.v[c] = acc[c][e] * inv;
+        if (ch + C <= a.head_dim) {
+            store_vec<float, C>(dst + ch, y);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (ch + c < a.head_dim) dst[ch + c] = y.v[c];
+        }
+    }
+}
+
+// Blocks of a batch at most: one of each sequence is not full.
+uint64_t blocks_most(const PromptArgs &a, uint32_t block_rows) {
+    return (static_cast<uint64_t>(a.tokens) * a.group + static_cast<uint64_t>(std::min(a.sequences, a.tokens)) * (block_rows - 1)) / block_rows;
+}
+template <auto KERNEL>
+hipError_t launch(const PromptArgs &a, uint32_t block_rows, size_t lds, hipStream_t stream) {
+    // once for each device: the call takes longer than the launch
+    static std::atomic<uint64_t> ready{0};
+    int id = 0;
+    hipError_t e = hipGetDevice(&id);
     if (e != hipSuccess) return e;
-    // at most one block of each sequence is not full
-    const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, used = std::min(a.sequences, a.tokens);
-    const uint32_t blocks = static_cast<uint32_t>((rows + used * (kBlockRows - 1)) / kBlockRows);
-    hipLaunchKernelGGL((prompt_attention_kernel<T, W, KT, DIRECT>), dim3(blocks * a.kv_heads), dim3(kThreads), lds, stream, a);
+    const uint64_t device = id < 64 ? 1ull << id : 0;
+    if (!(ready.load(std::memory_order_acquire) & device)) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+        if (e != hipSuccess) return e;
+        ready.fetch_or(device, std::memory_order_release);
+    }
+    hipLaunchKernelGGL(KERNEL, dim3(static_cast<uint32_t>(blocks_most(a, block_rows)) * a.kv_heads), dim3(kThreads), lds, stream, a);
     return hipGetLastError();
 }
-template <typename T, int W, int KT>
-hipError_t launch_tile(const PromptArgs &a, hipStream_t stream) {
+template <typename T, int W, int KT, int RW>
+hipError_t launch_rows(const PromptArgs &a, hipStream_t stream) {
+    constexpr size_t lds = std::max(2 * tile_bytes<T, W, KT>, join_bytes<W / 32, RW, kWaves>);
+    static_assert(lds <= 128 * 1024, "a workgroup's LDS");
     // loads to LDS take whole chunks of 16 bytes, aligned
     const uint64_t sizes = (static_cast<uint64_t>(a.head_dim) | a.key_stride | a.value_stride) * sizeof(T) |
                            reinterpret_cast<uintptr_t>(a.key) | reinterpret_cast<uintptr_t>(a.value);
-    return sizes % 16 == 0 ? launch_loads<T, W, KT, true>(a, stream) : launch_loads<T, W, KT, false>(a, stream);
+    return sizes % 16 == 0 ? launch<&prompt_attention_kernel<T, W, KT, RW, true>>(a, RW * kWaveRows, lds, stream)
+                           : launch<&prompt_attention_kernel<T, W, KT, RW, false>>(a, RW * kWaveRows, lds, stream);
+}
+template <int W>
+hipError_t launch_f32(const PromptArgs &a, hipStream_t stream) {
+    constexpr size_t lds = std::max(join_bytes<W / 32, 1, kWaves>, kQueryInLds<W> ? kWaves * kWaveSize * W * 2 : size_t(0));
+    static_assert(lds <= 128 * 1024, "a workgroup's LDS");
+    return a.head_dim == W ? launch<&prompt_attention_f32_kernel<W, true>>(a, kWaveRows, lds, stream)
+                           : launch<&prompt_attention_f32_kernel<W, false>>(a, kWaveRows, lds, stream);
+}
+// Where blocks of 128 rows are too few to fill the GPU, blocks of 64 with two waves
+// for the same rows.
+template <typename T, int W>
+hipError_t launch_width(const PromptArgs &a, hipStream_t stream) {
+    if constexpr (sizeof(T) == 4) {
+        return launch_f32<W>(a, stream);
+    } else {
+        return blocks_most(a, 4 * kWaveRows) * a.kv_heads >= kManyGroups ? launch_rows<T, W, W == 256 ? 32 : 64, 4>(a, stream)
+                                                                         : launch_rows<T, W, 64, 2>(a, stream);
+    }
 }
 template <typename T>
 hipError_t launch_prompt(const PromptArgs &a, hipStream_t stream) {
-    if (a.head_dim <= 64) return launch_tile<T, 64, sizeof(T) == 4 ? 32 : 64>(a, stream);
-    if (a.head_dim <= 128) return launch_tile<T, 128, sizeof(T) == 4 ? 32 : 64>(a, stream);
-    return launch_tile<T, 256, 32>(a, stream);
+    return a.head_dim <= 64 ? launch_width<T, 64>(a, stream) : a.head_dim <= 128 ? launch_width<T, 128>(a, stream) : launch_width<T, 256>(a, stream);
 }
 
 }  // namespace
@@ -544,7 +806,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_prompt_attention_device(QwnCudaContextHandle *h
     a.group = r->query_heads / r->kv_heads;
     // rows and blocks are counted in 32 bits
     const uint64_t all = rows * a.group;
-    if (all > 0x7fffffffu || (all / kBlockRows + std::min(r->sequences, r->tokens)) * r->kv_heads > 0x7fffffffu) {
+    if (all > 0x7fffffffu || (all / kWaveRows + std::min(r->sequences, r->tokens)) * r->kv_heads > 0x7fffffffu) {
         set_error("prompt attention: %u tokens of %u heads are too many for one call", r->tokens, r->query_heads);
         return QWN_CUDA_STATUS_UNSUPPORTED;
     }

@@ -463,9 +463,9 @@ QWN_CUDA_ABI_API int qwn_hip_ext_logits_process_device(QwnCudaContextHandle *con
  * the pairs, sections[0] belong to axis 0, sections[1] to axis 1, ... (they add
  * up to rope_dims / 2): one section after the other, or, with in_turn not 0,
  * dealt to the axes in turn, past those that have all of theirs.  Axes 0, 1 and 2
- * may be time, height and width; text has the same position in all.  In 64 bits,
- * rounded to fp32 and to dtype.  An output may be its input with that one's
- * stride. */
+ * may be time, height and width; text has the same position in all.  Angles are
+ * computed in 64 bits; fp32 rows are, too, and rounded once, 16-bit ones in fp32.
+ * An output may be its input with that one's stride. */
 #define QWN_HIP_ROTARY_AXES 4u
 typedef struct {
     QwnCudaAbiHeader header;
@@ -538,7 +538,8 @@ QWN_CUDA_ABI_API int qwn_hip_ext_prompt_attention_device(QwnCudaContextHandle *c
  * last.  next_*: of those the first `beams` whose token is none of end_tokens, the
  * same way.  No candidates come from a beam whose score is not finite, from
  * logits that are -inf or NaN (they do not count in the sum), or from a row with a
- * logit of +inf.  The order is that of 64-bit values; `values` are rounded to fp32.
+ * logit of +inf.  A row's sum is one of fp32 powers; values are added up in 64 bits,
+ * ordered there, and rounded to fp32.
  * The workspace (qwn_hip_ext_beam_select_workspace_bytes, 0 for sizes that are
  * refused; 16-byte aligned) holds nothing between calls, and may not be shared by
  * calls that run at the same time. */

@@ -25,75 +25,117 @@ template <typename T>
 constexpr uint32_t kSlice = kThreads * kLoads * (16 / sizeof(T));  // tokens of the vocabulary a workgroup takes
 
 // Candidates in order: a larger value, then the smaller place, is the larger key;
-// 0 is none.  Of a row, places are tokens and values fp32 logits; of a sequence,
-// places are beams and tokens and values 64 bits.
-__device__ __forceinline__ uint64_t row_key(float v, uint32_t token) {
-    if (!(v > -INFINITY)) return 0;  // -inf and NaN are no candidates
+// the value 0 is none.  Of a row, values are fp32 logits and places tokens; of a
+// sequence, 64-bit sums, and beams and tokens.
+__device__ __forceinline__ uint32_t ordered(float v) {  // 0 for -inf and NaN, which are no candidates
+    if (!(v > -INFINITY)) return 0;
     const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // -0 is 0
-    const uint32_t ord = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    return (static_cast<uint64_t>(ord) << 32) | (kNone - token);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float row_value(uint64_t key) {
-    const uint32_t ord = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ float unordered(uint32_t ord) {
     return __builtin_bit_cast(float, (ord & 0x80000000u) ? ord & 0x7fffffffu : ~ord);
 }
-__device__ __forceinline__ uint32_t row_token(uint64_t key) { return kNone - static_cast<uint32_t>(key); }
-
-struct BeamKey {
-    uint64_t value, place;  // ordered bits of the value; ~(beam, token)
+__device__ __forceinline__ uint64_t ordered(double v) {
+    if (!(v > -INFINITY)) return 0;
+    const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
+    return (b >> 63) ? ~b : (b | 1ull << 63);
+}
+__device__ __forceinline__ double unordered(uint64_t ord) {
+    return __builtin_bit_cast(double, (ord >> 63) ? ord & ~(1ull << 63) : ~ord);
+}
+struct Key {
+    uint64_t value, place;  // ordered bits; ~(beam, token), or ~token
 };
-__device__ __forceinline__ bool larger(uint64_t a, uint64_t b) { return a > b; }
-__device__ __forceinline__ bool larger(const BeamKey &a, const BeamKey &b) {
+__device__ __forceinline__ bool larger(const Key &a, const Key &b) {
     return a.value > b.value || (a.value == b.value && a.place > b.place);
 }
-__device__ __forceinline__ void clear(uint64_t &k) { k = 0; }
-__device__ __forceinline__ void clear(BeamKey &k) { k.value = k.place = 0; }
-__device__ __forceinline__ bool some(uint64_t k) { return k != 0; }
-__device__ __forceinline__ bool some(const BeamKey &k) { return k.value != 0; }
 
-// The `count` largest of the workgroup's keys, N a thread, largest first, in
-// list[0 .. count); none where there are fewer.  The result does not fall below the
-// count-th largest of the threads' own largest keys, and no more than count * N
-// keys are as large; of those, each one's place is the number that are larger.
-// found: room for kCountMost * N keys.
-template <typename K>
-struct Held {
-    K bound;
-    uint32_t count;
-};
-template <int N, typename K>
-__device__ __forceinline__ void select_keys(const K (&keys)[N], uint32_t count, K *tops, K *found, Held<K> *held, K *list) {
-    const uint32_t tid = threadIdx.x;
-    K top = keys[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i)
-        if (larger(keys[i], top)) top = keys[i];
-    tops[tid] = top;
-    if (tid == 0) {
-        held->count = 0;
-        clear(held->bound);
+// The count-th largest of the workgroup's 256 numbers, 0 where fewer are not 0.
+// Every wave searches for itself, two bits a step.
+__device__ __forceinline__ uint32_t find_bound(const uint32_t *numbers, uint32_t count) {
+    const uint4 x = reinterpret_cast<const uint4 *>(numbers)[threadIdx.x % kWaveSize];
+    auto above = [&](uint32_t t) {
+        return static_cast<uint32_t>(__popcll(__ballot(x.x >= t)) + __popcll(__ballot(x.y >= t)) + __popcll(__ballot(x.z >= t)) +
+                                     __popcll(__ballot(x.w >= t)));
+    };
+    uint32_t bound = 0;
+#pragma unroll 1
+    for (int bit = 30; bit >= 0; bit -= 2) {
+        const uint32_t one = 1u << bit;
+        const uint32_t n1 = above(bound | one), n2 = above(bound | one << 1), n3 = above(bound | one << 1 | one);
+        bound |= n3 >= count ? one << 1 | one : n2 >= count ? one << 1 : n1 >= count ? one : 0u;
     }
-    for (uint32_t i = tid; i < count; i += kThreads) clear(list[i]);
+    return bound;
+}
+
+// The `count` largest of the workgroup's candidates, N a thread, largest first, in
+// list[0 .. count); the value 0 where there are fewer.  key(i): the thread's i-th;
+// upper(i): what its value's upper bits are (0: none), a number that does not
+// decrease with the value; top: the largest of them.  The result does not
+// fall below the count-th largest `top`, and few candidates are as large; of those,
+// each one's place is the number that are larger.  Where they are more than kFound
+// (many are alike), the largest are taken out one by one.
+constexpr uint32_t kFound = 512;
+struct Selection {
+    uint32_t tops[kThreads];
+    Key found[kFound];
+    Key list[kCountMost];
+    Key best[kThreads / kWaveSize];
+    uint32_t held;
+};
+template <int N, typename U, typename K>
+__device__ __forceinline__ void select_keys(Selection &s, uint32_t count, uint32_t top, U upper, K key) {
+    const uint32_t tid = threadIdx.x;
+    s.tops[tid] = top;
+    if (tid == 0) s.held = 0;
     lds_barrier();
-    uint32_t rank = 0;
-    for (uint32_t i = 0; i < kThreads; ++i) rank += larger(tops[i], top) ? 1u : 0u;
-    if (rank == count - 1 && some(top)) held->bound = top;  // one thread's: keys differ, unless they are none
-    lds_barrier();
-    if (rank < count) {
-        const K bound = held->bound;
+    for (uint32_t i = tid; i < count; i += kThreads) s.list[i] = Key{0, 0};
+    const uint32_t bound = max(1u, find_bound(s.tops, count));
+    if (top >= bound) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (some(keys[i]) && !larger(bound, keys[i])) found[atomicAdd(&held->count, 1u)] = keys[i];
+            if (upper(i) >= bound) {
+                const uint32_t to = atomicAdd(&s.held, 1u);
+                if (to < kFound) s.found[to] = key(i);
+            }
     }
     lds_barrier();
-    const uint32_t n = held->count;
-    for (uint32_t e = tid; e < n; e += kThreads) {
-        const K mine = found[e];
-        uint32_t place = 0;
-        for (uint32_t i = 0; i < n; ++i) place += larger(found[i], mine) ? 1u : 0u;
-        if (place < count) list[place] = mine;
+    const uint32_t n = s.held;
+    if (n <= kFound) {
+        for (uint32_t e = tid; e < n; e += kThreads) {
+            const Key mine = s.found[e];
+            uint32_t place = 0;
+            for (uint32_t i = 0; i < n; ++i) place += larger(s.found[i], mine) ? 1u : 0u;
+            if (place < count) s.list[place] = mine;
+        }
+        lds_barrier();
+        return;
     }
-    lds_barrier();
+    Key last{~0ull, ~0ull};
+#pragma unroll 1
+    for (uint32_t k = 0; k < count; ++k) {
+        Key best{0, 0};
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+            if (upper(i) < bound) continue;
+            const Key x = key(i);
+            if (larger(last, x) && larger(x, best)) best = x;
+        }
+#pragma unroll
+        for (int off = kWaveSize / 2; off > 0; off >>= 1) {
+            const Key o{__shfl_xor(best.value, off), __shfl_xor(best.place, off)};
+            if (larger(o, best)) best = o;
+        }
+        if (tid % kWaveSize == 0) s.best[tid / kWaveSize] = best;
+        lds_barrier();
+        best = s.best[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kThreads / kWaveSize; ++w)
+            if (larger(s.best[w], best)) best = s.best[w];
+        if (tid == 0) s.list[k] = best;
+        last = best;
+        lds_barrier();  // `best` is read
+    }
 }
 
 struct SelectArgs {
@@ -112,13 +154,11 @@ struct SelectArgs {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void beam_rows_kernel(SelectArgs a) {
     constexpr int VEC = 16 / sizeof(T), N = kLoads * VEC;
-    __shared__ uint64_t tops[kThreads], found[kCountMost * N], list[kCountMost];
-    __shared__ Held<uint64_t> held;
+    __shared__ Selection select;
     __shared__ float2 red[kThreads / kWaveSize];
     const uint32_t r = blockIdx.y, v0 = blockIdx.x * kSlice<T>, tid = threadIdx.x;
     const T *in = static_cast<const T *>(a.logits) + static_cast<size_t>(r) * a.in_stride;
     float x[N];
-    uint64_t keys[N];
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
         const uint32_t v = v0 + (tid + kThreads * k) * VEC;
@@ -131,47 +171,65 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(SelectArgs a) {
             for (int i = 0; i < VEC; ++i) x[k * VEC + i] = v + i < a.vocab ? to_float(in[v + i]) : -INFINITY;
         }
     }
-    float m = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
-    m = wave_max_all(m);
+    for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
+    const float m = wave_max_all(top);
+    // logits are few steps of fp32 below m where they count: the difference and its
+    // product are rounded by 2^-24 of at most 40
+    constexpr float kLog2e = 1.44269504088896340736f;
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint32_t v = v0 + (tid + kThreads * (i / VEC)) * VEC + i % VEC;
-        keys[i] = row_key(x[i], v);
-        s += x[i] > -INFINITY ? expf(x[i] - m) : 0.0f;
-    }
+    for (int i = 0; i < N; ++i) s += x[i] > -INFINITY ? __builtin_amdgcn_exp2f((x[i] - m) * kLog2e) : 0.0f;
     s = wave_sum_all(s);
     if (tid % kWaveSize == 0) red[tid / kWaveSize] = make_float2(m, s);
-    select_keys(keys, a.count, tops, found, &held, list);
+    select_keys<N>(select, a.count, ordered(top), [&](int i) { return ordered(x[i]); },
+                   [&](int i) {
+                       const uint32_t v = v0 + (tid + kThreads * (i / VEC)) * VEC + i % VEC;
+                       return Key{ordered(x[i]), ~static_cast<uint64_t>(v)};
+                   });
     const size_t part = static_cast<size_t>(r) * a.parts + blockIdx.x;
-    for (uint32_t i = tid; i < a.count; i += kThreads) a.keys[part * a.count + i] = list[i];
+    for (uint32_t i = tid; i < a.count; i += kThreads)
+        a.keys[part * a.count + i] = select.list[i].value << 32 | static_cast<uint32_t>(~select.list[i].place);
     if (tid == 0) {
-        float top = red[0].x, sum = 0.0f;
-        for (uint32_t w = 1; w < kThreads / kWaveSize; ++w) top = fmaxf(top, red[w].x);
-        for (uint32_t w = 0; w < kThreads / kWaveSize; ++w) sum += red[w].x > -INFINITY ? red[w].y * expf(red[w].x - top) : 0.0f;
-        a.sums[part] = make_float2(top, sum);
+        float most = red[0].x, sum = 0.0f;
+        for (uint32_t w = 1; w < kThreads / kWaveSize; ++w) most = fmaxf(most, red[w].x);
+        for (uint32_t w = 0; w < kThreads / kWaveSize; ++w)
+            sum += red[w].x > -INFINITY ? red[w].y * __builtin_amdgcn_exp2f((red[w].x - most) * kLog2e) : 0.0f;
+        a.sums[part] = make_float2(most, sum);
     }
 }
 
 // grid (sequences): the rows' sums, and the largest of their parts' candidates.
 __global__ __launch_bounds__(kThreads) void beam_sequences_kernel(SelectArgs a) {
-    constexpr int N = 4;
-    __shared__ BeamKey tops[kThreads], found[kCountMost * N], list[kCountMost];
+    constexpr int N = 8;                 // keys of a thread in a round, one more of what is left of the round before
+    __shared__ Selection select;
     __shared__ double base[kBeamsMost], most[kBeamsMost];  // of a beam: its score less the logarithm of its sum, -inf: no
                                                            // candidates; its largest logit
-    __shared__ Held<BeamKey> held;
     const uint32_t tid = threadIdx.x, lane = tid % kWaveSize, wave = tid / kWaveSize, row0 = blockIdx.x * a.beams;
+    const uint32_t of_row = a.parts * a.count, all = a.beams * of_row;
+    const uint64_t *keys = a.keys + static_cast<size_t>(row0) * of_row;
+    uint64_t next[N];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t i = i0 + tid + kThreads * e;
+            next[e] = i < all ? keys[i] : 0u;
+        }
+    };
+    load(0);
     for (uint32_t b = wave; b < a.beams; b += kThreads / kWaveSize) {
         const float2 *sums = a.sums + static_cast<size_t>(row0 + b) * a.parts;
         const float score = a.scores[row0 + b];
-        float m = -INFINITY;
-        for (uint32_t i = lane; i < a.parts; i += kWaveSize) m = fmaxf(m, sums[i].x);
+        const float2 mine = lane < a.parts ? sums[lane] : make_float2(-INFINITY, 0.0f);
+        float m = mine.x;
+        for (uint32_t i = lane + kWaveSize; i < a.parts; i += kWaveSize) m = fmaxf(m, sums[i].x);
         m = wave_max_all(m);
-        double s = 0.0;
-        for (uint32_t i = lane; i < a.parts; i += kWaveSize)
-            if (sums[i].x > -INFINITY) s += static_cast<double>(sums[i].y) * exp(static_cast<double>(sums[i].x) - static_cast<double>(m));
+        auto share = [&](float2 x) {
+            return x.x > -INFINITY ? static_cast<double>(x.y) * exp(static_cast<double>(x.x) - static_cast<double>(m)) : 0.0;
+        };
+        double s = share(mine);
+        for (uint32_t i = lane + kWaveSize; i < a.parts; i += kWaveSize) s += share(sums[i]);
         s = wave_sum_f64(s);
         if (lane == 0) {
             base[b] = isfinite(m) && isfinite(score) ? static_cast<double>(score) - log(s) : -INFINITY;
@@ -179,44 +237,38 @@ __global__ __launch_bounds__(kThreads) void beam_sequences_kernel(SelectArgs a) 
         }
     }
     lds_barrier();
-    const uint32_t of_row = a.parts * a.count, all = a.beams * of_row;
-    const uint64_t *keys = a.keys + static_cast<size_t>(row0) * of_row;
-    for (uint32_t i0 = 0; i0 == 0 || i0 < all;) {
-        // what is left of the round before, and the next keys
-        BeamKey k[N];
-        const bool first = i0 == 0;
-        const uint32_t step = first ? N * kThreads : (N - 1) * kThreads;
+    for (uint32_t i0 = 0; i0 < all; i0 += N * kThreads) {
+        double v[N + 1];
+        uint64_t place[N + 1], top = 0;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            clear(k[e]);
-            if (!first && e == N - 1) {
-                if (tid < a.count) k[e] = list[tid];
-                continue;
-            }
-            const uint32_t i = i0 + tid + kThreads * e;
-            if (i >= all) continue;
-            const uint64_t key = keys[i];
-            const uint32_t b = i / of_row;
-            if (key == 0 || !(base[b] > -INFINITY)) continue;
-            const uint64_t v = __builtin_bit_cast(uint64_t, base[b] + (static_cast<double>(row_value(key)) - most[b]) + 0.0);
-            k[e].value = (v >> 63) ? ~v : (v | 1ull << 63);
-            k[e].place = ~(static_cast<uint64_t>(b) << 32 | row_token(key));
+            const uint32_t b = min((i0 + tid + kThreads * e) / of_row, a.beams - 1);
+            v[e] = next[e] ? base[b] + (static_cast<double>(unordered(static_cast<uint32_t>(next[e] >> 32))) - most[b]) : -INFINITY;
+            place[e] = ~(static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(next[e]));
         }
-        i0 += step;
-        lds_barrier();  // the list is read
-        select_keys(k, a.count, tops, found, &held, list);
+        v[N] = -INFINITY;
+        if (i0 > 0 && tid < a.count && select.list[tid].value) {
+            v[N] = unordered(select.list[tid].value);
+            place[N] = select.list[tid].place;
+        }
+        if (i0 + N * kThreads < all) load(i0 + N * kThreads);
+#pragma unroll
+        for (int e = 0; e <= N; ++e) top = max(top, ordered(v[e]));
+        if (i0 > 0) lds_barrier();  // the list is read
+        select_keys<N + 1>(select, a.count, static_cast<uint32_t>(top >> 32), [&](int i) { return static_cast<uint32_t>(ordered(v[i]) >> 32); },
+                           [&](int i) { return Key{ordered(v[i]), place[i]}; });
     }
     // the list is one wave's: place, and place among those that go on
     if (wave > 0) return;
-    const size_t out = static_cast<size_t>(blockIdx.x) * a.count, next = static_cast<size_t>(blockIdx.x) * a.beams;
+    const size_t out = static_cast<size_t>(blockIdx.x) * a.count, out_next = static_cast<size_t>(blockIdx.x) * a.beams;
     float value = -INFINITY;
     int32_t parent = -1, token = -1;
-    const bool real = lane < a.count && some(list[lane]);
+    const bool real = lane < a.count && select.list[lane].value;
     if (real) {
-        const uint64_t o = list[lane].value, place = ~list[lane].place;
-        value = static_cast<float>(__builtin_bit_cast(double, (o >> 63) ? o & ~(1ull << 63) : ~o));
-        parent = static_cast<int32_t>(row0 + static_cast<uint32_t>(place >> 32));
-        token = static_cast<int32_t>(static_cast<uint32_t>(place));
+        const uint64_t at = ~select.list[lane].place;
+        value = static_cast<float>(unordered(select.list[lane].value));
+        parent = static_cast<int32_t>(row0 + static_cast<uint32_t>(at >> 32));
+        token = static_cast<int32_t>(static_cast<uint32_t>(at));
     }
     if (lane < a.count) {
         a.values[out + lane] = value;
@@ -227,16 +279,16 @@ __global__ __launch_bounds__(kThreads) void beam_sequences_kernel(SelectArgs a) 
     bool goes = real;
     for (uint32_t i = 0; i < a.end_count; ++i) goes = goes && token != a.end_tokens[i];
     const uint64_t on = __ballot(goes);
-    const uint32_t place = __popcll(on & ((1ull << lane) - 1)), n = __popcll(on);
-    if (goes && place < a.beams) {
-        a.next_scores[next + place] = value;
-        a.next_parents[next + place] = parent;
-        a.next_tokens[next + place] = token;
+    const uint32_t to = __popcll(on & ((1ull << lane) - 1)), n = __popcll(on);
+    if (goes && to < a.beams) {
+        a.next_scores[out_next + to] = value;
+        a.next_parents[out_next + to] = parent;
+        a.next_tokens[out_next + to] = token;
     }
     if (lane >= n && lane < a.beams) {
-        a.next_scores[next + lane] = -INFINITY;
-        a.next_parents[next + lane] = -1;
-        a.next_tokens[next + lane] = -1;
+        a.next_scores[out_next + lane] = -INFINITY;
+        a.next_parents[out_next + lane] = -1;
+        a.next_tokens[out_next + lane] = -1;
     }
 }
 

@@ -14,7 +14,6 @@ namespace {
 using namespace qwn;
 
 constexpr uint32_t kPairsMost = 128;
-constexpr uint32_t kTokensMost = 4;     // of a workgroup
 constexpr uint32_t kThreadsMost = 512;
 
 struct RotaryArgs {
@@ -24,9 +23,9 @@ struct RotaryArgs {
     const int32_t *positions;
     uint32_t heads[2], in_stride[2], out_stride[2];
     uint32_t tokens, head_dim, rope, position_stride, lanes;  // lanes: of a head, a power of two
-    float eps;
+    double eps, inv_dim;
     uint8_t axis[kPairsMost];
-    double freq[kPairsMost];
+    double turns[kPairsMost];  // theta^(-2 i / rope_dims) / (2 pi)
 };
 
 // N elements [c, c + N) of a row, zeros from `end` on.
@@ -47,8 +46,8 @@ __device__ __forceinline__ Vec<T, N> load_part(const T *row, uint32_t c, uint32_
     }
     return x;
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_part(T *row, uint32_t c, uint32_t end, const double y[N]) {
+template <typename T, int N, typename R>
+__device__ __forceinline__ void store_part(T *row, uint32_t c, uint32_t end, const R y[N]) {
     constexpr int VEC = 16 / sizeof(T);
     if (c + N <= end) {
 #pragma unroll
@@ -65,98 +64,141 @@ __device__ __forceinline__ void store_part(T *row, uint32_t c, uint32_t end, con
     }
 }
 
-// A task is 8 pairs of a head (both channels of a pair in one thread: results
-// may be in place), or 16 of the channels behind the rotated ones; a head's
-// tasks lie in `lanes` lanes next to each other, which add up its squares.  A
-// workgroup takes up to 4 tokens, whose angles are computed once, in 64 bits (at
-// position 100000 an fp32 angle would be off by hundredths), while the first
-// loads are in flight.  64-bit arithmetic runs at the fp32 rate here and the bytes
-// bound the pass, so values are rounded once.
+// v of the lanes next to each other added up, `lanes` (a power of two up to 32) at a
+// time, to all of them.
+template <int CTRL>
+__device__ __forceinline__ float lane_moved(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double lane_moved(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, 0xf, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <typename R>
+__device__ __forceinline__ R lanes_sum(R v, uint32_t lanes) {
+    if (lanes > 1) v += lane_moved<0xb1>(v);   // quad_perm [1, 0, 3, 2]
+    if (lanes > 2) v += lane_moved<0x4e>(v);   // quad_perm [2, 3, 0, 1]
+    if (lanes > 4) v += lane_moved<0x141>(v);  // row_half_mirror: the other four
+    if (lanes > 8) v += lane_moved<0x140>(v);  // row_mirror: the other eight
+    if (lanes > 16) v += __shfl_xor(v, 16);
+    return v;
+}
+
+// Cosine and sine of t turns: what is left of the nearest quarter, at most pi / 4, by
+// Taylor's series to the 12th and 11th power (the next terms are below 2^-37).  The
+// library's functions take 90 registers more, which is a third of the waves.
+__device__ __forceinline__ double2 angle(double t) {
+    const double quarters = rint(4.0 * t), x = (4.0 * t - quarters) * 1.57079632679489661923, y = x * x;
+    const double c = 1.0 + y * (-1.0 / 2 + y * (1.0 / 24 + y * (-1.0 / 720 + y * (1.0 / 40320 + y * (-1.0 / 3628800 + y * (1.0 / 479001600))))));
+    const double s = x * (1.0 + y * (-1.0 / 6 + y * (1.0 / 120 + y * (-1.0 / 5040 + y * (1.0 / 362880 + y * (-1.0 / 39916800))))));
+    const int64_t q = static_cast<int64_t>(quarters);
+    const double a = q & 1 ? s : c, b = q & 1 ? c : s;
+    return make_double2((q + 1) & 2 ? -a : a, q & 2 ? -b : b);
+}
+
+// What fp32 rows are computed in, and 16-bit ones, whose own rounding is 2^-11 and
+// more: with fp32 for both, 64 bits would take twice the registers and half the waves.
 template <typename T>
-__global__ __launch_bounds__(kThreadsMost) void rotary_kernel(RotaryArgs a, uint32_t per_group) {
-    __shared__ double2 cs[kTokensMost][kPairsMost];
-    const uint32_t half = a.rope / 2, pair_tasks = (half + 7) / 8, D = a.head_dim;
-    const uint32_t heads = a.heads[0] + a.heads[1];
-    const uint32_t token0 = blockIdx.x * per_group, tokens = min(per_group, a.tokens - token0);
-    const uint32_t tasks = tokens * heads * a.lanes, nt = blockDim.x;
-    struct Task {
-        uint32_t token, head, kind, lane;
-    };
-    auto task_of = [&](uint32_t i) {
-        Task t;
-        t.lane = i % a.lanes;
-        const uint32_t j = i / a.lanes;
-        t.token = j / heads;
-        t.head = j % heads;
-        t.kind = t.head >= a.heads[0];
-        if (t.kind) t.head -= a.heads[0];
-        return t;
-    };
-    // the 16 channels of a task: the pairs' first and second ones, or one run of channels in two halves
-    auto first_of = [&](const Task &t) { return t.lane < pair_tasks ? t.lane * 8 : a.rope + (t.lane - pair_tasks) * 16; };
-    auto load = [&](uint32_t i, Vec<T, 8> &x, Vec<T, 8> &y) {
-        const Task t = task_of(i);
-        const T *row = static_cast<const T *>(a.in[t.kind]) + static_cast<size_t>(token0 + t.token) * a.in_stride[t.kind] +
-                       static_cast<size_t>(t.head) * D;
-        const uint32_t c = first_of(t);
-        if (t.lane < pair_tasks) {
-            x = load_part<T, 8>(row, c, half);
-            y = load_part<T, 8>(row + half, c, half);
-        } else {
-            x = load_part<T, 8>(row, c, D);
-            y = load_part<T, 8>(row, c + 8, D);
+struct Work {
+    typedef float real;
+    typedef float2 pair;
+};
+template <>
+struct Work<float> {
+    typedef double real;
+    typedef double2 pair;
+};
+__device__ __forceinline__ float root(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double root(double v) { return rsqrt(v); }
+
+// A thread takes 8 pairs of a head (both channels of a pair in one thread: results
+// may be in place), or 16 of the channels behind the rotated ones, of TOKENS tokens;
+// the `lanes` threads of a head, next to each other, add up its squares.
+// grid (tokens, heads): all loads are issued first; while they are on their way the
+// tokens' angles are computed, in 64 bits (at position 100000 an fp32 angle would be
+// off by hundredths).
+template <typename T, int TOKENS>
+__global__ __launch_bounds__(kThreadsMost, sizeof(T) == 4 ? 3 : 4) void rotary_kernel(RotaryArgs a) {
+    using R = typename Work<T>::real;
+    __shared__ typename Work<T>::pair cs[TOKENS][kPairsMost];  // pair f at f % 8 * 16 + f / 8: lanes read next to each other
+    const uint32_t half = a.rope / 2, pair_lanes = (half + 7) / 8, D = a.head_dim;
+    const uint32_t token0 = blockIdx.x * TOKENS, x = blockIdx.y * blockDim.x + threadIdx.x;
+    const uint32_t lane = x % a.lanes, h = x / a.lanes;  // lanes: a power of two
+    const bool real = h < a.heads[0] + a.heads[1];
+    const uint32_t kind = real && h >= a.heads[0] ? 1u : 0u, head = real ? h - (kind ? a.heads[0] : 0u) : 0u;
+    const bool pair = lane < pair_lanes;
+    // first and second channels of the pairs, or 8 channels and the 8 behind them
+    const uint32_t c = pair ? lane * 8 : a.rope + (lane - pair_lanes) * 16, next = pair ? half : 8u, end = pair ? half : D;
+    const uint32_t end2 = pair ? half : D > 8 ? D - 8 : 0u;  // of the second ones, counted from `next`
+    const T *in = static_cast<const T *>(kind ? a.in[1] : a.in[0]) + static_cast<size_t>(head) * D;
+    T *out = static_cast<T *>(kind ? a.out[1] : a.out[0]) + static_cast<size_t>(head) * D;
+    const size_t in_stride = kind ? a.in_stride[1] : a.in_stride[0], out_stride = kind ? a.out_stride[1] : a.out_stride[0];
+    const float *norm = kind ? a.norm[1] : a.norm[0];
+    Vec<T, 8> u[TOKENS], v[TOKENS];
+    if (real) {
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) {
+            const T *row = in + min(token0 + t, a.tokens - 1) * in_stride;
+            u[t] = load_part<T, 8>(row, c, end);
+            v[t] = load_part<T, 8>(row + next, c, end2);
         }
-    };
-    Vec<T, 8> x, y;
-    if (threadIdx.x < tasks) load(threadIdx.x, x, y);
-    for (uint32_t i = threadIdx.x; i < tokens * half; i += nt) {
+    }
+    Vec<float, 8> wu, wv;
+    if (real && norm) {
+        wu = load_part<float, 8>(norm, c, end);
+        wv = load_part<float, 8>(norm + next, c, end2);
+    }
+    for (uint32_t i = threadIdx.x; i < TOKENS * half; i += blockDim.x) {
         const uint32_t t = i / half, f = i % half;
-        const double p = a.positions[static_cast<size_t>(a.axis[f]) * a.position_stride + token0 + t];
-        double2 v;
-        sincos(p * a.freq[f], &v.y, &v.x);
-        cs[t][f] = v;
+        const double p = a.positions[static_cast<size_t>(a.axis[f]) * a.position_stride + min(token0 + t, a.tokens - 1)];
+        const double2 r = angle(p * a.turns[f]);
+        cs[t][f % 8 * 16 + f / 8] = {static_cast<R>(r.x), static_cast<R>(r.y)};
     }
     lds_barrier();
-    // whole waves go on, as lanes exchange
-    for (uint32_t i0 = 0; i0 < tasks; i0 += nt) {
-        const uint32_t i = i0 + threadIdx.x;
-        if (i0 > 0 && i < tasks) load(i, x, y);
-        const Task t = task_of(min(i, tasks - 1));
-        const bool pair = t.lane < pair_tasks, real = i < tasks;
-        const uint32_t c = first_of(t);
-        double u[8], v[8];
+    if (!real) return;  // all the lanes of a head
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = to_float(x.v[e]), v[e] = to_float(y.v[e]);
-        if (a.norm[0] || a.norm[1]) {
-            double sum = 0.0;
+    for (int t = 0; t < TOKENS; ++t) {
+        if (token0 + t >= a.tokens) return;
+        __builtin_amdgcn_sched_barrier(0);
+        R p[8], q[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum += u[e] * u[e] + v[e] * v[e];
-            for (uint32_t off = 1; off < a.lanes; off <<= 1) sum += __shfl_xor(sum, static_cast<int>(off));
-            if (const float *w = a.norm[t.kind]) {
-                const double inv = 1.0 / sqrt(sum / static_cast<double>(D) + static_cast<double>(a.eps));
-                const Vec<float, 8> wu = load_part<float, 8>(w, c, pair ? half : D);
-                const Vec<float, 8> wv = pair ? load_part<float, 8>(w + half, c, half) : load_part<float, 8>(w, c + 8, D);
+        for (int e = 0; e < 8; ++e) p[e] = to_float(u[t].v[e]), q[e] = to_float(v[t].v[e]);
+        if (norm) {
+            R sum = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) u[e] *= inv * wu.v[e], v[e] *= inv * wv.v[e];
-            }
+            for (int e = 0; e < 8; ++e) sum += p[e] * p[e] + q[e] * q[e];
+            const R inv = root(lanes_sum(sum, a.lanes) * static_cast<R>(a.inv_dim) + static_cast<R>(a.eps));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] *= inv * wu.v[e], q[e] *= inv * wv.v[e];
         }
-        if (!real) continue;
-        T *row = static_cast<T *>(a.out[t.kind]) + static_cast<size_t>(token0 + t.token) * a.out_stride[t.kind] +
-                 static_cast<size_t>(t.head) * D;
         if (pair) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const double2 r = cs[t.token][min(c + e, half - 1)];
-                const double p = u[e] * r.x - v[e] * r.y;
-                v[e] = u[e] * r.y + v[e] * r.x;
-                u[e] = p;
+                const auto r = cs[t][e * 16 + lane];  // past the last pair: anything, not stored
+                const R first = p[e] * r.x - q[e] * r.y;
+                q[e] = p[e] * r.y + q[e] * r.x;
+                p[e] = first;
             }
-            store_part<T, 8>(row, c, half, u);
-            store_part<T, 8>(row + half, c, half, v);
-        } else {
-            store_part<T, 8>(row, c, D, u);
-            store_part<T, 8>(row, c + 8, D, v);
         }
+        T *row = out + (token0 + t) * out_stride;
+        store_part<T, 8, R>(row, c, end, p);
+        store_part<T, 8, R>(row + next, c, end2, q);
+    }
+}
+
+// Tokens of a workgroup: more where the grid fills the GPU all the same.
+constexpr uint32_t kManyTokens = 2048, kTokens = 2;
+template <typename T>
+void launch_rotary(const RotaryArgs &a, uint64_t threads, hipStream_t stream) {
+    const uint32_t block = static_cast<uint32_t>(std::min<uint64_t>(kThreadsMost, (threads + kWaveSize - 1) / kWaveSize * kWaveSize));
+    const uint32_t groups = static_cast<uint32_t>((threads + block - 1) / block);
+    if (a.tokens >= kManyTokens) {
+        hipLaunchKernelGGL((rotary_kernel<T, kTokens>), dim3((a.tokens + kTokens - 1) / kTokens, groups), dim3(block), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((rotary_kernel<T, 1>), dim3(a.tokens, groups), dim3(block), 0, stream, a);
     }
 }
 
@@ -229,30 +271,27 @@ QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *handle, con
         a.axis[i] = static_cast<uint8_t>(x);
         --left[x];
         if (r->in_turn) x = (x + 1) % QWN_HIP_ROTARY_AXES;
-        a.freq[i] = std::pow(static_cast<double>(r->rope_theta), -2.0 * i / static_cast<double>(r->rope_dims));
+        a.turns[i] = std::pow(static_cast<double>(r->rope_theta), -2.0 * i / static_cast<double>(r->rope_dims)) / 6.28318530717958647693;
     }
     a.positions = r->positions;
     a.tokens = r->tokens;
     a.head_dim = r->head_dim;
     a.rope = r->rope_dims;
     a.eps = r->eps;
+    a.inv_dim = 1.0 / r->head_dim;
     const uint32_t lanes = (half + 7) / 8 + (r->head_dim - r->rope_dims + 15) / 16;  // at most 17
     for (a.lanes = 1; a.lanes < lanes;) a.lanes *= 2;
-    // a token of a workgroup, or, where they fill the GPU all the same, 4
-    const uint32_t per_group = r->tokens >= 1024 * kTokensMost ? kTokensMost : 1;
-    const uint64_t tasks = static_cast<uint64_t>(heads[0] + heads[1]) * a.lanes * per_group;
-    const uint32_t threads = static_cast<uint32_t>(std::min<uint64_t>(kThreadsMost, (tasks + kWaveSize - 1) / kWaveSize * kWaveSize));
-    const dim3 grid((r->tokens + per_group - 1) / per_group);
     std::lock_guard<std::mutex> lock(ctx->mutex);
     DeviceScope device(ctx->device);
     if (device.error() != hipSuccess) return hip_fail("rotary device", device.error());
     hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
+    const uint64_t threads = static_cast<uint64_t>(heads[0] + heads[1]) * a.lanes;
     if (r->dtype == QWN_HIP_DTYPE_F32) {
-        hipLaunchKernelGGL(rotary_kernel<float>, grid, dim3(threads), 0, s, a, per_group);
+        launch_rotary<float>(a, threads, s);
     } else if (r->dtype == QWN_HIP_DTYPE_F16) {
-        hipLaunchKernelGGL(rotary_kernel<f16>, grid, dim3(threads), 0, s, a, per_group);
+        launch_rotary<f16>(a, threads, s);
     } else {
-        hipLaunchKernelGGL(rotary_kernel<bf16>, grid, dim3(threads), 0, s, a, per_group);
+        launch_rotary<bf16>(a, threads, s);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? QWN_CUDA_STATUS_OK : hip_fail("rotary launch", e);

@@ -57,23 +57,36 @@ def reference(logits, scores, beams, vocab, count, ends=()):
     return value, parent, token, *nxt, c
 
 
-# The kernel's logarithm of a row's sum: each term off by 2^-23 of itself (the exponential) and by
-# 2^-24 of its exponent, at most 40 where it counts; chains of 16 to 32 fp32 sums and 8 of waves and parts.
-LSE = 2.0 ** -23 + 40 * 2.0 ** -24 + 40 * 2.0 ** -24
+# The kernel's logarithm of a row's sum: each term is off by 2^-23 of itself (the power of 2) and, of
+# its exponent of at most 40 / ln 2 where it counts, by three roundings (the difference, log2 e, their
+# product), 2^-24 each: 3 * 40 * 2^-24 of the term.  Chains of at most 32 + 8 fp32 sums.
+LSE = 2.0 ** -23 + 3 * 40 * 2.0 ** -24 + 40 * 2.0 ** -24
 
 
-def check(got, want):
+def check(got, want, vocab):
     value, parent, token, ns, np_, nt, c = want
-    # where two candidates of one sequence are further apart than sums may be off, or in one row, the order is decided
-    top = c.sort(dim=1, descending=True).values[:, :value.shape[1] + 1]
-    gap = (top[:, :-1] - top[:, 1:])[torch.isfinite(top[:, 1:])]
-    assert not bool(((gap > 0) & (gap < 2 * LSE)).any()), "two candidates that the test cannot tell apart"
-    assert torch.equal(got[1].long(), parent) and torch.equal(got[2].long(), token)
+    beams = c.shape[1] // vocab
+    # Candidates of one row are in the order of their logits, whatever its sum; of two rows, where they
+    # are further apart than the sums may be off.  Else each is as large as the one of its place, none
+    # comes twice, and those of a row are in order.
+    top, at = (x[:, :value.shape[1] + 1] for x in c.sort(dim=1, descending=True, stable=True))
+    gap, row = top[:, :-1] - top[:, 1:], at // vocab
+    near = (row[:, :-1] != row[:, 1:]) & (gap < 2 * LSE) & (top[:, 1:] > -math.inf) & (gap > 0)
+    for s in range(c.shape[0]):
+        if not bool(near[s].any()):
+            assert torch.equal(got[1][s].long(), parent[s]) and torch.equal(got[2][s].long(), token[s])
+            assert got[4][s].tolist() == np_[s] and got[5][s].tolist() == nt[s]
+            continue
+        n = int((value[s] > -math.inf).sum())
+        places = (got[1][s].long() - s * beams) * vocab + got[2][s].long()
+        assert bool(((c[s][places[:n]] - value[s][:n]).abs() <= 2 * LSE).all()) and len(set(places[:n].tolist())) == n
+        for b in range(beams):
+            mine = places[:n][places[:n] // vocab == b]
+            assert torch.equal(mine, at[s][:-1][row[s][:-1] == b][:len(mine)])
     for a, b in ((got[0], value), (got[3], torch.tensor(ns, dtype=torch.float64))):
         inf = b == -math.inf
         assert torch.equal(a == -math.inf, inf)
-        assert bool(((a.double() - b).abs()[~inf] <= LSE + 2.0 ** -24 * b.abs()[~inf]).all())
-    assert got[4].tolist() == np_ and got[5].tolist() == nt
+        assert bool(((a.double() - b).abs()[~inf] <= 2 * LSE + 2.0 ** -24 * b.abs()[~inf]).all())
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -89,7 +102,7 @@ def test_select(gpu_ctx, dtype, seqs, beams, vocab, count, odd):
     scores = -10 * torch.rand(seqs, beams, generator=g) - 0.37 * torch.arange(beams)
     ends = [int(i) for i in torch.randint(0, vocab, (2,), generator=g)]
     want = reference(x, scores, beams, vocab, count, ends)
-    check(select(gpu_ctx, x, scores, beams, vocab, count, dtype, ends, stride=vocab + odd), want)
+    check(select(gpu_ctx, x, scores, beams, vocab, count, dtype, ends, stride=vocab + odd), want, vocab)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -125,7 +138,7 @@ def test_beams_and_logits_that_are_left_out(gpu_ctx, dtype):
     x[13, 1:] = -math.inf
     want = reference(x, scores, beams, vocab, 16, [5])
     got = select(gpu_ctx, x, scores, beams, vocab, 16, dtype, [5])
-    check(got, want)
+    check(got, want, vocab)
     assert got[1][2].tolist() == [11] * 3 + [-1] * 13
     assert got[3][2].tolist()[3:] == [-math.inf] and got[4][2].tolist()[3:] == [-1]
     everything = select(gpu_ctx, torch.full_like(x, -math.inf), scores, beams, vocab, 16, dtype)
@@ -229,7 +242,7 @@ def test_select_captured_and_on_two_streams(gpu_ctx):
             gpu_ctx.beam_select_device(b[3], stream=sv.stream())
         torch.cuda.synchronize()
         assert torch.equal(a[0], b[0]) and all(torch.equal(p, q) for p, q in zip(a[1], b[1]))
-        check([t.cpu() for t in (*a[1][:3], a[0], a[1][3], a[1][4])], reference(x.cpu(), before, beams, vocab, count, [3]))
+        check([t.cpu() for t in (*a[1][:3], a[0], a[1][3], a[1][4])], reference(x.cpu(), before, beams, vocab, count, [3]), vocab)
 
 
 # ---- what the beams keep ----------------------------------------------------------

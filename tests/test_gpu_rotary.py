@@ -43,10 +43,16 @@ def reference(x, heads, d, rope, positions, sections, in_turn, norm, theta=THETA
 
 
 def check(got, want, size, dtype):
-    """64 bits rounded to fp32 and to the type, each by at most half a step; the angle, of up to 2^18,
-    in 64 bits (2^-33), twice over for the frequency's own rounding."""
+    """fp32: 64 bits rounded once, by at most half a step; the angle, of up to 2^18, in 64 bits (2^-33),
+    twice over for the frequency's own rounding.  16 bits: fp32, rounded to the type.  A square sum of up
+    to 256 channels is off by at most 22 roundings (products, chains of 16, 5 lanes), the root of it
+    by half of them and 2; weight, product, angle and two products of the rotation are 5 more: 18 of
+    2^-24 of what the element is computed from."""
     tiny = 2.0 ** -25 if dtype == "f16" else 2.0 ** -134 if dtype == "bf16" else 2.0 ** -150
-    tol = (2.0 ** -24 + (sv.HALF[dtype] if dtype != "f32" else 0.0)) * (1 + 1e-6) * want.abs() + 2.0 ** -31 * size + tiny
+    if dtype == "f32":
+        tol = 2.0 ** -24 * (1 + 1e-6) * want.abs() + 2.0 ** -31 * size + tiny
+    else:
+        tol = sv.HALF[dtype] * want.abs() + (1 + sv.HALF[dtype]) * 18 * 2.0 ** -24 * size + tiny
     assert bool(((got.double() - want).abs() <= tol).all())
 
 

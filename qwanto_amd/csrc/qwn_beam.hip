@@ -50,32 +50,28 @@ __device__ __forceinline__ bool larger(const Key &a, const Key &b) {
     return a.value > b.value || (a.value == b.value && a.place > b.place);
 }
 
-// The count-th largest of the workgroup's 256 numbers, 0 where fewer are not 0.
-// Every wave searches for itself, two bits a step.
+// The count-th largest of 64 numbers, each the largest of 4 of the workgroup's; 0
+// where fewer are not 0.  Every wave searches for itself.
 __device__ __forceinline__ uint32_t find_bound(const uint32_t *numbers, uint32_t count) {
     const uint4 x = reinterpret_cast<const uint4 *>(numbers)[threadIdx.x % kWaveSize];
-    auto above = [&](uint32_t t) {
-        return static_cast<uint32_t>(__popcll(__ballot(x.x >= t)) + __popcll(__ballot(x.y >= t)) + __popcll(__ballot(x.z >= t)) +
-                                     __popcll(__ballot(x.w >= t)));
-    };
+    const uint32_t most = max(max(x.x, x.y), max(x.z, x.w));
     uint32_t bound = 0;
-#pragma unroll 1
-    for (int bit = 30; bit >= 0; bit -= 2) {
-        const uint32_t one = 1u << bit;
-        const uint32_t n1 = above(bound | one), n2 = above(bound | one << 1), n3 = above(bound | one << 1 | one);
-        bound |= n3 >= count ? one << 1 | one : n2 >= count ? one << 1 : n1 >= count ? one : 0u;
-    }
+#pragma unroll 4
+    for (uint32_t bit = 1u << 31; bit; bit >>= 1)
+        if (static_cast<uint32_t>(__popcll(__ballot(most >= (bound | bit)))) >= count) bound |= bit;
     return bound;
 }
 
 // The `count` largest of the workgroup's candidates, N a thread, largest first, in
 // list[0 .. count); the value 0 where there are fewer.  key(i): the thread's i-th;
-// upper(i): what its value's upper bits are (0: none), a number that does not
-// decrease with the value; top: the largest of them.  The result does not
-// fall below the count-th largest `top`, and few candidates are as large; of those,
+// reaches(i, bound): whether its value's upper bits, of a number that does not
+// decrease with the value, are bound or more; top: the largest of them, 0 for none.
+// The result does not
+// fall below the count-th largest of 64 of these, and few candidates are as large; of those,
 // each one's place is the number that are larger.  Where they are more than kFound
 // (many are alike), the largest are taken out one by one.
 constexpr uint32_t kFound = 512;
+constexpr uint32_t kLeast = 0x00100000u;  // below what any number's upper bits are ordered as, above none's
 struct Selection {
     uint32_t tops[kThreads];
     Key found[kFound];
@@ -83,18 +79,18 @@ struct Selection {
     Key best[kThreads / kWaveSize];
     uint32_t held;
 };
-template <int N, typename U, typename K>
-__device__ __forceinline__ void select_keys(Selection &s, uint32_t count, uint32_t top, U upper, K key) {
+template <int N, typename R, typename K>
+__device__ __forceinline__ void select_keys(Selection &s, uint32_t count, uint32_t top, R reaches, K key) {
     const uint32_t tid = threadIdx.x;
     s.tops[tid] = top;
     if (tid == 0) s.held = 0;
     lds_barrier();
     for (uint32_t i = tid; i < count; i += kThreads) s.list[i] = Key{0, 0};
-    const uint32_t bound = max(1u, find_bound(s.tops, count));
+    const uint32_t bound = max(kLeast, find_bound(s.tops, count));
     if (top >= bound) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (upper(i) >= bound) {
+            if (reaches(i, bound)) {
                 const uint32_t to = atomicAdd(&s.held, 1u);
                 if (to < kFound) s.found[to] = key(i);
             }
@@ -117,7 +113,7 @@ __device__ __forceinline__ void select_keys(Selection &s, uint32_t count, uint32
         Key best{0, 0};
 #pragma unroll 1
         for (int i = 0; i < N; ++i) {
-            if (upper(i) < bound) continue;
+            if (!reaches(i, bound)) continue;
             const Key x = key(i);
             if (larger(last, x) && larger(x, best)) best = x;
         }
@@ -171,19 +167,23 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(SelectArgs a) {
             for (int i = 0; i < VEC; ++i) x[k * VEC + i] = v + i < a.vocab ? to_float(in[v + i]) : -INFINITY;
         }
     }
+    constexpr float kLowest = -3.402823466e38f;
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
-    const float m = wave_max_all(top);
+    for (int i = 0; i < N; ++i) {
+        x[i] = fmaxf(x[i], -INFINITY);  // NaN counts as -inf
+        top = fmaxf(top, x[i]);
+    }
+    const float m = fmaxf(wave_max_all(top), kLowest);
     // logits are few steps of fp32 below m where they count: the difference and its
     // product are rounded by 2^-24 of at most 40
     constexpr float kLog2e = 1.44269504088896340736f;
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += x[i] > -INFINITY ? __builtin_amdgcn_exp2f((x[i] - m) * kLog2e) : 0.0f;
+    for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f((x[i] - m) * kLog2e);
     s = wave_sum_all(s);
     if (tid % kWaveSize == 0) red[tid / kWaveSize] = make_float2(m, s);
-    select_keys<N>(select, a.count, ordered(top), [&](int i) { return ordered(x[i]); },
+    select_keys<N>(select, a.count, ordered(top), [&](int i, uint32_t bound) { return x[i] >= fmaxf(unordered(bound), kLowest); },
                    [&](int i) {
                        const uint32_t v = v0 + (tid + kThreads * (i / VEC)) * VEC + i % VEC;
                        return Key{ordered(x[i]), ~static_cast<uint64_t>(v)};
@@ -194,9 +194,8 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(SelectArgs a) {
     if (tid == 0) {
         float most = red[0].x, sum = 0.0f;
         for (uint32_t w = 1; w < kThreads / kWaveSize; ++w) most = fmaxf(most, red[w].x);
-        for (uint32_t w = 0; w < kThreads / kWaveSize; ++w)
-            sum += red[w].x > -INFINITY ? red[w].y * __builtin_amdgcn_exp2f((red[w].x - most) * kLog2e) : 0.0f;
-        a.sums[part] = make_float2(most, sum);
+        for (uint32_t w = 0; w < kThreads / kWaveSize; ++w) sum += red[w].y * __builtin_amdgcn_exp2f((red[w].x - most) * kLog2e);
+        a.sums[part] = make_float2(most > kLowest || sum > 0.0f ? most : -INFINITY, sum);  // else nothing but -inf and NaN
     }
 }
 
@@ -255,7 +254,7 @@ __global__ __launch_bounds__(kThreads) void beam_sequences_kernel(SelectArgs a) 
 #pragma unroll
         for (int e = 0; e <= N; ++e) top = max(top, ordered(v[e]));
         if (i0 > 0) lds_barrier();  // the list is read
-        select_keys<N + 1>(select, a.count, static_cast<uint32_t>(top >> 32), [&](int i) { return static_cast<uint32_t>(ordered(v[i]) >> 32); },
+        select_keys<N + 1>(select, a.count, static_cast<uint32_t>(top >> 32), [&](int i, uint32_t bound) { return static_cast<uint32_t>(ordered(v[i]) >> 32) >= bound; },
                            [&](int i) { return Key{ordered(v[i]), place[i]}; });
     }
     // the list is one wave's: place, and place among those that go on
@@ -372,19 +371,18 @@ __device__ __forceinline__ Kin kin_of(const AdvanceArgs &a, uint32_t row0, uint3
     return k;
 }
 
-// grid (rows, caches, at least one): the slots of the parent's page in use to the
-// row's spare, in one cache; the first of a row's workgroups writes its length
-// and the spare it gets.  Bytes bound it.
-__global__ __launch_bounds__(kThreads) void beam_copy_kernel(CopyArgs args) {
+// The slots of the parent's page in use to the row's spare, in one cache; the first
+// of a row's workgroups writes its length and the spare it gets.  Bytes bound it.
+__device__ __forceinline__ void copy_pages(const CopyArgs &args, uint32_t r, uint32_t cache) {
     const AdvanceArgs &a = args.a;
-    const uint32_t r = blockIdx.x, row0 = r / a.beams * a.beams, lane = threadIdx.x % kWaveSize;
+    const uint32_t row0 = r / a.beams * a.beams, lane = threadIdx.x % kWaveSize;
     const Kin k = kin_of(a, row0, lane);
     const int b = static_cast<int>(r - row0);
     const bool goes = lane_of(k.goes, b), later = lane_of(k.later, b);
     const uint32_t parent = lane_of(k.g.parent, b), length = lane_of(k.g.length, b);
     const uint32_t full = length >> a.page_shift, used = length & ((1u << a.page_shift) - 1);
     const int32_t spare = a.spare[r];
-    if (blockIdx.y == 0 && threadIdx.x == 0) {
+    if (cache == 0 && threadIdx.x == 0) {
         int32_t next = spare;
         if (goes && used == 0) {
             next = -1;
@@ -403,27 +401,26 @@ __global__ __launch_bounds__(kThreads) void beam_copy_kernel(CopyArgs args) {
         a.past_out[r] = goes ? static_cast<int32_t>(length) : a.past[r];
         a.spare_out[r] = next;
     }
-    if (!goes || !later || used == 0 || !args.pools[blockIdx.y]) return;
+    if (!goes || !later || used == 0 || !args.pools[cache]) return;
     const PagedKv &c = args.c;
     const int32_t from = page_of(a, parent, full);
     if (from < 0 || static_cast<uint32_t>(from) >= c.pages || spare < 0 || static_cast<uint32_t>(spare) >= c.pages || from == spare) return;
     const uint32_t tiles = (used + kPagedTile - 1) / kPagedTile, words = tiles * (paged_block_bytes(c.width) / 16);
     for (uint32_t i = threadIdx.x; i < c.kv_heads * words; i += kThreads) {
         const uint32_t head = i / words, w = i % words;
-        uint8_t *pool = args.pools[blockIdx.y];
+        uint8_t *pool = args.pools[cache];
         reinterpret_cast<uint4 *>(pool + paged_block_at(c, static_cast<uint32_t>(spare), 0, head))[w] =
             reinterpret_cast<const uint4 *>(pool + paged_block_at(c, static_cast<uint32_t>(from), 0, head))[w];
     }
 }
 
-// grid (columns, sequences): a thread moves a column of the table or of the
-// histories in all of the sequence's rows, reading all of them first, so that they
-// may be in place.
-__global__ __launch_bounds__(kThreads) void beam_rows_move_kernel(AdvanceArgs a, uint32_t table_groups) {
-    const uint32_t row0 = blockIdx.y * a.beams, lane = threadIdx.x % kWaveSize;
+// A thread moves a column of the table or of the histories in all of the
+// sequence's rows, reading all of them first, so that they may be in place.
+__device__ __forceinline__ void move_columns(const AdvanceArgs &a, uint32_t sequence, uint32_t group, uint32_t table_groups) {
+    const uint32_t row0 = sequence * a.beams, lane = threadIdx.x % kWaveSize;
     const Kin k = kin_of(a, row0, lane);
-    const bool table = blockIdx.x < table_groups;
-    const uint32_t column = (table ? blockIdx.x : blockIdx.x - table_groups) * kThreads + threadIdx.x;
+    const bool table = group < table_groups;
+    const uint32_t column = (table ? group : group - table_groups) * kThreads + threadIdx.x;
     const uint32_t stride = table ? a.table_stride : a.history_length;
     const bool in = column < stride;
     const int32_t *from = table ? a.table : a.history;
@@ -449,6 +446,18 @@ __global__ __launch_bounds__(kThreads) void beam_rows_move_kernel(AdvanceArgs a,
 #pragma unroll
     for (uint32_t b = 0; b < kBeamsMost; ++b)
         if (b < a.beams) to[static_cast<size_t>(row0 + b) * stride + column] = v[b];
+}
+
+// grid: workgroups from `first` on of those that copy (a row and a cache each, at
+// least one cache), then of those that move (a sequence, and 256 columns).
+__global__ __launch_bounds__(kThreads) void beam_advance_kernel(CopyArgs args, uint32_t first, uint32_t copies, uint32_t rows,
+                                                                uint32_t groups, uint32_t table_groups) {
+    const uint32_t i = first + blockIdx.x;
+    if (i < copies) {
+        copy_pages(args, i % rows, i / rows);
+    } else {
+        move_columns(args.a, (i - copies) / groups, (i - copies) % groups, table_groups);
+    }
 }
 
 }  // namespace
@@ -532,7 +541,8 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_beam_advance_device(QwnCudaContextHand
     const uint64_t rows = static_cast<uint64_t>(r->sequences) * r->beams;
     const uint64_t table_groups = (static_cast<uint64_t>(r->table_stride) + kThreads - 1) / kThreads;
     const uint64_t history_groups = r->history ? (static_cast<uint64_t>(r->history_length) + kThreads - 1) / kThreads : 0;
-    if (r->beams > kBeamsMost || rows > 65535 || count > kCachesMost) {
+    const uint64_t groups = table_groups + history_groups;
+    if (r->beams > kBeamsMost || rows > 65535 || count > kCachesMost || rows * std::max(1u, count) + r->sequences * groups > 0x7fffffffu) {
         set_error("unsupported beam advance: %u sequences of %u beams, %u caches", r->sequences, r->beams, count);
         return QWN_CUDA_STATUS_UNSUPPORTED;
     }
@@ -588,14 +598,16 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_beam_advance_device(QwnCudaContextHand
     a.added = r->added;
     a.history_length = r->history_length;
     hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
-    // the copies read the tables as they were: a launch of their own
-    hipLaunchKernelGGL(beam_copy_kernel, dim3(static_cast<uint32_t>(rows), std::max(1u, count)), dim3(kThreads), 0, s, c);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess) {
-        hipLaunchKernelGGL(beam_rows_move_kernel, dim3(static_cast<uint32_t>(table_groups + history_groups), r->sequences), dim3(kThreads), 0,
-                           s, a, static_cast<uint32_t>(table_groups));
-        e = hipGetLastError();
-    }
+    // the copies read the tables as they were: a launch of their own where these are in place
+    const uint32_t copies = static_cast<uint32_t>(rows * std::max(1u, count)), moves = static_cast<uint32_t>(r->sequences * groups);
+    const bool in_two = r->page_table_out == r->page_table;
+    auto launch = [&](uint32_t first, uint32_t n) {
+        hipLaunchKernelGGL(beam_advance_kernel, dim3(n), dim3(kThreads), 0, s, c, first, copies, static_cast<uint32_t>(rows),
+                           static_cast<uint32_t>(groups), static_cast<uint32_t>(table_groups));
+        return hipGetLastError();
+    };
+    hipError_t e = launch(0, in_two ? copies : copies + moves);
+    if (e == hipSuccess && in_two) e = launch(copies, moves);
     if (e != hipSuccess) return hip_fail("beam advance launch", e);
     ctx->telemetry.kv_cache_kernel_count++;
     return QWN_CUDA_STATUS_OK;

@@ -617,17 +617,20 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
 
 // fp32.  A product of two fp32 operands (v_mfma_f32_32x32x2_f32) takes 64 cycles for
 // an operand of 4 bytes a lane, 16 times as long as the 16-bit ones for theirs: L2
-// brings a wave's operands in the time, so there is no LDS and no barrier.  The four
-// waves of a workgroup take the same 32 rows and every fourth tile of 32 tokens; a tile's values come
-// while its scores are computed, the next tile's keys from then on, in one set of
-// registers each.  A lane's values are W / 32 channels next to each other: block
-// c of the output's rows are channels c, c + W / 32, ...  WHOLE: heads of W channels.
-// Of 256 channels the output, keys and values have 384 registers: the lane's query
-// stays in LDS.
-template <int W>
-constexpr bool kQueryInLds = W == 256;
+// brings a wave's operands in the time, so keys and values need no LDS and no barrier
+// (through LDS one call of four prompts of up to 1024 tokens, 12 heads, took 225 us, and
+// takes 77).  The four waves of a workgroup take the same 32 rows and every fourth
+// tile of 32 tokens.  A tile's values are loaded when its scores are there, into the
+// registers that held its keys, the next keys after its sums: with the rows' query
+// in LDS two waves a SIMD (of 64 channels three) fit, one's products run while the
+// other waits (one wave with loads ahead: 32 heads of 128 channels, 4096 tokens, 1440 us
+// for 1176; of 256 channels, where they did not fit, 430 for 176).
+// A lane's values are W / 32 channels next to each other: block c of the output's
+// rows are channels c, c + W / 32, ...  WHOLE: heads of W channels.
+// Bound by the matrix unit: those 1176 us are 117 TFLOP/s, of 154 that a large product
+// reaches; few rows by the longest one's chain of tiles.
 template <int W, bool WHOLE>
-__global__ __launch_bounds__(kThreads, W == 64 ? 2 : 1) void prompt_attention_f32_kernel(PromptArgs a) {
+__global__ __launch_bounds__(kThreads, W <= 128 ? 2 : 1) void prompt_attention_f32_kernel(PromptArgs a) {
     constexpr uint32_t KT = 32, KW = kWaves;
     constexpr int C = W / 32, J = W / 8;
     extern __shared__ v4u lds[];
@@ -672,15 +675,16 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 2 : 1) void prompt_attention_f3
             }
         }
     };
-    if (part < count) load_keys(part);
     v4u qf[J];
     Softmax soft;
     load_query<float>(a, b, r, h, qf, soft.mul);
-    v4u *own = lds + wave * J * kWaveSize + lane;
-    if constexpr (kQueryInLds<W>) {
+    v4u *const query = lds + lane;
+    if (wave == 0) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) own[j * kWaveSize] = qf[j];
+        for (int j = 0; j < J; ++j) query[j * kWaveSize] = qf[j];
     }
+    lds_barrier();
+    if (part < count) load_keys(part);
     v16f acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -688,26 +692,21 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 2 : 1) void prompt_attention_f3
         for (int e = 0; e < 16; ++e) acc[c][e] = 0.0f;
 
     for (uint32_t i = part; i < count; i += KW) {
-        if constexpr (!kQueryInLds<W>) {
-            load_values(i);
-            __builtin_amdgcn_sched_barrier(0);  // or they are put off until they are needed
-        }
         const uint32_t t0 = i * KT;
         v16f sc[1], odd;  // two chains of products
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[0][e] = odd[e] = 0.0f;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const v4f q4 = __builtin_bit_cast(v4f, kQueryInLds<W> ? own[j * kWaveSize] : qf[j]);
+            const v4f q4 = __builtin_bit_cast(v4f, query[j * kWaveSize]);
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
                 sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j].v[e], q4[e], sc[0], 0, 0, 0);
                 odd = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j].v[e + 1], q4[e + 1], odd, 0, 0, 0);
             }
         }
-        if constexpr (kQueryInLds<W>) load_values(i);
-        load_keys(min(i + KW, count - 1));  // past the last tile too: how many loads are in flight does not depend on a branch
-        __builtin_amdgcn_sched_barrier(0);
+        load_values(i);
+        __builtin_amdgcn_sched_barrier(0);  // or they are put off until they are needed
         sc[0] += odd;
         uint32_t bad = 0;  // tokens of a masked tile with values that are not finite
         if (t0 + KT > r.w_least) {
@@ -732,6 +731,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 2 : 1) void prompt_attention_f3
         for (int e = 0; e < 16; ++e)
 #pragma unroll
             for (int c = 0; c < C; ++c) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[e].v[c], p[0][e], acc[c], 0, 0, 0);
+        load_keys(min(i + KW, count - 1));  // past the last tile too: how many loads are in flight does not depend on a branch
         for (; bad; bad &= bad - 1) {
             const uint32_t t = t0 + __ffs(static_cast<int>(bad)) - 1;
             if (t >= r.visible) continue;
@@ -799,7 +799,7 @@ hipError_t launch_rows(const PromptArgs &a, hipStream_t stream) {
 }
 template <int W>
 hipError_t launch_f32(const PromptArgs &a, hipStream_t stream) {
-    constexpr size_t lds = std::max(join_bytes<W / 32, 1, kWaves>, kQueryInLds<W> ? kWaves * kWaveSize * W * 2 : size_t(0));
+    constexpr size_t lds = std::max<size_t>(join_bytes<W / 32, 1, kWaves>, kWaveSize * W * 2);
     static_assert(lds <= 128 * 1024, "a workgroup's LDS");
     return a.head_dim == W ? launch<&prompt_attention_f32_kernel<W, true>>(a, kWaveRows, lds, stream)
                            : launch<&prompt_attention_f32_kernel<W, false>>(a, kWaveRows, lds, stream);

@@ -500,11 +500,13 @@ QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *context, co
  * starts[sequences] belong to no sequence: they are not read, and the output
  * keeps what it held there; a sequence whose rows do not lie in 0 .. tokens is
  * left out.  Scores and sums are fp32, probabilities are rounded to dtype; fp32 is
- * fp32 throughout.  Scores may be of any size, past fp32's too (of fp32 and bf16, a
- * channel counts as zero where the key is below 2^-100, or the query below 2^-100 of
- * its row's largest).  A row with a score that is NaN or infinite, or with a
- * scale that is, is NaN; a value that is not finite makes its channel so in the
- * rows that attend to it, and in no other.  For single tokens behind a cache:
+ * fp32 throughout.  Finite queries, keys and scale have their softmax whatever the
+ * scores' size, past fp32's too (of fp32 and bf16, a channel counts as zero where the
+ * key is below 2^-100, or the query below 2^-100 of its row's largest).  A key or query
+ * with an infinity: a score of -inf has probability 0, a row with one that is +inf or
+ * NaN, and a row with a scale that is not finite, is NaN.  A value that is not finite
+ * makes its channel so in the rows that attend to it, and in no other.  For single
+ * tokens behind a cache:
  * qwn_hip_ext_paged_kv_attention_device. */
 typedef struct {
     QwnCudaAbiHeader header;

@@ -120,6 +120,9 @@ __device__ __forceinline__ double root(double v) { return rsqrt(v); }
 // grid (tokens, heads): all loads are issued first; while they are on their way the
 // tokens' angles are computed, in 64 bits (at position 100000 an fp32 angle would be
 // off by hundredths).
+// Bound by HBM: 4099 tokens of 40 bf16 heads of 128 with norms, 84 MB, 21 us, 4 TB/s of the
+// 5.1 that a large copy reaches; few tokens by a launch and two loads, one
+// after the other, 2.9 us.
 template <typename T, int TOKENS>
 __global__ __launch_bounds__(kThreadsMost, sizeof(T) == 4 ? 3 : 4) void rotary_kernel(RotaryArgs a) {
     using R = typename Work<T>::real;

@@ -546,7 +546,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_paged_kv_beam_advance_device(QwnCudaContextHand
     const uint64_t table_groups = (static_cast<uint64_t>(r->table_stride) + kThreads - 1) / kThreads;
     const uint64_t history_groups = r->history ? (static_cast<uint64_t>(r->history_length) + kThreads - 1) / kThreads : 0;
     const uint64_t groups = table_groups + history_groups;
-    if (r->beams > kBeamsMost || rows > 65535 || count > kCachesMost || rows * std::max(1u, count) + r->sequences * groups > 0x7fffffffu) {
+    if (r->beams > kBeamsMost || rows > 65535 || count > kCachesMost || rows * std::max(1u, count) + r->sequences * groups > 0xffffffffu / kThreads) {
         set_error("unsupported beam advance: %u sequences of %u beams, %u caches", r->sequences, r->beams, count);
         return QWN_CUDA_STATUS_UNSUPPORTED;
     }

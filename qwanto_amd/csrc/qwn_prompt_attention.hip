@@ -861,9 +861,9 @@ QWN_CUDA_ABI_API int qwn_hip_ext_prompt_attention_device(QwnCudaContextHandle *h
         return QWN_CUDA_STATUS_INVALID_ARGUMENT;
     }
     a.group = r->query_heads / r->kv_heads;
-    // rows and blocks are counted in 32 bits
+    // rows are counted in 32 bits, the threads of a launch, too
     const uint64_t all = rows * a.group;
-    if (all > 0x7fffffffu || (all / kWaveRows + std::min(r->sequences, r->tokens)) * r->kv_heads > 0x7fffffffu) {
+    if (all > 0x7fffffffu || (all / kWaveRows + std::min(r->sequences, r->tokens)) * r->kv_heads > 0xffffffffu / kThreads) {
         set_error("prompt attention: %u tokens of %u heads are too many for one call", r->tokens, r->query_heads);
         return QWN_CUDA_STATUS_UNSUPPORTED;
     }

@@ -194,9 +194,12 @@ __global__ __launch_bounds__(kThreadsMost, sizeof(T) == 4 ? 3 : 4) void rotary_k
 
 // Tokens of a workgroup: more where the grid fills the GPU all the same.
 constexpr uint32_t kManyTokens = 2048, kTokens = 2;
+uint32_t block_of(uint64_t threads) {
+    return static_cast<uint32_t>(std::min<uint64_t>(kThreadsMost, (threads + kWaveSize - 1) / kWaveSize * kWaveSize));
+}
 template <typename T>
 void launch_rotary(const RotaryArgs &a, uint64_t threads, hipStream_t stream) {
-    const uint32_t block = static_cast<uint32_t>(std::min<uint64_t>(kThreadsMost, (threads + kWaveSize - 1) / kWaveSize * kWaveSize));
+    const uint32_t block = block_of(threads);
     const uint32_t groups = static_cast<uint32_t>((threads + block - 1) / block);
     if (a.tokens >= kManyTokens) {
         hipLaunchKernelGGL((rotary_kernel<T, kTokens>), dim3((a.tokens + kTokens - 1) / kTokens, groups), dim3(block), 0, stream, a);
@@ -284,11 +287,15 @@ QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *handle, con
     a.inv_dim = 1.0 / r->head_dim;
     const uint32_t lanes = (half + 7) / 8 + (r->head_dim - r->rope_dims + 15) / 16;  // at most 17
     for (a.lanes = 1; a.lanes < lanes;) a.lanes *= 2;
+    const uint64_t threads = static_cast<uint64_t>(heads[0] + heads[1]) * a.lanes;
+    if ((tokens + kTokens - 1) / kTokens * block_of(threads) > 0xffffffffu) {  // a launch's threads are counted in 32 bits
+        set_error("unsupported rotary request: %u tokens of %u heads in one call", r->tokens, heads[0] + heads[1]);
+        return QWN_CUDA_STATUS_UNSUPPORTED;
+    }
     std::lock_guard<std::mutex> lock(ctx->mutex);
     DeviceScope device(ctx->device);
     if (device.error() != hipSuccess) return hip_fail("rotary device", device.error());
     hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
-    const uint64_t threads = static_cast<uint64_t>(heads[0] + heads[1]) * a.lanes;
     if (r->dtype == QWN_HIP_DTYPE_F32) {
         launch_rotary<float>(a, threads, s);
     } else if (r->dtype == QWN_HIP_DTYPE_F16) {

@@ -9,7 +9,8 @@ import pytest
 import torch
 
 import serving as sv
-from test_gpu_beam import advance_reference
+from qwanto_amd import abi
+from test_gpu_beam import Beams, advance_reference
 from test_gpu_beam import check as check_select
 from test_gpu_beam import reference as select_reference
 from test_gpu_prompt_attention import check as check_prompt
@@ -309,3 +310,24 @@ def test_two_at_once(gpu_ctx):
     finally:
         for g in gens:
             g.close()
+
+
+def test_more_than_a_launch_counts(gpu_ctx):
+    """A launch has less than 2^32 threads: more are refused on the host, before anything is read."""
+    far = lambda i: (1 << 44) + (i << 42)  # noqa: E731
+    b = Beams(gpu_ctx, 1, 4, 16, 20)
+    try:
+        calls = [
+            (gpu_ctx.rotary_device, (gpu_ctx.rotary_request(2 ** 31 - 1, "f16", DIM, DIM, THETA, far(0), query_heads=2, q_ptr=far(1),
+                                                            q_out_ptr=far(2)),)),
+            (gpu_ctx.prompt_attention_device, (gpu_ctx.prompt_attention_request(1, 1 << 26, far(0), "bf16", 32, 8, 1, far(1), far(2), far(3), far(4),
+                                                                                1.0),)),
+            (gpu_ctx.paged_kv_beam_advance_device, (b.caches * 128, gpu_ctx.beam_advance_request(16383, 4, 16, 2, *(far(i) for i in range(7))))),
+        ]
+        for call, args in calls:
+            with pytest.raises(abi.AbiError) as e:
+                call(*args, stream=sv.stream())
+            assert e.value.status == -5, call
+        torch.cuda.synchronize()
+    finally:
+        b.close()

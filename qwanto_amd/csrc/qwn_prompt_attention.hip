@@ -44,6 +44,13 @@ constexpr float kFar = 0x1p20f;               // of references: past it their ro
 // prompt of 512 tokens, 128 groups, 18 us and in blocks of 64 14; of 1777 and eight
 // shorter, 728 groups, 52 and 59).
 constexpr uint64_t kManyGroups = 320;
+// Heads of 64 channels have half the products between two barriers: in sequences of that
+// many tokens on average tiles of 128, until so many workgroups hide the barriers by
+// themselves (16 heads: one prompt of 2048 tokens 23 us for 27, of 3000, 1200 and 300 45 for
+// 50; but 30 of 200, whose last tiles are mostly masked, 19 for 16, and one of 8192, 1024
+// groups, 165 for 160).
+constexpr uint32_t kLongTokens = 512;
+constexpr uint64_t kFullGroups = 1024;
 
 struct PromptArgs {
     const void *query, *key, *value;
@@ -816,8 +823,12 @@ hipError_t launch_width(const PromptArgs &a, hipStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         return launch_f32<W>(a, stream);
     } else {
-        return blocks_most(a, 4 * kWaveRows) * a.kv_heads >= kManyGroups ? launch_rows<T, W, W == 256 ? 32 : 64, 4>(a, stream)
-                                                                         : launch_rows<T, W, 64, 2>(a, stream);
+        const uint64_t groups = blocks_most(a, 4 * kWaveRows) * a.kv_heads;
+        if constexpr (W == 64) {
+            if (a.tokens / a.sequences >= kLongTokens && groups < kFullGroups)
+                return groups >= kManyGroups ? launch_rows<T, W, 128, 4>(a, stream) : launch_rows<T, W, 128, 2>(a, stream);
+        }
+        return groups >= kManyGroups ? launch_rows<T, W, W == 256 ? 32 : 64, 4>(a, stream) : launch_rows<T, W, 64, 2>(a, stream);
     }
 }
 template <typename T>

@@ -110,6 +110,30 @@ def test_sizes(gpu_ctx, dtype, heads, kv_heads, d, lengths, pad):
     check(got, q, k, v, lengths, heads, kv_heads, d, d ** -0.5, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d,lengths,pad", [(32, 16, 64, [1300, 0, 700, 511, 129], 2), (8, 2, 64, [640, 1, 1100], 0),
+                                                          (4, 1, 40, [1029], 1), (40, 40, 56, [515], 0), (3, 1, 63, [900, 127, 640], 3)])
+def test_long_sequences_of_small_heads(gpu_ctx, dtype, heads, kv_heads, d, lengths, pad):
+    """Sequences of 512 tokens and more on average, heads of up to 64 channels: larger tiles."""
+    q, k, v = inputs(sum(lengths) + d, sum(lengths) + pad, heads, kv_heads, d, dtype)
+    check(attend(gpu_ctx, q, k, v, lengths, heads, kv_heads, d, d ** -0.5, dtype), q, k, v, lengths, heads, kv_heads, d, d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_masked_values_in_larger_tiles(gpu_ctx, dtype):
+    """Values that are not finite in the last tiles reach the rows that see them, and no other."""
+    n, d = 700, 64
+    q, k, v = inputs(3, n, 4, 2, d, dtype)
+    clean = attend(gpu_ctx, q, k, v, [n], 4, 2, d, 0.125, dtype).cpu()
+    for t in (0, 63, 64, 127, 128, 300, 447, 640, 699):
+        b = v.clone()
+        b[t, 5], b[t, d + 9] = math.inf, math.nan
+        got = attend(gpu_ctx, q, k, b, [n], 4, 2, d, 0.125, dtype).cpu()
+        assert bool((got[t:, [5, d + 5]] == math.inf).all()) and bool(torch.isnan(got[t:, [2 * d + 9, 3 * d + 9]]).all()), t
+        got[t:, [5, d + 5, 2 * d + 9, 3 * d + 9]] = clean[t:, [5, d + 5, 2 * d + 9, 3 * d + 9]]
+        assert torch.equal(got, clean), t
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_many_sequences(gpu_ctx, dtype):
     """More sequences than a wave has lanes, most of one token and some of none."""

@@ -579,10 +579,12 @@ QWN_CUDA_ABI_API int qwn_hip_ext_beam_select_device(QwnCudaContextHandle *contex
  * that are full are shared; the one in use goes on with the first row that has
  * this parent, and each further one takes the page `spare` that it holds, to
  * which the slots are copied in every cache given, and in exchange the page in
- * use of a row that nothing goes on from becomes its spare.  Where the page in
- * use has just become full, every row takes its spare as the next one, and has
- * none (-1) until the caller hands it another.  So a row owns two pages, one in
- * use and one spare, and no row's table names another's; the caller takes back
+ * use of a row that nothing goes on from becomes its spare, as long as there are such
+ * rows (a row of a negative length leaves no page).  Where the page in
+ * use has just become full, the row takes its spare as the next one, and has
+ * none (-1) until the caller hands it another, or gets a page in use that no
+ * copy has taken, which only a row of another length leaves.  So a row owns two pages, one in
+ * use and one spare, no row's table names another's, and none in use is lost; the caller takes back
  * full pages that no table names any more.  Table entries past the page in use are
  * -1.  A row whose parent is none of its sequence (-1) goes on from itself, with no
  * token; one whose parent's length is negative, too (its own negative: nothing of

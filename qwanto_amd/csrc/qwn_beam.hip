@@ -374,6 +374,38 @@ __device__ __forceinline__ Kin kin_of(const AdvanceArgs &a, uint32_t row0, uint3
     return k;
 }
 
+// The n-th of some bits (from 0); none past the last.
+__device__ __forceinline__ uint32_t nth_of(uint64_t bits, uint32_t n) {
+    for (; n > 0 && bits; --n) bits &= bits - 1;
+    return bits ? __ffsll(static_cast<unsigned long long>(bits)) - 1 : kNone;
+}
+// The spare that the lane's row has afterwards.  Pages in use are left by rows that nothing
+// goes on from, where they have a length and a page that has not just become full.  A
+// row that copies takes the one of the row that has its place among the childless, if it
+// left one, else the first that nobody took so, in order; those that are left then go to rows that
+// begin a page (of other lengths: of one length there are none left).  So a page in use is
+// lost only where no row has room for it.
+__device__ __forceinline__ int32_t spare_of(const AdvanceArgs &a, const Kin &k, uint32_t row0, uint32_t lane) {
+    const bool row = lane < a.beams;
+    const uint32_t slots = (1u << a.page_shift) - 1;
+    const int32_t past = row ? a.past[row0 + lane] : -1;
+    const int64_t length = static_cast<int64_t>(past) + a.added;
+    const int32_t page = past >= 0 && (length & slots) && length >> a.page_shift < a.table_stride
+                             ? page_of(a, row0 + lane, static_cast<uint32_t>(length >> a.page_shift)) : -1;
+    const bool copies = k.later && (k.g.length & slots), begins = k.goes && !(k.g.length & slots);
+    const uint64_t below = (1ull << lane) - 1, all_copy = __ballot(copies), left = __ballot(((k.childless >> lane) & 1) && page >= 0);
+    // by place: the lane's row as one that copies, and as one that leaves its page
+    const uint32_t giver = nth_of(k.childless, __popcll(k.laters & below)), taker = nth_of(k.laters, __popcll(k.childless & below));
+    const bool served = copies && giver != kNone && (left >> giver & 1), gives = taker != kNone && (all_copy >> taker & 1);
+    // in order: who has none yet, then who begins a page; of what is left
+    const uint64_t free = __ballot((left >> lane & 1) && !gives), want = __ballot(copies && !served), later_want = __ballot(begins);
+    const uint32_t place = begins ? __popcll(want) + __popcll(later_want & below) : __popcll(want & below);
+    const uint32_t from = served ? giver : nth_of(free, place);
+    const int32_t taken = __shfl(page, static_cast<int>(from == kNone ? 0u : from));
+    const int32_t spare = row ? a.spare[row0 + lane] : -1;
+    return copies || begins ? (from == kNone ? -1 : taken) : spare;
+}
+
 // The slots of the parent's page in use to the row's spare, in one cache; the first
 // of a row's workgroups writes its length and the spare it gets.  Bytes bound it.
 __device__ __forceinline__ void copy_pages(const CopyArgs &args, uint32_t r, uint32_t cache) {
@@ -385,24 +417,12 @@ __device__ __forceinline__ void copy_pages(const CopyArgs &args, uint32_t r, uin
     const uint32_t parent = lane_of(k.g.parent, b), length = lane_of(k.g.length, b);
     const uint32_t full = length >> a.page_shift, used = length & ((1u << a.page_shift) - 1);
     const int32_t spare = a.spare[r];
-    if (cache == 0 && threadIdx.x == 0) {
-        int32_t next = spare;
-        if (goes && used == 0) {
-            next = -1;
-        } else if (goes && later) {
-            // of the rows that nothing goes on from, the one with this row's place among those that copy
-            uint64_t left = k.childless;
-            for (uint64_t before = k.laters & ((1ull << b) - 1); before; before &= before - 1) left &= left - 1;
-            next = -1;
-            if (left) {
-                const uint32_t q = row0 + __ffsll(static_cast<unsigned long long>(left)) - 1;
-                const int64_t past = static_cast<int64_t>(a.past[q]) + a.added;
-                if (a.past[q] >= 0 && (past & ((1 << a.page_shift) - 1)))
-                    next = page_of(a, q, static_cast<uint32_t>(min(past >> a.page_shift, static_cast<int64_t>(a.table_stride))));
-            }
+    if (cache == 0 && threadIdx.x < kWaveSize) {
+        const int32_t next = spare_of(a, k, row0, lane);
+        if (lane == static_cast<uint32_t>(b)) {
+            a.past_out[r] = goes ? static_cast<int32_t>(length) : a.past[r];
+            a.spare_out[r] = next;
         }
-        a.past_out[r] = goes ? static_cast<int32_t>(length) : a.past[r];
-        a.spare_out[r] = next;
     }
     if (!goes || !later || used == 0 || !args.pools[cache]) return;
     const PagedKv &c = args.c;

@@ -430,6 +430,106 @@ def test_advance_parents_of_every_kind(gpu_ctx):
         b.close()
 
 
+class Owned:
+    """A sequence's rows as a caller keeps them, at lengths of their own: every page in use and every spare has one
+    owner, whole pages are shared; rows of a negative length have a spare and nothing else."""
+
+    def __init__(self, b, past, rng):
+        page, width = b.page, b.stride
+        pages = list(range(b.pages))
+        rng.shuffle(pages)
+        whole = [pages.pop() for _ in range(3)]
+        self.past = torch.tensor(past, dtype=torch.int32)
+        self.table = torch.full((len(past), width), -1, dtype=torch.int32)
+        for r, n in enumerate(past):
+            for c in range(n // page if n >= 0 else 0):
+                self.table[r, c] = whole[c]
+            if n >= 0 and n // page < width:
+                self.table[r, n // page] = pages.pop()
+        self.spare = torch.tensor([pages.pop() for _ in past], dtype=torch.int32)
+        self.history = torch.zeros(len(past), 4, dtype=torch.int32)
+
+    def state(self):
+        return self.past, self.table, self.spare, self.history
+
+
+def check_ownership(b, parents, before, after):
+    """A step of one token by the rule of ownership.  Of the rows' pages, in use before or spare, each is afterwards the
+    page in use or the spare of one row, as long as there are rows without a spare to take it; the first row with a
+    parent goes on in that one's page in use, further ones and rows that begin a page in their own spare."""
+    past, table, spare, _ = before
+    past2, table2, spare2, _ = after
+    rows, width, page = len(past), table.shape[1], b.page
+    real = [0 <= int(p) < rows and int(past[p]) >= 0 for p in parents]
+    parent = [int(p) if ok else r for r, (p, ok) in enumerate(zip(parents, real))]
+    goes = [int(past[parent[r]]) >= 0 for r in range(rows)]
+    cell = lambda t, r, n: int(t[r, n // page]) if n // page < width else -1  # noqa: E731
+    gone_on, mine, given = set(), {}, set()
+    for r in range(rows):
+        if not goes[r]:
+            assert int(past2[r]) == int(past[r]) and torch.equal(table2[r], table[r]) and int(spare2[r]) == int(spare[r])
+            continue
+        p, n = parent[r], int(past[parent[r]]) + 1
+        assert int(past2[r]) == n
+        takes = n % page == 0 or p in gone_on
+        gone_on.add(p)
+        assert cell(table2, r, n) == (int(spare[r]) if takes else cell(table, p, n))
+        mine[r] = cell(table2, r, n)
+        if not takes:
+            assert int(spare2[r]) == int(spare[r])
+        elif int(spare2[r]) >= 0:
+            given.add(int(spare2[r]))
+    # what rows that nothing goes on from leave: their pages in use
+    left = {cell(table, q, int(past[q]) + 1) for q in range(rows) if int(past[q]) >= 0 and q not in gone_on and (int(past[q]) + 1) % page} - {-1}
+    assert given <= left
+    without = [r for r in range(rows) if goes[r] and int(spare2[r]) < 0]
+    assert given == left or not without, (given, left, without)
+    owned_now = list(mine.values()) + [int(s) for s in spare2 if s >= 0]
+    assert len(owned_now) == len(set(owned_now))
+    return left - given
+
+
+@pytest.mark.parametrize("past,parents", [
+    ([-1, 21, 21, 21], [-1, 1, 1, 2]),                                           # a row without a length before one that leaves a page
+    ([-1, 5, 5], [-1, 1, 1]),
+    ([5, -1, 5, -1, 5, 5], [4, 4, 4, -1, 4, 4]),
+    ([21, 31, 21, 21], [2, 1, 2, 2]),                                            # rows that nothing goes on from, one with a page just full
+    ([31, 21, 31, 21, 21], [0, 3, 0, 3, 3]),                                     # a row that begins a page among those that copy
+    ([21, 15], [1, 1]),                                                          # a page in use is left, and only rows that begin one
+    ([46, 46, 46], [1, 1, 1]),
+])
+def test_advance_loses_no_page(gpu_ctx, past, parents):
+    b = Beams(gpu_ctx, 1, len(past), 16, 20, layers=1)                           # tables of 3 pages
+    try:
+        o = Owned(b, past, random.Random(1))
+        contents = b.contents()
+        got = b.run(torch.tensor(parents, dtype=torch.int32), torch.arange(len(past), dtype=torch.int32), state=o.state())
+        assert not check_ownership(b, parents, o.state(), got)
+        after = b.contents()
+        for r, p in enumerate(parents):                                          # every row has its parent's tokens
+            p = p if p >= 0 else r
+            for t in range(int(o.past[p]) + 1 if int(o.past[p]) >= 0 else 0):
+                src, dst = int(o.table[p, t // 16]), int(got[1][r, t // 16])
+                assert torch.equal(after[:, :, dst, t % 16], contents[:, :, src, t % 16])
+    finally:
+        b.close()
+
+
+def test_advance_owns_pages_at_any_lengths(gpu_ctx):
+    rng = random.Random(7)
+    b = Beams(gpu_ctx, 1, 8, 16, 20, layers=1)
+    try:
+        for _ in range(150):
+            alike = rng.randrange(1, 46)
+            past = [alike if rng.random() < 0.6 else rng.choice([-1, 14, 15, 16, 30, 31, rng.randrange(0, 46)]) for _ in range(8)]
+            parents = [rng.choice([-1, *range(8), *[rng.randrange(8)] * 8]) for _ in range(8)]
+            o = Owned(b, past, rng)
+            got = b.run(torch.tensor(parents, dtype=torch.int32), torch.arange(8, dtype=torch.int32), state=o.state())
+            assert not check_ownership(b, parents, o.state(), got), (past, parents)
+    finally:
+        b.close()
+
+
 def test_advance_without_caches_tokens_or_histories(gpu_ctx):
     b = Beams(gpu_ctx, 1, 4, 16, 20)
     try:

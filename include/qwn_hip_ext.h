@@ -583,9 +583,10 @@ QWN_CUDA_ABI_API int qwn_hip_ext_beam_select_device(QwnCudaContextHandle *contex
  * rows (a row of a negative length leaves no page).  Where the page in
  * use has just become full, the row takes its spare as the next one, and has
  * none (-1) until the caller hands it another, or gets a page in use that no
- * copy has taken, which only a row of another length leaves.  So a row owns two pages, one in
- * use and one spare, no row's table names another's, and none in use is lost; the caller takes back
- * full pages that no table names any more.  Table entries past the page in use are
+ * copy has taken, which only a row of another length leaves; where its table ends there, the spare
+ * stays what it is.  So a row owns two pages, one in
+ * use and one spare, no row's table names another's, and none in use is lost that a row has
+ * room for; the caller takes back full pages that no table names any more.  Table entries past the page in use are
  * -1.  A row whose parent is none of its sequence (-1) goes on from itself, with no
  * token; one whose parent's length is negative, too (its own negative: nothing of
  * it changes).  Pages that are not the caches' are not copied to or from.  Tables and histories may be in

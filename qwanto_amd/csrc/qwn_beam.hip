@@ -392,7 +392,8 @@ __device__ __forceinline__ int32_t spare_of(const AdvanceArgs &a, const Kin &k, 
     const int64_t length = static_cast<int64_t>(past) + a.added;
     const int32_t page = past >= 0 && (length & slots) && length >> a.page_shift < a.table_stride
                              ? page_of(a, row0 + lane, static_cast<uint32_t>(length >> a.page_shift)) : -1;
-    const bool copies = k.later && (k.g.length & slots), begins = k.goes && !(k.g.length & slots);
+    const bool copies = k.later && (k.g.length & slots),
+               begins = k.goes && !(k.g.length & slots) && k.g.length >> a.page_shift < a.table_stride;  // else the table has no place for a page
     const uint64_t below = (1ull << lane) - 1, all_copy = __ballot(copies), left = __ballot(((k.childless >> lane) & 1) && page >= 0);
     // by place: the lane's row as one that copies, and as one that leaves its page
     const uint32_t giver = nth_of(k.childless, __popcll(k.laters & below)), taker = nth_of(k.laters, __popcll(k.childless & below));

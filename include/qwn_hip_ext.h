@@ -505,7 +505,8 @@ QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *context, co
  * key is below 2^-100, or the query below 2^-100 of its row's largest).  A key or query
  * with an infinity: a score of -inf has probability 0, a row with one that is +inf or
  * NaN, and a row with a scale that is not finite, is NaN.  A value that is not finite
- * makes its channel so in the rows that attend to it, and in no other.  For single
+ * makes its channel so in the rows that attend to it, and in no other; of finite values, up to
+ * the type's largest, the average is finite.  For single
  * tokens behind a cache:
  * qwn_hip_ext_paged_kv_attention_device. */
 typedef struct {

@@ -83,6 +83,19 @@ constexpr int kQueryBits = std::is_same_v<T, f16> ? 15 : -9;
 // What a lane's probabilities of a tile may add up to: of f16 none passes it.
 template <typename T>
 constexpr float kMost = std::is_same_v<T, f16> ? 0x1p15f : 0x1p40f;
+// Probabilities of up to 2^40 times values past 2^88, or a sum of values next to the
+// type's largest, are past fp32 although their average is not.  A block where an average has
+// come out infinite or NaN is gone through again, with probabilities 2^-34 as large and references at each
+// row's largest so far: those of 2^31 tokens add up to less than 1 (f16's products are
+// below 2^32, its averages only rounded past the largest).  Only what was not finite and now is
+// takes the second result, so what one channel holds shows in no other.
+template <typename T>
+constexpr float kSecondLift = std::is_same_v<T, f16> ? 0.0f : -34.0f;
+template <typename T>
+constexpr float kSecondMost = std::is_same_v<T, f16> ? kMost<T> : 0.0f;
+// The type's largest number: an average of finite values is not past it, but may be rounded past it.
+template <typename T>
+constexpr float kLargest = std::is_same_v<T, f16> ? 65504.0f : std::is_same_v<T, bf16> ? 0x1.fep127f : 0x1.fffffep127f;
 
 struct Span {
     uint32_t row = 0, rows = 0;  // of a sequence; none where its starts do not lie in the batch
@@ -98,9 +111,9 @@ __device__ __forceinline__ Span span_of(const PromptArgs &a, uint32_t s) {
 }
 // The sequence that holds block `index` of the batch, and its number there;
 // false past the last.  Every wave searches for itself, 64 sequences a step.
-__device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t block_rows, uint32_t index, Span &q, uint32_t &at) {
+__device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t lane, uint32_t block_rows, uint32_t index, Span &q, uint32_t &at) {
     for (uint32_t s0 = 0; s0 < a.sequences; s0 += kWaveSize) {
-        const Span mine = span_of(a, s0 + threadIdx.x % kWaveSize);
+        const Span mine = span_of(a, s0 + lane);
         const uint32_t n = (mine.rows * a.group + block_rows - 1) / block_rows, end = wave_scan(n);
         const uint64_t past = __ballot(end > index);
         if (past) {
@@ -145,18 +158,20 @@ __device__ __forceinline__ float halves_sum(float v) {
     return b.low + b.high;
 }
 
-// What sums are multiplied by as the reference goes from (m, ref) to (mx, to):
-// exponents were taken from ref itself where it is near, else from m times mul as it is.
-__device__ __forceinline__ float moved(float m, float ref, float mx, float to, float mul) {
-    const bool was = fabsf(ref) < kFar, is = fabsf(to) < kFar;
-    return __builtin_amdgcn_exp2f(was ? (is ? ref - to : fmaf(-mx, mul, ref)) : is ? fmaf(m, mul, -to) : (m - mx) * mul);
-}
-
-// A row's softmax so far: the reference as a product, and times mul; far: some row of
-// the wave has one too far to be rounded.  m is 0 of a row that has seen nothing.
+// A row's softmax so far: the reference as a product, and what exponents are taken from,
+// mul times it less lift; far: some row of the wave has one too far to be rounded.  m is 0 of a
+// row that has seen nothing.  lift: the exponent of the reference's own probability.
 struct Softmax {
-    float m = 0.0f, ref = 0.0f, sum = 0.0f, mul = 0.0f;
+    float m = 0.0f, ref = 0.0f, sum = 0.0f, mul = 0.0f, lift = 0.0f;
     bool far = false;
+    __device__ __forceinline__ float reference(float mx) const { return mul_rounded(mx, mul) - lift; }
+    // What sums are multiplied by as the reference goes from (from, was) to (to, is): exponents
+    // were taken from `was` itself where it is near, else from `from` times mul as it is.
+    __device__ __forceinline__ float moved(float from, float was, float to, float is) const {
+        const bool near = fabsf(was) < kFar, stays = fabsf(is) < kFar;
+        return __builtin_amdgcn_exp2f(near ? (stays ? was - is : fmaf(-to, mul, was) + lift)
+                                           : stays ? fmaf(from, mul, -is) - lift : (from - to) * mul);
+    }
 };
 template <int S>
 __device__ __forceinline__ float largest_of(const v16f (&sc)[S]) {
@@ -173,7 +188,7 @@ __device__ __forceinline__ float weigh(const v16f (&sc)[S], const Softmax &x, fl
     float add = 0.0f;
     if (x.far) {  // of rows with a far reference the product is taken off first
         const bool mine = !(fabsf(x.ref) < kFar);
-        const float off = mine ? x.m : 0.0f, less = mine ? 0.0f : x.ref;
+        const float off = mine ? x.m : 0.0f, less = mine ? -x.lift : x.ref;
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -199,15 +214,15 @@ __device__ __forceinline__ void softmax_tile(const v16f (&sc)[S], Softmax &x, fl
                                              float top) {
     if (first) {
         x.m = sees ? fmaxf(largest_of(sc), kLowest) : 0.0f;
-        x.ref = mul_rounded(x.m, x.mul);
+        x.ref = x.reference(x.m);
         x.far = __any(!(fabsf(x.ref) < kFar));
     }
     float add = weigh(sc, x, p);
     if (__any(!(add < top))) {
         // of the rows that pass it, which does not depend on other rows
         const bool over = halves_max(add < top ? 0.0f : 1.0f) > 0.0f;
-        const float mx = over ? fmaxf(x.m, largest_of(sc)) : x.m, to = mul_rounded(mx, x.mul);
-        const float alpha = moved(x.m, x.ref, mx, to, x.mul);
+        const float mx = over ? fmaxf(x.m, largest_of(sc)) : x.m, to = x.reference(mx);
+        const float alpha = x.moved(x.m, x.ref, mx, to);
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] *= alpha;
         x.sum *= alpha;
@@ -247,7 +262,7 @@ __device__ __forceinline__ bool join_parts(v4u *lds, uint32_t wave, uint32_t lan
             const float4 o = state[(wave + k * RW) * kWaveSize + lane];
             if (o.w > 0.0f) mx = fmaxf(mx, o.x);
         }
-        const float to = mul_rounded(mx, x.mul), mine = moved(x.m, x.ref, mx, to, x.mul);
+        const float to = x.reference(mx), mine = x.moved(x.m, x.ref, mx, to);
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] *= mine;
         x.sum *= mine;
@@ -255,7 +270,7 @@ __device__ __forceinline__ bool join_parts(v4u *lds, uint32_t wave, uint32_t lan
         for (int k = 1; k < KW; ++k) {
             const float4 o = state[(wave + k * RW) * kWaveSize + lane];
             const bool any = o.w > 0.0f;
-            const float f = any ? moved(o.x, o.y, mx, to, x.mul) : 0.0f;
+            const float f = any ? x.moved(o.x, o.y, mx, to) : 0.0f;
             x.sum += any ? o.z * f : 0.0f;
 #pragma unroll
             for (int c = 0; c < C; ++c)
@@ -276,10 +291,10 @@ struct Block {
     uint32_t most, least;        // tokens that any row sees, and every one
 };
 template <uint32_t ROWS>
-__device__ __forceinline__ bool block_of(const PromptArgs &a, Block &b) {
+__device__ __forceinline__ bool block_of(const PromptArgs &a, uint32_t lane, Block &b) {
     uint32_t at;
     b.head = blockIdx.x % a.kv_heads;
-    if (!find_block(a, ROWS, blockIdx.x / a.kv_heads, b.q, at)) return false;
+    if (!find_block(a, lane, ROWS, blockIdx.x / a.kv_heads, b.q, at)) return false;
     const uint32_t all = b.q.rows * a.group, blocks = (all + ROWS - 1) / ROWS;
     b.row0 = (blocks - 1 - at) * ROWS;  // a sequence's longest contexts first
     b.last = min(b.row0 + ROWS, all) - 1;
@@ -344,6 +359,43 @@ __device__ __forceinline__ bool finite(T v) {
     }
 }
 
+// The lane's number, from the hardware: what is made of it before a loop need not be kept over it.
+__device__ __forceinline__ uint32_t lane_anew() {
+    uint32_t lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+    return lane;
+}
+
+// N of a row's sums from channel ch on as averages.  odd: not finite afterwards where one may have come out so.
+template <typename T, int N>
+__device__ __forceinline__ void store_averages(T *dst, uint32_t ch, uint32_t channels, const float (&sums)[N], float inv, float &odd) {
+    constexpr float kPast = 0x1.fffffep127f / kLargest<T> * 1.0001f;  // takes what rounds to an infinity past fp32
+    Vec<T, N> y;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const float v = sums[k] * inv;
+        y.v[k] = from_float<T>(v);
+        odd = fmaf(v, kPast, odd);
+    }
+    if (ch + N <= channels) {
+        store_vec<T, N>(dst + ch, y);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (ch + k < channels) dst[ch + k] = y.v[k];
+    }
+}
+// The second time: to what is not finite there, and now is.
+template <typename T, int N>
+__device__ __forceinline__ void mend_averages(T *dst, uint32_t ch, uint32_t channels, const float (&sums)[N], float inv) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const float v = sums[k] * inv;
+        if (ch + k < channels && fabsf(sums[k]) < INFINITY && !finite(dst[ch + k]))
+            dst[ch + k] = from_float<T>(fabsf(v) > kLargest<T> ? copysignf(kLargest<T>, v) : v);
+    }
+}
+
 // Keys and values of a tile, and how many tiles LDS is given room for.
 template <typename T, int W, int KT>
 constexpr size_t tile_bytes = 2 * KT * W * sizeof(T);
@@ -397,8 +449,8 @@ __device__ __forceinline__ void load_query(const PromptArgs &a, const Block &b, 
 // 32 heads of 128, one prompt of 8192 tokens 521 to 552 us (1 PFLOP/s, of 1.17 that a
 // large product reaches); short ones by the longest block's chain of tiles: nine of up to
 // 1777 tokens 45 us, of which a large product would take 25.
-template <typename T, int W, int KT, int RW, bool DIRECT>
-__global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_kernel(PromptArgs a) {
+template <typename T, int W, int KT, int RW, bool DIRECT, bool again>
+__device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave, uint32_t lane) {
     using M = Matrix<T>;
     using L = Tile<T, W>;
     constexpr uint32_t CE = L::CE, NC = L::NC;
@@ -408,11 +460,11 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
     static_assert(kChunks % kThreads == 0 && S > 0, "whole rounds of loads, a part for each wave");
     extern __shared__ v4u tiles[];          // two times keys, then values
     constexpr uint32_t kMasked = kBlockRows / KT + 2;
+    __shared__ uint32_t again_wanted;
     __shared__ uint32_t odd[kMasked][KT / 32];  // of the masked tiles: tokens with values that are not finite
-    const uint32_t tid = threadIdx.x, lane = tid % kWaveSize, wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
-    const uint32_t n = lane % 32, h = lane / 32, part = wave / RW;  // of a tile's tokens
+    const uint32_t tid = wave * kWaveSize + lane, n = lane % 32, h = lane / 32, part = wave / RW;  // of a tile's tokens
     Block b;
-    if (!block_of<kBlockRows>(a, b)) return;
+    if (!block_of<kBlockRows>(a, lane, b)) return false;
     const uint32_t count = (b.most + KT - 1) / KT, masked = b.least / KT;  // tiles, and the first that not every row sees all of
     const T *keys = static_cast<const T *>(a.key) + static_cast<size_t>(b.q.row) * a.key_stride + b.head * a.head_dim;
     const T *values = static_cast<const T *>(a.value) + static_cast<size_t>(b.q.row) * a.value_stride + b.head * a.head_dim;
@@ -455,11 +507,6 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
             }
         }
     };
-    if (DIRECT && a.head_dim != W) {
-#pragma unroll
-        for (uint32_t e = 0; e < 4 * kOfThread; ++e)
-            if (channel(e % kSame) >= a.head_dim) tiles[tid + kThreads * e] = (v4u){0, 0, 0, 0};
-    }
     // what was brought is in LDS
     auto settle = [&](uint32_t i) {
         if constexpr (DIRECT) {
@@ -490,13 +537,20 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         }
         lds_barrier();
     };
+    if (DIRECT && a.head_dim != W) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4 * kOfThread; ++e)
+            if (channel(e % kSame) >= a.head_dim) tiles[tid + kThreads * e] = (v4u){0, 0, 0, 0};
+    }
     bring(0);
 
     // this lane's row, as a column of the products
     const Row r = row_of(a, b, b.row0 + wave % RW * kWaveRows, n);
     v4u qf[J];
     Softmax soft;
+    if (again) soft.lift = kSecondLift<T>;
     load_query<T>(a, b, r, h, qf, soft.mul);
+    if (tid == 0) again_wanted = 0;
     if (tid < kMasked * (KT / 32)) odd[tid / (KT / 32)][tid % (KT / 32)] = 0;
 
     // where a lane's operands lie in a buffer: of keys piece 2 j + h of token n, of V^T
@@ -555,7 +609,7 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
                     if (32 * s + 8 * (e / 4) + e % 4 >= seen) sc[s][e] = -INFINITY;
         }
         float p[S][16];
-        softmax_tile(sc, soft, p, acc, i == 0, r.visible > t0, kMost<T>);
+        softmax_tile(sc, soft, p, acc, i == 0, r.visible > t0, again ? kSecondMost<T> : kMost<T>);
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -606,25 +660,71 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
         }
     }
 
-    if (!join_parts<C, RW, kWaves>(tiles, wave, lane, r.visible > part * S * 32, soft, acc) || r.visible == 0) return;
-    const float inv = 1.0f / soft.sum;
-    T *dst = static_cast<T *>(a.output) + static_cast<size_t>(b.q.row + r.token) * a.output_stride + r.at;
+    float odd_sums = 0.0f;
+    if (join_parts<C, RW, kWaves>(tiles, wave, lane, r.visible > part * S * 32, soft, acc) && r.visible > 0) {
+        const float inv = 1.0f / soft.sum;
+        T *dst = static_cast<T *>(a.output) + static_cast<size_t>(b.q.row + r.token) * a.output_stride + r.at;
+        auto each = [&](auto take) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const uint32_t ch = 32 * c + 8 * (e / 4) + 4 * h;
-            Vec<T, 4> y;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y.v[k] = from_float<T>(acc[c][e + k] * inv);
-            if (ch + 4 <= a.head_dim) {
-                store_vec<T, 4>(dst + ch, y);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (ch + k < a.head_dim) dst[ch + k] = y.v[k];
-            }
+                for (int e = 0; e < 16; e += 4) {
+                    const float sums[4] = {acc[c][e], acc[c][e + 1], acc[c][e + 2], acc[c][e + 3]};
+                    take(32 * c + 8 * (e / 4) + 4 * h, sums);
+                }
+        };
+        if (!again) {
+            each([&](uint32_t ch, const float (&sums)[4]) {
+                store_averages<T, 4>(dst, ch, a.head_dim, sums, inv, odd_sums);
+            });
+        } else {
+            each([&](uint32_t ch, const float (&sums)[4]) { mend_averages<T, 4>(dst, ch, a.head_dim, sums, inv); });
         }
+    }
+    if (again) return false;
+    if (!(fabsf(odd_sums) < INFINITY)) again_wanted = 1;
+    lds_barrier();
+    return __builtin_amdgcn_readfirstlane(again_wanted);
+}
+
+// What a workgroup does, and again where the first pass asks for it (it returns whether).  The second is code of its
+// own, with arguments and lanes taken anew: as a loop over one code both passes
+// spilled registers (the first now has none more than alone; 16 tokens 8.3 us for 8.1, 8192 the same).
+__device__ __forceinline__ PromptArgs arguments_at(uint64_t args) {
+    auto word = [&](size_t at) { return *reinterpret_cast<const __attribute__((address_space(4))) uint32_t *>(args + at); };
+    auto pointer = [&](size_t at) {
+        const uint64_t p = *reinterpret_cast<const __attribute__((address_space(4))) uint64_t *>(args + at);
+        return (void *)reinterpret_cast<__attribute__((address_space(1))) void *>(p);
+    };
+    PromptArgs a;
+    a.query = pointer(offsetof(PromptArgs, query));
+    a.key = pointer(offsetof(PromptArgs, key));
+    a.value = pointer(offsetof(PromptArgs, value));
+    a.output = pointer(offsetof(PromptArgs, output));
+    a.starts = static_cast<const int32_t *>(pointer(offsetof(PromptArgs, starts)));
+    a.sequences = word(offsetof(PromptArgs, sequences));
+    a.tokens = word(offsetof(PromptArgs, tokens));
+    a.kv_heads = word(offsetof(PromptArgs, kv_heads));
+    a.group = word(offsetof(PromptArgs, group));
+    a.head_dim = word(offsetof(PromptArgs, head_dim));
+    a.query_stride = word(offsetof(PromptArgs, query_stride));
+    a.key_stride = word(offsetof(PromptArgs, key_stride));
+    a.value_stride = word(offsetof(PromptArgs, value_stride));
+    a.output_stride = word(offsetof(PromptArgs, output_stride));
+    a.scale = __builtin_bit_cast(float, word(offsetof(PromptArgs, scale)));
+    return a;
+}
+template <auto FIRST, auto SECOND>
+__device__ __forceinline__ void once_or_twice(const PromptArgs &a) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    if (!FIRST(a, wave, threadIdx.x % kWaveSize)) return;
+    uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    SECOND(arguments_at(args), wave, lane_anew());
+}
+template <typename T, int W, int KT, int RW, bool DIRECT>
+__global__ __launch_bounds__(kThreads, W == 256 ? 1 : W == 64 && KT == 64 ? 3 : 2) void prompt_attention_kernel(PromptArgs a) {
+    once_or_twice<&attend_block<T, W, KT, RW, DIRECT, false>, &attend_block<T, W, KT, RW, DIRECT, true>>(a);
 }
 
 // fp32.  A product of two fp32 operands (v_mfma_f32_32x32x2_f32) takes 64 cycles for
@@ -641,41 +741,50 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : 2) void prompt_attention_k
 // rows are channels c, c + W / 32, ...  WHOLE: heads of W channels.
 // Bound by the matrix unit: those 1176 us are 117 TFLOP/s, of 154 that a large product
 // reaches; few rows by the longest one's chain of tiles.
-template <int W, bool WHOLE>
-__global__ __launch_bounds__(kThreads, W <= 128 ? 2 : 1) void prompt_attention_f32_kernel(PromptArgs a) {
+template <int W, bool WHOLE, bool again>
+__device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, uint32_t wave, uint32_t lane) {
     constexpr uint32_t KT = 32, KW = kWaves;
     constexpr int C = W / 32, J = W / 8;
     extern __shared__ v4u lds[];
-    const uint32_t tid = threadIdx.x, lane = tid % kWaveSize, wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
-    const uint32_t n = lane % 32, h = lane / 32, part = wave;
+    __shared__ uint32_t again_wanted;
+    const uint32_t tid = wave * kWaveSize + lane, n = lane % 32, h = lane / 32, part = wave;
     Block b;
-    if (!block_of<kWaveRows>(a, b)) return;
+    if (!block_of<kWaveRows>(a, lane, b)) return false;
     const Row r = row_of(a, b, b.row0, n);
     const uint32_t count = (r.w_most + KT - 1) / KT;
     const float *keys = static_cast<const float *>(a.key) + static_cast<size_t>(b.q.row) * a.key_stride + b.head * a.head_dim;
     const float *values = static_cast<const float *>(a.value) + static_cast<size_t>(b.q.row) * a.value_stride + b.head * a.head_dim;
-    auto piece = [&](const float *row, uint32_t c) {
+    auto piece = [&](const float *row, uint32_t c, uint32_t d) {
         if constexpr (WHOLE) {
             return load_vec<float, 4>(row + c);
         } else {
-            return __builtin_bit_cast(Vec<float, 4>, load_chunk(row, c, a.head_dim));
+            return __builtin_bit_cast(Vec<float, 4>, load_chunk(row, c, d));
         }
+    };
+    // compared for each tile: masks kept over the loop would not have the registers (96 channels, four
+    // prompts of 1024, 500, 300 and 100 tokens 94 us for 99; of 256, where they are twice as many, 190 for 165)
+    auto channels = [&]() {
+        uint32_t d = a.head_dim;
+        if constexpr (!WHOLE && W <= 128) asm volatile("" : "+s"(d));
+        return d;
     };
     Vec<float, 4> kf[J];
     Vec<float, C> vf[16];
     auto load_keys = [&](uint32_t i) {
+        const uint32_t d = channels();
         const float *row = keys + static_cast<size_t>(min(i * KT + n, b.most - 1)) * a.key_stride;
 #pragma unroll
-        for (int j = 0; j < J; ++j) kf[j] = piece(row, (2 * j + h) * 4);
+        for (int j = 0; j < J; ++j) kf[j] = piece(row, (2 * j + h) * 4, d);
     };
     auto load_values = [&](uint32_t i) {
+        const uint32_t d = channels();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const float *row = values + static_cast<size_t>(min(i * KT + 8 * (e / 4) + 4 * h + e % 4, b.most - 1)) * a.value_stride;
             if constexpr (C >= 4) {
 #pragma unroll
                 for (int x = 0; x < C / 4; ++x) {
-                    const Vec<float, 4> v = piece(row, C * n + 4 * x);
+                    const Vec<float, 4> v = piece(row, C * n + 4 * x, d);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) vf[e].v[4 * x + k] = v.v[k];
                 }
@@ -683,14 +792,16 @@ __global__ __launch_bounds__(kThreads, W <= 128 ? 2 : 1) void prompt_attention_f
                 vf[e] = load_vec<float, C>(row + C * n);
             } else {
 #pragma unroll
-                for (int k = 0; k < C; ++k) vf[e].v[k] = C * n + k < a.head_dim ? row[C * n + k] : 0.0f;
+                for (int k = 0; k < C; ++k) vf[e].v[k] = C * n + k < d ? row[C * n + k] : 0.0f;
             }
         }
     };
     v4u qf[J];
     Softmax soft;
+    if (again) soft.lift = kSecondLift<float>;
     load_query<float>(a, b, r, h, qf, soft.mul);
     v4u *const query = lds + lane;
+    if (tid == 0) again_wanted = 0;
     if (wave == 0) {
 #pragma unroll
         for (int j = 0; j < J; ++j) query[j * kWaveSize] = qf[j];
@@ -738,7 +849,7 @@ __global__ __launch_bounds__(kThreads, W <= 128 ? 2 : 1) void prompt_attention_f
             }
         }
         float p[1][16];
-        softmax_tile(sc, soft, p, acc, i == part, r.visible > t0, kMost<float>);
+        softmax_tile(sc, soft, p, acc, i == part, r.visible > t0, again ? kSecondMost<float> : kMost<float>);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
 #pragma unroll
@@ -760,23 +871,38 @@ __global__ __launch_bounds__(kThreads, W <= 128 ? 2 : 1) void prompt_attention_f
         }
     }
 
-    if (!join_parts<C, 1, kWaves>(lds, wave, lane, r.visible > part * KT, soft, acc) || r.visible == 0) return;
-    const float inv = 1.0f / soft.sum;
-    float *dst = static_cast<float *>(a.output) + static_cast<size_t>(b.q.row + r.token) * a.output_stride + r.at;
+    float odd_sums = 0.0f;
+    const uint32_t late = lane_anew();
+    const Row row = row_of(a, b, b.row0, late % 32);
+    if (join_parts<C, 1, kWaves>(lds, wave, late, row.visible > part * KT, soft, acc) && row.visible > 0) {
+        const float inv = 1.0f / soft.sum;
+        float *dst = static_cast<float *>(a.output) + static_cast<size_t>(b.q.row + row.token) * a.output_stride + row.at;
+        auto each = [&](auto take) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const uint32_t ch = C * (8 * (e / 4) + 4 * h + e % 4);
-        Vec<float, C> y;
+            for (int e = 0; e < 16; ++e) {
+                float sums[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) y.v[c] = acc[c][e] * inv;
-        if (ch + C <= a.head_dim) {
-            store_vec<float, C>(dst + ch, y);
+                for (int c = 0; c < C; ++c) sums[c] = acc[c][e];
+                take(C * (8 * (e / 4) + 4 * (late / 32) + e % 4), sums);
+            }
+        };
+        if (!again) {
+            each([&](uint32_t ch, const float (&sums)[C]) {
+                store_averages<float, C>(dst, ch, a.head_dim, sums, inv, odd_sums);
+            });
         } else {
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (ch + c < a.head_dim) dst[ch + c] = y.v[c];
+            each([&](uint32_t ch, const float (&sums)[C]) { mend_averages<float, C>(dst, ch, a.head_dim, sums, inv); });
         }
     }
+    if (again) return false;
+    if (!(fabsf(odd_sums) < INFINITY)) again_wanted = 1;
+    lds_barrier();
+    return __builtin_amdgcn_readfirstlane(again_wanted);
+}
+
+template <int W, bool WHOLE>
+__global__ __launch_bounds__(kThreads, W <= 128 ? 2 : 1) void prompt_attention_f32_kernel(PromptArgs a) {
+    once_or_twice<&attend_block_f32<W, WHOLE, false>, &attend_block_f32<W, WHOLE, true>>(a);
 }
 
 // Blocks of a batch at most: one of each sequence is not full.

@@ -265,6 +265,64 @@ def test_queries_and_scales_that_are_not_finite(gpu_ctx, dtype):
         assert bool(torch.isnan(attend(gpu_ctx, q, k, v, [40], 2, 1, 64, bad, dtype)).all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,heads,kv_heads,lengths", [(64, 2, 1, [300, 40]), (64, 2, 1, [600]), (128, 2, 2, [300]), (256, 1, 1, [200, 70]),
+                                                      (96, 2, 1, [150]), (33, 1, 1, [140]), (64, 80, 80, [200, 190]), (128, 80, 80, [150, 140]),
+                                                      (256, 80, 80, [150, 140])])
+def test_large_values(gpu_ctx, dtype, d, heads, kv_heads, lengths):
+    """Finite values up to the type's largest, scores that rise along the sequence or not: outputs are averages of values,
+    so they are finite, and those of other channels are what they were to the bit."""
+    n, top = sum(lengths), torch.finfo(sv.DTYPES[dtype]).max
+    q, k, v = inputs(d + heads, n, heads, kv_heads, d, dtype)
+    t = torch.cat([torch.arange(m) for m in lengths])
+    for rise in (0.0, 0.3, 3.0):
+        q2, k2 = q.clone(), k.clone()
+        if rise:                                                                  # scores of about rise * token, of any query
+            q2.reshape(n, heads, d)[:, :, 0] = 4.0
+            k2.reshape(n, kv_heads, d)[:, :, 0] = (rise / 0.4 * t)[:, None].to(k.dtype)
+        clean = attend(gpu_ctx, q2, k2, v, lengths, heads, kv_heads, d, 0.1, dtype).cpu().reshape(n, heads, d)
+        check(clean.reshape(n, -1), q2, k2, v, lengths, heads, kv_heads, d, 0.1, dtype)
+        for size in (top, 0.99 * top, 2.0 ** 100 if dtype != "f16" else 2.0 ** 14):
+            b = v.clone()
+            x = b.reshape(n, kv_heads, d)
+            x[:, :, 3] = size                                                     # all alike: the row's, too
+            x[:, :, 7] = (size * (2 * torch.rand(n, kv_heads, generator=sv.gen(1)) - 1)).to(v.dtype)
+            x[-1, :, 9] = -size
+            got = attend(gpu_ctx, q2, k2, b, lengths, heads, kv_heads, d, 0.1, dtype).cpu()
+            assert bool(torch.isfinite(got).all())
+            got = got.reshape(n, heads, d)
+            others = [c for c in range(d) if c not in (3, 7, 9)]
+            assert torch.equal(got[:, :, others], clean[:, :, others])
+            assert torch.equal(got[:-1, :, 9], clean[:-1, :, 9])
+            big = torch.zeros_like(b).reshape(n, kv_heads, d)
+            big[:, :, [3, 7, 9]] = x[:, :, [3, 7, 9]]
+            alone = torch.zeros_like(got)
+            alone[:, :, [3, 7, 9]] = got[:, :, [3, 7, 9]]
+            # the large channels by themselves: their sizes, not the others', are what they may be off by
+            for ch in (3, 7, 9):
+                one, mine = torch.zeros_like(big), torch.zeros_like(alone)
+                one[:, :, ch], mine[:, :, ch] = big[:, :, ch], alone[:, :, ch]
+                check(mine.reshape(n, -1), q2, k2, one.reshape(n, -1), lengths, heads, kv_heads, d, 0.1, dtype)
+
+
+def test_large_values_beside_what_is_not_finite(gpu_ctx):
+    """A row with an infinite value in one channel and large finite ones in another, in tiles that are masked and
+    that are not."""
+    n, d = 260, 64
+    for dtype in ("f32", "bf16"):
+        top = torch.finfo(sv.DTYPES[dtype]).max
+        q, k, v = inputs(8, n, 1, 1, d, dtype)
+        q[:, 0], k[:, 0] = 4.0, torch.arange(n).to(q.dtype)
+        v[:, 5] = top
+        v[100, 9], v[230, 11] = math.inf, math.nan
+        got = attend(gpu_ctx, q, k, v, [n], 1, 1, d, 0.1, dtype).cpu().double()
+        assert bool(((got[:, 5] - top).abs() <= ((2 * sv.HALF[dtype] if dtype == "bf16" else 0) + 2.0 ** -20) * top).all())
+        assert bool(torch.isfinite(got[:100]).all()) and bool(torch.isfinite(got[:230, 11]).all())
+        assert bool((got[100:, 9] == math.inf).all()) and bool(torch.isnan(got[230:, 11]).all())
+        rest = [c for c in range(d) if c not in (9, 11)]
+        assert bool(torch.isfinite(got[:, rest]).all())
+
+
 def test_starts_that_are_none(gpu_ctx):
     """Sequences whose rows do not lie in the batch are left out, the others are not."""
     q, k, v = inputs(4, 100, 2, 1, 64, "bf16")

@@ -369,13 +369,12 @@ __device__ __forceinline__ uint32_t lane_anew() {
 // N of a row's sums from channel ch on as averages.  odd: not finite afterwards where one may have come out so.
 template <typename T, int N>
 __device__ __forceinline__ void store_averages(T *dst, uint32_t ch, uint32_t channels, const float (&sums)[N], float inv, float &odd) {
-    constexpr float kPast = 0x1.fffffep127f / kLargest<T> * 1.0001f;  // takes what rounds to an infinity past fp32
+    const float past = inv * (0x1.fffffep127f / kLargest<T> * 1.0001f);  // takes what rounds to an infinity past fp32
     Vec<T, N> y;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const float v = sums[k] * inv;
-        y.v[k] = from_float<T>(v);
-        odd = fmaf(v, kPast, odd);
+        y.v[k] = from_float<T>(sums[k] * inv);  // f16: one instruction, one rounding
+        odd = fmaf(sums[k], past, odd);
     }
     if (ch + N <= channels) {
         store_vec<T, N>(dst + ch, y);

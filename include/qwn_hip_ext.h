@@ -499,8 +499,8 @@ QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *context, co
  * query head h to KV head h / (query_heads / kv_heads).  Rows behind
  * starts[sequences] belong to no sequence: they are not read, and the output
  * keeps what it held there; a sequence whose rows do not lie in 0 .. tokens is
- * left out.  Scores and sums are fp32, probabilities are rounded to dtype; fp32 is
- * fp32 throughout.  Finite queries, keys and scale have their softmax whatever the
+ * left out.  Scores and sums are fp32, probabilities are rounded to dtype (f16: below 2^-20 of
+ * the row's largest to steps of 2^-30 of that); fp32 is fp32 throughout.  Finite queries, keys and scale have their softmax whatever the
  * scores' size, past fp32's too (of fp32 and bf16, a channel counts as zero where the
  * key is below 2^-100, or the query below 2^-100 of its row's largest).  A key or query
  * with an infinity: a score of -inf has probability 0, a row with one that is +inf or

@@ -13,7 +13,8 @@
 //
 // Scores and sums are fp32; probabilities are rounded to the inputs' type for the
 // second product (by at most 2^-8 of each in bf16, 2^-11 in f16, as the output itself is; over
-// the tokens it averages out), and fp32 goes in fp32 throughout.
+// the tokens it averages out; in f16 those below 2^-20 of the row's largest by up to 2^-31 of that),
+// and fp32 goes in fp32 throughout.
 #include "qwn_context.h"
 #include "qwn_device.h"
 #include "qwn_hip_ext.h"
@@ -80,9 +81,15 @@ struct Matrix<bf16> {
 // the others, with any finite key, below 2^127.
 template <typename T>
 constexpr int kQueryBits = std::is_same_v<T, f16> ? 15 : -9;
+// The exponent of the reference's own probability.  Of f16 numbers below 2^-14 lose bits: with 2^6, a
+// probability is off by 2^-11 of itself, or by 2^-31 of the row's largest, so that 2^20 tokens with next
+// to none of the weight still add up to it within f16's own rounding.  (A larger one leaves less room until the
+// reference moves: scores spread by 4, 1500 tokens of 128 channels 30 us, with 2^8 32, with 1 27.)
+template <typename T>
+constexpr float kLift = std::is_same_v<T, f16> ? 6.0f : 0.0f;
 // What a lane's probabilities of a tile may add up to: of f16 none passes it.
 template <typename T>
-constexpr float kMost = std::is_same_v<T, f16> ? 0x1p15f : 0x1p40f;
+constexpr float kMost = std::is_same_v<T, f16> ? 65504.0f : 0x1p40f;
 // Probabilities of up to 2^40 times values past 2^88, or a sum of values next to the
 // type's largest, are past fp32 although their average is not.  A block where an average has
 // come out infinite or NaN is gone through again, with probabilities 2^-34 as large and references at each
@@ -90,7 +97,7 @@ constexpr float kMost = std::is_same_v<T, f16> ? 0x1p15f : 0x1p40f;
 // below 2^32, its averages only rounded past the largest).  Only what was not finite and now is
 // takes the second result, so what one channel holds shows in no other.
 template <typename T>
-constexpr float kSecondLift = std::is_same_v<T, f16> ? 0.0f : -34.0f;
+constexpr float kSecondLift = std::is_same_v<T, f16> ? kLift<T> : -34.0f;
 template <typename T>
 constexpr float kSecondMost = std::is_same_v<T, f16> ? kMost<T> : 0.0f;
 // The type's largest number: an average of finite values is not past it, but may be rounded past it.
@@ -547,7 +554,7 @@ __device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave,
     const Row r = row_of(a, b, b.row0 + wave % RW * kWaveRows, n);
     v4u qf[J];
     Softmax soft;
-    if (again) soft.lift = kSecondLift<T>;
+    soft.lift = again ? kSecondLift<T> : kLift<T>;
     load_query<T>(a, b, r, h, qf, soft.mul);
     if (tid == 0) again_wanted = 0;
     if (tid < kMasked * (KT / 32)) odd[tid / (KT / 32)][tid % (KT / 32)] = 0;
@@ -797,7 +804,7 @@ __device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, uint32_t w
     };
     v4u qf[J];
     Softmax soft;
-    if (again) soft.lift = kSecondLift<float>;
+    soft.lift = again ? kSecondLift<float> : kLift<float>;
     load_query<float>(a, b, r, h, qf, soft.mul);
     v4u *const query = lds + lane;
     if (tid == 0) again_wanted = 0;

@@ -323,6 +323,31 @@ def test_large_values_beside_what_is_not_finite(gpu_ctx):
         assert bool(torch.isfinite(got[:, rest]).all())
 
 
+@pytest.mark.parametrize("d,heads,n,late", [(64, 1, 1500, 0), (64, 48, 1100, 3), (128, 1, 1500, 70), (256, 1, 700, 0), (128, 40, 1100, 0)])
+@pytest.mark.parametrize("below", [18.0, 20.5, 23.3, 25.0, 27.7])
+def test_small_probabilities_add_up(gpu_ctx, below, d, heads, n, late):
+    """One token has nearly all of the weight and a value of nothing, the others 2^-18 of it and less each: what they add
+    up to is there in f16, too.  A probability that is rounded to f16 2^6 times as large as it is to the row's largest is
+    off by 2^-11 of itself, or by 2^-31 of the largest where it is below f16's normal numbers; beside that the fp32 chains
+    and roundings of rows_of, in whole: 2^-16 of a probability."""
+    g = sv.gen(int(10 * below) + d)
+    q, k = torch.zeros(n, heads, d), torch.zeros(n, 1, d)
+    q[:, :, 0], q[:, :, 1] = 1.0, 1.0
+    k[:, 0, 0] = -below * math.log(2.0)                                          # scale 1: rounded to f16, and taken as it is
+    k[:, 0, 1] = 0.1 * sv.normal(g, n)
+    k[late, 0, :2] = 0.0
+    v = 0.5 + torch.rand(n, 1, d, generator=g)
+    v[late] = 0.0
+    q, k, v = (x.half().reshape(n, -1) for x in (q, k, v))
+    got = attend(gpu_ctx, q, k, v, [n], heads, 1, d, 1.0, "f16").cpu().double().reshape(n, heads, d)
+    s = (q.double()[:, :d] @ k.double().t()).masked_fill(torch.ones(n, n).triu(1) > 0, -math.inf)
+    p = torch.softmax(s, dim=1)
+    want = (p @ v.double())[:, None]
+    size = v.double().abs()
+    off = (2.0 ** -11 + 2.0 ** -16) * (p @ size) + 2.0 ** -31 * (p.amax(1, keepdim=True) * torch.tril(torch.ones(n, n)).double()) @ size
+    assert bool(((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + off[:, None]).all())
+
+
 def test_starts_that_are_none(gpu_ctx):
     """Sequences whose rows do not lie in the batch are left out, the others are not."""
     q, k, v = inputs(4, 100, 2, 1, 64, "bf16")

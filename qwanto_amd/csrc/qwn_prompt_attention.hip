@@ -77,10 +77,10 @@ struct Matrix<bf16> {
     typedef __bf16 pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ v16f mul(frag a, frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
-// Queries are scaled to below 2^kQueryBits: of f16 products are then below 2^40, of
-// the others, with any finite key, below 2^127.
+// Queries are scaled to below 2^kQueryBits: of f16 products are then below 2^40, and no query is
+// scaled down, which its smallest channels have no bits for; of the others, with any finite key, below 2^127.
 template <typename T>
-constexpr int kQueryBits = std::is_same_v<T, f16> ? 15 : -9;
+constexpr int kQueryBits = std::is_same_v<T, f16> ? 16 : -9;
 // The exponent of the reference's own probability.  Of f16 numbers below 2^-14 lose bits: with 2^6, a
 // probability is off by 2^-11 of itself, or by 2^-31 of the row's largest, so that 2^20 tokens with next
 // to none of the weight still add up to it within f16's own rounding.  (A larger one leaves less room until the
@@ -425,8 +425,8 @@ __device__ __forceinline__ void load_query(const PromptArgs &a, const Block &b, 
 #pragma unroll
         for (uint32_t e = 0; e < CE; ++e) top = fmaxf(top, fabsf(to_float(raw[j].v[e])));
     top = halves_max(top);
-    int e2 = 0;  // top < 2^e2
-    if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e2);
+    int e2 = kQueryBits<T>;  // top < 2^e2, and as it is where that is not finite (its row is NaN)
+    if (top < INFINITY) (void)frexpf(top, &e2);
     e2 = max(e2, -100);
     float up = ldexpf(1.0f, kQueryBits<T> - e2);
     mul = exponents_of(a.scale, e2 - kQueryBits<T>, up);

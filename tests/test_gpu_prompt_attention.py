@@ -348,6 +348,20 @@ def test_small_probabilities_add_up(gpu_ctx, below, d, heads, n, late):
     assert bool(((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + off[:, None]).all())
 
 
+def test_query_channels_far_apart(gpu_ctx):
+    """f16 queries with a channel of the type's largest and others of its smallest numbers, which decide."""
+    d, n = 64, 50
+    g = sv.gen(11)
+    q, k = torch.zeros(n, d), torch.zeros(n, d)
+    q[:, 0] = 65504.0
+    q[:, 1:9] = 2.0 ** -24 * torch.randint(1, 8, (n, 8), generator=g)
+    k[:, 1:9] = 60000 * (2 * torch.rand(n, 8, generator=g) - 1)
+    q, k, v = q.half(), k.half(), sv.normal(g, n, d).half()
+    for scale in (1.0, 100.0, -30.0):
+        got = attend(gpu_ctx, q, k, v, [n], 1, 1, d, scale, "f16")
+        check(got, q, k, v, [n], 1, 1, d, scale, "f16")
+
+
 def test_starts_that_are_none(gpu_ctx):
     """Sequences whose rows do not lie in the batch are left out, the others are not."""
     q, k, v = inputs(4, 100, 2, 1, 64, "bf16")

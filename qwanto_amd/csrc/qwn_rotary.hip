@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -111,6 +112,10 @@ struct Work<float> {
     typedef double real;
     typedef double2 pair;
 };
+// A mean square of bf16 may be past fp32, or lie where its squares lose bits: such heads are
+// normed in 64 bits.  f16's squares cannot be.
+template <typename T>
+constexpr bool kWide = std::is_same_v<T, bf16>;
 __device__ __forceinline__ float root(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double root(double v) { return rsqrt(v); }
 
@@ -162,34 +167,48 @@ __global__ __launch_bounds__(kThreadsMost, sizeof(T) == 4 ? 3 : 4) void rotary_k
     }
     lds_barrier();
     if (!real) return;  // all the lanes of a head
+    uint32_t wide = 0;  // tokens
+    auto finish = [&](auto in_64) {
 #pragma unroll
-    for (int t = 0; t < TOKENS; ++t) {
-        if (token0 + t >= a.tokens) return;
-        __builtin_amdgcn_sched_barrier(0);
-        R p[8], q[8];
+        for (int t = 0; t < TOKENS; ++t) {
+            if (token0 + t >= a.tokens) break;
+            if (decltype(in_64)::value && !(wide >> t & 1)) continue;
+            __builtin_amdgcn_sched_barrier(0);
+            R p[8], q[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = to_float(u[t].v[e]), q[e] = to_float(v[t].v[e]);
-        if (norm) {
-            R sum = 0;
+            for (int e = 0; e < 8; ++e) p[e] = to_float(u[t].v[e]), q[e] = to_float(v[t].v[e]);
+            if constexpr (decltype(in_64)::value) {
+                double sum = 0.0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum += p[e] * p[e] + q[e] * q[e];
-            const R inv = root(lanes_sum(sum, a.lanes) * static_cast<R>(a.inv_dim) + static_cast<R>(a.eps));
+                for (int e = 0; e < 8; ++e) sum += static_cast<double>(p[e]) * p[e] + static_cast<double>(q[e]) * q[e];
+                const double inv = root(lanes_sum(sum, a.lanes) * a.inv_dim + a.eps);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] *= inv * wu.v[e], q[e] *= inv * wv.v[e];
-        }
-        if (pair) {
+                for (int e = 0; e < 8; ++e) p[e] = static_cast<R>(p[e] * inv * wu.v[e]), q[e] = static_cast<R>(q[e] * inv * wv.v[e]);
+            } else if (norm) {
+                R sum = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const auto r = cs[t][e * 16 + lane];  // past the last pair: anything, not stored
-                const R first = p[e] * r.x - q[e] * r.y;
-                q[e] = p[e] * r.y + q[e] * r.x;
-                p[e] = first;
+                for (int e = 0; e < 8; ++e) sum += p[e] * p[e] + q[e] * q[e];
+                const R mean = lanes_sum(sum, a.lanes) * static_cast<R>(a.inv_dim) + static_cast<R>(a.eps), inv = root(mean);
+                wide |= mean > 0x1p-80f && mean < INFINITY ? 0u : 1u << t;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] *= inv * wu.v[e], q[e] *= inv * wv.v[e];
             }
+            if (pair) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const auto r = cs[t][e * 16 + lane];  // past the last pair: anything, not stored
+                    const R first = p[e] * r.x - q[e] * r.y;
+                    q[e] = p[e] * r.y + q[e] * r.x;
+                    p[e] = first;
+                }
+            }
+            T *row = out + (token0 + t) * out_stride;
+            store_part<T, 8, R>(row, c, end, p);
+            store_part<T, 8, R>(row + next, c, end2, q);
         }
-        T *row = out + (token0 + t) * out_stride;
-        store_part<T, 8, R>(row, c, end, p);
-        store_part<T, 8, R>(row + next, c, end2, q);
-    }
+    };
+    finish(std::false_type{});
+    if (kWide<T> && wide) finish(std::true_type{});  // again, from what was loaded (decided before: 3 to 10 % more for all)
 }
 
 // Tokens of a workgroup: more where the grid fills the GPU all the same.

@@ -150,6 +150,47 @@ def test_values_that_are_not_finite_stay_in_their_head(gpu_ctx):
         check(got[fine], want[fine], size[fine], "f32")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,rope", [(128, 128), (256, 64), (80, 80), (1, 0)])
+def test_norms_of_any_size(gpu_ctx, dtype, d, rope):
+    """Heads whose squares' sum is past fp32's range, or below it, beside ordinary ones and zeros: of each its norm."""
+    g = sv.gen(d)
+    info = torch.finfo(sv.DTYPES[dtype])
+    sizes = [1.0, 0.9 * info.max, info.max ** 0.5, 1e-3 * info.max, info.tiny ** 0.5, 3 * info.tiny, info.tiny / 16, 0.0]
+    heads, tokens = len(sizes), 5
+    x = 2 * torch.rand(tokens, heads, d, generator=g) - 1
+    x = (x * torch.tensor(sizes)[:, None]).to(sv.DTYPES[dtype]).reshape(tokens, heads * d)
+    p, w = positions_of(g, 1, tokens), 1 + 0.2 * sv.normal(g, d)
+    xd, pd, wd = x.to(sv.DEV), p.to(sv.DEV), w.to(sv.DEV)
+    out = torch.zeros_like(xd)
+    for eps in (0.0, 1e-30, 1e-6):
+        gpu_ctx.rotary_device(gpu_ctx.rotary_request(tokens, dtype, d, rope, THETA, sv.ptr(pd), query_heads=heads, q_ptr=sv.ptr(xd),
+                                                     q_out_ptr=sv.ptr(out), q_norm_ptr=sv.ptr(wd), eps=eps), stream=sv.stream())
+        eps = float(torch.tensor(eps, dtype=torch.float32))
+        want, size = reference(x, heads, d, rope, p, [rope // 2], False, w, eps=eps)
+        got = out.cpu()
+        zeros = x.reshape(tokens, heads, d).double().square().sum(-1).eq(0).repeat_interleave(d, 1)
+        if eps == 0.0:
+            assert bool(torch.isnan(got[zeros]).all())                           # 0 / 0
+        else:
+            assert bool((got[zeros] == 0).all())
+        check(got[~zeros], want[~zeros], size[~zeros], dtype)
+    # many tokens, the odd ones ordinary: theirs is what it is beside ordinary ones, to the bit; in place
+    many = x.repeat(820, 1)
+    many[1::2] = (2 * torch.rand(2050, heads * d, generator=g) - 1).to(many.dtype)
+    calm = many.clone()
+    calm[0::2] = calm[1::2]
+    p = positions_of(g, 1, 4100).to(sv.DEV)
+    out = [t.to(sv.DEV) for t in (many, calm)]
+    for o in out:
+        gpu_ctx.rotary_device(gpu_ctx.rotary_request(4100, dtype, d, rope, THETA, sv.ptr(p), query_heads=heads, q_ptr=sv.ptr(o),
+                                                     q_out_ptr=sv.ptr(o), q_norm_ptr=sv.ptr(wd), eps=1e-30), stream=sv.stream())
+    torch.cuda.synchronize()
+    assert torch.equal(out[0][1::2], out[1][1::2])
+    want, size = reference(many, heads, d, rope, p.cpu(), [rope // 2], False, w, eps=float(torch.tensor(1e-30)))
+    check(out[0].cpu(), want, size, dtype)
+
+
 def test_refusals(gpu_ctx):
     t, d = 4, 64
     q, k = torch.zeros(t, 2 * d, device=sv.DEV), torch.zeros(t, d, device=sv.DEV)

@@ -542,7 +542,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_prompt_attention_device(QwnCudaContextHandle *c
  * same way.  No candidates come from a beam whose score is not finite, from
  * logits that are -inf or NaN (they do not count in the sum), or from a row with a
  * logit of +inf.  A row's sum is one of fp32 powers; values are added up in 64 bits,
- * ordered there, and rounded to fp32.
+ * ordered there (a beam's that are one number there, by their logits), and rounded to fp32.
  * The workspace (qwn_hip_ext_beam_select_workspace_bytes, 0 for sizes that are
  * refused; 16-byte aligned) holds nothing between calls, and may not be shared by
  * calls that run at the same time. */

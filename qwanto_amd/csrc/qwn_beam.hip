@@ -24,9 +24,10 @@ constexpr int kLoads = 4;               // vectors of 16 bytes that a thread tak
 template <typename T>
 constexpr uint32_t kSlice = kThreads * kLoads * (16 / sizeof(T));  // tokens of the vocabulary a workgroup takes
 
-// Candidates in order: a larger value, then the smaller place, is the larger key;
-// the value 0 is none.  Of a row, values are fp32 logits and places tokens; of a
-// sequence, 64-bit sums, and beams and tokens.
+// Candidates in order: a larger value, then the larger place, is the larger key;
+// the value 0 is none.  Of a row, values are fp32 logits and places its tokens from the last; of a
+// sequence, 64-bit sums, and places the beams from the last, then the logits (sums of one beam may
+// be one number where they are not), then the tokens from the last.
 __device__ __forceinline__ uint32_t ordered(float v) {  // 0 for -inf and NaN, which are no candidates
     if (!(v > -INFINITY)) return 0;
     const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // -0 is 0
@@ -44,8 +45,14 @@ __device__ __forceinline__ double unordered(uint64_t ord) {
     return __builtin_bit_cast(double, (ord >> 63) ? ord & ~(1ull << 63) : ~ord);
 }
 struct Key {
-    uint64_t value, place;  // ordered bits; ~(beam, token), or ~token
+    uint64_t value, place;  // ordered bits
 };
+constexpr uint32_t kTokenBits = 24, kTokens = 1u << kTokenBits;  // of a place in a sequence: above them 32 of the logit, then the beam
+__device__ __forceinline__ uint64_t place_of(uint32_t beam, uint32_t logit, uint32_t token) {
+    return static_cast<uint64_t>(kBeamsMost - 1 - beam) << (kTokenBits + 32) | static_cast<uint64_t>(logit) << kTokenBits | (kTokens - 1 - token);
+}
+__device__ __forceinline__ uint32_t beam_of(uint64_t place) { return kBeamsMost - 1 - static_cast<uint32_t>(place >> (kTokenBits + 32)); }
+__device__ __forceinline__ uint32_t token_of(uint64_t place) { return kTokens - 1 - (static_cast<uint32_t>(place) & (kTokens - 1)); }
 __device__ __forceinline__ bool larger(const Key &a, const Key &b) {
     return a.value > b.value || (a.value == b.value && a.place > b.place);
 }
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void beam_sequences_kernel(SelectArgs a) 
         for (int e = 0; e < N; ++e) {
             const uint32_t b = min((i0 + tid + kThreads * e) / of_row, a.beams - 1);
             v[e] = next[e] ? base[b] + (static_cast<double>(unordered(static_cast<uint32_t>(next[e] >> 32))) - most[b]) : -INFINITY;
-            place[e] = ~(static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(next[e]));
+            place[e] = place_of(b, static_cast<uint32_t>(next[e] >> 32), static_cast<uint32_t>(next[e]));
         }
         v[N] = -INFINITY;
         if (i0 > 0 && tid < a.count && select.list[tid].value) {
@@ -267,10 +274,10 @@ __global__ __launch_bounds__(kThreads) void beam_sequences_kernel(SelectArgs a) 
     int32_t parent = -1, token = -1;
     const bool real = lane < a.count && select.list[lane].value;
     if (real) {
-        const uint64_t at = ~select.list[lane].place;
+        const uint64_t at = select.list[lane].place;
         value = static_cast<float>(unordered(select.list[lane].value));
-        parent = static_cast<int32_t>(row0 + static_cast<uint32_t>(at >> 32));
-        token = static_cast<int32_t>(static_cast<uint32_t>(at));
+        parent = static_cast<int32_t>(row0 + beam_of(at));
+        token = static_cast<int32_t>(token_of(at));
     }
     if (lane < a.count) {
         a.values[out + lane] = value;
@@ -313,7 +320,7 @@ hipError_t launch_select(SelectArgs a, uint32_t sequences, void *workspace, hipS
 
 bool select_sizes(uint32_t sequences, uint32_t beams, uint32_t vocab, uint32_t count) {
     return sequences > 0 && beams > 0 && beams <= kBeamsMost && static_cast<uint64_t>(sequences) * beams <= 65535 && vocab > 0 &&
-           vocab <= 1u << 24 && count > 0 && count <= kCountMost;
+           vocab <= kTokens && count > 0 && count <= kCountMost;
 }
 
 // ---- what the beams keep ------------------------------------------------------

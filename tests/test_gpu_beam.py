@@ -167,6 +167,38 @@ def test_logits_of_any_size(gpu_ctx, size):
     assert bool((((got[0].double() - want[0]).abs() <= tol) | (got[0].double() == want[0].float().double())).all())
 
 
+def best_by_logit(logits, scores, beams, vocab, count):
+    """[seqs][count] rows and tokens by value (a beam's by their logits: its sum and score are the same to all of
+    them), the lower beam, the lower token; for beams whose values lie far apart."""
+    rows, tokens = [], []
+    for s in range(scores.shape[0]):
+        order = sorted(((b, t) for b in range(beams) for t in range(vocab) if float(logits[s * beams + b, t]) > -math.inf),
+                       key=lambda c: (-float(scores[s, c[0]]), c[0], -float(logits[s * beams + c[0], c[1]]), c[1]))[:count]
+        rows.append([s * beams + b for b, _ in order])
+        tokens.append([t for _, t in order])
+    return rows, tokens
+
+
+@pytest.mark.parametrize("size,score", [(1e-30, 0.0), (2.0 ** -40, -1.0), (1e-3, -1e9), (0.25, -1e12), (1.0, -3e38)])
+def test_logits_apart_by_less_than_their_value_shows(gpu_ctx, size, score):
+    """Of one beam the larger logits come first, also where score + logit is one 64-bit number for all of them (a
+    score of -1e9 for beams that are not yet in use): over several parts of the vocabulary, in both orders."""
+    vocab, count = 9001, 12
+    g = sv.gen(int(-score) % 1000)
+    up = (torch.arange(vocab) + 1.0) * (size / vocab)
+    for x in (up, up.flip(0), up[torch.randperm(vocab, generator=g)]):
+        logits = torch.full((2, vocab), -math.inf)
+        logits[0, [5, 4097]] = torch.tensor([2.0, 3.0])
+        logits[1] = x
+        scores = torch.tensor([[score / 2 + 1.0, score]])
+        if score == 0.0:
+            scores = torch.tensor([[50.0, score]])
+        got = select(gpu_ctx, logits, scores, 2, vocab, count, "f32")
+        rows, tokens = best_by_logit(logits, scores, 2, vocab, count)
+        assert rows[0][:2] == [0, 0] and rows[0][2:] == [1] * (count - 2)
+        assert got[1].tolist() == rows and got[2].tolist() == tokens
+
+
 def test_select_refusals(gpu_ctx):
     seqs, beams, vocab, count = 2, 3, 50, 6
     x = torch.zeros(seqs * beams, 2 * vocab, device=sv.DEV)

@@ -80,7 +80,7 @@ __device__ __forceinline__ uint32_t find_bound(const uint32_t *numbers, uint32_t
 constexpr uint32_t kFound = 512;
 constexpr uint32_t kLeast = 0x00100000u;  // below what any number's upper bits are ordered as, above none's
 struct Selection {
-    uint32_t tops[kThreads];
+    alignas(16) uint32_t tops[kThreads];  // read four at a time
     Key found[kFound];
     Key list[kCountMost];
     Key best[kThreads / kWaveSize];

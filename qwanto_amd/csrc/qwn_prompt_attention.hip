@@ -351,11 +351,15 @@ __device__ __forceinline__ v4u load_chunk(const T *row, uint32_t c, uint32_t n) 
 }
 // 16 bytes a lane into LDS, the wave's next to each other from `to` on.  In
 // assembly, as the compiler would wait for all such loads before the transposing reads
-// of the other buffer; it does not count them: wait_vmcnt does.
+// of the other buffer; it does not count them: wait_vmcnt does.  m0 is one of the compiler's own
+// registers, of which it warns; named, it knows that what m0 held is gone.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(const void *from, v4u *to) {
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)to));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <typename T>
 __device__ __forceinline__ bool finite(T v) {
     if constexpr (sizeof(T) == 4) {

@@ -91,15 +91,14 @@ constexpr float kLift = std::is_same_v<T, f16> ? 6.0f : 0.0f;
 template <typename T>
 constexpr float kMost = std::is_same_v<T, f16> ? 65504.0f : 0x1p40f;
 // Probabilities of up to 2^40 times values past 2^88, or a sum of values next to the
-// type's largest, are past fp32 although their average is not.  A block where an average has
-// come out infinite or NaN is gone through again, with probabilities 2^-34 as large and references at each
-// row's largest so far: those of 2^31 tokens add up to less than 1 (f16's products are
-// below 2^32, its averages only rounded past the largest).  Only what was not finite and now is
-// takes the second result, so what one channel holds shows in no other.
+// type's largest, are past fp32 although their average is not.  A block with sums near that is
+// gone through again, with probabilities 2^-34 as large and references at each
+// row's largest so far: those of 2^31 tokens add up to less than 1.  Only what was not finite and
+// now is takes the second result, so what one channel holds shows in no other.  f16's products
+// are below 2^32: its averages may only be rounded past the largest.
+constexpr float kSecondLift = -34.0f;
 template <typename T>
-constexpr float kSecondLift = std::is_same_v<T, f16> ? kLift<T> : -34.0f;
-template <typename T>
-constexpr float kSecondMost = std::is_same_v<T, f16> ? kMost<T> : 0.0f;
+constexpr bool kTwice = !std::is_same_v<T, f16>;
 // The type's largest number: an average of finite values is not past it, but may be rounded past it.
 template <typename T>
 constexpr float kLargest = std::is_same_v<T, f16> ? 65504.0f : std::is_same_v<T, bf16> ? 0x1.fep127f : 0x1.fffffep127f;
@@ -377,16 +376,23 @@ __device__ __forceinline__ uint32_t lane_anew() {
     return lane;
 }
 
-// N of a row's sums from channel ch on as averages.  odd: not finite afterwards where one may have come out so.
+// Whether some of a part's sums are past 2^-4 of fp32's largest, or NaN: else the joined ones, of four parts at
+// most, are finite, and so are their averages.  (More is taken for it where several come near; that costs a pass.)
+template <int C>
+__device__ __forceinline__ bool past_range(const v16f (&acc)[C]) {
+    float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) odd[e % 4] = fmaf(acc[c][e], 16.0f, odd[e % 4]);
+    return !(fabsf((odd[0] + odd[1]) + (odd[2] + odd[3])) < INFINITY);
+}
+// N of a row's sums from channel ch on as averages.
 template <typename T, int N>
-__device__ __forceinline__ void store_averages(T *dst, uint32_t ch, uint32_t channels, const float (&sums)[N], float inv, float &odd) {
-    const float past = inv * (0x1.fffffep127f / kLargest<T> * 1.0001f);  // takes what rounds to an infinity past fp32
+__device__ __forceinline__ void store_averages(T *dst, uint32_t ch, uint32_t channels, const float (&sums)[N], float inv) {
     Vec<T, N> y;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        y.v[k] = from_float<T>(sums[k] * inv);  // f16: one instruction, one rounding
-        odd = fmaf(sums[k], past, odd);
-    }
+    for (int k = 0; k < N; ++k) y.v[k] = from_float<T>(sums[k] * inv);
     if (ch + N <= channels) {
         store_vec<T, N>(dst + ch, y);
     } else {
@@ -395,7 +401,7 @@ __device__ __forceinline__ void store_averages(T *dst, uint32_t ch, uint32_t cha
             if (ch + k < channels) dst[ch + k] = y.v[k];
     }
 }
-// The second time: to what is not finite there, and now is.
+// The same where what is there is not finite, and can be.
 template <typename T, int N>
 __device__ __forceinline__ void mend_averages(T *dst, uint32_t ch, uint32_t channels, const float (&sums)[N], float inv) {
 #pragma unroll
@@ -459,8 +465,8 @@ __device__ __forceinline__ void load_query(const PromptArgs &a, const Block &b, 
 // 32 heads of 128, one prompt of 8192 tokens 521 to 552 us (1 PFLOP/s, of 1.17 that a
 // large product reaches); short ones by the longest block's chain of tiles: nine of up to
 // 1777 tokens 45 us, of which a large product would take 25.
-template <typename T, int W, int KT, int RW, bool DIRECT, bool again>
-__device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave, uint32_t lane) {
+template <typename T, int W, int KT, int RW, bool DIRECT, bool AGAIN>
+__device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t &again_wanted, uint32_t wave, uint32_t lane) {
     using M = Matrix<T>;
     using L = Tile<T, W>;
     constexpr uint32_t CE = L::CE, NC = L::NC;
@@ -470,7 +476,6 @@ __device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave,
     static_assert(kChunks % kThreads == 0 && S > 0, "whole rounds of loads, a part for each wave");
     extern __shared__ v4u tiles[];          // two times keys, then values
     constexpr uint32_t kMasked = kBlockRows / KT + 2;
-    __shared__ uint32_t again_wanted;
     __shared__ uint32_t odd[kMasked][KT / 32];  // of the masked tiles: tokens with values that are not finite
     const uint32_t tid = wave * kWaveSize + lane, n = lane % 32, h = lane / 32, part = wave / RW;  // of a tile's tokens
     Block b;
@@ -558,9 +563,9 @@ __device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave,
     const Row r = row_of(a, b, b.row0 + wave % RW * kWaveRows, n);
     v4u qf[J];
     Softmax soft;
-    soft.lift = again ? kSecondLift<T> : kLift<T>;
+    soft.lift = AGAIN ? kSecondLift : kLift<T>;
     load_query<T>(a, b, r, h, qf, soft.mul);
-    if (tid == 0) again_wanted = 0;
+    if (!AGAIN && tid == 0) again_wanted = 0;
     if (tid < kMasked * (KT / 32)) odd[tid / (KT / 32)][tid % (KT / 32)] = 0;
 
     // where a lane's operands lie in a buffer: of keys piece 2 j + h of token n, of V^T
@@ -619,7 +624,7 @@ __device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave,
                     if (32 * s + 8 * (e / 4) + e % 4 >= seen) sc[s][e] = -INFINITY;
         }
         float p[S][16];
-        softmax_tile(sc, soft, p, acc, i == 0, r.visible > t0, again ? kSecondMost<T> : kMost<T>);
+        softmax_tile(sc, soft, p, acc, i == 0, r.visible > t0, AGAIN ? 0.0f : kMost<T>);
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -670,7 +675,7 @@ __device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave,
         }
     }
 
-    float odd_sums = 0.0f;
+    if (!AGAIN && kTwice<T> && past_range(acc)) again_wanted = 1;
     if (join_parts<C, RW, kWaves>(tiles, wave, lane, r.visible > part * S * 32, soft, acc) && r.visible > 0) {
         const float inv = 1.0f / soft.sum;
         T *dst = static_cast<T *>(a.output) + static_cast<size_t>(b.q.row + r.token) * a.output_stride + r.at;
@@ -683,23 +688,25 @@ __device__ __forceinline__ bool attend_block(const PromptArgs &a, uint32_t wave,
                     take(32 * c + 8 * (e / 4) + 4 * h, sums);
                 }
         };
-        if (!again) {
-            each([&](uint32_t ch, const float (&sums)[4]) {
-                store_averages<T, 4>(dst, ch, a.head_dim, sums, inv, odd_sums);
+        if (!AGAIN) each([&](uint32_t ch, const float (&sums)[4]) { store_averages<T, 4>(dst, ch, a.head_dim, sums, inv); });
+        if constexpr (!kTwice<T>) {
+            float odd = 0.0f;  // infinite or NaN where an average past the type's largest is added
+            each([&](uint32_t, const float (&sums)[4]) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) odd = fmaf(sums[k], inv * (0x1.fffffep127f / kLargest<T> * 1.0001f), odd);
             });
-        } else {
-            each([&](uint32_t ch, const float (&sums)[4]) { mend_averages<T, 4>(dst, ch, a.head_dim, sums, inv); });
+            if (fabsf(odd) < INFINITY) return false;
         }
+        if (AGAIN || !kTwice<T>) each([&](uint32_t ch, const float (&sums)[4]) { mend_averages<T, 4>(dst, ch, a.head_dim, sums, inv); });
     }
-    if (again) return false;
-    if (!(fabsf(odd_sums) < INFINITY)) again_wanted = 1;
-    lds_barrier();
+    if (AGAIN || !kTwice<T>) return false;
+    if (KW == 1) lds_barrier();  // else the join has come past some since
     return __builtin_amdgcn_readfirstlane(again_wanted);
 }
 
-// What a workgroup does, and again where the first pass asks for it (it returns whether).  The second is code of its
-// own, with arguments and lanes taken anew: as a loop over one code both passes
-// spilled registers (the first now has none more than alone; 16 tokens 8.3 us for 8.1, 8192 the same).
+// What a workgroup does, and again where the first pass asks for it (every wave returns whether).  The second is
+// code of its own, with arguments and lanes taken anew, so that the first keeps nothing in registers for it: as a
+// loop over one code both spilled.  The first one's times are what they are without a second, to 0.3 us.
 __device__ __forceinline__ PromptArgs arguments_at(uint64_t args) {
     auto word = [&](size_t at) { return *reinterpret_cast<const __attribute__((address_space(4))) uint32_t *>(args + at); };
     auto pointer = [&](size_t at) {
@@ -724,17 +731,23 @@ __device__ __forceinline__ PromptArgs arguments_at(uint64_t args) {
     a.scale = __builtin_bit_cast(float, word(offsetof(PromptArgs, scale)));
     return a;
 }
-template <auto FIRST, auto SECOND>
-__device__ __forceinline__ void once_or_twice(const PromptArgs &a) {
+template <auto FIRST, auto SECOND, typename K>
+__device__ __forceinline__ void once_or_twice(const PromptArgs &a, K &kept) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-    if (!FIRST(a, wave, threadIdx.x % kWaveSize)) return;
+    if (!FIRST(a, kept, wave, threadIdx.x % kWaveSize)) return;
+    lds_barrier();  // the first pass's LDS is read
     uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(args));
-    SECOND(arguments_at(args), wave, lane_anew());
+    SECOND(arguments_at(args), kept, wave, lane_anew());
 }
 template <typename T, int W, int KT, int RW, bool DIRECT>
 __global__ __launch_bounds__(kThreads, W == 256 ? 1 : W == 64 && KT == 64 ? 3 : 2) void prompt_attention_kernel(PromptArgs a) {
-    once_or_twice<&attend_block<T, W, KT, RW, DIRECT, false>, &attend_block<T, W, KT, RW, DIRECT, true>>(a);
+    __shared__ uint32_t again_wanted;
+    if constexpr (kTwice<T>) {
+        once_or_twice<&attend_block<T, W, KT, RW, DIRECT, false>, &attend_block<T, W, KT, RW, DIRECT, true>>(a, again_wanted);
+    } else {
+        attend_block<T, W, KT, RW, DIRECT, false>(a, again_wanted, __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize), threadIdx.x % kWaveSize);
+    }
 }
 
 // fp32.  A product of two fp32 operands (v_mfma_f32_32x32x2_f32) takes 64 cycles for
@@ -751,12 +764,20 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : W == 64 && KT == 64 ? 3 : 
 // rows are channels c, c + W / 32, ...  WHOLE: heads of W channels.
 // Bound by the matrix unit: those 1176 us are 117 TFLOP/s, of 154 that a large product
 // reaches; few rows by the longest one's chain of tiles.
-template <int W, bool WHOLE, bool again>
-__device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, uint32_t wave, uint32_t lane) {
+// One for both passes: 128 channels take 53.2 KB for the join, of which three workgroups have room in a CU's LDS
+// as long as there are 512 bytes more at most; the third starts while the first waves of two write their output
+// (four prompts of 1024, 687, 598 and 171 tokens 97 us without, 93 with).
+struct Kept {
+    uint32_t again_wanted;
+    uint2 rows[kWaveRows];  // token and place of each, until its output
+};
+template <int W, bool WHOLE, bool AGAIN>
+__device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, Kept &kept, uint32_t wave, uint32_t lane) {
     constexpr uint32_t KT = 32, KW = kWaves;
     constexpr int C = W / 32, J = W / 8;
     extern __shared__ v4u lds[];
-    __shared__ uint32_t again_wanted;
+    uint2 *const rows = kept.rows;
+    uint32_t &again_wanted = kept.again_wanted;
     const uint32_t tid = wave * kWaveSize + lane, n = lane % 32, h = lane / 32, part = wave;
     Block b;
     if (!block_of<kWaveRows>(a, lane, b)) return false;
@@ -808,13 +829,14 @@ __device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, uint32_t w
     };
     v4u qf[J];
     Softmax soft;
-    soft.lift = again ? kSecondLift<float> : kLift<float>;
+    soft.lift = AGAIN ? kSecondLift : kLift<float>;
     load_query<float>(a, b, r, h, qf, soft.mul);
     v4u *const query = lds + lane;
-    if (tid == 0) again_wanted = 0;
+    if (!AGAIN && tid == 0) again_wanted = 0;
     if (wave == 0) {
 #pragma unroll
         for (int j = 0; j < J; ++j) query[j * kWaveSize] = qf[j];
+        rows[n] = make_uint2(r.token, r.at);
     }
     lds_barrier();
     if (part < count) load_keys(part);
@@ -859,7 +881,7 @@ __device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, uint32_t w
             }
         }
         float p[1][16];
-        softmax_tile(sc, soft, p, acc, i == part, r.visible > t0, again ? kSecondMost<float> : kMost<float>);
+        softmax_tile(sc, soft, p, acc, i == part, r.visible > t0, AGAIN ? 0.0f : kMost<float>);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
 #pragma unroll
@@ -881,38 +903,32 @@ __device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, uint32_t w
         }
     }
 
-    float odd_sums = 0.0f;
-    const uint32_t late = lane_anew();
-    const Row row = row_of(a, b, b.row0, late % 32);
-    if (join_parts<C, 1, kWaves>(lds, wave, late, row.visible > part * KT, soft, acc) && row.visible > 0) {
+    if (!AGAIN && past_range(acc)) again_wanted = 1;
+    const uint32_t late = lane_anew(), token = rows[late % 32].x, at = rows[late % 32].y;
+    const uint32_t visible = b.row0 + late % 32 <= b.last ? token + 1 : 0u;
+    if (join_parts<C, 1, kWaves>(lds, wave, late, visible > part * KT, soft, acc) && visible > 0) {
         const float inv = 1.0f / soft.sum;
-        float *dst = static_cast<float *>(a.output) + static_cast<size_t>(b.q.row + row.token) * a.output_stride + row.at;
-        auto each = [&](auto take) {
+        float *dst = static_cast<float *>(a.output) + static_cast<size_t>(b.q.row + token) * a.output_stride + at;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float sums[C];
+        for (int e = 0; e < 16; ++e) {
+            const uint32_t ch = C * (8 * (e / 4) + 4 * (late / 32) + e % 4);
+            float sums[C];
 #pragma unroll
-                for (int c = 0; c < C; ++c) sums[c] = acc[c][e];
-                take(C * (8 * (e / 4) + 4 * (late / 32) + e % 4), sums);
+            for (int c = 0; c < C; ++c) sums[c] = acc[c][e];
+            if (AGAIN) {
+                mend_averages<float, C>(dst, ch, a.head_dim, sums, inv);
+            } else {
+                store_averages<float, C>(dst, ch, a.head_dim, sums, inv);
             }
-        };
-        if (!again) {
-            each([&](uint32_t ch, const float (&sums)[C]) {
-                store_averages<float, C>(dst, ch, a.head_dim, sums, inv, odd_sums);
-            });
-        } else {
-            each([&](uint32_t ch, const float (&sums)[C]) { mend_averages<float, C>(dst, ch, a.head_dim, sums, inv); });
         }
     }
-    if (again) return false;
-    if (!(fabsf(odd_sums) < INFINITY)) again_wanted = 1;
-    lds_barrier();
-    return __builtin_amdgcn_readfirstlane(again_wanted);
+    return !AGAIN && __builtin_amdgcn_readfirstlane(again_wanted);
 }
 
 template <int W, bool WHOLE>
 __global__ __launch_bounds__(kThreads, W <= 128 ? 2 : 1) void prompt_attention_f32_kernel(PromptArgs a) {
-    once_or_twice<&attend_block_f32<W, WHOLE, false>, &attend_block_f32<W, WHOLE, true>>(a);
+    __shared__ Kept kept;
+    once_or_twice<&attend_block_f32<W, WHOLE, false>, &attend_block_f32<W, WHOLE, true>>(a, kept);
 }
 
 // Blocks of a batch at most: one of each sequence is not full.

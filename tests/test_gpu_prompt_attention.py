@@ -455,3 +455,83 @@ def test_captured_and_on_two_streams(gpu_ctx, dtype):
         torch.cuda.synchronize()
         assert torch.equal(out, want), starts
         assert bool((out[starts[-1]:] == 2.0).all())
+
+
+def groups_of(lengths, heads, kv_heads, pad=0):
+    """Workgroups that blocks of 128 rows would make: from 320 on these are taken."""
+    tokens, group = sum(lengths) + pad, heads // kv_heads
+    return (tokens * group + min(len(lengths), tokens) * 127) // 128 * kv_heads
+
+
+LARGE = [(32, 8, 128, [700, 0, 530, 1, 129], 3), (16, 16, 96, [1300, 1200], 0), (40, 40, 256, [600, 450], 1), (40, 40, 200, [700, 300], 0),
+         (36, 36, 33, [640, 500], 2), (32, 32, 80, [257, 900], 0), (64, 32, 64, [100] * 7, 1), (48, 48, 40, [900], 0)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d,lengths,pad", LARGE)
+def test_blocks_of_128_rows(gpu_ctx, dtype, heads, kv_heads, d, lengths, pad):
+    """Batches that fill the GPU, in blocks of 128 rows: every width, heads narrower than it, unaligned rows."""
+    assert groups_of(lengths, heads, kv_heads, pad) >= 320
+    q, k, v = inputs(d + sum(lengths), sum(lengths) + pad, heads, kv_heads, d, dtype)
+    got = attend(gpu_ctx, q, k, v, lengths, heads, kv_heads, d, d ** -0.5, dtype)
+    check(got, q, k, v, lengths, heads, kv_heads, d, d ** -0.5, dtype)
+    # columns of one buffer, at an odd element
+    n = q.shape[0]
+    buf = torch.cat([torch.full((n, 3), float("nan")).to(q.dtype), q, k, v], dim=1).to(sv.DEV).contiguous()
+    a, b = 3 + heads * d, 3 + (heads + kv_heads) * d
+    odd = torch.full_like(got, 5.0)
+    attend(gpu_ctx, buf[:, 3:], buf[:, a:], buf[:, b:], lengths, heads, kv_heads, d, d ** -0.5, dtype, out=odd, query_stride=buf.shape[1],
+           key_stride=buf.shape[1], value_stride=buf.shape[1], output_stride=heads * d)
+    assert torch.equal(odd, got)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d,n", [(32, 8, 128, 1280), (40, 40, 256, 1027), (36, 36, 33, 1150), (64, 32, 64, 700), (24, 24, 200, 1707)])
+def test_what_is_masked_in_blocks_of_128_rows(gpu_ctx, dtype, heads, kv_heads, d, n):
+    """Values and keys that are not finite leave the rows before them, and other heads and channels, as they were to the
+    bit; values show in their channel of the rows that see them."""
+    assert groups_of([n], heads, kv_heads) >= 320
+    group = heads // kv_heads
+    q, k, v = (x.to(sv.DEV) for x in inputs(n, n, heads, kv_heads, d, dtype))
+    clean = attend(gpu_ctx, q, k, v, [n], heads, kv_heads, d, 0.1, dtype)
+    for t in (0, 31, 32, 63, 64, 127, 128, 500, n - 33, n - 1):
+        b = v.clone()
+        b[t, 5], b[t, (kv_heads - 1) * d + 9] = -math.inf, math.nan
+        got = attend(gpu_ctx, q, k, b, [n], heads, kv_heads, d, 0.1, dtype).reshape(n, heads, d)
+        assert bool((got[t:, :group, 5] == -math.inf).all()) and bool(torch.isnan(got[t:, heads - group:, 9]).all()), t
+        got[t:, :group, 5] = clean.reshape(n, heads, d)[t:, :group, 5]
+        got[t:, heads - group:, 9] = clean.reshape(n, heads, d)[t:, heads - group:, 9]
+        assert torch.equal(got.reshape(n, -1), clean), t
+        b = k.clone()
+        b[t, d:] = math.nan                                                      # all KV heads but the first
+        got = attend(gpu_ctx, q, b, v, [n], heads, kv_heads, d, 0.1, dtype)
+        assert torch.equal(got[:t], clean[:t]) and torch.equal(got[:, :group * d], clean[:, :group * d]), t
+        assert bool(torch.isnan(got[t:, group * d:]).all()), t
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,n", [("bf16", 32, 8, 128, 1400), ("f16", 64, 32, 64, 800)])
+def test_blocks_of_128_rows_captured_and_on_two_streams(gpu_ctx, dtype, heads, kv_heads, d, n):
+    q, k, v = (x.to(sv.DEV) for x in inputs(7, n, heads, kv_heads, d, dtype))
+    st = torch.zeros(4, dtype=torch.int32, device=sv.DEV)
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    req = lambda o: gpu_ctx.prompt_attention_request(3, n, sv.ptr(st), dtype, heads, kv_heads, d, sv.ptr(q), sv.ptr(k), sv.ptr(v),  # noqa: E731
+                                                     sv.ptr(o), 0.1)
+    assert groups_of([n, 0, 0], heads, kv_heads) >= 320
+    r, e = req(out), req(want)
+    gpu_ctx.prompt_attention_device(e, stream=sv.stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu_ctx.prompt_attention_device(r, stream=sv.stream())
+    side = torch.cuda.Stream()
+    for starts in ([0, n, n, n], [0, 1, 200, n - 70], [0, 0, 130, 260], [0, n - 1, n - 1, n]):
+        st.copy_(torch.tensor(starts, dtype=torch.int32))
+        out.fill_(2.0)
+        want.fill_(2.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            gpu_ctx.prompt_attention_device(e, stream=sv.stream())
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), starts
+        assert bool((out[starts[-1]:] == 2.0).all())

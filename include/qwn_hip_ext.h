@@ -490,7 +490,7 @@ typedef struct {
     void *key_out;
     const float *query_norm;       /* NULL, or [head_dim] */
     const float *key_norm;
-    const int32_t *positions;      /* [axes with a section][position_stride] */
+    const int32_t *positions;      /* [axis][position_stride], axes up to the last that has a section */
 } QwnHipRotaryRequest;
 QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *context, const QwnHipRotaryRequest *request, void *stream);
 

@@ -818,7 +818,8 @@ class Context:
                        k_ptr: int | None = None, k_out_ptr: int | None = None, q_norm_ptr: int | None = None,
                        k_norm_ptr: int | None = None, eps: float = 0.0, query_stride: int = 0, key_stride: int = 0,
                        query_out_stride: int = 0, key_out_stride: int = 0, position_stride: int = 0) -> RotaryRequest:
-        """`sections`: pairs of each axis, up to 4 (None: all of them the first axis')."""
+        """`sections`: pairs of each axis, up to 4 (None: all of them the first axis'); the positions have a row
+        for every axis up to the last that has pairs."""
         sections = [rope_dims // 2] if sections is None else list(sections)
         return RotaryRequest(tokens=tokens, dtype=ACTIVATION[dtype], query_heads=query_heads, key_heads=key_heads,
                              head_dim=head_dim, rope_dims=rope_dims, sections=(ctypes.c_uint32 * 4)(*sections),

@@ -191,6 +191,35 @@ def test_norms_of_any_size(gpu_ctx, dtype, d, rope):
     check(out[0].cpu(), want, size, dtype)
 
 
+def test_axes_without_a_section_have_a_row(gpu_ctx):
+    """Positions are found by the axis' number, so an axis without pairs has a row of its own, too, which does not count;
+    rows up to the last axis with pairs are an input, which an output may not overlap."""
+    tokens, d = 7, 64
+    g = sv.gen(3)
+    x, p = sv.normal(g, tokens, d), positions_of(g, 4, tokens)
+    xd, out = x.to(sv.DEV), torch.zeros(tokens, d, device=sv.DEV)
+    for sections in ([4, 0, 28], [0, 0, 0, 32], [0, 32], [16, 0, 0, 16]):
+        want, size = reference(x, 1, d, d, p, sections, False, None)
+        for other in (0, 2 ** 31 - 1):
+            q = p.clone()
+            for a, n in enumerate(sections):
+                if not n:
+                    q[a] = other
+            qd = q[:len(sections)].contiguous().to(sv.DEV)
+            gpu_ctx.rotary_device(gpu_ctx.rotary_request(tokens, "f32", d, d, THETA, sv.ptr(qd), sections=sections, query_heads=1, q_ptr=sv.ptr(xd),
+                                                         q_out_ptr=sv.ptr(out)), stream=sv.stream())
+            torch.cuda.synchronize()
+            check(out.cpu(), want, size, "f32")
+    both = torch.zeros(3 * tokens + tokens * d, dtype=torch.int32, device=sv.DEV)
+    req = lambda sections, at: gpu_ctx.rotary_request(tokens, "f32", d, d, THETA, sv.ptr(both), sections=sections, query_heads=1,  # noqa: E731
+                                                      q_ptr=sv.ptr(xd), q_out_ptr=sv.ptr(both) + 4 * at)
+    gpu_ctx.rotary_device(req([32, 0], tokens), stream=sv.stream())
+    gpu_ctx.rotary_device(req([4, 0, 28], 3 * tokens), stream=sv.stream())
+    with pytest.raises(abi.AbiError):
+        gpu_ctx.rotary_device(req([4, 0, 28], 2 * tokens), stream=sv.stream())
+    torch.cuda.synchronize()
+
+
 def test_refusals(gpu_ctx):
     t, d = 4, 64
     q, k = torch.zeros(t, 2 * d, device=sv.DEV), torch.zeros(t, d, device=sv.DEV)

@@ -502,7 +502,7 @@ QWN_CUDA_ABI_API int qwn_hip_ext_rotary_device(QwnCudaContextHandle *context, co
  * left out.  Scores and sums are fp32, probabilities are rounded to dtype (f16: below 2^-20 of
  * the row's largest to steps of 2^-30 of that); fp32 is fp32 throughout.  Finite queries, keys and scale have their softmax whatever the
  * scores' size, past fp32's too (of fp32 and bf16, a channel counts as zero where the
- * key is below 2^-100, or the query below 2^-100 of its row's largest).  A key or query
+ * key times the query, taken as its share of its row's largest, is below 2^-116).  A key or query
  * with an infinity: a score of -inf has probability 0, a row with one that is +inf or
  * NaN, and a row with a scale that is not finite, is NaN.  A value that is not finite
  * makes its channel so in the rows that attend to it, and in no other; of finite values, up to

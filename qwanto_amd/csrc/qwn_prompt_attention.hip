@@ -135,11 +135,12 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t lane, u
 }
 
 // What a row's products, of queries times the power of two `up`, are multiplied
-// by to be exponents of 2: positive, the scale's sign is the queries'.  Below
-// 2^-100 all scores are alike; past fp32 the largest fp32 stands in its place.
+// by to be exponents of 2: positive, the scale's sign is the queries'.  Products are below 2^127:
+// where it is below fp32's numbers all scores are alike (its rounding to the smallest of them is off by
+// 2^-22 of an exponent); past fp32 the largest fp32 stands in its place.
 __device__ __forceinline__ float exponents_of(float scale, int bits, float &up) {
     const float mul = fminf(ldexpf(fabsf(scale), bits) * 1.44269504088896340736f, 3.402823466e38f);
-    const bool alike = mul < 0x1p-100f;
+    const bool alike = mul == 0.0f;
     up = alike ? 0.0f : copysignf(up, scale);
     if (!isfinite(scale)) up = __builtin_nanf("");  // the row is NaN, whatever the keys are
     return alike ? 1.0f : mul;

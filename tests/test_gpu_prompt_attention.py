@@ -251,6 +251,21 @@ def test_scores_past_fp32(gpu_ctx, dtype):
         assert bool(((got - want).abs() <= (sv.HALF[dtype] + 2.0 ** -22) * want.abs()).all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("q_size,k_size,scale", [(1.0, 1e36, 1e-36), (1e-30, 1e36, 1e-6), (1e-20, 3e37, 1e-18), (1e30, 1e-30, 1.0), (1e-36, 1e36, -1.0),
+                                                 (30.0, 3e37, 1e-38), (1e-5, 1e37, 2e-33), (1e38, 1e-34, 1e-4), (1e-38, 1e38, 1.0)])
+@pytest.mark.parametrize("d,n", [(64, 150), (128, 70)])
+def test_ordinary_scores_of_factors_of_any_size(gpu_ctx, dtype, q_size, k_size, scale, d, n):
+    """Queries, keys and a scale of which no product is out of the ordinary, though each may be."""
+    g = sv.gen(12)
+    dt = sv.DTYPES[dtype]
+    q, k, v = ((s * (2 * torch.rand(n, d, generator=g) - 1)).to(dt) for s in (q_size, k_size, 1.0))
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    s = q.double() @ k.double().t() * scale
+    assert 0.01 < float(s.std()) < 100
+    check(attend(gpu_ctx, q, k, v, [n], 1, 1, d, scale, dtype), q, k, v, [n], 1, 1, d, scale, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_queries_and_scales_that_are_not_finite(gpu_ctx, dtype):
     q, k, v = inputs(2, 40, 2, 1, 64, dtype)

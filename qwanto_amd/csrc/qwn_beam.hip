@@ -480,8 +480,8 @@ __device__ __forceinline__ void move_columns(const AdvanceArgs &a, uint32_t sequ
 }
 
 // grid: workgroups from `first` on of those that copy (a row and a cache each, at
-// least one cache), then of those that move (a sequence, and 256 columns).  4 rows 4.1 us, a
-// launch and three loads one after the other; 64 rows of 28 caches 10.8, copies of up to 18 KB each.
+// least one cache), then of those that move (a sequence, and 256 columns).  4 rows 4.2 us, a
+// launch and three loads one after the other; 64 rows of 28 caches 10.9, copies of up to 18 KB each.
 __global__ __launch_bounds__(kThreads) void beam_advance_kernel(CopyArgs args, uint32_t first, uint32_t copies, uint32_t rows,
                                                                 uint32_t groups, uint32_t table_groups) {
     const uint32_t i = first + blockIdx.x;

@@ -47,9 +47,11 @@ constexpr float kFar = 0x1p20f;               // of references: past it their ro
 constexpr uint64_t kManyGroups = 320;
 // Heads of 64 channels have half the products between two barriers: in sequences of that
 // many tokens on average tiles of 128, until so many workgroups hide the barriers by
-// themselves (16 heads: one prompt of 2048 tokens 23 us for 27, of 3000, 1200 and 300 45 for
-// 50; but 30 of 200, whose last tiles are mostly masked, 19 for 16, and one of 8192, 1024
-// groups, 165 for 160).
+// themselves.  16 heads, tiles of 128 and of 64: one prompt of 300 tokens 8.6 and 8.6 us, of 500 9.6 and
+// 10.4, of 2000 21.7 and 25.0, of 3000, 1200 and 300 41 and 45; six of 400 13.7 and 13.2, four of 500 12.1
+// and 12.4, but of 600 15.6 and 13.8, three of 800 16.5 and 15.2, two of 1000 16.8 and 17.2: where a sequence
+// ends in its tiles counts as much as the average, which is what the host knows.  30 of 200 tokens 19 and
+// 16; one of 8192, 1024 groups, 165 and 160.
 constexpr uint32_t kLongTokens = 512;
 constexpr uint64_t kFullGroups = 1024;
 
@@ -751,27 +753,30 @@ __global__ __launch_bounds__(kThreads, W == 256 ? 1 : W == 64 && KT == 64 ? 3 : 
     }
 }
 
-// fp32.  A product of two fp32 operands (v_mfma_f32_32x32x2_f32) takes 64 cycles for
-// an operand of 4 bytes a lane, 16 times as long as the 16-bit ones for theirs: L2
-// brings a wave's operands in the time, so keys and values need no LDS and no barrier
-// (through LDS one call of four prompts of up to 1024 tokens, 12 heads, took 225 us, and
-// takes 77).  The four waves of a workgroup take the same 32 rows and every fourth
-// tile of 32 tokens.  A tile's values are loaded when its scores are there, into the
-// registers that held its keys, the next keys after its sums: with the rows' query
-// in LDS two waves a SIMD (of 64 channels three) fit, one's products run while the
-// other waits (one wave with loads ahead: 32 heads of 128 channels, 4096 tokens, 1440 us
-// for 1176; of 256 channels, where they did not fit, 430 for 176).
-// A lane's values are W / 32 channels next to each other: block c of the output's
-// rows are channels c, c + W / 32, ...  WHOLE: heads of W channels.
-// Bound by the matrix unit: those 1176 us are 117 TFLOP/s, of 154 that a large product
-// reaches; few rows by the longest one's chain of tiles.
-// One for both passes: 128 channels take 53.2 KB for the join, of which three workgroups have room in a CU's LDS
+// What fp32's two passes share: 128 channels take 53.2 KB for the join, of which three workgroups have room in a CU's LDS
 // as long as there are 512 bytes more at most; the third starts while the first waves of two write their output
-// (four prompts of 1024, 687, 598 and 171 tokens 97 us without, 93 with).
+// (four prompts of 1024, 687, 598 and 171 tokens 97 us without it, 93 with it).
 struct Kept {
     uint32_t again_wanted;
     uint2 rows[kWaveRows];  // token and place of each, until its output
 };
+
+// fp32.  A product of two fp32 operands (v_mfma_f32_32x32x2_f32) takes 64 cycles for
+// an operand of 4 bytes a lane, 16 times as long as the 16-bit ones for theirs: L2
+// brings a wave's operands in the time, so keys and values need no LDS and no barrier
+// (through LDS one call of four prompts of 1024, 300, 100 and 500 tokens, 12 heads, took 225 us, and
+// takes 73).  The four waves of a workgroup take the same 32 rows and every fourth
+// tile of 32 tokens.  A tile's values are loaded when its scores are there, into the
+// registers that held its keys, the next keys after its sums: with the rows' query
+// in LDS two waves a SIMD fit (three of 64 channels were not faster, 332 us for 310), one's products run
+// while the other waits (one wave with loads ahead: 32 heads of 128 channels, 4096 tokens, 1440 us
+// for 1170; of 256 channels, where they did not fit, 430 for 175).  Heads between 128 and 256
+// channels have more addresses and compared channels than registers (468 bytes a lane go to
+// scratch in both passes): 200 channels, 1024 tokens of 8 heads 163 us.
+// A lane's values are W / 32 channels next to each other: block c of the output's
+// rows are channels c, c + W / 32, ...  WHOLE: heads of W channels.
+// Bound by the matrix unit: those 1160 to 1184 us are 117 TFLOP/s, of 154 that a large product
+// reaches; few rows by the longest one's chain of tiles.
 template <int W, bool WHOLE, bool AGAIN>
 __device__ __forceinline__ bool attend_block_f32(const PromptArgs &a, Kept &kept, uint32_t wave, uint32_t lane) {
     constexpr uint32_t KT = 32, KW = kWaves;

@@ -101,7 +101,7 @@ __device__ __forceinline__ double2 angle(double t) {
 }
 
 // What fp32 rows are computed in, and 16-bit ones, whose own rounding is 2^-11 and
-// more: with fp32 for both, 64 bits would take twice the registers and half the waves.
+// more (64 bits take twice the registers and half the waves).
 template <typename T>
 struct Work {
     typedef float real;
@@ -125,7 +125,7 @@ __device__ __forceinline__ double root(double v) { return rsqrt(v); }
 // grid (tokens, heads): all loads are issued first; while they are on their way the
 // tokens' angles are computed, in 64 bits (at position 100000 an fp32 angle would be
 // off by hundredths).
-// Bound by HBM: 4099 tokens of 40 bf16 heads of 128 with norms, 84 MB, 21 us, 4 TB/s of the
+// Bound by HBM: 4099 tokens of 40 bf16 heads of 128 with norms, 84 MB, 20 us, 4.2 TB/s of the
 // 5.1 that a large copy reaches; few tokens by a launch and two loads, one
 // after the other, 2.9 us.
 template <typename T, int TOKENS>

@@ -550,3 +550,38 @@ def test_blocks_of_128_rows_captured_and_on_two_streams(gpu_ctx, dtype, heads, k
         torch.cuda.synchronize()
         assert torch.equal(out, want), starts
         assert bool((out[starts[-1]:] == 2.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d,lengths,pad", LARGE + [(64, 64, 64, [640], 0), (64, 64, 24, [640], 0)])
+def test_large_values_in_blocks_of_128_rows(gpu_ctx, dtype, heads, kv_heads, d, lengths, pad):
+    """A channel of the type's largest in every token is that in every row, whatever the weights; the other channels are
+    what they are without it, to the bit; eager and replayed."""
+    assert groups_of(lengths, heads, kv_heads, pad) >= 320
+    n, top = sum(lengths), torch.finfo(sv.DTYPES[dtype]).max
+    q, k, v = (x.to(sv.DEV) for x in inputs(d, n + pad, heads, kv_heads, d, dtype))
+    q.reshape(n + pad, heads, d)[:, :, 0] = 4.0
+    k.reshape(n + pad, kv_heads, d)[:, :, 0] = torch.arange(n + pad, device=sv.DEV)[:, None].to(k.dtype)
+    clean = attend(gpu_ctx, q, k, v, lengths, heads, kv_heads, d, 0.1, dtype).reshape(-1, heads, d)
+    v.reshape(n + pad, kv_heads, d)[:, -1, 3] = top
+    st, out = starts_of(lengths).to(sv.DEV), torch.full_like(q, 5.0)
+    r = gpu_ctx.prompt_attention_request(len(lengths), n + pad, sv.ptr(st), dtype, heads, kv_heads, d, sv.ptr(q), sv.ptr(k), sv.ptr(v),
+                                         sv.ptr(out), 0.1)
+    gpu_ctx.prompt_attention_device(r, stream=sv.stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu_ctx.prompt_attention_device(r, stream=sv.stream())
+    last = heads - heads // kv_heads
+    for replay in range(3):
+        if replay:
+            out.fill_(5.0)
+            graph.replay()
+            torch.cuda.synchronize()
+        got = out.reshape(-1, heads, d)
+        # every weight is off by half a step of the type, and so is the output; sums and powers by less than 2^-18
+        assert bool((got[:n, last:, 3].double() >= top * (1 - 2 * sv.HALF[dtype] - 2.0 ** -18)).all())
+        assert bool(torch.isfinite(got).all())
+        rest = got.clone()
+        rest[:n, last:, 3] = clean[:n, last:, 3]
+        assert torch.equal(rest, clean)

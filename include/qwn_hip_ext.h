@@ -464,7 +464,8 @@ QWN_CUDA_ABI_API int qwn_hip_ext_logits_process_device(QwnCudaContextHandle *con
  * up to rope_dims / 2): one section after the other, or, with in_turn not 0,
  * dealt to the axes in turn, past those that have all of theirs.  Axes 0, 1 and 2
  * may be time, height and width; text has the same position in all.  Angles are
- * computed in 64 bits; fp32 rows are, too, and rounded once, 16-bit ones in fp32.
+ * computed in 64 bits; fp32 rows are, too, and rounded once, 16-bit ones in fp32 (norms
+ * of heads whose mean square is no number of fp32 in 64 bits).
  * An output may be its input with that one's stride. */
 #define QWN_HIP_ROTARY_AXES 4u
 typedef struct {
